@@ -43,6 +43,13 @@ typedef enum {
     LYRAQ_E4M3 = 4 /* FP8 e4m3 codes, one byte each (only where an entry point says so) */
 } lyraq_dtype_t;
 
+/* Microscaled FP4 formats: e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two to a byte, the even element in the low
+ * nibble, and a scale byte per block of consecutive values. */
+typedef enum {
+    LYRAQ_NVFP4 = 0, /* blocks of 16, scale e4m3, times a tensor scale (a positive power of two) */
+    LYRAQ_MXFP4 = 1  /* blocks of 32, scale e8m0 */
+} lyraq_fp4_format_t;
+
 /* How the activation scale of an INT8 quantize / GEMM is given. */
 typedef enum {
     LYRAQ_SCALE_PER_TENSOR = 0,       /* one fp32 scalar on the device */
@@ -103,6 +110,10 @@ LYRAQ_API int lyraq_debug_skinny_wait_test(int stalled_rank, unsigned int wait_l
  * way (0, default), so that a test reaches that kernel with small problems.  Process-wide, not thread-safe.  No counterpart in the
  * reference, which has one W4A4 kernel (src/lyradiff/kernels/w4a4_gemm/w4a4_gemm.cu). */
 LYRAQ_API int lyraq_debug_force_w4a4_wide(int on);
+
+/* Test / sweep hook: the kernel of lyraq_gemm_fp4.  0 = automatic (default); 2562 = CTA pair, 256 x 256 tile; 1281 = one CTA, 128 x 128.
+ * Process-wide, not thread-safe.  It has no counterpart in the reference, which has no FP4 linears. */
+LYRAQ_API int lyraq_debug_force_fp4_tile(int code);
 
 /* Test / sweep hook for the row kernels (quantize, LayerNorm, AdaLN, GEGLU): the most 16-byte vectors one thread
  * holds (4 or 6, default 6) before a row is given to a team twice as large.  Process-wide, not thread-safe.
@@ -171,6 +182,29 @@ LYRAQ_API int lyraq_weight_quant_int8(float* w_scale, int8_t* qw, const void* w,
 LYRAQ_API int lyraq_weight_quant_int4_g64(uint8_t* qw, void* w_scale, int scale_dtype, const void* w, int w_dtype,
                                 size_t n, size_t k, void* stream);
 
+/* Microscaled FP4 quantize of x [rows, k] (row pitch ldx elements; f16, bf16 or f32), k a multiple of 32.
+ *   LYRAQ_NVFP4: a = max|x| of 16 values; s = e4m3(a / (6 g)), nearest, ties to even, at most 448; codes = e2m1(x / (s g)), nearest, ties to
+ *   even, saturating; 0 where s = 0.  g = tensor_scale[0], a positive power of two (NULL: 1).  Another g works too, but a quotient within
+ *   2^-23 of a tie may then go either way.
+ *   LYRAQ_MXFP4: s = 2^(floor(log2 a) - 2), at least 2^-127; codes = e2m1(x / s), saturating.  tensor_scale is not read.
+ * A block that holds a NaN or an infinity gets the scale NaN and zero codes: all of it stands for NaN.
+ * q: [rows, k / 2] bytes.  q_scale: lyraq_fp4_scale_bytes(rows, k, format) bytes, the block scales in the order the tensor cores take
+ * them: atoms of 512 bytes for 128 rows x 4 blocks, byte (row % 32) * 16 + (row % 128) / 32 * 4 + block % 4, an atom for every 4 blocks
+ * along k and then the next 128 rows.  Scales of absent blocks of a row are written as 0, those of absent rows are left as they were.
+ * x, q and q_scale 16-byte aligned, ldx a multiple of 16 bytes.  It has no counterpart in the reference, whose 4-bit
+ * format is lyraq_quant_int4_g64's. */
+LYRAQ_API int lyraq_quant_fp4(uint8_t* q, uint8_t* q_scale, const void* x, int x_dtype, size_t ldx, const float* tensor_scale, int format,
+                              size_t rows, size_t k, void* stream);
+
+/* Size of the block scales of lyraq_quant_fp4 for [rows, k] (0 for an unknown format; no counterpart in the reference). */
+LYRAQ_API size_t lyraq_fp4_scale_bytes(size_t rows, size_t k, int format);
+
+/* FP4 weight quantize in one call, on `stream` without a host step.  LYRAQ_NVFP4: tensor_scale[0] = the least power of two g with
+ * max|w| <= 6 * 448 * g over the finite weights (0 for a weight of zeros), then lyraq_quant_fp4 with it; LYRAQ_MXFP4: lyraq_quant_fp4,
+ * tensor_scale may be NULL.  w [n, k] contiguous.  What lyraq_weight_quant_fp8 is for e4m3; no counterpart in the reference. */
+LYRAQ_API int lyraq_weight_quant_fp4(uint8_t* qw, uint8_t* w_scale, float* tensor_scale, const void* w, int w_dtype, int format, size_t n,
+                                     size_t k, void* stream);
+
 /* ------------------------------------------------------------------ fused producers */
 
 /* AdaLN-Zero modulation y = LN(x)*(1+scale_b)+shift_b (eps, no affine), x [B,S,D], scale/shift [B,D].
@@ -217,7 +251,9 @@ enum {
     LYRAQ_OP_LINEAR_INT8 = 3,
     LYRAQ_OP_LINEAR_FP8 = 4,
     LYRAQ_OP_LINEAR_W4A4 = 5,
-    LYRAQ_OP_LINEAR_W4A4_LORA = 6
+    LYRAQ_OP_LINEAR_W4A4_LORA = 6,
+    LYRAQ_OP_GEMM_FP4 = 7,
+    LYRAQ_OP_LINEAR_FP4 = 8
 };
 
 /* Bytes of workspace an operation can use for (m, n, k).  0 for the INT8 and FP8 GEMMs (no split-K; the call is kept so that
@@ -312,6 +348,14 @@ LYRAQ_API int lyraq_gemm_w4a4(const uint8_t* A, const uint8_t* B, const float* s
                     const void* bias, const void* residual, int epilogue, int m, int n, int k,
                     void* workspace, size_t workspace_bytes, void* stream);
 
+/* Microscaled FP4: Y[m,n] = T( epi( g_x g_w * sum_k X[m,k] W[n,k] + beta * R[m,n] + bias[n] ) ), X and W codes with block scales as
+ * lyraq_quant_fp4 lays them out, both of the same `format`, g_x and g_w fp32 [1] or NULL (= 1), exact products, fp32 accumulation, epi =
+ * identity or tanh-GELU, T = c_dtype (F16, BF16, F32), bias and R of c_dtype or NULL; Y may alias R.  k a multiple of 32; all pointers
+ * 16-byte aligned.  The FP4 form of lyraq_gemm_fp8; no counterpart in the reference. */
+LYRAQ_API int lyraq_gemm_fp4(const uint8_t* X, const uint8_t* x_scale, const float* x_tensor_scale, const uint8_t* W, const uint8_t* w_scale,
+                             const float* w_tensor_scale, int format, void* Y, int c_dtype, const void* bias, const void* residual,
+                             float beta, int epilogue, int m, int n, int k, void* stream);
+
 /* ------------------------------------------------------------------ between the linears of a FLUX block
  * (the callers either side of the quantized-linear path) */
 
@@ -380,6 +424,13 @@ LYRAQ_API int lyraq_load_lora(void* weight, const void* lora, int dtype, float a
 LYRAQ_API int lyraq_linear_fp8_forward(void* Y, const void* x, int dtype, const float* x_scale, const uint8_t* W,
                                        const float* w_scale, const void* bias, const void* residual, float beta, int epilogue,
                                        int m, int n, int k, void* workspace, size_t workspace_bytes, void* stream);
+
+/* FP4 linear: x [m, k] (row pitch ldx elements) -> FP4 with the tensor scale x_tensor_scale[0], then lyraq_gemm_fp4.  The workspace of
+ * LYRAQ_OP_LINEAR_FP4 suffices for either format.  The FP4 form of lyraq_linear_fp8_forward; no counterpart in the reference. */
+LYRAQ_API int lyraq_linear_fp4_forward(void* Y, const void* x, int dtype, size_t ldx, const float* x_tensor_scale, const uint8_t* W,
+                                       const uint8_t* w_scale, const float* w_tensor_scale, int format, const void* bias,
+                                       const void* residual, float beta, int epilogue, int m, int n, int k, void* workspace,
+                                       size_t workspace_bytes, void* stream);
 
 /* INT8 SmoothQuant linear: x -> int8 (scale_mode as in lyraq_quant_int8; PER_TOKEN_DYNAMIC keeps the computed scales in
  * the workspace), then lyraq_gemm_int8 with bias.  Replaces the invokeSqInputQuant + runGemmInt8 pair of the SDXL INT8

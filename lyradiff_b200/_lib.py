@@ -23,6 +23,7 @@ SIGNATURES = {
     "lyraq_debug_attention_wait_test": (c_int, [c_int, ctypes.c_uint]),
     "lyraq_debug_skinny_wait_test": (c_int, [c_int, ctypes.c_uint]),
     "lyraq_debug_force_w4a4_wide": (c_int, [c_int]),
+    "lyraq_debug_force_fp4_tile": (c_int, [c_int]),
     "lyraq_last_cuda_error": (ctypes.c_char_p, []),
     "lyraq_debug_set_row_vectors_per_thread": (c_int, [c_int]),
     "lyraq_debug_set_special_row_kernels": (c_int, [c_int]),
@@ -34,6 +35,9 @@ SIGNATURES = {
                                      c_size_t, c_void_p]),
     "lyraq_weight_quant_int8": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_size_t, c_void_p]),
     "lyraq_weight_quant_int4_g64": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int, c_size_t, c_size_t, c_void_p]),
+    "lyraq_quant_fp4": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_size_t, c_void_p, c_int, c_size_t, c_size_t, c_void_p]),
+    "lyraq_fp4_scale_bytes": (c_size_t, [c_size_t, c_size_t, c_int]),
+    "lyraq_weight_quant_fp4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_size_t, c_size_t, c_void_p]),
     "lyraq_adaln_quant": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
                                   c_void_p, c_size_t, c_size_t, c_size_t, c_double, c_void_p]),
     "lyraq_adaln_quant_fp8x2": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
@@ -67,6 +71,10 @@ SIGNATURES = {
     "lyraq_gate_residual": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_size_t, c_size_t, c_size_t, c_void_p]),
     "lyraq_gemm_w4a4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p,
                                 c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "lyraq_gemm_fp4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p,
+                               c_float, c_int, c_int, c_int, c_int, c_void_p]),
+    "lyraq_linear_fp4_forward": (c_int, [c_void_p, c_void_p, c_int, c_size_t, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
+                                         c_void_p, c_float, c_int, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "lyraq_linear_fp8_forward": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float,
                                          c_int, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "lyraq_linear_int8_forward": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,

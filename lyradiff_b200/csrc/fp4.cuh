@@ -1,0 +1,147 @@
+// Microscaled FP4: the two formats, the layout of their block scales, and the quantize of one block.
+//
+// A row of k values is stored as k / 2 bytes of e2m1 codes (the even element in the low nibble) and one scale byte per block:
+//   nvfp4  blocks of 16, scale e4m3 (never negative), and a tensor scale g, a power of two, beside both:  value = code * s * g
+//   mxfp4  blocks of 32, scale e8m0, a power of two:                                                      value = code * s
+// Block scales lie in atoms of 512 bytes, 128 rows x 4 consecutive blocks, in the order in which tcgen05.cp spreads them over tensor
+// memory: byte (row % 32) * 16 + (row % 128) / 32 * 4 + block % 4; the atoms of 128 rows follow each other along k, then the next 128 rows.
+// Blocks of a row beyond k (k is a multiple of 32, an atom spans 64 or 128 values) have scale 0; rows beyond the last are never read
+// into a result and stay as they were.
+#pragma once
+
+#include "common.cuh"
+
+namespace lyraq {
+
+__host__ __device__ constexpr int fp4_group(int format) { return format == LYRAQ_NVFP4 ? 16 : 32; }
+// atoms along k, and the values of a row one atom scales
+__host__ __device__ constexpr int    fp4_atom_k(int format) { return 4 * fp4_group(format); }
+__host__ __device__ constexpr size_t fp4_atoms(size_t k, int format) { return (k + (size_t)fp4_atom_k(format) - 1) / (size_t)fp4_atom_k(format); }
+
+__host__ __device__ inline size_t fp4_scale_offset(size_t row, size_t atoms, size_t atom)
+{
+    return ((row >> 7) * atoms + atom) * 512 + (row & 31) * 16 + ((row & 127) >> 5) * 4;
+}
+
+// Eight floats -> eight e2m1 codes (nearest, ties to the even code, saturating at 6), element j at bits 4 j.
+__device__ __forceinline__ uint32_t f32x8_to_e2m1x8(const float* v)
+{
+    uint32_t r;
+    asm("{\n\t"
+        ".reg .b8 b0, b1, b2, b3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+        "mov.b32 %0, {b0, b1, b2, b3};\n\t"
+        "}\n"
+        : "=r"(r)
+        : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+    return r;
+}
+
+// Scale of one block from the largest magnitude in it: the stored byte and what the block's values are divided by.
+struct Fp4Block {
+    uint32_t code;
+    float    t;      // 0: every code is 0
+    float    r;      // 1 / t, rounded once
+    bool     exact;  // the division of this block may go through r
+};
+
+// amax_bits: the largest |x| of the block as fp32 bits, taken as an integer maximum, so that a NaN beats an infinity and both beat every
+// number.  A block that holds either gets the scale NaN and zero codes: all of it reads back as NaN.
+//   nvfp4: s = e4m3(amax / (6 g)), t = s g;  mxfp4: s = t = 2^(floor(log2 amax) - 2), at least 2^-127
+// With g a power of two t has four significant bits, s and every code are the nearest to the exact quotient, ties to even: a quotient
+// that is not a tie differs from one by more than half an ulp (numerator and tie times t both lie on the numerator's grid).
+template<int FORMAT> __device__ __forceinline__ Fp4Block fp4_block(uint32_t amax_bits, float g)
+{
+    Fp4Block b;
+    if (amax_bits >= 0x7f800000u) {
+        b.code  = FORMAT == LYRAQ_NVFP4 ? 0x7fu : 0xffu;
+        b.t     = 0.0f;
+        b.r     = 0.0f;
+        b.exact = true;
+        return b;
+    }
+    const float amax = __uint_as_float(amax_bits);
+    if (FORMAT == LYRAQ_NVFP4) {
+        const float ratio = amax_bits == 0u ? 0.0f : amax / (6.0f * g);
+        b.code            = f32x2_to_e4m3x2(ratio, 0.0f) & 0xffu;
+        // e4m3 -> fp32: the code's seven bits under fp16's exponent read 2^-8 times its value, subnormals included
+        b.t     = __half2float(__ushort_as_half((unsigned short)(b.code << 7))) * 256.0f * g;
+        b.r     = b.t > 0.0f ? 1.0f / b.t : 0.0f;
+        b.exact = b.t == 0.0f || (b.t >= 7.9e-31f && b.t <= 1.2e30f && amax <= b.t * 1048576.0f);
+    } else {
+        const uint32_t e = amax_bits >> 23;                                  // biased; 0 for subnormals
+        b.code           = e > 2u ? e - 2u : 0u;
+        b.t              = b.code != 0u ? __uint_as_float(b.code << 23) : __uint_as_float(0x00400000u);
+        // 2^-(code - 127) is a number for every code (2^127 down to 2^-125), so the product with it is the quotient itself
+        b.r     = __uint_as_float((254u - b.code) << 23);
+        b.exact = true;
+    }
+    return b;
+}
+
+// The codes of eight values of a block.  nvfp4: q = fl(x / t) without a division: q0 = x r, then one correction by the exact remainder
+// x - q0 t, which gives the correctly rounded quotient (Markstein) where nothing over- or underflows on the way; blocks outside that range
+// divide.  A quotient that over- or underflows saturates or rounds to zero like any other.
+template<int FORMAT> __device__ __forceinline__ uint32_t fp4_encode8(const float* x, const Fp4Block& b)
+{
+    float q[8];
+    if (b.t == 0.0f) {
+        return 0u;
+    }
+    if (FORMAT != LYRAQ_NVFP4) {
+        const float2 r2 = make_float2(b.r, b.r);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 p = mul_f32x2(make_float2(x[2 * j], x[2 * j + 1]), r2);
+            q[2 * j]       = p.x;
+            q[2 * j + 1]   = p.y;
+        }
+    } else if (b.exact) {
+        const float2 r2 = make_float2(b.r, b.r);
+        const float2 m2 = make_float2(-b.t, -b.t);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 v   = make_float2(x[2 * j], x[2 * j + 1]);
+            const float2 q0  = mul_f32x2(v, r2);
+            const float2 rem = fma_f32x2(q0, m2, v);
+            const float2 q1  = fma_f32x2(rem, r2, q0);
+            q[2 * j]         = q1.x;
+            q[2 * j + 1]     = q1.y;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            q[j] = x[j] / b.t;
+        }
+    }
+    return f32x8_to_e2m1x8(q);
+}
+
+// Largest magnitude of a 16-byte vector of T, as fp32 bits (see fp4_block).
+template<typename T> __device__ __forceinline__ uint32_t amax_bits_of(const Vec16& v);
+template<> __device__ __forceinline__ uint32_t amax_bits_of<float>(const Vec16& v)
+{
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        m = max(m, v.w[i] & 0x7fffffffu);
+    }
+    return m;
+}
+__device__ __forceinline__ uint32_t amax16_of(const Vec16& v)
+{
+    uint32_t m = __vmaxu2(__vmaxu2(v.w[0] & 0x7fff7fffu, v.w[1] & 0x7fff7fffu), __vmaxu2(v.w[2] & 0x7fff7fffu, v.w[3] & 0x7fff7fffu));
+    return max(m & 0xffffu, m >> 16);
+}
+template<> __device__ __forceinline__ uint32_t amax_bits_of<__nv_bfloat16>(const Vec16& v) { return amax16_of(v) << 16; }
+template<> __device__ __forceinline__ uint32_t amax_bits_of<__half>(const Vec16& v)
+{
+    const uint32_t m = amax16_of(v);
+    // half -> float keeps order, infinities and NaN
+    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m))) & 0x7fffffffu;
+}
+
+}  // namespace lyraq

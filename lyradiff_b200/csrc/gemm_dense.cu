@@ -1089,7 +1089,7 @@ int make_tmap_bytes_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64
 
 // Tensor map of a row-major [rows, cols] matrix of 1- or 2-byte elements for TMA stores of 32 x 32 boxes whose
 // shared-memory image uses the swizzle that matches the box's row size (32 or 64 bytes).
-int make_tmap_store(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, int elem_bytes, bool wide = false)
+int make_tmap_store(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, int elem_bytes, bool wide)
 {
     const TmapKey key{base, cols, rows, ld * (uint64_t)elem_bytes, wide ? 64u : 32u, 32, 16 + elem_bytes + (wide ? 8 : 0)};
     if (tmap_cache().find(key, map)) {
@@ -1110,6 +1110,33 @@ int make_tmap_store(CUtensorMap* map, const void* base, uint64_t rows, uint64_t 
                             CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
         record_cuda_error(cudaErrorInvalidValue, "cuTensorMapEncodeTiled refused the output tensor map");
+        return LYRAQ_ERR_CUDA;
+    }
+    tmap_cache().put(key, *map);
+    return LYRAQ_OK;
+}
+
+// Tensor map of FP4 block scales (fp4.cuh): [row blocks][atoms][512 bytes], boxes of box_blocks x box_atoms whole atoms; atoms that do not
+// exist read as zero.
+int make_tmap_atoms(CUtensorMap* map, const void* base, uint64_t row_blocks, uint64_t atoms, uint32_t box_blocks, uint32_t box_atoms)
+{
+    const TmapKey key{base, atoms, row_blocks, 512, box_atoms, box_blocks, 64};
+    if (tmap_cache().find(key, map)) {
+        return LYRAQ_OK;
+    }
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (fn == nullptr) {
+        return LYRAQ_ERR_CUDA;
+    }
+    const cuuint64_t dims[3]    = {128, atoms, row_blocks};
+    const cuuint64_t strides[2] = {512, atoms * 512};
+    const cuuint32_t box[3]     = {128, box_atoms, box_blocks};
+    const cuuint32_t estr[3]    = {1, 1, 1};
+    const CUresult   r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(base), dims, strides, box, estr,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        record_cuda_error(cudaErrorInvalidValue, "cuTensorMapEncodeTiled refused the scale tensor map");
         return LYRAQ_ERR_CUDA;
     }
     tmap_cache().put(key, *map);
@@ -1187,7 +1214,7 @@ static int launch_gemm(const void* A, const void* B, GemmParams p, int sms, cuda
     p.epi.tma_store = 0;
     if (p.epi.out_q_scale != nullptr) {
         if ((p.N & 15) == 0 && (p.epi.ldc & 15) == 0) {
-            st = make_tmap_store(&tc, p.epi.C, (uint64_t)p.M, (uint64_t)p.N, (uint64_t)p.epi.ldc, 1);
+            st = make_tmap_store(&tc, p.epi.C, (uint64_t)p.M, (uint64_t)p.N, (uint64_t)p.epi.ldc, 1, false);
             if (st != LYRAQ_OK) {
                 return st;
             }

@@ -2,6 +2,7 @@
 // the quantized activation (and its scales) held in caller-provided workspace.  These are what the reference's layers
 // do around every quantized linear with buffers from their allocator; here the caller owns the buffer.
 #include "common.cuh"
+#include "fp4.cuh"
 #include "gemm_w4a4.cuh"
 
 namespace lyraq {
@@ -15,6 +16,7 @@ static inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; 
 //   LINEAR_INT8 : int8 activation [m, k] | fp32 per-token scales [m]
 //   LINEAR_W4A4 : packed int4 activation [m, k/2] | fp32 group scales [m, k/64]
 //   LINEAR_W4A4_LORA : the same, then the fp32 low-rank activation [m, 32]
+//   LINEAR_FP4  : e2m1 activation [m, k/2] | block scales (nvfp4's, the larger)
 // The W4A4 forwards hand what a larger workspace has left to the GEMM, for its wide form (gemm_w4a4_wide.cu): w4a4_wide_bytes.
 size_t linear_workspace_bytes(int op, size_t m, size_t k)
 {
@@ -24,6 +26,7 @@ size_t linear_workspace_bytes(int op, size_t m, size_t k)
         case LYRAQ_OP_LINEAR_W4A4: return align_up(m * k / 2, 256) + align_up(4 * m * (k / 64), 256);
         case LYRAQ_OP_LINEAR_W4A4_LORA:
             return align_up(m * k / 2, 256) + align_up(4 * m * (k / 64), 256) + align_up(4 * m * 32, 256);
+        case LYRAQ_OP_LINEAR_FP4: return align_up(m * k / 2, 256) + lyraq_fp4_scale_bytes(m, k, LYRAQ_NVFP4);
         default: return 0;
     }
 }
@@ -77,6 +80,37 @@ int lyraq_linear_fp8_forward(void* Y, const void* x, int dtype, const float* x_s
         return st;
     }
     return lyraq_gemm_fp8(qx, x_scale, W, w_scale, Y, dtype, bias, residual, 1.0f, beta, epilogue, m, n, k, nullptr, 0, stream);
+}
+
+int lyraq_linear_fp4_forward(void* Y, const void* x, int dtype, size_t ldx, const float* x_tensor_scale, const uint8_t* W,
+                             const uint8_t* w_scale, const float* w_tensor_scale, int format, const void* bias, const void* residual,
+                             float beta, int epilogue, int m, int n, int k, void* workspace, size_t workspace_bytes, void* stream)
+{
+    if (m < 0 || n < 0 || k < 0 || (format != LYRAQ_NVFP4 && format != LYRAQ_MXFP4)) {
+        return LYRAQ_ERR_INVALID_ARG;
+    }
+    if (m == 0 || n == 0) {
+        return LYRAQ_OK;
+    }
+    if (k == 0 || (k & 31) != 0) {
+        return LYRAQ_ERR_UNSUPPORTED;
+    }
+    if (workspace == nullptr || workspace_bytes < linear_workspace_bytes(LYRAQ_OP_LINEAR_FP4, (size_t)m, (size_t)k) || !aligned16(workspace)) {
+        return LYRAQ_ERR_WORKSPACE;
+    }
+    // whatever the product would refuse is refused before the quantize runs
+    if (Y == nullptr || W == nullptr || w_scale == nullptr || !aligned16(Y) || !aligned16(W) || !aligned16(w_scale) ||
+        (bias != nullptr && !aligned16(bias)) || (residual != nullptr && !aligned16(residual)) ||
+        (epilogue != LYRAQ_EPI_NONE && epilogue != LYRAQ_EPI_GELU_TANH)) {
+        return LYRAQ_ERR_INVALID_ARG;
+    }
+    uint8_t* qx = static_cast<uint8_t*>(workspace);
+    uint8_t* sx = qx + align_up((size_t)m * (size_t)k / 2, 256);
+    int      st = lyraq_quant_fp4(qx, sx, x, dtype, ldx, x_tensor_scale, format, (size_t)m, (size_t)k, stream);
+    if (st != LYRAQ_OK) {
+        return st;
+    }
+    return lyraq_gemm_fp4(qx, sx, x_tensor_scale, W, w_scale, w_tensor_scale, format, Y, dtype, bias, residual, beta, epilogue, m, n, k, stream);
 }
 
 int lyraq_linear_int8_forward(void* Y, const void* x, int dtype, const float* pre_quant_scale, const float* input_scale,

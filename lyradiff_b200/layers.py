@@ -10,7 +10,7 @@ import torch
 
 from . import _lib, ops
 
-OP_LINEAR_INT8, OP_LINEAR_FP8, OP_LINEAR_W4A4, OP_LINEAR_W4A4_LORA = 3, 4, 5, 6
+OP_LINEAR_INT8, OP_LINEAR_FP8, OP_LINEAR_W4A4, OP_LINEAR_W4A4_LORA, OP_LINEAR_FP4 = 3, 4, 5, 6, 8
 
 
 def _workspace(op, m, n, k, device, current):
@@ -47,6 +47,69 @@ class Fp8Linear:
             self.k, ops._p(self._ws), self._ws.numel(), ops._stream())
         _lib.check(st, "lyraq_linear_fp8_forward")
         return y.reshape(*x.shape[:-1], self.n)
+
+
+class Fp4Linear:
+    """Linear in microscaled FP4 (nvfp4 or mxfp4) on the tensor cores' 4-bit path: weight quantized on load, activations by the forward,
+    bias / GELU-tanh / residual fused into the GEMM epilogue.  input_scale (nvfp4): the static tensor scale of the activations, the largest
+    magnitude they should keep over 6 * 448; it is rounded up to a power of two, with which the quantizer is exact (None: 1).  The
+    quantized activation lives in memory taken from torch's allocator per call, so calls on several streams and captured graphs do not
+    share it.  The reference has no FP4 linear; this is Fp8Linear's counterpart."""
+
+    def __init__(self, weight, bias=None, input_scale=None, gelu=False, fmt="nvfp4"):
+        n, k = weight.shape
+        dev = weight.device
+        self.n, self.k, self.gelu, self.fmt = n, k, gelu, fmt
+        self.weight = ops.weight_quant_fp4(weight.contiguous(), fmt)
+        self.bias = None if bias is None else bias.contiguous()
+        if input_scale is None or fmt != "nvfp4":
+            self.input_scale = None
+        else:
+            s = input_scale.detach().reshape(1).double()
+            m, e = torch.frexp(s)
+            if not bool((torch.isfinite(s) & (s > 0)).all()):
+                raise ValueError("input_scale must be positive and finite")
+            self.input_scale = torch.ldexp(torch.ones_like(s), torch.where(m == 0.5, e - 1, e)).to(device=dev, dtype=torch.float32)
+
+    def _out(self, shape, dtype, device, out):
+        m = 1
+        for d in shape:
+            m *= d
+        if out is None:
+            return m, torch.empty(m, self.n, dtype=dtype, device=device)
+        if out.dtype != dtype or out.numel() != m * self.n or out.shape[-1] != self.n:
+            raise ValueError("out must be [..., %d] of x's dtype" % self.n)
+        return m, out.view(m, self.n)
+
+    def forward(self, x, residual=None, beta=1.0, out=None):
+        lead = x.shape[:-1]
+        if x.shape[-1] != self.k:
+            raise ValueError("expected [..., %d], got %s" % (self.k, tuple(x.shape)))
+        m, y = self._out(lead, x.dtype, x.device, out)
+        x2 = x.reshape(m, self.k)
+        ldx = ops._rows_of(x2)
+        ops._check_epilogue(y, self.bias, residual, m, self.n)
+        ops._same_device(x, y, residual, self.weight.codes)
+        need = _lib.lib().lyraq_workspace_bytes(OP_LINEAR_FP4, m, self.n, self.k)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        w = self.weight
+        st = _lib.lib().lyraq_linear_fp4_forward(
+            ops._p(y), x2.data_ptr(), ops._dt(x2), ldx, ops._p(self.input_scale), ops._p(w.codes), ops._p(w.scales), ops._p(w.tensor_scale),
+            ops.FP4_FORMATS[self.fmt], ops._p(self.bias), ops._p(residual), float(beta), ops.EPI_GELU_TANH if self.gelu else ops.EPI_NONE,
+            m, self.n, self.k, ops._p(ws), need, ops._stream())
+        _lib.check(st, "lyraq_linear_fp4_forward")
+        return y.reshape(*lead, self.n)
+
+    def empty_input(self, rows):
+        """An Fp4Tensor for `rows` rows of this layer's input, for producers that write FP4 themselves (ops.gated_residual_norm)."""
+        return ops.Fp4Tensor.empty(rows, self.k, self.fmt, self.input_scale, self.weight.codes.device)
+
+    def forward_quantized(self, x, dtype, residual=None, beta=1.0, out=None):
+        """The product alone, for an input that is FP4 already (empty_input): [rows, n] of `dtype`."""
+        if x.tensor_scale is not self.input_scale:
+            raise ValueError("the input was not quantized for this layer (empty_input)")
+        y = self._out((x.rows,), dtype, x.codes.device, out)[1]
+        return ops.gemm_fp4(self.weight, x, y, self.bias, residual, beta, self.gelu)
 
 
 class SmoothQuantLinear:

@@ -14,6 +14,7 @@ F16, BF16, F32, S32, E4M3 = 0, 1, 2, 3, 4
 SCALE_PER_TENSOR, SCALE_PER_TOKEN, SCALE_PER_TOKEN_DYNAMIC = 0, 1, 2
 EPI_NONE, EPI_GELU_TANH, EPI_ROUND_EACH = 0, 1, 2
 OP_GEMM_W4A4 = 2
+FP4_FORMATS = {"nvfp4": 0, "mxfp4": 1}
 
 _DTYPES = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32, torch.int32: S32}
 
@@ -117,6 +118,86 @@ def weight_quant_int4_g64(qw, w_scale, w):
     return qw, w_scale
 
 
+def _same_device(*tensors):
+    """The tensors of one call are on the current device, whose stream the call runs on."""
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != here:
+            raise ValueError("tensor on %s, but the current device is cuda:%d" % (t.device, here))
+
+
+def _fp4_format(fmt):
+    try:
+        return FP4_FORMATS[fmt]
+    except KeyError:
+        raise ValueError("unknown FP4 format %r (nvfp4 or mxfp4)" % (fmt,))
+
+
+class Fp4Tensor:
+    """A matrix in microscaled FP4 (lyraq_quant_fp4): codes uint8 [rows, k / 2], the block scales in the tensor cores' order (scales, uint8),
+    the format, and for nvfp4 the tensor scale (fp32 [1], a power of two; None: 1)."""
+
+    __slots__ = ("rows", "k", "fmt", "codes", "scales", "tensor_scale")
+
+    def __init__(self, rows, k, fmt, codes, scales, tensor_scale=None):
+        self.rows, self.k, self.fmt, self.codes, self.scales, self.tensor_scale = rows, k, fmt, codes, scales, tensor_scale
+
+    @classmethod
+    def empty(cls, rows, k, fmt="nvfp4", tensor_scale=None, device="cuda"):
+        n = _lib.lib().lyraq_fp4_scale_bytes(rows, k, _fp4_format(fmt))
+        return cls(rows, k, fmt, torch.empty(rows, k // 2, dtype=torch.uint8, device=device), torch.empty(n, dtype=torch.uint8, device=device),
+                   tensor_scale)
+
+    def check(self):
+        """Refuses parts that do not fit together: a kernel would read past them."""
+        if self.k % 32 or tuple(self.codes.shape) != (self.rows, self.k // 2) or self.codes.dtype != torch.uint8:
+            raise ValueError("FP4 codes must be uint8 [%d, %d / 2], k a multiple of 32" % (self.rows, self.k))
+        if self.scales.dtype != torch.uint8 or self.scales.numel() != _lib.lib().lyraq_fp4_scale_bytes(self.rows, self.k, _fp4_format(self.fmt)):
+            raise ValueError("FP4 block scales do not fit [%d, %d] in %s" % (self.rows, self.k, self.fmt))
+        _fp4_tensor_scale(self.tensor_scale)
+        return self
+
+
+def _fp4_tensor_scale(t):
+    if t is not None and (t.dtype != torch.float32 or t.numel() != 1):
+        raise ValueError("an FP4 tensor scale is one fp32 number")
+
+
+def _rows_of(x):
+    """x [rows, k] with contiguous rows -> its row pitch in elements."""
+    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+        raise ValueError("expected a matrix with contiguous rows that do not overlap")
+    if not x.is_cuda:
+        raise ValueError("expected a CUDA tensor")
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def quant_fp4(x, tensor_scale=None, fmt="nvfp4", out=None):
+    """Microscaled FP4 quantize (lyraq_quant_fp4) of x [rows, k], whose rows may lie further apart than k.  Returns an Fp4Tensor; `out`
+    reuses one (its tensor scale is the one that counts then)."""
+    ldx = _rows_of(x)
+    if out is None:
+        out = Fp4Tensor.empty(x.shape[0], x.shape[1], fmt, tensor_scale, x.device)
+    elif tensor_scale is not None or (out.rows, out.k) != tuple(x.shape):
+        raise ValueError("out must have x's shape and carries its own tensor scale")
+    out.check()
+    _same_device(x, out.codes, out.scales, out.tensor_scale)
+    st = _lib.lib().lyraq_quant_fp4(_p(out.codes), _p(out.scales), x.data_ptr(), _dt(x), ldx, _p(out.tensor_scale), _fp4_format(out.fmt),
+                                    out.rows, out.k, _stream())
+    _lib.check(st, "lyraq_quant_fp4")
+    return out
+
+
+def weight_quant_fp4(w, fmt="nvfp4"):
+    """FP4 weight quantize (lyraq_weight_quant_fp4): w [n, k] -> Fp4Tensor, with the weight's own tensor scale for nvfp4."""
+    n, k = w.shape
+    out = Fp4Tensor.empty(n, k, fmt, torch.empty(1, dtype=torch.float32, device=w.device) if fmt == "nvfp4" else None, w.device).check()
+    _same_device(w)
+    st = _lib.lib().lyraq_weight_quant_fp4(_p(out.codes), _p(out.scales), _p(out.tensor_scale), _p(w), _dt(w), _fp4_format(fmt), n, k, _stream())
+    _lib.check(st, "lyraq_weight_quant_fp4")
+    return out
+
+
 # ----------------------------------------------------------------------------- fused producers
 def invoke_layer_norm_with_shift_and_scale(dst, src, scale, shift, eps=1e-6, q8=None, q8_scale=None, qf8=None,
                                            f8_scale=None, pre_quant_scale=None):
@@ -201,6 +282,30 @@ def gemm_with_residual_and_bias_fp8(W, w_scale, X, x_scale, Y, bias=None, residu
                                    _stream())
     _lib.check(st, "lyraq_gemm_fp8")
     return Y
+
+
+def gemm_fp4(W, X, Y, bias=None, residual=None, beta=1.0, is_gelu=False):
+    """Microscaled FP4 GEMM (lyraq_gemm_fp4), weight first as in gemm_with_residual_and_bias_fp8: Y[m,n] = epi(X W^T + beta * R + bias) for
+    two Fp4Tensors of one format."""
+    m, n = X.rows, W.rows
+    if X.fmt != W.fmt or X.k != W.k or tuple(Y.shape) != (m, n):
+        raise ValueError("shape or format mismatch")
+    X.check()
+    W.check()
+    _check_epilogue(Y, bias, residual, m, n)
+    _same_device(Y, bias, residual, X.codes, X.scales, X.tensor_scale, W.codes, W.scales, W.tensor_scale)
+    st = _lib.lib().lyraq_gemm_fp4(_p(X.codes), _p(X.scales), _p(X.tensor_scale), _p(W.codes), _p(W.scales), _p(W.tensor_scale),
+                                   _fp4_format(X.fmt), _p(Y), _dt(Y), _p(bias), _p(residual), float(beta),
+                                   EPI_GELU_TANH if is_gelu else EPI_NONE, m, n, X.k, _stream())
+    _lib.check(st, "lyraq_gemm_fp4")
+    return Y
+
+
+def _check_epilogue(Y, bias, residual, m, n):
+    if bias is not None and (bias.dtype != Y.dtype or tuple(bias.shape) != (n,)):
+        raise ValueError("bias must be [%d] of Y's dtype" % n)
+    if residual is not None and (residual.dtype != Y.dtype or residual.numel() != m * n or residual.shape[-1] != n):
+        raise ValueError("residual must have the shape and dtype of Y")
 
 
 def gemm_fp8_qk_rope(W, w_scale, X, x_scale, Y, qk_scale, rope_emb, heads, head_dim, bias=None, eps=1e-6):

@@ -1,0 +1,219 @@
+"""GPU tests of the microscaled FP4 operators against the 64-bit restatement in oracle/fp4.py."""
+
+import pytest
+import torch
+
+from oracle import fp4
+from tests.util import check_status, cu
+
+pytestmark = pytest.mark.gpu
+
+FORMATS = ["nvfp4", "mxfp4"]
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from lyradiff_b200 import ops as _ops
+    return _ops
+
+
+@pytest.fixture
+def tile():
+    from lyradiff_b200 import _lib
+    yield lambda code: _lib.check(_lib.lib().lyraq_debug_force_fp4_tile(code), "lyraq_debug_force_fp4_tile")
+    _lib.lib().lyraq_debug_force_fp4_tile(0)
+
+
+def assert_quantized(t, x, fmt, g=1.0):
+    """Codes (as values: the sign of a zero does not matter) and scale bytes are exactly those of the definition, and blocks that a
+    row does not have carry scale 0."""
+    codes, s = fp4.encode(x, fmt, g)
+    rows, k = x.shape
+    got = fp4.unpack(t.codes.cpu())
+    blocks = k // fp4.GROUP[fmt]
+    sb = t.scales.cpu()
+    assert torch.equal(sb[fp4.scale_offsets(rows, blocks)], s)
+    pad = (blocks + 3) // 4 * 4
+    assert not bool(sb[fp4.scale_offsets(rows, pad)][:, blocks:].any())
+    sign = lambda c: torch.where(c == 8, 0, c)   # noqa: E731
+    assert torch.equal(sign(got), sign(codes))
+
+
+def inputs(rows, k, dtype, seed, spread=3.0):
+    """Values over several binades, so that blocks differ in scale, with exact ties, zeros and a block of zeros among them."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, k, generator=g) * torch.exp2(spread * torch.randn(rows, k // 32, generator=g)).repeat_interleave(32, dim=1)
+    ties = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0]) * torch.tensor([1.0, -1.0] * 4)
+    x[::3, :8], x[1::4, 8:16] = ties, ties * 1.125 / 4
+    x[::5, :32] = 0
+    x[:, -1] = -x[:, -1]
+    return x.clamp(-60000, 60000).to(dtype)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,k", [(1, 32), (3, 96), (31, 160), (33, 64), (128, 256), (130, 1056), (300, 640)])
+def test_quantize_is_exact(ops, fmt, dtype, rows, k):
+    x = inputs(rows, k, dtype, rows + k)
+    for g in ((1.0, 2.0 ** -5) if fmt == "nvfp4" else (None,)):
+        t = ops.quant_fp4(cu(x), None if g is None else torch.tensor([g], device="cuda"), fmt)
+        check_status()
+        assert_quantized(t, x, fmt, g or 1.0)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_quantize_of_the_types_extremes(ops, fmt):
+    """Subnormals, the largest numbers, infinities and NaN, a block scale that underflows, one that saturates."""
+    x = torch.zeros(9, 64)
+    x[0] = 1e-42
+    x[1, 5] = 3.0e38
+    x[1, 40] = -3.0e38
+    x[2, 7], x[2, 50] = float("inf"), float("nan")
+    x[3] = torch.linspace(-1e-3, 1e-3, 64)
+    x[4] = 2.0 ** -126
+    x[5, ::2] = -0.0
+    x[6] = torch.tensor([448.0 * 6 * 4, 1.0] * 32)
+    x[7, 63] = float("-inf")
+    x[8] = torch.linspace(1e-38, 5e-38, 64)
+    t = ops.quant_fp4(cu(x), None, fmt)
+    check_status()
+    assert_quantized(t, x, fmt)
+    h = x.clamp(-3e38, 3e38).nan_to_num(0).bfloat16()
+    assert_quantized(ops.quant_fp4(cu(h), None, fmt), h, fmt)
+
+
+def test_tensor_scales_far_from_one(ops):
+    """The division-free path gives way to divisions where a reciprocal would over- or underflow."""
+    g = torch.Generator().manual_seed(4)
+    base = torch.randn(4, 64, generator=g)
+    for e, ge in ((-100, -108), (110, 104), (-30, 90), (100, -120), (0, -126), (0, 120)):
+        x = base * 2.0 ** e
+        t = ops.quant_fp4(cu(x), torch.tensor([2.0 ** ge], device="cuda"), "nvfp4")
+        assert_quantized(t, x, "nvfp4", 2.0 ** ge)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_quantize_takes_rows_apart_and_leaves_absent_rows_alone(ops, fmt):
+    x = inputs(70, 192, torch.bfloat16, 3)
+    wide = torch.full((70, 448), float("nan"), dtype=torch.bfloat16, device="cuda")
+    wide[:, 128:320] = x.cuda()
+    out = ops.Fp4Tensor.empty(70, 192, fmt)
+    out.scales.fill_(0xAB)
+    ops.quant_fp4(wide[:, 128:320], out=out)
+    check_status()
+    assert_quantized(out, x, fmt)
+    blocks = 192 // fp4.GROUP[fmt]
+    rest = torch.ones(out.scales.numel(), dtype=torch.bool)
+    rest[fp4.scale_offsets(70, (blocks + 3) // 4 * 4).flatten()] = False
+    assert bool((out.scales.cpu()[rest] == 0xAB).all())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_weight_quantize(ops, fmt, dtype):
+    g = torch.Generator().manual_seed(9)
+    w = (torch.randn(200, 352, generator=g) * 0.02).to(dtype)
+    w[3, 7] = float("inf")
+    for scale in (1.0, 0.0):
+        t = ops.weight_quant_fp4(cu(w * scale if scale else torch.zeros_like(w)), fmt)
+        check_status()
+        ref = w if scale else torch.zeros_like(w)
+        gs = fp4.tensor_scale(ref)
+        if fmt == "nvfp4":
+            assert float(t.tensor_scale) == gs
+        assert_quantized(t, ref, fmt, gs or 1.0)
+
+
+# ----------------------------------------------------------------------------- the product
+def problem(m, n, k, fmt, dtype, seed, bias=True, residual=False, g=(0.5, 2.0 ** -7)):
+    gen = torch.Generator().manual_seed(seed)
+    xc, xs = fp4.encode(torch.randn(m, k, generator=gen) * 2, fmt, g[0])
+    wc, ws = fp4.encode(torch.randn(n, k, generator=gen) * 0.05, fmt, g[1])
+    b = torch.randn(n, generator=gen).to(dtype) if bias else None
+    r = torch.randn(m, n, generator=gen).to(dtype) if residual else None
+    return (xc, xs, g[0] if fmt == "nvfp4" else 1.0), (wc, ws, g[1] if fmt == "nvfp4" else 1.0), b, r
+
+
+def to_device(ops, part, fmt, fill=0xAB):
+    codes, s, g = part
+    rows, k = codes.shape
+    blocks = s.shape[1]
+    t = ops.Fp4Tensor.empty(rows, k, fmt, torch.tensor([g], device="cuda") if fmt == "nvfp4" else None)
+    t.codes.copy_(fp4.pack(codes))
+    sb = torch.full((t.scales.numel(),), fill, dtype=torch.uint8)     # scales of absent rows: anything
+    pad = fp4.scale_offsets(rows, (blocks + 3) // 4 * 4)
+    sb[pad.flatten()] = 0
+    sb[pad[:, :blocks].flatten()] = s.flatten()
+    t.scales.copy_(sb)
+    return t
+
+
+def assert_product(got, x, w, fmt, bias=None, residual=None, beta=1.0, gelu=False):
+    """Against 64 bits.  The products of two FP4 values and their scales are exact; the sum of K of them runs through the fp32 accumulator in
+    K / 64 instructions, each of which may lose an ulp of what it adds up (2^-23 of the sum of magnitudes; 2 more for the sum inside it);
+    the epilogue adds at most four fp32 roundings, tanh.approx has a relative error of 2^-10.9 (half of which reaches the result), and the
+    result is rounded to its type: half a step."""
+    xv, wv = fp4.decode(*x[:2], fmt, x[2]), fp4.decode(*w[:2], fmt, w[2])
+    y, mag = xv @ wv.t(), xv.abs() @ wv.abs().t()
+    k = xv.shape[1]
+    if residual is not None:
+        y, mag = y + beta * residual.double(), mag + abs(beta) * residual.double().abs()
+    if bias is not None:
+        y, mag = y + bias.double(), mag + bias.double().abs()
+    tol = ((k + 63) // 64 + 2 + 4) * 2.0 ** -23 * mag
+    if gelu:
+        tol = 1.13 * tol + 0.5 * y.abs() * 2.0 ** -10.9 + 2.0 ** -21 * y.abs()
+        y = fp4.gelu_tanh(y)
+    half = torch.finfo(got.dtype).eps / 2
+    tiny = torch.finfo(got.dtype).tiny * half * 2
+    tol = tol * (1 + half) + half * y.abs() + tiny
+    err = (got.cpu().double() - y).abs()
+    assert bool((err <= tol).all()), "off by %g of the tolerance at %s" % (float((err / tol).max()), (err / tol).argmax())
+
+
+SHAPES = [(1, 8, 32), (5, 24, 64), (128, 128, 256), (130, 200, 288), (257, 129, 512), (300, 520, 1056), (64, 100, 3200)]
+
+
+@pytest.mark.parametrize("code", [1281, 2562])
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_product_of_every_tile(ops, tile, code, fmt, m, n, k):
+    tile(code)
+    x, w, b, _ = problem(m, n, k, fmt, torch.bfloat16, m + n + k)
+    y = torch.full((m, n), float("nan"), dtype=torch.bfloat16, device="cuda")
+    ops.gemm_fp4(to_device(ops, w, fmt), to_device(ops, x, fmt), y, cu(b))
+    check_status()
+    assert_product(y, x, w, fmt, b)
+
+
+@pytest.mark.parametrize("code", [0, 1281, 2562])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("gelu,bias,residual", [(True, True, False), (False, False, True), (True, True, True)])
+@pytest.mark.parametrize("m,n", [(3, 72), (140, 300), (260, 131)])
+def test_epilogues_and_types(ops, tile, code, dtype, gelu, bias, residual, m, n):
+    tile(code)
+    x, w, b, r = problem(m, n, 320, "nvfp4", dtype, 5, bias, residual)
+    y = torch.full((m, n), float("nan"), dtype=dtype, device="cuda")
+    ops.gemm_fp4(to_device(ops, w, "nvfp4"), to_device(ops, x, "nvfp4"), y, cu(b), cu(r), 0.75, gelu)
+    check_status()
+    assert_product(y, x, w, "nvfp4", b, r, 0.75, gelu)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_scales_of_every_row_and_block_reach_their_values(ops, tile, fmt):
+    """One value in each (row, block), all scales different: a scale taken from another row or block shows."""
+    for code, m, n, k in ((1281, 128, 128, 512), (2562, 256, 256, 512), (0, 16, 128, 512)):
+        tile(code)
+        blocks = k // fp4.GROUP[fmt]
+        xc = torch.zeros(m, k, dtype=torch.uint8)
+        wc = torch.zeros(n, k, dtype=torch.uint8)
+        xc[:, ::fp4.GROUP[fmt]] = 2
+        wc[:, ::fp4.GROUP[fmt]] = 2
+        i, j, b = torch.arange(m)[:, None], torch.arange(n)[:, None], torch.arange(blocks)[None]
+        xs = (48 + (i * 7 + b * 3) % 23 + (70 if fmt == "mxfp4" else 0)).to(torch.uint8)
+        ws = (48 + (j * 5 + b * 11) % 19 + (70 if fmt == "mxfp4" else 0)).to(torch.uint8)
+        x, w = (xc, xs, 1.0), (wc, ws, 1.0)
+        y = torch.empty(m, n, dtype=torch.float32, device="cuda")
+        ops.gemm_fp4(to_device(ops, w, fmt), to_device(ops, x, fmt), y)
+        check_status()
+        assert_product(y, x, w, fmt)
