@@ -40,7 +40,8 @@ typedef enum {
     LYRAQ_BF16 = 1,
     LYRAQ_F32 = 2,
     LYRAQ_S32 = 3,
-    LYRAQ_E4M3 = 4 /* FP8 e4m3 codes, one byte each (only where an entry point says so) */
+    LYRAQ_E4M3 = 4, /* FP8 e4m3 codes, one byte each (only where an entry point says so) */
+    LYRAQ_S64 = 5   /* only where an entry point says so */
 } lyraq_dtype_t;
 
 /* Microscaled FP4 formats: e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two to a byte, the even element in the low
@@ -111,9 +112,11 @@ LYRAQ_API int lyraq_debug_skinny_wait_test(int stalled_rank, unsigned int wait_l
  * reference, which has one W4A4 kernel (src/lyradiff/kernels/w4a4_gemm/w4a4_gemm.cu). */
 LYRAQ_API int lyraq_debug_force_w4a4_wide(int on);
 
-/* Test / sweep hook: the kernel of lyraq_gemm_fp4.  0 = automatic (default); 2562 = CTA pair, 256 x 256 tile; 1281 = one CTA, 128 x 128.
- * Process-wide, not thread-safe.  It has no counterpart in the reference, which has no FP4 linears. */
+/* Test / sweep hook: the kernel of lyraq_gemm_fp4.  0 = automatic (default); 2562 = CTA pair, 256 x 256 tile; 1281 = one CTA, 128 x 128; 16 = the few-row kernel wherever it can (16 rows), the automatic choice elsewhere.  Process-wide, not thread-safe.  It has no counterpart in the reference, which has no FP4 linears. */
 LYRAQ_API int lyraq_debug_force_fp4_tile(int code);
+
+/* lyraq_debug_skinny_wait_test for the few-row FP4 kernel.  It has no counterpart in the reference. */
+LYRAQ_API int lyraq_debug_fp4_skinny_wait_test(int stalled_rank, unsigned int wait_limit_ms);
 
 /* Test / sweep hook for the row kernels (quantize, LayerNorm, AdaLN, GEGLU): the most 16-byte vectors one thread
  * holds (4 or 6, default 6) before a row is given to a team twice as large.  Process-wide, not thread-safe.
@@ -406,6 +409,66 @@ LYRAQ_API int lyraq_quant_fp8_2d(uint8_t* dst, size_t dst_ld, const void* src, i
  * 152-160). */
 LYRAQ_API int lyraq_gate_residual(void* out, const void* y, const void* gate, const void* x, int dtype, size_t batch,
                                   size_t seq_len, size_t dim, void* stream);
+
+/* Arguments of lyraq_rope_axes.  Element (b, s, h, 0) of q lies q_batch * b + q_token * s + q_head * h elements behind its pointer, and so on: any
+ * layout whose heads are contiguous; position (b, s, a) likewise (pos_batch = 0: one set for all). */
+typedef struct {
+    const void *q, *k;                       /* [batch, seq_len, heads, head_dim] by strides */
+    size_t q_batch, q_token, q_head, k_batch, k_token, k_head;
+    void *q_out, *k_out;                     /* may be q and k */
+    size_t q_out_batch, q_out_token, q_out_head, k_out_batch, k_out_token, k_out_head;
+    const void *q_norm, *k_norm;             /* RMS norm weights [head_dim], or NULL: not normalised */
+    const void* positions;
+    size_t pos_batch, pos_token, pos_axis;
+    const uint64_t* turns;                   /* [pairs]: frequency of each pair in turns per position, times 2^64, rounded */
+    const unsigned char* axis;               /* [pairs]: the position axis of each pair */
+    int pos_dtype;                           /* S32, S64 or F32 */
+    int dtype;                               /* F16 or BF16 */
+    int q_heads, k_heads, head_dim, pairs;
+    int interleaved;                         /* pair i is (x[2 i], x[2 i + 1]); else (x[i], x[i + pairs]) */
+    float eps;
+    size_t batch, seq_len;
+} lyraq_rope_axes_t;
+
+/* Rotary embedding over several position axes (time, height, width), from the positions: pair i < pairs of every q and k head turns by
+ * positions[b, s, axis[i]] * turns[i] / 2^64 turns, exact for any integer position; elements from 2 * pairs on pass through.  Heads with norm
+ * weights are RMS-normalised first.  fp32, rounded once.  A position that is not finite gives NaN.  head_dim even, at most 256; either of q
+ * and k may be absent (heads 0).  No alignment is required beyond the element; 16-byte aligned heads are faster.  What the reference does with a table
+ * in invokeFusedRmsNormAndRope<T> (src/lyradiff/kernels/rope/flux_apply_rope.h:20-30), for other layouts, head counts and without the table. */
+LYRAQ_API int lyraq_rope_axes(const lyraq_rope_axes_t* args, void* stream);
+
+/* Norms of lyraq_gated_residual_norm. */
+enum { LYRAQ_NORM_NONE = 0, LYRAQ_NORM_RMS = 1, LYRAQ_NORM_LAYER = 2 };
+
+/* Arguments of lyraq_gated_residual_norm.  Row r of batch entry b of a [batch, seq_len, dim] tensor begins *_batch * b + *_row * r elements
+ * behind its pointer; gate, scale and shift have one row per batch entry (*_batch = 0: one for all).  All strides are multiples of 8. */
+typedef struct {
+    const void *y, *x;                       /* the block's output and the residual stream */
+    size_t y_batch, y_row, x_batch, x_row;
+    void *x_out, *h;                         /* the new stream and its norm; either may be NULL */
+    size_t x_out_batch, x_out_row, h_batch, h_row;
+    uint8_t* qf8;                            /* e4m3 codes of h / f8_scale[0], [batch * seq_len, dim], or NULL */
+    const float* f8_scale;
+    uint8_t *q4, *q4_scales;                 /* h in FP4 as lyraq_quant_fp4 makes it of [batch * seq_len, dim], or NULL */
+    const float* q4_tensor_scale;            /* its tensor scale, NULL = 1 */
+    int q4_format;
+    const void *gate, *scale, *shift;        /* NULL: 1, 0, 0 */
+    size_t gate_batch, scale_batch, shift_batch;
+    const void *post_weight, *pre_weight;    /* [dim] or NULL (= ones) */
+    int post, pre;                           /* LYRAQ_NORM_*; pre is RMS or LAYER */
+    float residual_scale, eps;
+    int dtype;                               /* F16 or BF16, of every 16-bit tensor */
+    size_t batch, seq_len, dim;
+} lyraq_gated_norm_t;
+
+/* Norms before and after a block with its gate and residual in one pass:
+ *   u = post(y) * post_weight;  v = residual_scale * x + gate_b * u;  x_out = T(v);  h = T( pre(v) * pre_weight * (1 + scale_b) + shift_b )
+ * RMS: v / sqrt(mean(v^2) + eps); LAYER: the mean subtracted first.  fp32 throughout, each output rounded once; pre sees v before its rounding.
+ * qf8 and q4 hold the codes that lyraq_quant_fp8 and lyraq_quant_fp4 make of T(h).  x_out may be x and h may be y (same strides).  dim a
+ * multiple of 8 (32 with q4), at most 16384; pointers 16-byte aligned (qf8: 8).  The fused form of what the reference runs as
+ * invokeFusedGateAndResidual (src/lyradiff/kernels/flux_single_transformer_block/flux_single_transformer_kernels.cu:43-65) and
+ * invokeLayerNormWithShiftAndScale (src/lyradiff/kernels/norms/layer_norm.h:19); the norm after a block has no counterpart there. */
+LYRAQ_API int lyraq_gated_residual_norm(const lyraq_gated_norm_t* args, void* stream);
 
 /* LoRA hot-swap on a 16-bit weight: weight[i] = T(weight[i] + T(lora[i] * T(alpha))), i < n, in place; every step rounds to
  * T as the reference's 16-bit operators do.  The FP8 layers follow it with lyraq_weight_quant_fp8 on the merged weight

@@ -13,6 +13,28 @@ c_size_t = ctypes.c_size_t
 c_float = ctypes.c_float
 c_double = ctypes.c_double
 
+
+
+class GatedNormArgs(ctypes.Structure):
+    """lyraq_gated_norm_t."""
+    _fields_ = ([(n, c_void_p) for n in ("y", "x")] + [(n, c_size_t) for n in ("y_batch", "y_row", "x_batch", "x_row")]
+                + [(n, c_void_p) for n in ("x_out", "h")] + [(n, c_size_t) for n in ("x_out_batch", "x_out_row", "h_batch", "h_row")]
+                + [(n, c_void_p) for n in ("qf8", "f8_scale", "q4", "q4_scales", "q4_tensor_scale")] + [("q4_format", c_int)]
+                + [(n, c_void_p) for n in ("gate", "scale", "shift")] + [(n, c_size_t) for n in ("gate_batch", "scale_batch", "shift_batch")]
+                + [(n, c_void_p) for n in ("post_weight", "pre_weight")] + [("post", c_int), ("pre", c_int)]
+                + [("residual_scale", c_float), ("eps", c_float), ("dtype", c_int)] + [(n, c_size_t) for n in ("batch", "seq_len", "dim")])
+
+
+class RopeAxesArgs(ctypes.Structure):
+    """lyraq_rope_axes_t."""
+    _fields_ = ([(n, c_void_p) for n in ("q", "k")] + [(a + n, c_size_t) for a in ("q_", "k_") for n in ("batch", "token", "head")]
+                + [(n, c_void_p) for n in ("q_out", "k_out")] + [(a + n, c_size_t) for a in ("q_out_", "k_out_") for n in ("batch", "token", "head")]
+                + [(n, c_void_p) for n in ("q_norm", "k_norm", "positions")] + [(n, c_size_t) for n in ("pos_batch", "pos_token", "pos_axis")]
+                + [(n, c_void_p) for n in ("turns", "axis")]
+                + [(n, c_int) for n in ("pos_dtype", "dtype", "q_heads", "k_heads", "head_dim", "pairs", "interleaved")] + [("eps", c_float)]
+                + [(n, c_size_t) for n in ("batch", "seq_len")])
+
+
 # name -> (restype, argtypes); mirrors include/lyraq.h declaration by declaration
 SIGNATURES = {
     "lyraq_version": (ctypes.c_char_p, []),
@@ -24,6 +46,7 @@ SIGNATURES = {
     "lyraq_debug_skinny_wait_test": (c_int, [c_int, ctypes.c_uint]),
     "lyraq_debug_force_w4a4_wide": (c_int, [c_int]),
     "lyraq_debug_force_fp4_tile": (c_int, [c_int]),
+    "lyraq_debug_fp4_skinny_wait_test": (c_int, [c_int, ctypes.c_uint]),
     "lyraq_last_cuda_error": (ctypes.c_char_p, []),
     "lyraq_debug_set_row_vectors_per_thread": (c_int, [c_int]),
     "lyraq_debug_set_special_row_kernels": (c_int, [c_int]),
@@ -69,6 +92,8 @@ SIGNATURES = {
     "lyraq_quant_fp8_2d": (c_int, [c_void_p, c_size_t, c_void_p, c_int, c_void_p, c_size_t, c_size_t, c_void_p]),
     "lyraq_load_lora": (c_int, [c_void_p, c_void_p, c_int, c_float, c_size_t, c_void_p]),
     "lyraq_gate_residual": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_size_t, c_size_t, c_size_t, c_void_p]),
+    "lyraq_rope_axes": (c_int, [ctypes.POINTER(RopeAxesArgs), c_void_p]),
+    "lyraq_gated_residual_norm": (c_int, [ctypes.POINTER(GatedNormArgs), c_void_p]),
     "lyraq_gemm_w4a4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p,
                                 c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "lyraq_gemm_fp4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p,

@@ -40,76 +40,104 @@ __device__ __forceinline__ uint32_t f32x8_to_e2m1x8(const float* v)
     return r;
 }
 
+// 1 / v, off by an ulp at most.
+__device__ __forceinline__ float rcp_approx(float v)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// What the blocks of a tensor share: its scale g, 6 g and about 1 / (6 g).
+struct Fp4Tensor {
+    float g, g6, r6;
+    bool  plain;    // 6 g is far from where its reciprocal or a remainder over- or underflows
+};
+template<int FORMAT> __device__ __forceinline__ Fp4Tensor fp4_tensor(const float* tensor_scale)
+{
+    Fp4Tensor t{1.0f, 6.0f, 0.0f, true};
+    if (FORMAT == LYRAQ_NVFP4) {
+        t.g     = tensor_scale != nullptr ? ld_f32(tensor_scale) : 1.0f;
+        t.g6    = 6.0f * t.g;
+        t.r6    = rcp_approx(t.g6);
+        t.plain = t.g6 >= 7.9e-31f && t.g6 <= 1.2e30f;
+    }
+    return t;
+}
+
+// Quotients without a division: q0 = a r with r about 1 / b, then q0 + (a - q0 b) r.  The remainder is exact, so what is rounded to the result is off
+// by 2^-45 of it.  Here b has few significant bits (three times or a four-bit number times a power of two), and so does every tie of the number
+// formats times b: a quotient that is a tie comes out as it, one that is not lies more than half an ulp and 2^-31 away from any.  So
+// roundings decide as the exact quotient would, ties included.
+//
 // Scale of one block from the largest magnitude in it: the stored byte and what the block's values are divided by.
 struct Fp4Block {
     uint32_t code;
     float    t;      // 0: every code is 0
-    float    r;      // 1 / t, rounded once
-    bool     exact;  // the division of this block may go through r
+    float    r;      // 1 / t: exact for mxfp4, about so for nvfp4
+    bool     plain;  // nothing over- or underflows on the way of the values' quotients
 };
 
 // amax_bits: the largest |x| of the block as fp32 bits, taken as an integer maximum, so that a NaN beats an infinity and both beat every
 // number.  A block that holds either gets the scale NaN and zero codes: all of it reads back as NaN.
 //   nvfp4: s = e4m3(amax / (6 g)), t = s g;  mxfp4: s = t = 2^(floor(log2 amax) - 2), at least 2^-127
-// With g a power of two t has four significant bits, s and every code are the nearest to the exact quotient, ties to even: a quotient
-// that is not a tie differs from one by more than half an ulp (numerator and tie times t both lie on the numerator's grid).
-template<int FORMAT> __device__ __forceinline__ Fp4Block fp4_block(uint32_t amax_bits, float g)
+template<int FORMAT> __device__ __forceinline__ Fp4Block fp4_block(uint32_t amax_bits, const Fp4Tensor& s)
 {
     Fp4Block b;
     if (amax_bits >= 0x7f800000u) {
         b.code  = FORMAT == LYRAQ_NVFP4 ? 0x7fu : 0xffu;
         b.t     = 0.0f;
         b.r     = 0.0f;
-        b.exact = true;
+        b.plain = true;
         return b;
     }
-    const float amax = __uint_as_float(amax_bits);
     if (FORMAT == LYRAQ_NVFP4) {
-        const float ratio = amax_bits == 0u ? 0.0f : amax / (6.0f * g);
-        b.code            = f32x2_to_e4m3x2(ratio, 0.0f) & 0xffu;
+        const float amax  = __uint_as_float(amax_bits);
+        const float q0    = amax * s.r6;
+        float       ratio = fmaf(fmaf(-q0, s.g6, amax), s.r6, q0);
+        if (!s.plain || amax > s.g6 * 1024.0f) {   // the second saturates
+            ratio = amax_bits == 0u ? 0.0f : amax / s.g6;
+        }
+        b.code = f32x2_to_e4m3x2(ratio, 0.0f) & 0xffu;
         // e4m3 -> fp32: the code's seven bits under fp16's exponent read 2^-8 times its value, subnormals included
-        b.t     = __half2float(__ushort_as_half((unsigned short)(b.code << 7))) * 256.0f * g;
-        b.r     = b.t > 0.0f ? 1.0f / b.t : 0.0f;
-        b.exact = b.t == 0.0f || (b.t >= 7.9e-31f && b.t <= 1.2e30f && amax <= b.t * 1048576.0f);
+        b.t     = __half2float(__ushort_as_half((unsigned short)(b.code << 7))) * 256.0f * s.g;
+        b.r     = rcp_approx(b.t);
+        b.plain = b.t >= 7.9e-31f && b.t <= 1.2e30f && amax <= b.t * 1048576.0f;
     } else {
         const uint32_t e = amax_bits >> 23;                                  // biased; 0 for subnormals
         b.code           = e > 2u ? e - 2u : 0u;
         b.t              = b.code != 0u ? __uint_as_float(b.code << 23) : __uint_as_float(0x00400000u);
         // 2^-(code - 127) is a number for every code (2^127 down to 2^-125), so the product with it is the quotient itself
         b.r     = __uint_as_float((254u - b.code) << 23);
-        b.exact = true;
+        b.plain = true;
     }
     return b;
 }
 
-// The codes of eight values of a block.  nvfp4: q = fl(x / t) without a division: q0 = x r, then one correction by the exact remainder
-// x - q0 t, which gives the correctly rounded quotient (Markstein) where nothing over- or underflows on the way; blocks outside that range
-// divide.  A quotient that over- or underflows saturates or rounds to zero like any other.
+// The codes of eight values of a block.  A quotient that over- or underflows saturates or rounds to zero like any other.
 template<int FORMAT> __device__ __forceinline__ uint32_t fp4_encode8(const float* x, const Fp4Block& b)
 {
-    float q[8];
+    float        q[8];
+    const float2 r2 = make_float2(b.r, b.r);
     if (b.t == 0.0f) {
         return 0u;
     }
     if (FORMAT != LYRAQ_NVFP4) {
-        const float2 r2 = make_float2(b.r, b.r);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float2 p = mul_f32x2(make_float2(x[2 * j], x[2 * j + 1]), r2);
             q[2 * j]       = p.x;
             q[2 * j + 1]   = p.y;
         }
-    } else if (b.exact) {
-        const float2 r2 = make_float2(b.r, b.r);
+    } else if (b.plain) {
         const float2 m2 = make_float2(-b.t, -b.t);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float2 v   = make_float2(x[2 * j], x[2 * j + 1]);
-            const float2 q0  = mul_f32x2(v, r2);
-            const float2 rem = fma_f32x2(q0, m2, v);
-            const float2 q1  = fma_f32x2(rem, r2, q0);
-            q[2 * j]         = q1.x;
-            q[2 * j + 1]     = q1.y;
+            const float2 v  = make_float2(x[2 * j], x[2 * j + 1]);
+            const float2 q0 = mul_f32x2(v, r2);
+            const float2 q1 = fma_f32x2(fma_f32x2(q0, m2, v), r2, q0);
+            q[2 * j]        = q1.x;
+            q[2 * j + 1]    = q1.y;
         }
     } else {
 #pragma unroll

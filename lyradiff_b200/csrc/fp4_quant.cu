@@ -6,28 +6,29 @@ namespace lyraq {
 int device_sm_count();  // gemm_dense.cu
 
 // Activations (and weights, once their tensor scale is known).  A pass over memory: 2 bytes a value are read, half a byte and a
-// sixteenth or a thirty-second of one are written.  A thread owns one block, so nothing is exchanged but the four scale bytes of an
-// atom's row, which one of four neighbours stores as a word.  A warp takes the same atom of eight rows, r and r + 1 in each quarter of the
-// 128: it reads whole 128-byte lines of every row and its scale words fill one 32-byte sector.
+// sixteenth or a thirty-second of one are written.  A thread owns 32 values, two blocks or one, four lanes 128 of a row; nothing is exchanged
+// but the scale bytes of an atom's row, which one lane stores as a word.  A warp takes the same 128 columns of eight rows, r and r + 1 in
+// each quarter of the 128: whole lines of every row, and scale words that fill 32-byte sectors.
 template<typename T, int FORMAT>
 __global__ void __launch_bounds__(256)
-fp4_quant_kernel(uint8_t* q, uint8_t* sf, const T* x, size_t ldx, const float* tensor_scale, size_t rows, size_t k, unsigned atoms,
+fp4_quant_kernel(uint8_t* q, uint8_t* sf, const T* x, size_t ldx, const float* tensor_scale, size_t rows, size_t k, unsigned chunks,
                  unsigned octets, size_t tasks)
 {
-    constexpr int kGroup = fp4_group(FORMAT);
-    constexpr int kPer   = 16 / (int)sizeof(T);     // values of a 16-byte vector
-    constexpr int kVecs  = kGroup / kPer;
+    constexpr int kGroup  = fp4_group(FORMAT);
+    constexpr int kBlocks = 32 / kGroup;            // of one thread
+    constexpr int kPer    = 16 / (int)sizeof(T);    // values of a 16-byte vector
+    constexpr int kVecs   = 32 / kPer;
     grid_launch_dependents();
     const size_t   task  = (size_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
     const unsigned lane  = threadIdx.x & 31;
-    const size_t   rest  = task / atoms;
-    const unsigned atom  = (unsigned)(task - rest * atoms);
+    const size_t   rest  = task / chunks;
+    const unsigned chunk = (unsigned)(task - rest * chunks);
     const size_t   rb    = rest / octets;
     const unsigned octet = (unsigned)(rest - rb * octets);
     const unsigned i     = lane >> 2, j = lane & 3;
     const size_t   row   = rb * 128 + 2 * octet + (i >> 2) + 32 * (i & 3);
-    const size_t   col   = (size_t)atom * fp4_atom_k(FORMAT) + (size_t)j * kGroup;
-    const bool     in    = task < tasks && row < rows && col < k;   // k is a multiple of 32: a block is whole or absent
+    const size_t   col   = (size_t)chunk * 128 + (size_t)j * 32;
+    const bool     in    = task < tasks && row < rows && col < k;   // k is a multiple of 32: a thread's values are there or not
     grid_dependency_wait();
 
     Vec16 v[kVecs];
@@ -38,44 +39,45 @@ fp4_quant_kernel(uint8_t* q, uint8_t* sf, const T* x, size_t ldx, const float* t
             v[a] = ld_nc_16(src + a * kPer);
         }
     }
-    const float g    = tensor_scale != nullptr ? ld_f32(tensor_scale) : 1.0f;
-    uint32_t    code = 0;
+    const Fp4Tensor tensor = fp4_tensor<FORMAT>(tensor_scale);
+    uint32_t        code   = 0;
     if (in) {
-        uint32_t amax = 0;
+        Vec16 o;
 #pragma unroll
-        for (int a = 0; a < kVecs; ++a) {
-            amax = max(amax, amax_bits_of<T>(v[a]));
-        }
-        const Fp4Block b = fp4_block<FORMAT>(amax, g);
-        code             = b.code;
-        uint32_t w[kGroup / 8];
+        for (int b = 0; b < kBlocks; ++b) {
+            constexpr int kV = kVecs / kBlocks;
+            uint32_t      amax = 0;
 #pragma unroll
-        for (int a = 0; a < kGroup / 8; ++a) {
-            float f[8];
-            if constexpr (sizeof(T) == 4) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    f[e] = __uint_as_float(v[2 * a + (e >> 2)].w[e & 3]);
-                }
-            } else {
-                unpack8<T>(v[a], f);
+            for (int a = 0; a < kV; ++a) {
+                amax = max(amax, amax_bits_of<T>(v[b * kV + a]));
             }
-            w[a] = fp4_encode8<FORMAT>(f, b);
+            const Fp4Block blk = fp4_block<FORMAT>(amax, tensor);
+            code |= blk.code << (8 * b);
+#pragma unroll
+            for (int a = 0; a < kGroup / 8; ++a) {
+                float f[8];
+                if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        f[e] = __uint_as_float(v[b * kV + 2 * a + (e >> 2)].w[e & 3]);
+                    }
+                } else {
+                    unpack8<T>(v[b * kV + a], f);
+                }
+                o.w[b * (kGroup / 8) + a] = fp4_encode8<FORMAT>(f, blk);
+            }
         }
-        uint8_t* dst = q + row * (k >> 1) + (col >> 1);
-        if constexpr (kGroup == 16) {
-            st_8(dst, w[0], w[1]);
-        } else {
-            Vec16 o;
-            o.w[0] = w[0]; o.w[1] = w[1]; o.w[2] = w[2]; o.w[3] = w[3];
-            st_16(dst, o);
-        }
+        st_16(q + row * (k >> 1) + (col >> 1), o);
     }
     // blocks beyond k have scale 0, so the word of an existing row is always written whole
-    uint32_t word = code << (8 * j);
+    constexpr unsigned kLanes = 4 / kBlocks;    // that share a word
+    uint32_t           word   = code << (8 * kBlocks * (j % kLanes));
     word |= __shfl_xor_sync(0xffffffffu, word, 1);
-    word |= __shfl_xor_sync(0xffffffffu, word, 2);
-    if (j == 0 && task < tasks && row < rows) {
+    if (kLanes == 4) {
+        word |= __shfl_xor_sync(0xffffffffu, word, 2);
+    }
+    const size_t atom = (size_t)chunk * (4 / kLanes) + j / kLanes, atoms = fp4_atoms(k, FORMAT);
+    if (j % kLanes == 0 && task < tasks && row < rows && atom < atoms) {
         *reinterpret_cast<uint32_t*>(sf + fp4_scale_offset(row, atoms, atom)) = word;
     }
 }
@@ -161,16 +163,16 @@ static int check_fp4(const void* q, const void* sf, const void* x, int dtype, si
 static int run_quant(uint8_t* q, uint8_t* sf, const void* x, int dtype, size_t ldx, const float* tensor_scale, int format, size_t rows,
                      size_t k, cudaStream_t s)
 {
-    const size_t atoms   = fp4_atoms(k, format);
+    const size_t chunks  = (k + 127) / 128;
     const size_t octets  = rows >= 32 ? 16 : (rows + 1) / 2;     // fewer than 32 rows lie in the first quarter of their 128
-    const size_t tasks   = (rows + 127) / 128 * octets * atoms;  // one warp each
+    const size_t tasks   = (rows + 127) / 128 * octets * chunks;  // one warp each
     const size_t blocks  = (tasks + 7) / 8;
     if (blocks > 0x7fffffffu) {
         return LYRAQ_ERR_UNSUPPORTED;
     }
     auto launch = [&](auto* kernel, auto type) {
         using T = decltype(type);
-        return launch_kernel(kernel, (unsigned)blocks, 256u, (size_t)0, s, 1u, q, sf, (const T*)x, ldx, tensor_scale, rows, k, (unsigned)atoms,
+        return launch_kernel(kernel, (unsigned)blocks, 256u, (size_t)0, s, 1u, q, sf, (const T*)x, ldx, tensor_scale, rows, k, (unsigned)chunks,
                              (unsigned)octets, tasks);
     };
     auto pick = [&](auto type) {

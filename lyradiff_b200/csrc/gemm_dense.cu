@@ -1116,11 +1116,12 @@ int make_tmap_store(CUtensorMap* map, const void* base, uint64_t rows, uint64_t 
     return LYRAQ_OK;
 }
 
-// Tensor map of FP4 block scales (fp4.cuh): [row blocks][atoms][512 bytes], boxes of box_blocks x box_atoms whole atoms; atoms that do not
-// exist read as zero.
-int make_tmap_atoms(CUtensorMap* map, const void* base, uint64_t row_blocks, uint64_t atoms, uint32_t box_blocks, uint32_t box_atoms)
+// Tensor map of FP4 block scales (fp4.cuh): [row blocks][atoms][128 words], boxes of box_blocks x box_atoms atoms, the first box_words words of
+// each; atoms that do not exist read as zero.
+int make_tmap_atoms(CUtensorMap* map, const void* base, uint64_t row_blocks, uint64_t atoms, uint32_t box_blocks, uint32_t box_atoms,
+                    uint32_t box_words)
 {
-    const TmapKey key{base, atoms, row_blocks, 512, box_atoms, box_blocks, 64};
+    const TmapKey key{base, atoms, row_blocks, 512, box_atoms, box_blocks, 64 + (int)box_words};
     if (tmap_cache().find(key, map)) {
         return LYRAQ_OK;
     }
@@ -1130,7 +1131,7 @@ int make_tmap_atoms(CUtensorMap* map, const void* base, uint64_t row_blocks, uin
     }
     const cuuint64_t dims[3]    = {128, atoms, row_blocks};
     const cuuint64_t strides[2] = {512, atoms * 512};
-    const cuuint32_t box[3]     = {128, box_atoms, box_blocks};
+    const cuuint32_t box[3]     = {box_words, box_atoms, box_blocks};
     const cuuint32_t estr[3]    = {1, 1, 1};
     const CUresult   r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(base), dims, strides, box, estr,
                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,

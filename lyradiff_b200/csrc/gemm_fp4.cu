@@ -28,7 +28,8 @@ int device_sm_count();                                                          
 int make_tmap_bytes_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t k_bytes, uint64_t row_stride_bytes,    // gemm_dense.cu
                        uint32_t box_rows, uint32_t box_bytes, bool swizzle128);
 int make_tmap_store(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, int elem_bytes, bool wide);  // gemm_dense.cu
-int make_tmap_atoms(CUtensorMap* map, const void* base, uint64_t row_blocks, uint64_t atoms, uint32_t box_blocks, uint32_t box_atoms);  // gemm_dense.cu
+int make_tmap_atoms(CUtensorMap* map, const void* base, uint64_t row_blocks, uint64_t atoms, uint32_t box_blocks, uint32_t box_atoms,  // gemm_dense.cu
+                    uint32_t box_words);
 
 namespace fp4 {
 
@@ -38,7 +39,8 @@ constexpr int kBlockK    = 256;
 constexpr int kThreads   = 384;
 constexpr int kEpiWarp0  = 4;
 constexpr int kEpiWarps  = 8;
-constexpr int kBox       = 32 * 128;     // one warp's staging box: 32 rows x 64 columns of a 16-bit type
+constexpr int kBox       = 32 * 64;      // one warp's staging box: 32 rows x 32 columns of a 16-bit type
+constexpr int kBiasBytes = 128 * 4;      // one warp's bias: up to 128 columns in fp32
 constexpr int kBarBytes  = 256;
 constexpr int kOtherRegs = 72;
 constexpr int kEpiRegs   = 216;
@@ -46,21 +48,24 @@ static_assert(128 * kOtherRegs + 256 * kEpiRegs <= kThreads * 168, "the split dr
 
 template<int FORMAT, int BLOCK_N, int CTAS> struct Smem {
     static constexpr int kAtoms      = kBlockK / fp4_atom_k(FORMAT);    // scale atoms of 128 rows in a K block: 4 or 2
+    static constexpr int kSbBlocks   = BLOCK_N / 128;                   // row blocks of 128 in a tile's B rows
     static constexpr int kABytes     = kBlockM * kRowBytes;
     static constexpr int kBBytes     = BLOCK_N / CTAS * kRowBytes;
     static constexpr int kSfaBytes   = kAtoms * 512;
-    static constexpr int kSfbBytes   = BLOCK_N / 128 * kAtoms * 512;
+    static constexpr int kSfbBytes   = kSbBlocks * kAtoms * 512;
     static constexpr int kStageBytes = kABytes + kBBytes + kSfaBytes + kSfbBytes;
-    static constexpr int kStages     = 5;
+    static constexpr int kEpiBytes   = kEpiWarps * (kBox + kBiasBytes);
+    static constexpr int kStages     = (227 * 1024 - 1024 - kBarBytes - kEpiBytes) / kStageBytes;
     static constexpr int kEpiOffset  = kStages * kStageBytes;
-    static constexpr int kBarOffset  = kEpiOffset + kEpiWarps * kBox;
+    static constexpr int kBarOffset  = kEpiOffset + kEpiBytes;
     static constexpr int kTotal      = kBarOffset + kBarBytes + 1024;   // + alignment slack
-    // tensor memory
-    static constexpr int kAccBufs    = 256 / BLOCK_N;
-    static constexpr int kScaleCols  = kAtoms * 4 * (1 + BLOCK_N / 128);
+    // tensor memory: accumulators, then each stage's scales
+    static constexpr int kAccBufs    = BLOCK_N == 256 ? 1 : 2;
+    static constexpr int kAccCols    = kAccBufs * BLOCK_N;
+    static constexpr int kScaleCols  = kAtoms * 4 * (1 + kSbBlocks);
     static_assert(kStageBytes % 1024 == 0, "the swizzle pattern is anchored to 1024 bytes");
-    static_assert(kTotal <= 227 * 1024, "");
-    static_assert(256 + kStages * kScaleCols <= 512, "");
+    static_assert(8 * (2 * kStages + 4) + 8 <= kBarBytes, "");
+    static_assert(kAccCols + kStages * kScaleCols <= 512, "");
 };
 
 // Bands of 8 tile rows swept along N: the tiles that run at the same time share A and B tiles through L2.
@@ -76,9 +81,9 @@ __device__ __forceinline__ void tile_coords(int tile, int m_tiles, int n_tiles, 
     n_blk               = in_group / rows;
 }
 
-// 32 columns of one row: accumulators -> fp32 results, in the order beta R, bias, GELU.
+// 32 columns of one row: accumulators -> fp32 results, in the order beta R, bias, GELU.  bias: the columns' own in shared memory.
 template<typename T, bool RES>
-__device__ __forceinline__ void finish32(const Fp4GemmParams& p, const uint32_t* acc, float scale, int row, int col0, int valid, bool vec_ok, float* v)
+__device__ __forceinline__ void finish32(const Fp4GemmParams& p, const uint32_t* acc, const float* bias, float scale, int row, int col0, int valid, bool vec_ok, float* v)
 {
     constexpr int kPer = 16 / (int)sizeof(T);
     const float2  s2 = make_float2(scale, scale);
@@ -118,32 +123,12 @@ __device__ __forceinline__ void finish32(const Fp4GemmParams& p, const uint32_t*
         }
     }
     if (p.bias != nullptr) {
-        const T* b = reinterpret_cast<const T*>(p.bias) + col0;
-        if (valid >= 32) {   // every lane reads the same 16 bytes
 #pragma unroll
-            for (int q = 0; q < 32 / kPer; ++q) {
-                const Vec16 x = ld_nc_16_keep(b + q * kPer);
-                float       f[8];
-                if constexpr (sizeof(T) == 4) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        f[j] = __uint_as_float(x.w[j]);
-                    }
-                } else {
-                    unpack8<T>(x, f);
-                }
-#pragma unroll
-                for (int j = 0; j < kPer; ++j) {
-                    v[q * kPer + j] += f[j];
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                if (i < valid) {
-                    v[i] += to_f32(b[i]);
-                }
-            }
+        for (int q = 0; q < 8; ++q) {   // every lane reads the same 16 bytes
+            const float4 b = *reinterpret_cast<const float4*>(bias + 4 * q);
+            const float2 a0 = add_f32x2(make_float2(v[4 * q], v[4 * q + 1]), make_float2(b.x, b.y));
+            const float2 a1 = add_f32x2(make_float2(v[4 * q + 2], v[4 * q + 3]), make_float2(b.z, b.w));
+            v[4 * q] = a0.x; v[4 * q + 1] = a0.y; v[4 * q + 2] = a1.x; v[4 * q + 3] = a1.y;
         }
     }
     if (p.gelu) {
@@ -324,7 +309,6 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             uint32_t phase = 0;
             int      local = 0;
             bool     ok = true;
-            const uint32_t peer = (CTAS == 2) ? 1u : 0u;
             for (int tile = unit; ok && tile < num_tiles; tile += n_units, ++local) {
                 const int      buf       = S::kAccBufs == 2 ? (local & 1) : 0;
                 const uint32_t acc_phase = (uint32_t)(S::kAccBufs == 2 ? local >> 1 : local) & 1u;
@@ -343,12 +327,12 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                         break;
                     }
                     tc_fence_after_sync();
-                    const uint32_t sa    = smem_base + stage * S::kStageBytes;
-                    const uint64_t adesc = umma_desc_k_sw128(sa);
-                    const uint64_t bdesc = umma_desc_k_sw128(sa + S::kABytes);
+                    const uint32_t sa     = smem_base + stage * S::kStageBytes;
+                    const uint64_t adesc  = umma_desc_k_sw128(sa);
+                    const uint64_t bdesc  = umma_desc_k_sw128(sa + S::kABytes);
                     const uint64_t sadesc = umma_desc_scales(sa + S::kABytes + S::kBBytes);
                     const uint64_t sbdesc = umma_desc_scales(sa + S::kABytes + S::kBBytes + S::kSfaBytes);
-                    const uint32_t sfa    = tmem_base + 256u + (uint32_t)(stage * S::kScaleCols);
+                    const uint32_t sfa    = tmem_base + (uint32_t)(S::kAccCols + stage * S::kScaleCols);
                     const uint32_t sfb    = sfa + S::kAtoms * 4;
                     const int      steps  = min(kBlockK, p.K - kb * kBlockK + 63) / 64;   // MMAs of this K block
                     const bool     last   = kb + 1 == num_kb;
@@ -356,11 +340,11 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
 #pragma unroll
                         for (int a = 0; a < S::kAtoms; ++a) {
                             if (a * (4 / S::kAtoms) < steps) {
-                                // in tensor memory an atom's row blocks stand side by side
+                                // in tensor memory the row blocks of an atom stand side by side
                                 tmem_copy_scales<CTAS>(sfa + a * 4, sadesc + (uint64_t)(a * 32));
 #pragma unroll
-                                for (int rb = 0; rb < BLOCK_N / 128; ++rb) {
-                                    tmem_copy_scales<CTAS>(sfb + a * (BLOCK_N / 32) + rb * 4, sbdesc + (uint64_t)((rb * S::kAtoms + a) * 32));
+                                for (int rb = 0; rb < S::kSbBlocks; ++rb) {
+                                    tmem_copy_scales<CTAS>(sfb + a * (4 * S::kSbBlocks) + rb * 4, sbdesc + (uint64_t)((rb * S::kAtoms + a) * 32));
                                 }
 #pragma unroll
                                 for (int h = 0; h < 4 / S::kAtoms; ++h) {
@@ -368,17 +352,15 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                                     if (k < steps) {
                                         mma_fp4<FORMAT, CTAS>(d_tmem, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k),
                                                               umma_idesc_fp4(FORMAT, kTileM, BLOCK_N, 2u * h), sfa + a * 4,
-                                                              sfb + a * (BLOCK_N / 32), (kb > 0 || k > 0) ? 1u : 0u);
+                                                              sfb + a * (4 * S::kSbBlocks), (kb > 0 || k > 0) ? 1u : 0u);
                                     }
                                 }
                             }
                         }
                         if (CTAS == 2) {
-                            tc_commit_pair(empty_bar(stage));
-                            tc_commit_pair(map_to_cta(empty_bar(stage), peer));
+                            tc_commit_both(empty_bar(stage));
                             if (last) {
-                                tc_commit_pair(tmem_full_bar(buf));
-                                tc_commit_pair(map_to_cta(tmem_full_bar(buf), peer));
+                                tc_commit_both(tmem_full_bar(buf));
                             }
                         } else {
                             tc_commit(empty_bar(stage));
@@ -402,6 +384,7 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
         uint8_t*       box       = gen_base + S::kEpiOffset + (warp - kEpiWarp0) * kBox;
         const uint32_t box_addr  = smem_base + S::kEpiOffset + (warp - kEpiWarp0) * kBox;
+        float*         bias      = reinterpret_cast<float*>(gen_base + S::kEpiOffset + kEpiWarps * kBox + (warp - kEpiWarp0) * kBiasBytes);
         const float    scale     = fp4_tensor_scale(p);
         const bool     vec_ok    = p.c_dtype == LYRAQ_F32 ? (p.N & 3) == 0 : (p.N & 7) == 0;
         int            local     = 0;
@@ -413,6 +396,26 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             const int row0  = m_blk * kTileM + (int)rank * kBlockM + quad * 32;  // first row of this warp
             const int row   = row0 + lane;
             const int ncol0 = n_blk * BLOCK_N + half * kHalfN;
+            if (p.bias != nullptr) {
+                // staged while the main loop of the tile still runs; the warp's own piece, so no other warp is waited for
+                float b[kHalfN / 32];
+#pragma unroll
+                for (int i = 0; i < kHalfN / 32; ++i) {
+                    const int col = ncol0 + lane + 32 * i;
+                    b[i]          = 0.0f;
+                    if (col < p.N) {
+                        b[i] = p.c_dtype == LYRAQ_F32    ? reinterpret_cast<const float*>(p.bias)[col]
+                               : p.c_dtype == LYRAQ_BF16 ? to_f32(reinterpret_cast<const __nv_bfloat16*>(p.bias)[col])
+                                                         : to_f32(reinterpret_cast<const __half*>(p.bias)[col]);
+                    }
+                }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < kHalfN / 32; ++i) {
+                    bias[lane + 32 * i] = b[i];
+                }
+                __syncwarp();
+            }
             if (RES && p.residual != nullptr && row < p.M) {
                 // the row's share of the residual is asked into L2 while the main loop of the tile still runs
                 const int      esz = p.c_dtype == LYRAQ_F32 ? 4 : 2;
@@ -431,83 +434,87 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                 break;
             }
             tc_fence_after_sync();
-            uint32_t acc[kHalfN];
+            const uint32_t t_addr = tmem_base + lane_addr + (uint32_t)(buf * BLOCK_N + half * kHalfN);
+            auto release = [&]() {   // this warp's share of the accumulator is in registers: the next tile may have its columns
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    if (CTAS == 2 && !leader) {
+                        mbar_arrive_cluster_relaxed(map_to_cta(tmem_empty_bar(buf), 0u));
+                    } else {
+                        mbar_arrive(tmem_empty_bar(buf));
+                    }
+                }
+            };
+            constexpr int kChunks = kHalfN / 32;
+            constexpr int kAhead  = S::kAccBufs == 1 ? kChunks : 2;   // chunks in registers: all of a lone accumulator
+            uint32_t acc[kAhead][32];
+            if (S::kAccBufs == 1) {
 #pragma unroll
-            for (int c = 0; c < kHalfN / 32; ++c) {
-                tmem_ld_32x32(tmem_base + lane_addr + (uint32_t)(buf * BLOCK_N + half * kHalfN + c * 32), acc + c * 32);
+                for (int c = 0; c < kChunks; ++c) {
+                    tmem_ld_32x32(t_addr + (uint32_t)(c * 32), acc[c % kAhead]);
+                }
+                tmem_ld_wait();
+                release();
+            } else {
+                tmem_ld_32x32(t_addr, acc[0]);
             }
-            tmem_ld_wait();
-            // the accumulator is in registers: the next tile may have its columns
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) {
-                if (CTAS == 2 && !leader) {
-                    mbar_arrive_cluster(map_to_cta(tmem_empty_bar(buf), 0u));
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+                if (S::kAccBufs == 2) {
+                    tmem_ld_wait();
+                    if (c + 1 < kChunks) {
+                        tmem_ld_32x32(t_addr + (uint32_t)((c + 1) * 32), acc[(c + 1) % kAhead]);
+                    } else {
+                        release();
+                    }
+                }
+                const int col0  = ncol0 + c * 32;
+                const int valid = p.N - col0;
+                if (valid <= 0) {
+                    continue;
+                }
+                float v[32];
+                if (p.c_dtype == LYRAQ_F32) {
+                    if (row < p.M) {
+                        finish32<float, RES>(p, acc[c % kAhead], bias + c * 32, scale, row, col0, valid, vec_ok, v);
+                        store32<float>(reinterpret_cast<float*>(p.C) + (size_t)row * (size_t)p.N + (size_t)col0, valid, vec_ok, v);
+                    }
+                    continue;
+                }
+                const bool bf16 = p.c_dtype == LYRAQ_BF16;
+                if (bf16) {
+                    finish32<__nv_bfloat16, RES>(p, acc[c % kAhead], bias + c * 32, scale, row, col0, valid, vec_ok, v);
                 } else {
-                    mbar_arrive(tmem_empty_bar(buf));
+                    finish32<__half, RES>(p, acc[c % kAhead], bias + c * 32, scale, row, col0, valid, vec_ok, v);
                 }
-            }
-#pragma unroll
-            for (int c2 = 0; c2 < kHalfN / 64; ++c2) {
-                uint32_t o[32];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int c     = c2 * 2 + h;
-                    const int col0  = ncol0 + c * 32;
-                    const int valid = p.N - col0;
-                    float     v[32];
-                    if (p.c_dtype == LYRAQ_F32) {
-                        if (row < p.M && valid > 0) {
-                            finish32<float, RES>(p, acc + c * 32, scale, row, col0, valid, vec_ok, v);
-                            store32<float>(reinterpret_cast<float*>(p.C) + (size_t)row * (size_t)p.N + (size_t)col0, valid, vec_ok, v);
-                        }
-                        continue;
-                    }
-                    if (valid > 0) {
-                        if (p.c_dtype == LYRAQ_BF16) {
-                            finish32<__nv_bfloat16, RES>(p, acc + c * 32, scale, row, col0, valid, vec_ok, v);
+                if (!p.tma_store) {
+                    if (row < p.M) {
+                        uint16_t* crow = reinterpret_cast<uint16_t*>(p.C) + (size_t)row * (size_t)p.N + (size_t)col0;
+                        if (bf16) {
+                            store32<__nv_bfloat16>(reinterpret_cast<__nv_bfloat16*>(crow), valid, vec_ok, v);
                         } else {
-                            finish32<__half, RES>(p, acc + c * 32, scale, row, col0, valid, vec_ok, v);
+                            store32<__half>(reinterpret_cast<__half*>(crow), valid, vec_ok, v);
                         }
                     }
-                    if (!p.tma_store) {
-                        if (row < p.M && valid > 0) {
-                            uint16_t* crow = reinterpret_cast<uint16_t*>(p.C) + (size_t)row * (size_t)p.N + (size_t)col0;
-                            if (p.c_dtype == LYRAQ_BF16) {
-                                store32<__nv_bfloat16>(reinterpret_cast<__nv_bfloat16*>(crow), valid, vec_ok, v);
-                            } else {
-                                store32<__half>(reinterpret_cast<__half*>(crow), valid, vec_ok, v);
-                            }
-                        }
-                        continue;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        o[h * 16 + i] = p.c_dtype == LYRAQ_BF16 ? Pair<__nv_bfloat16>::from_f32(v[2 * i], v[2 * i + 1])
-                                                                : Pair<__half>::from_f32(v[2 * i], v[2 * i + 1]);
-                    }
+                    continue;
                 }
-                if (p.tma_store) {
-                    // 32 rows x 128 bytes through this warp's box in the 128-byte swizzle, one TMA store; rows and columns beyond the
-                    // matrix are clipped
-                    if (lane == 0) {
-                        tma_store_wait_read();  // the previous store has drained the box
-                    }
-                    __syncwarp();
-                    uint8_t*  brow = box + lane * 128;
-                    const int sw   = lane & 7;
+                // 32 rows x 64 bytes through this warp's box in the 64-byte swizzle, one TMA store; rows and columns beyond the matrix are clipped
+                if (lane == 0) {
+                    tma_store_wait_read();  // the previous store has drained the box
+                }
+                __syncwarp();
+                uint8_t*  brow = box + lane * 64;
+                const int sw   = (lane >> 1) & 3;
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) {
-                        Vec16 w;
-                        w.w[0] = o[4 * q]; w.w[1] = o[4 * q + 1]; w.w[2] = o[4 * q + 2]; w.w[3] = o[4 * q + 3];
-                        *reinterpret_cast<Vec16*>(brow + ((q ^ sw) << 4)) = w;
-                    }
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0 && row0 < p.M && ncol0 + c2 * 64 < p.N) {
-                        tma_store_2d(&tmap_c, box_addr, ncol0 + c2 * 64, row0);
-                        tma_store_commit();
-                    }
+                for (int q = 0; q < 4; ++q) {
+                    *reinterpret_cast<Vec16*>(brow + ((q ^ sw) << 4)) = bf16 ? pack8<__nv_bfloat16>(v + 8 * q) : pack8<__half>(v + 8 * q);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0 && row0 < p.M) {
+                    tma_store_2d(&tmap_c, box_addr, col0, row0);
+                    tma_store_commit();
                 }
             }
         }
@@ -544,21 +551,21 @@ static int launch(const uint8_t* X, const uint8_t* xs, const uint8_t* W, const u
         st = make_tmap_bytes_2d(&tb, W, (uint64_t)p.N, kb, kb, BLOCK_N / CTAS, kRowBytes, true);
     }
     if (st == LYRAQ_OK) {
-        st = make_tmap_atoms(&tsa, xs, ((uint64_t)p.M + 127) / 128, atoms, 1, S::kAtoms);
+        st = make_tmap_atoms(&tsa, xs, ((uint64_t)p.M + 127) / 128, atoms, 1, S::kAtoms, 128);
     }
     if (st == LYRAQ_OK) {
-        st = make_tmap_atoms(&tsb, ws, ((uint64_t)p.N + 127) / 128, atoms, BLOCK_N / 128, S::kAtoms);
+        st = make_tmap_atoms(&tsb, ws, ((uint64_t)p.N + 127) / 128, atoms, S::kSbBlocks, S::kAtoms, 128);
     }
     CUtensorMap tc = ta;   // never used where the output is stored directly
     p.tma_store    = p.c_dtype != LYRAQ_F32 && (p.N & 7) == 0;
     if (st == LYRAQ_OK && p.tma_store) {
-        st = make_tmap_store(&tc, p.C, (uint64_t)p.M, (uint64_t)p.N, (uint64_t)p.N, 2, true);
+        st = make_tmap_store(&tc, p.C, (uint64_t)p.M, (uint64_t)p.N, (uint64_t)p.N, 2, false);
     }
     if (st != LYRAQ_OK) {
         return st;
     }
-    p.m_tiles = (p.M + kBlockM * CTAS - 1) / (kBlockM * CTAS);
-    p.n_tiles = (p.N + BLOCK_N - 1) / BLOCK_N;
+    p.m_tiles = (int)(((long)p.M + kBlockM * CTAS - 1) / (kBlockM * CTAS));
+    p.n_tiles = (int)(((long)p.N + BLOCK_N - 1) / BLOCK_N);
     const long long tiles = (long long)p.m_tiles * p.n_tiles;
     if (tiles > 0x40000000ll) {
         return LYRAQ_ERR_UNSUPPORTED;
@@ -575,20 +582,28 @@ static int launch(const uint8_t* X, const uint8_t* xs, const uint8_t* W, const u
                        "cudaLaunchKernelEx(gemm_fp4_kernel)");
 }
 
-// forced tile for tests and sweeps: 0 = automatic, 2562 = CTA pair with 256 x 256, 1281 = one CTA with 128 x 128
+// forced kernel for tests and sweeps: 0 = automatic, 16 = the few-row kernel (up to 16 rows), 2562 = CTA pair with 256 x 256, 1281 = one CTA with 128 x 128
 static int g_forced_tile = 0;
 
 static int run(const uint8_t* X, const uint8_t* xs, const uint8_t* W, const uint8_t* ws, int format, const Fp4GemmParams& p, int sms,
                cudaStream_t stream)
 {
-    const long m128 = (p.M + 127) / 128, n128 = (p.N + 127) / 128, m256 = (p.M + 255) / 256, n256 = (p.N + 255) / 256;
+    const long m128 = ((long)p.M + 127) / 128, n128 = ((long)p.N + 127) / 128, m256 = ((long)p.M + 255) / 256, n256 = ((long)p.N + 255) / 256;
     const long pairs = sms / 2;
     const long c1 = (m128 * n128 + sms - 1) / sms, c2 = 2 * ((m256 * n256 + pairs - 1) / pairs);
-    const bool pair = g_forced_tile != 0 ? g_forced_tile == 2562 : c2 <= c1;
+    // The few-row kernel's time grows with the rows (their partial sums cross shared memory and leave row by row), the other's does not; what it
+    // gains grows with K.  Dense against few-row, us: 4 rows of [256, 256] 2.8 / 3.1, of [1280, 1280] 4.3 / 4.1, 8 rows of it 4.3 / 5.2; 16
+    // rows of [1280, 2048] 5.1 / 4.7, of [3072, 3072] 6.4 / 5.6, of [3072, 12288] 17.4 / 8.2; one row of [9216, 3072] 8.3 / 5.4.
+    const int num_kb = (p.K + kBlockK - 1) / kBlockK;
+    if (p.M <= kFp4SkinnyRows && (g_forced_tile == 16 || (g_forced_tile == 0 && (num_kb >= 8 || p.M <= 2 + num_kb / 2)))) {
+        return launch_skinny(X, xs, W, ws, format, p, sms, stream);
+    }
+    const int  tile = g_forced_tile > 16 ? g_forced_tile : c2 <= c1 ? 2562 : 1281;
     auto pick = [&](auto fmt, auto res) {
         constexpr int  kFmt = decltype(fmt)::value;
         constexpr bool kRes = decltype(res)::value;
-        return pair ? launch<kFmt, 256, 2, kRes>(X, xs, W, ws, p, sms, stream) : launch<kFmt, 128, 1, kRes>(X, xs, W, ws, p, sms, stream);
+        return tile == 2562 ? launch<kFmt, 256, 2, kRes>(X, xs, W, ws, p, sms, stream)
+                            : launch<kFmt, 128, 1, kRes>(X, xs, W, ws, p, sms, stream);
     };
     auto pick_res = [&](auto fmt) {
         return p.residual != nullptr ? pick(fmt, std::integral_constant<bool, true>{}) : pick(fmt, std::integral_constant<bool, false>{});
@@ -605,7 +620,7 @@ extern "C" {
 
 int lyraq_debug_force_fp4_tile(int code)
 {
-    if (code != 0 && code != 1281 && code != 2562) {
+    if (code != 0 && code != 16 && code != 1281 && code != 2562) {
         return LYRAQ_ERR_INVALID_ARG;
     }
     fp4::g_forced_tile = code;
@@ -624,7 +639,7 @@ int lyraq_gemm_fp4(const uint8_t* X, const uint8_t* x_scale, const float* x_tens
     if (m == 0 || n == 0) {
         return LYRAQ_OK;
     }
-    if (k == 0 || (k & 31) != 0) {
+    if (k == 0 || (k & 31) != 0 || m > 0x7fffff00 || n > 0x7fffff00 || k > 0x7fffff00) {   // row and column numbers of a last tile stay within 31 bits
         return LYRAQ_ERR_UNSUPPORTED;
     }
     if (X == nullptr || x_scale == nullptr || W == nullptr || w_scale == nullptr || Y == nullptr || !aligned16(X) || !aligned16(x_scale) ||

@@ -21,6 +21,12 @@ struct Fp4GemmParams {
     int           gelu;
 };
 
+namespace fp4 {
+constexpr int kFp4SkinnyRows = 16;   // most rows of X that gemm_fp4_skinny.cu takes
+int launch_skinny(const uint8_t* X, const uint8_t* xs, const uint8_t* W, const uint8_t* ws, int format, const Fp4GemmParams& p, int sms,
+                  cudaStream_t stream);
+}  // namespace fp4
+
 __device__ __forceinline__ float fp4_tensor_scale(const Fp4GemmParams& p)
 {
     return (p.s_x != nullptr ? ld_f32(p.s_x) : 1.0f) * (p.s_w != nullptr ? ld_f32(p.s_w) : 1.0f);
@@ -42,6 +48,20 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t smem_dst, const CUtens
         "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
         ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(leader_bar), "r"(x), "r"(y), "r"(z)
         : "memory");
+}
+
+// Arrive on another CTA's barrier when all that has to be ordered before it is complete already (tensor-memory loads behind their wait).  The
+// releasing form makes the warp's earlier memory accesses visible first, which took a pair's second CTA 900 ns per tile.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr)
+{
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// Arrive on the barrier at this offset in both CTAs of a pair once all MMAs issued so far have completed.
+__device__ __forceinline__ void tc_commit_both(uint32_t bar)
+{
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3)
+                 : "memory");
 }
 
 // Shared memory -> tensor memory, 32 rows of 16 bytes, the same to each of the four lane quadrants: one atom of block scales, four columns.

@@ -1,0 +1,334 @@
+// Rotary embedding over several position axes, from the positions: no table is built, stored or read.
+//
+// Pair i of a head turns by pos[token, axis(i)] * f(i).  Angles are 64-bit fractions of a turn: F(i) = f(i) / 2 pi * 2^64, and the product of
+// an integer position with it, kept to its low 64 bits, IS the angle modulo a turn, at position one as at a billion (in fp32, position 10^6
+// times 1 rad would be off by 0.03 rad).  The top 32 bits go through sincospi.  A fractional position multiplies its 24-bit significand and
+// shifts.
+//
+// q and k heads are normalised first where weights are given (RMS over the head, fp32), rotated in fp32 and rounded once; what lies behind the
+// rotated part of a head is normalised and copied.
+//
+// Bound by memory: q and k in and out.  A block takes a few tokens; its threads first form the tokens' cosines and sines in shared memory, once for all
+// heads, then a group of L lanes takes a head, every lane VEC pairs (16 bytes of either half, or 32 in a row), two heads of every
+// thread in flight.  A lane's cosines stay in registers while it goes through the heads of a token.
+#include "common.cuh"
+
+namespace lyraq {
+
+int device_sm_count();  // gemm_dense.cu
+
+struct RopeAxesParams {
+    const void*          src[2];      // q, k
+    void*                dst[2];
+    const void*          norm[2];
+    size_t               src_batch[2], src_token[2], src_head[2], dst_batch[2], dst_token[2], dst_head[2];   // strides in elements
+    const void*          pos;
+    size_t               pos_batch, pos_token, pos_axis;
+    const uint64_t*      turns;       // [pairs]
+    const unsigned char* axis;        // [pairs]
+    int                  pos_dtype;
+    int                  heads[2];
+    int                  head_dim, pairs, lanes_log2, groups, chunks, tokens_per_block;
+    size_t               tokens, seq;
+    float                eps;
+};
+
+// Angle of one pair as a fraction of a turn, in 1 / 2^64.
+__device__ __forceinline__ bool angle_of(const RopeAxesParams& p, size_t at, uint64_t turns, uint64_t& phase)
+{
+    if (p.pos_dtype == LYRAQ_S32) {
+        phase = (uint64_t)(int64_t)reinterpret_cast<const int*>(p.pos)[at] * turns;
+        return true;
+    }
+    if (p.pos_dtype == LYRAQ_S64) {
+        phase = (uint64_t)reinterpret_cast<const int64_t*>(p.pos)[at] * turns;
+        return true;
+    }
+    const uint32_t b = __float_as_uint(reinterpret_cast<const float*>(p.pos)[at]);
+    const uint32_t e = (b >> 23) & 0xffu;
+    if (e == 0xffu) {
+        return false;
+    }
+    const uint64_t m  = (uint64_t)((b & 0x7fffffu) | (e != 0u ? 0x800000u : 0u));
+    const int      sh = (int)(e != 0u ? e : 1u) - 150;       // position = m 2^sh
+    const uint64_t lo = m * turns, hi = __umul64hi(m, turns);
+    uint64_t       v;
+    if (sh >= 0) {
+        v = sh < 64 ? lo << sh : 0u;                         // whole turns beyond
+    } else if (sh > -64) {
+        v = (lo >> -sh) | (hi << (64 + sh));
+    } else {
+        v = sh > -128 ? hi >> (-sh - 64) : 0u;
+    }
+    phase = (b >> 31) != 0u ? 0u - v : v;
+    return true;
+}
+
+template<typename T, int VEC> struct Piece;   // VEC values of T
+template<typename T> struct Piece<T, 8> {
+    Vec16 v;
+    __device__ __forceinline__ void load(const T* p) { v = ld_16(p); }
+    __device__ __forceinline__ void store(T* p) const { st_16(p, v); }
+    __device__ __forceinline__ void get(float* f) const { unpack8<T>(v, f); }
+    __device__ __forceinline__ void set(const float* f) { v = pack8<T>(f); }
+};
+template<typename T> struct Piece<T, 4> {
+    uint32_t a, b;
+    __device__ __forceinline__ void load(const T* p) { asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(a), "=r"(b) : "l"(p)); }
+    __device__ __forceinline__ void store(T* p) const { st_8(p, a, b); }
+    __device__ __forceinline__ void get(float* f) const
+    {
+        const float2 x = Pair<T>::to_f32(a), y = Pair<T>::to_f32(b);
+        f[0] = x.x; f[1] = x.y; f[2] = y.x; f[3] = y.y;
+    }
+    __device__ __forceinline__ void set(const float* f)
+    {
+        a = Pair<T>::from_f32(f[0], f[1]);
+        b = Pair<T>::from_f32(f[2], f[3]);
+    }
+};
+template<typename T> struct Piece<T, 1> {
+    T v;
+    __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const volatile T*>(p); }
+    __device__ __forceinline__ void store(T* p) const { *p = v; }
+    __device__ __forceinline__ void get(float* f) const { f[0] = to_f32(v); }
+    __device__ __forceinline__ void set(const float* f) { v = from_f32<T>(f[0]); }
+};
+template<> __device__ __forceinline__ void Piece<__half, 1>::load(const __half* p) { v = __ushort_as_half((unsigned short)ld_u16(p)); }
+template<> __device__ __forceinline__ void Piece<__nv_bfloat16, 1>::load(const __nv_bfloat16* p) { v = __ushort_as_bfloat16((unsigned short)ld_u16(p)); }
+
+// VEC: pairs of a lane's unit; NU: units of a lane (more than one only for single pairs of long heads); HALVES: pair i is (x[i], x[i + pairs]), else
+// (x[2 i], x[2 i + 1]); NORM: q or k is normalised.
+template<typename T, int VEC, int NU, bool HALVES, bool NORM>
+__global__ void __launch_bounds__(256) rope_axes_kernel(const RopeAxesParams p)
+{
+    extern __shared__ float2 turn[];      // [tokens_per_block][pairs]: cosine, sine
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int    chunk = (int)(blockIdx.x % (unsigned)p.chunks);
+    const size_t t0    = (size_t)(blockIdx.x / (unsigned)p.chunks) * (size_t)p.tokens_per_block;
+    const int    n_tok = (int)min((size_t)p.tokens_per_block, p.tokens - t0);
+    for (int i = threadIdx.x; i < n_tok * p.pairs; i += blockDim.x) {
+        const int    tk = i / p.pairs, pair = i - tk * p.pairs;
+        const size_t token = t0 + tk, b = token / p.seq, s = token - b * p.seq;
+        uint64_t     phase = 0;
+        float2       cs;
+        if (angle_of(p, b * p.pos_batch + s * p.pos_token + (size_t)p.axis[pair] * p.pos_axis, p.turns[pair], phase)) {
+            // half turns in [-1, 1)
+            sincospif((float)(int)(uint32_t)(phase >> 32) * 4.656612873077393e-10f, &cs.y, &cs.x);
+        } else {
+            cs = make_float2(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
+        }
+        turn[i] = cs;
+    }
+    __syncthreads();
+
+    const int lanes = 1 << p.lanes_log2;
+    const int lane = (int)threadIdx.x & (lanes - 1), group = (int)threadIdx.x >> p.lanes_log2;
+    const int units = p.head_dim / (2 * VEC), turning = p.pairs / VEC;     // units of a head, those of them that turn
+    const int heads = p.heads[0] + p.heads[1];
+    // this block's share of the heads, dealt to groups
+    const int h0 = (int)((long long)heads * chunk / p.chunks), h1 = (int)((long long)heads * (chunk + 1) / p.chunks);
+    int  at_a[NU], at_b[NU];
+    bool there[NU], turns[NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+        const int unit = lane + u * lanes;
+        there[u] = unit < units;
+        turns[u] = unit < turning;
+        at_a[u]  = HALVES && turns[u] ? unit * VEC : unit * 2 * VEC;
+        at_b[u]  = HALVES && turns[u] ? p.pairs + unit * VEC : unit * 2 * VEC + VEC;
+    }
+    for (int tk = 0; tk < n_tok; ++tk) {
+        const size_t token = t0 + tk, b = token / p.seq, s = token - b * p.seq;
+        float2       cs[NU][VEC];
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                cs[u][j] = turns[u] ? turn[tk * p.pairs + (lane + u * lanes) * VEC + j] : make_float2(1.0f, 0.0f);
+            }
+        }
+        for (int hb = h0; hb < h1; hb += 2 * p.groups) {
+            Piece<T, VEC> a[2][NU], c[2][NU];
+            T*            out[2];
+            const T*      w[2];
+            bool          on[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int  head = hb + group + i * p.groups;
+                const bool is_k = head >= p.heads[0];
+                const int  k    = is_k ? 1 : 0, h = is_k ? head - p.heads[0] : head;
+                on[i]           = group < p.groups && head < h1;
+                const T* in     = reinterpret_cast<const T*>(p.src[k]) + b * p.src_batch[k] + s * p.src_token[k] + (size_t)h * p.src_head[k];
+                out[i]          = reinterpret_cast<T*>(p.dst[k]) + b * p.dst_batch[k] + s * p.dst_token[k] + (size_t)h * p.dst_head[k];
+                w[i]            = reinterpret_cast<const T*>(p.norm[k]);
+#pragma unroll
+                for (int u = 0; u < NU; ++u) {
+                    if (on[i] && there[u]) {
+                        a[i][u].load(in + at_a[u]);
+                        c[i][u].load(in + at_b[u]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float x[NU][2 * VEC];
+                float sq = 0.0f;
+#pragma unroll
+                for (int u = 0; u < NU; ++u) {
+#pragma unroll
+                    for (int j = 0; j < 2 * VEC; ++j) {
+                        x[u][j] = 0.0f;
+                    }
+                    if (on[i] && there[u]) {
+                        a[i][u].get(x[u]);
+                        c[i][u].get(x[u] + VEC);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2 * VEC; ++j) {
+                        sq = fmaf(x[u][j], x[u][j], sq);
+                    }
+                }
+                if (NORM) {
+                    for (int m = lanes >> 1; m > 0; m >>= 1) {
+                        sq += __shfl_xor_sync(0xffffffffu, sq, m);
+                    }
+                    const float inv = rsqrtf(sq / (float)p.head_dim + p.eps);
+                    if (w[i] != nullptr) {
+#pragma unroll
+                        for (int u = 0; u < NU; ++u) {
+                            if (on[i] && there[u]) {
+                                Piece<T, VEC> wa, wc;
+                                float         f[2 * VEC];
+                                wa.load(w[i] + at_a[u]);
+                                wc.load(w[i] + at_b[u]);
+                                wa.get(f);
+                                wc.get(f + VEC);
+#pragma unroll
+                                for (int j = 0; j < 2 * VEC; ++j) {
+                                    x[u][j] *= inv * f[j];
+                                }
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < NU; ++u) {
+                    if (on[i] && there[u]) {
+                        float y[2 * VEC];
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j) {
+                            // a pair beyond the turning part has cosine 1 and sine 0, but its partner may be anything: it is copied
+                            const int   p0 = HALVES ? j : 2 * j, p1 = HALVES ? VEC + j : 2 * j + 1;
+                            const float v0 = x[u][p0], v1 = x[u][p1];
+                            y[p0] = turns[u] ? fmaf(v0, cs[u][j].x, -v1 * cs[u][j].y) : v0;
+                            y[p1] = turns[u] ? fmaf(v0, cs[u][j].y, v1 * cs[u][j].x) : v1;
+                        }
+                        a[i][u].set(y);
+                        c[i][u].set(y + VEC);
+                        a[i][u].store(out[i] + at_a[u]);
+                        c[i][u].store(out[i] + at_b[u]);
+                    }
+                }
+            }
+        }
+    }
+}
+
+static bool even_strides(const void* p, size_t batch, size_t token, size_t head, unsigned vec)
+{
+    return (reinterpret_cast<uintptr_t>(p) & (2 * vec - 1)) == 0 && ((batch | token | head) & (vec - 1)) == 0;
+}
+
+}  // namespace lyraq
+
+using namespace lyraq;
+
+extern "C" int lyraq_rope_axes(const lyraq_rope_axes_t* a, void* stream)
+{
+    if (a == nullptr || (a->pos_dtype != LYRAQ_S32 && a->pos_dtype != LYRAQ_S64 && a->pos_dtype != LYRAQ_F32) || a->q_heads < 0 || a->k_heads < 0 ||
+        a->head_dim <= 0 || a->pairs < 0) {
+        return LYRAQ_ERR_INVALID_ARG;
+    }
+    const int heads = a->q_heads + a->k_heads;
+    if (a->batch * a->seq_len == 0 || heads == 0) {
+        return LYRAQ_OK;
+    }
+    if ((a->dtype != LYRAQ_F16 && a->dtype != LYRAQ_BF16) || a->head_dim > 256 || (a->head_dim & 1) != 0 || 2 * a->pairs > a->head_dim || heads > 65536 || a->q_heads > 65536 || a->k_heads > 65536 ||
+        a->batch > 0x7fffffffu || a->seq_len > 0x7fffffffu || a->batch * a->seq_len > 0x7fffffffu) {
+        return LYRAQ_ERR_UNSUPPORTED;
+    }
+    if ((a->q_heads > 0 && (a->q == nullptr || a->q_out == nullptr)) || (a->k_heads > 0 && (a->k == nullptr || a->k_out == nullptr)) ||
+        (a->pairs > 0 && (a->positions == nullptr || a->turns == nullptr || a->axis == nullptr))) {
+        return LYRAQ_ERR_INVALID_ARG;
+    }
+    const uintptr_t pos_align = a->pos_dtype == LYRAQ_S64 ? 7u : 3u;
+    if ((reinterpret_cast<uintptr_t>(a->positions) & pos_align) != 0 || (reinterpret_cast<uintptr_t>(a->turns) & 7u) != 0) {
+        return LYRAQ_ERR_INVALID_ARG;
+    }
+    if (((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->q_out) | reinterpret_cast<uintptr_t>(a->k) |
+          reinterpret_cast<uintptr_t>(a->k_out) | reinterpret_cast<uintptr_t>(a->q_norm) | reinterpret_cast<uintptr_t>(a->k_norm)) & 1u) != 0) {
+        return LYRAQ_ERR_INVALID_ARG;
+    }
+    const int sms = device_sm_count();
+    if (sms <= 0) {
+        return LYRAQ_ERR_CUDA;
+    }
+    RopeAxesParams p{};
+    p.src[0] = a->q; p.src[1] = a->k; p.dst[0] = a->q_out; p.dst[1] = a->k_out; p.norm[0] = a->q_norm; p.norm[1] = a->k_norm;
+    p.src_batch[0] = a->q_batch; p.src_token[0] = a->q_token; p.src_head[0] = a->q_head;
+    p.src_batch[1] = a->k_batch; p.src_token[1] = a->k_token; p.src_head[1] = a->k_head;
+    p.dst_batch[0] = a->q_out_batch; p.dst_token[0] = a->q_out_token; p.dst_head[0] = a->q_out_head;
+    p.dst_batch[1] = a->k_out_batch; p.dst_token[1] = a->k_out_token; p.dst_head[1] = a->k_out_head;
+    p.pos = a->positions; p.pos_batch = a->pos_batch; p.pos_token = a->pos_token; p.pos_axis = a->pos_axis; p.pos_dtype = a->pos_dtype;
+    p.turns = a->turns; p.axis = a->axis; p.heads[0] = a->q_heads; p.heads[1] = a->k_heads; p.head_dim = a->head_dim; p.pairs = a->pairs;
+    p.tokens = a->batch * a->seq_len; p.seq = a->seq_len; p.eps = a->eps;
+    // the widest pieces that sizes, strides and addresses allow
+    auto fits = [&](int vec) {
+        const int  rest = a->head_dim - 2 * a->pairs;
+        const bool size = a->pairs % vec == 0 && rest % (2 * vec) == 0;
+        const bool q = a->q_heads == 0 || (even_strides(a->q, a->q_batch, a->q_token, a->q_head, vec) &&
+                                           even_strides(a->q_out, a->q_out_batch, a->q_out_token, a->q_out_head, vec) && even_strides(a->q_norm, 0, 0, 0, vec));
+        const bool k = a->k_heads == 0 || (even_strides(a->k, a->k_batch, a->k_token, a->k_head, vec) &&
+                                           even_strides(a->k_out, a->k_out_batch, a->k_out_token, a->k_out_head, vec) && even_strides(a->k_norm, 0, 0, 0, vec));
+        return size && q && k;
+    };
+    const int vec   = fits(8) ? 8 : fits(4) ? 4 : 1;
+    const int units = a->head_dim / (2 * vec);
+    while ((1 << p.lanes_log2) < units && p.lanes_log2 < 5) {
+        ++p.lanes_log2;
+    }
+    // Groups: all heads of a token in as few rounds as 256 threads make of them, the rounds equally full.  Tokens: enough to share the
+    // cosines' cost, few enough to fill the chip; where there are few, a token's heads are dealt to several blocks.
+    const int lanes  = 1 << p.lanes_log2;
+    const int most   = 256 / lanes;
+    p.chunks         = p.tokens >= (size_t)sms * 2 ? 1 : (heads + most - 1) / most;
+    const int share  = (heads + p.chunks - 1) / p.chunks;
+    const int rounds = (share + most - 1) / most;
+    p.groups         = (share + rounds - 1) / rounds;
+    p.tokens_per_block = p.tokens >= (size_t)sms * 32 ? 4 : p.tokens >= (size_t)sms * 16 ? 2 : 1;
+    const unsigned threads = (unsigned)((p.groups * lanes + 31) / 32 * 32);
+    const unsigned grid    = (unsigned)((p.tokens + p.tokens_per_block - 1) / p.tokens_per_block) * (unsigned)p.chunks;
+    if (((p.tokens + p.tokens_per_block - 1) / p.tokens_per_block) * (size_t)p.chunks > 0x7fffffffu) {
+        return LYRAQ_ERR_UNSUPPORTED;
+    }
+    const size_t smem = sizeof(float2) * (size_t)p.tokens_per_block * (size_t)(p.pairs > 0 ? p.pairs : 1);
+    const bool   norm = a->q_norm != nullptr || a->k_norm != nullptr;
+    auto launch = [&](auto* kernel) { return launch_kernel(kernel, grid, threads, smem, (cudaStream_t)stream, 1u, p); };
+    auto pick = [&](auto type, auto halves, auto normed) {
+        using T           = decltype(type);
+        constexpr bool kH = decltype(halves)::value, kN = decltype(normed)::value;
+        return vec == 8   ? launch(rope_axes_kernel<T, 8, 1, kH, kN>)
+               : vec == 4 ? launch(rope_axes_kernel<T, 4, 1, kH, kN>)
+                          : launch(rope_axes_kernel<T, 1, 4, kH, kN>);
+    };
+    auto pick_norm = [&](auto type, auto halves) {
+        return norm ? pick(type, halves, std::integral_constant<bool, true>{}) : pick(type, halves, std::integral_constant<bool, false>{});
+    };
+    auto pick_style = [&](auto type) {
+        return a->interleaved ? pick_norm(type, std::integral_constant<bool, false>{}) : pick_norm(type, std::integral_constant<bool, true>{});
+    };
+    const cudaError_t e = a->dtype == LYRAQ_BF16 ? pick_style(__nv_bfloat16{}) : pick_style(__half{});
+    return cuda_status(e, "cudaLaunchKernelEx(rope_axes_kernel)");
+}

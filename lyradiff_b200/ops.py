@@ -376,6 +376,134 @@ def invoke_fused_gate_and_residual(out, y, gate, residual):
     return out
 
 
+_POSITIONS = {torch.int32: S32, torch.int64: 5, torch.float32: F32}
+
+
+def _overlaps(t):
+    """Whether a view may hold one element of memory twice (dimensions ordered by stride, each must step past what lies inside it)."""
+    span = 1
+    for stride, size in sorted((t.stride(d), t.shape[d]) for d in range(t.dim()) if t.shape[d] > 1):
+        if stride < span:
+            return True
+        span = stride * (size - 1) + span
+    return False
+
+
+def rope_axes(plan, positions, q, k=None, q_norm=None, k_norm=None, eps=1e-6, q_out=None, k_out=None):
+    """Rotary embedding over several position axes (lyraq_rope_axes).  plan: a rope.AxisRope; q [batch, seq, heads, head_dim] and optionally k
+    (its own number of heads), any strides with contiguous heads (views of a packed projection, heads before tokens by transpose);
+    positions [batch, seq, axes] or [seq, axes], int32, int64 or fp32, any strides.  q_norm / k_norm [head_dim]: RMS norm weights.  Returns
+    (q_out, k_out), created when omitted; they may be q and k."""
+    if q.dim() != 4 or (k is not None and k.dim() != 4):
+        raise ValueError("expected [batch, seq, heads, head_dim]")
+    batch, seq, _, d = q.shape
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if k is not None and k_out is None:
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    a = _lib.RopeAxesArgs(dtype=_dt(q), head_dim=d, pairs=plan.pairs, interleaved=1 if plan.interleaved else 0, eps=float(eps), batch=batch, seq_len=seq)
+    for name, t, out, norm in (("q", q, q_out, q_norm), ("k", k, k_out, k_norm)):
+        if t is None:
+            if norm is not None or out is not None:
+                raise ValueError("%s_norm or %s_out without %s" % (name, name, name))
+            continue
+        if t.dtype != q.dtype or t.shape[:2] != q.shape[:2] or t.shape[3] != d or out.shape != t.shape or out.dtype != q.dtype:
+            raise ValueError("%s and its output must be [%d, %d, heads, %d] of %s" % (name, batch, seq, d, q.dtype))
+        if d > 1 and (t.stride(3) != 1 or out.stride(3) != 1):
+            raise ValueError("%s: heads must be contiguous" % name)
+        if not t.is_cuda or not out.is_cuda:
+            raise ValueError("expected CUDA tensors")
+        if _overlaps(out):
+            raise ValueError("%s_out has overlapping elements" % name)
+        setattr(a, name, t.data_ptr())
+        setattr(a, name + "_out", out.data_ptr())
+        setattr(a, name + "_heads", t.shape[2])
+        for i, part in enumerate(("batch", "token", "head")):
+            setattr(a, "%s_%s" % (name, part), t.stride(i) if t.shape[i] > 1 else 0)
+            setattr(a, "%s_out_%s" % (name, part), out.stride(i) if t.shape[i] > 1 else 0)
+        if norm is not None:
+            if norm.dtype != q.dtype or tuple(norm.shape) != (d,):
+                raise ValueError("%s_norm must be [%d] of %s" % (name, d, q.dtype))
+            setattr(a, name + "_norm", _p(norm))
+    if positions.dtype not in _POSITIONS:
+        raise TypeError("positions must be int32, int64 or fp32")
+    if not positions.is_cuda or tuple(positions.shape) not in ((batch, seq, plan.axes), (seq, plan.axes)):
+        raise ValueError("positions must be a CUDA tensor [%d, %d, %d] or [%d, %d]" % (batch, seq, plan.axes, seq, plan.axes))
+    a.positions, a.pos_dtype = positions.data_ptr(), _POSITIONS[positions.dtype]
+    a.pos_batch = positions.stride(0) if positions.dim() == 3 else 0
+    a.pos_token, a.pos_axis = positions.stride(-2), positions.stride(-1)
+    a.turns, a.axis = _p(plan.turns), _p(plan.axis)
+    _same_device(q, k, q_out, k_out, q_norm, k_norm, positions, plan.turns, plan.axis)
+    _lib.check(_lib.lib().lyraq_rope_axes(a, _stream()), "lyraq_rope_axes")
+    return q_out, k_out
+
+
+_NORMS = {"none": 0, "rms": 1, "layer": 2}
+
+
+def _row_strides(t, what, shape, dtype):
+    """(pointer, batch stride, row stride) of a [batch, seq, dim] view whose rows are contiguous."""
+    if not t.is_cuda:
+        raise ValueError("%s: expected a CUDA tensor" % what)
+    if tuple(t.shape) != shape or t.dtype != dtype or (t.stride(2) != 1 and shape[2] > 1):
+        raise ValueError("%s must be %s of %s with contiguous rows" % (what, list(shape), dtype))
+    return t.data_ptr(), t.stride(0) if shape[0] > 1 else 0, t.stride(1) if shape[1] > 1 else 0
+
+
+def gated_residual_norm(y, x, gate=None, scale=None, shift=None, post_weight=None, pre_weight=None, post="rms", pre="rms", residual_scale=1.0,
+                        eps=1e-6, x_out=None, h=None, qf8=None, f8_scale=None, q4=None):
+    """Norms before and after a block fused with its gate and residual (lyraq_gated_residual_norm): for y, x [batch, seq, dim]
+        v = residual_scale * x + gate[b] * (post(y) * post_weight);  x_out = v;  h = pre(v) * pre_weight * (1 + scale[b]) + shift[b]
+    Returns (x_out, h).  gate, scale, shift: [batch, dim] (rows may lie apart, as chunks of one modulation tensor do) or [dim]; post: "none",
+    "rms" or "layer", pre: "rms" or "layer".  x_out is created when omitted, h when no other form of it is asked for.  qf8 (uint8, contiguous,
+    with f8_scale) takes e4m3 codes of h, q4 (an Fp4Tensor of [batch * seq, dim]) its FP4 form.  x_out may be x itself, h may be y."""
+    if y.dim() != 3:
+        raise ValueError("expected [batch, seq, dim]")
+    shape, dt = tuple(y.shape), y.dtype
+    batch, seq, dim = shape
+    if x_out is None:
+        x_out = torch.empty(shape, dtype=dt, device=y.device)
+    if h is None and qf8 is None and q4 is None:
+        h = torch.empty(shape, dtype=dt, device=y.device)
+    if post not in _NORMS or pre not in ("rms", "layer"):
+        raise ValueError("unknown norm %r / %r" % (post, pre))
+    a = _lib.GatedNormArgs(post=_NORMS[post], pre=_NORMS[pre], residual_scale=float(residual_scale), eps=float(eps), dtype=_dt(y), batch=batch,
+                           seq_len=seq, dim=dim)
+    a.y, a.y_batch, a.y_row = _row_strides(y, "y", shape, dt)
+    a.x, a.x_batch, a.x_row = _row_strides(x, "x", shape, dt)
+    a.x_out, a.x_out_batch, a.x_out_row = _row_strides(x_out, "x_out", shape, dt)
+    for i, t in enumerate((x_out, h)):
+        # rows of an output must not share memory with each other
+        if t is not None and ((seq > 1 and t.stride(1) < dim) or (batch > 1 and t.stride(0) < dim)):
+            raise ValueError("%s has overlapping rows" % ("x_out", "h")[i])
+    if h is not None:
+        a.h, a.h_batch, a.h_row = _row_strides(h, "h", shape, dt)
+    for name, t in (("gate", gate), ("scale", scale), ("shift", shift)):
+        if t is None:
+            continue
+        if t.dtype != dt or tuple(t.shape) not in ((batch, dim), (dim,)) or (t.stride(-1) != 1 and dim > 1) or not t.is_cuda:
+            raise ValueError("%s must be [%d, %d] or [%d] of %s" % (name, batch, dim, dim, dt))
+        setattr(a, name, t.data_ptr())
+        setattr(a, name + "_batch", t.stride(0) if t.dim() == 2 and batch > 1 else 0)
+    for name, t in (("post_weight", post_weight), ("pre_weight", pre_weight)):
+        if t is not None:
+            if t.dtype != dt or tuple(t.shape) != (dim,):
+                raise ValueError("%s must be [%d] of %s" % (name, dim, dt))
+            setattr(a, name, _p(t))
+    if qf8 is not None:
+        if f8_scale is None or f8_scale.dtype != torch.float32 or qf8.dtype != torch.uint8 or qf8.numel() != batch * seq * dim:
+            raise ValueError("qf8 must be uint8 of y's size, with an fp32 f8_scale")
+        a.qf8, a.f8_scale = _p(qf8), _p(f8_scale)
+    if q4 is not None:
+        if (q4.rows, q4.k) != (batch * seq, dim):
+            raise ValueError("q4 must be [%d, %d]" % (batch * seq, dim))
+        q4.check()
+        a.q4, a.q4_scales, a.q4_tensor_scale, a.q4_format = _p(q4.codes), _p(q4.scales), _p(q4.tensor_scale), _fp4_format(q4.fmt)
+    _same_device(y, x, x_out, h, gate, scale, shift, post_weight, pre_weight, qf8, f8_scale, *(() if q4 is None else (q4.codes, q4.scales, q4.tensor_scale)))
+    _lib.check(_lib.lib().lyraq_gated_residual_norm(a, _stream()), "lyraq_gated_residual_norm")
+    return x_out, h
+
+
 def invoke_load_lora(weight, lora, alpha):
     """invokeLoadLora<T> (src/lyradiff/kernels/lora/load_lora.h): weight += lora * alpha in place, in the weight's own 16-bit
     arithmetic (both steps rounded)."""

@@ -5,9 +5,81 @@ matrix [[cos, -sin], [sin, cos]] of each frequency; `lyraq_rmsnorm_rope` reads i
 table the reference's Python wrapper builds before calling the ops (`rope` / `EmbedND`,
 lyradiff/lyradiff_model/lyradiff_flux_transformer_model_v2.py:35-65): angles in float64, one block of frequencies per
 position axis, concatenated along the frequency axis.
+
+AxisRope is the plan of `lyraq_rope_axes` (ops.rope_axes), which needs no table: the frequency of every pair as a fraction of a turn, and the
+position axis it follows.
 """
 
+import decimal
+import fractions
+import math
+
 import torch
+
+_PI = "3.14159265358979323846264338327950288419716939937510582097494459230781640628620899"
+
+
+def _turns(freq):
+    """Frequency in radians per position, at least 0 and below a whole turn -> turns per position times 2^64, rounded, its bits as a signed
+    64-bit number."""
+    with decimal.localcontext() as ctx:
+        ctx.prec = 60
+        if not isinstance(freq, decimal.Decimal) and not math.isfinite(freq):
+            raise ValueError("rope: a frequency must be finite, got %s" % freq)
+        f = freq if isinstance(freq, decimal.Decimal) else decimal.Decimal(fractions.Fraction(freq).numerator) / fractions.Fraction(freq).denominator
+        if not 0 <= f < 2 * decimal.Decimal(_PI):
+            raise ValueError("rope: a frequency must be at least 0 and below 2 pi radians per position, got %s" % freq)
+        t = int((f / (2 * decimal.Decimal(_PI)) * 2 ** 64).to_integral_value()) % 2 ** 64
+    return t - 2 ** 64 if t >= 2 ** 63 else t
+
+
+class AxisRope:
+    """Which way each pair of a head turns: `turns` int64 [pairs] (turns per position, times 2^64), `axis` uint8 [pairs].
+
+    AxisRope(axes_dim, theta): one block of pairs per axis, each with its own frequencies theta^(-2 i / dim) (theta: a number, or one per axis), as
+    flux_rope_table lays them out.  AxisRope.sections: one ladder of frequencies over all pairs, cut into one section per axis.
+    AxisRope.from_pairs: any frequency and axis per pair (scaled or learned frequencies, axes dealt in turn).  interleaved: pair i is (x[2 i],
+    x[2 i + 1]), else (x[i], x[i + pairs]).  Elements of a head beyond 2 * pairs are left alone."""
+
+    def __init__(self, axes_dim, theta=10000.0, interleaved=True, device="cuda"):
+        thetas = list(theta) if isinstance(theta, (list, tuple)) else [theta] * len(axes_dim)
+        if len(thetas) != len(axes_dim):
+            raise ValueError("rope: %d axes and %d thetas" % (len(axes_dim), len(thetas)))
+        freq, axis = [], []
+        for a, (dim, th) in enumerate(zip(axes_dim, thetas)):
+            if dim % 2 or dim < 0:
+                raise ValueError("rope: the axis dimension must be even, got %d" % dim)
+            freq += self._ladder(dim, th)
+            axis += [a] * (dim // 2)
+        self._set(freq, axis, len(axes_dim), interleaved, device)
+
+    @staticmethod
+    def _ladder(dim, theta):
+        with decimal.localcontext() as ctx:
+            ctx.prec = 60
+            base = decimal.Decimal(fractions.Fraction(theta).numerator) / fractions.Fraction(theta).denominator
+            if not base > 0:
+                raise ValueError("rope: theta must be positive, got %s" % theta)
+            return [base ** (decimal.Decimal(-2 * i) / dim) for i in range(dim // 2)]
+
+    def _set(self, freq, axis, axes, interleaved, device):
+        if len(freq) != len(axis) or axes > 255 or any(not 0 <= a < axes for a in axis):
+            raise ValueError("rope: one axis below %d for each of %d pairs" % (min(axes, 255), len(freq)))
+        self.pairs, self.axes, self.interleaved = len(freq), axes, bool(interleaved)
+        self.turns = torch.tensor([_turns(f) for f in freq], dtype=torch.int64, device=device)
+        self.axis = torch.tensor(axis, dtype=torch.uint8, device=device)
+
+    @classmethod
+    def sections(cls, sections, theta=10000.0, interleaved=False, device="cuda"):
+        """sections: pairs per axis; pair i of all has frequency theta^(-i / pairs)."""
+        return cls.from_pairs(cls._ladder(2 * sum(sections), theta), [a for a, n in enumerate(sections) for _ in range(n)], len(sections), interleaved, device)
+
+    @classmethod
+    def from_pairs(cls, freq, axis, axes, interleaved=False, device="cuda"):
+        """freq: radians per position of each pair (floats), axis: its position axis, below `axes`."""
+        plan = cls.__new__(cls)
+        plan._set([f if isinstance(f, decimal.Decimal) else float(f) for f in freq], [int(a) for a in axis], axes, interleaved, device)
+        return plan
 
 
 def axis_table(pos, dim, theta):

@@ -217,3 +217,165 @@ def test_scales_of_every_row_and_block_reach_their_values(ops, tile, fmt):
         ops.gemm_fp4(to_device(ops, w, fmt), to_device(ops, x, fmt), y)
         check_status()
         assert_product(y, x, w, fmt)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("m,n,k", [(1, 8, 32), (1, 129, 96), (2, 300, 1312), (7, 136, 2048), (16, 520, 4096), (11, 4224, 576)])
+def test_few_rows(ops, tile, fmt, dtype, m, n, k):
+    tile(16)
+    x, w, b, r = problem(m, n, k, fmt, dtype, m * n + k, True, True)
+    for gelu in (False, True):
+        y = torch.full((m, n), float("nan"), dtype=dtype, device="cuda")
+        ops.gemm_fp4(to_device(ops, w, fmt, 0xFF), to_device(ops, x, fmt, 0xFF), y, cu(b), cu(r), -0.5, gelu)
+        check_status()
+        assert_product(y, x, w, fmt, b, r, -0.5, gelu)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m", [1, 5, 16])
+@pytest.mark.parametrize("n,k", [(264, 4096), (4224, 4096), (4352, 4096), (9088, 2048), (9216, 2048), (18944, 1024), (19072, 1024), (130, 32)])
+def test_few_rows_with_every_split_of_k(ops, fmt, m, n, k):
+    """One, two, four and eight CTAs along k, and both sides of the tile counts at which fewer are taken.  Codes of 0, 1, -1 and 2 under scales of
+    one make every partial sum an integer below 2^24: exact in any order."""
+    g = torch.Generator(device="cuda").manual_seed(n + m)
+    codes = torch.tensor([0, 2, 10, 4], dtype=torch.uint8, device="cuda")
+    values = torch.tensor([0.0, 1.0, -1.0, 2.0], dtype=torch.float64, device="cuda")
+    parts = []
+    for rows in (n, m):
+        i = torch.randint(0, 4, (rows, k), generator=g, device="cuda")
+        t = ops.Fp4Tensor.empty(rows, k, fmt)
+        c = codes[i]
+        t.codes.copy_(c[:, 0::2] | (c[:, 1::2] << 4))
+        t.scales.fill_(0x38 if fmt == "nvfp4" else 127)
+        parts.append((t, values[i]))
+    y = torch.empty(m, n, dtype=torch.float32, device="cuda")
+    ops.gemm_fp4(parts[0][0], parts[1][0], y)
+    check_status()
+    assert torch.equal(y.double(), parts[1][1] @ parts[0][1].t())
+
+
+def test_large_product_is_exact_and_the_same_with_every_tile(ops, tile):
+    """All rounds of a persistent grid, both accumulator buffers, the tile order's last band: integer operands again."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    m, n, k = 2309, 4808, 1120
+    codes = torch.tensor([0, 2, 10, 4], dtype=torch.uint8, device="cuda")
+    values = torch.tensor([0.0, 1.0, -1.0, 2.0], dtype=torch.float64, device="cuda")
+    for fmt in FORMATS:
+        parts = []
+        for rows in (n, m):
+            i = torch.randint(0, 4, (rows, k), generator=g, device="cuda")
+            t = ops.Fp4Tensor.empty(rows, k, fmt)
+            t.codes.copy_(codes[i][:, 0::2] | (codes[i][:, 1::2] << 4))
+            t.scales.zero_()
+            blocks = k // fp4.GROUP[fmt]
+            t.scales[fp4.scale_offsets(rows, blocks).flatten().cuda()] = 0x38 if fmt == "nvfp4" else 127
+            parts.append((t, values[i]))
+        want = parts[1][1] @ parts[0][1].t()
+        for code in (0, 1281, 2562):
+            tile(code)
+            y = torch.full((m, n), float("nan"), dtype=torch.float32, device="cuda")
+            ops.gemm_fp4(parts[0][0], parts[1][0], y)
+            check_status()
+            assert torch.equal(y.double(), want), (fmt, code)
+            h = torch.full((m, n), float("nan"), dtype=torch.bfloat16, device="cuda")
+            ops.gemm_fp4(parts[0][0], parts[1][0], h)
+            assert torch.equal(h, want.bfloat16()), (fmt, code)
+
+
+@pytest.mark.parametrize("stalled", [0, 1])
+def test_few_rows_wait_that_runs_out_stores_nothing(ops, stalled):
+    """One CTA of each cluster loads nothing (a debug switch, no fault): its wait ends with the status, and no CTA of the cluster stores."""
+    from lyradiff_b200 import _lib
+    lib = _lib.lib()
+    x, w, _, _ = problem(4, 512, 2048, "nvfp4", torch.bfloat16, 8)
+    X, W = to_device(ops, x, "nvfp4"), to_device(ops, w, "nvfp4")
+    good, out = (torch.full((4, 512), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    ops.gemm_fp4(W, X, good)
+    check_status()
+    assert lib.lyraq_debug_fp4_skinny_wait_test(stalled, 50) == 0
+    try:
+        ops.gemm_fp4(W, X, out)
+        torch.cuda.synchronize()
+        status, detail = ops.last_status()
+    finally:
+        assert lib.lyraq_debug_fp4_skinny_wait_test(-1, 0) == 0
+    assert status == 4 and 0x6000 <= detail < 0x7000, (status, hex(detail))
+    assert bool((out == 7.0).all())
+    ops.gemm_fp4(W, X, out)
+    check_status()
+    assert torch.equal(out, good)
+
+
+def test_blocks_of_nan_reach_their_outputs_and_no_others(ops):
+    x = torch.randn(40, 256, generator=torch.Generator().manual_seed(1)).bfloat16()
+    x[7, 33] = float("nan")
+    w = torch.randn(24, 256, generator=torch.Generator().manual_seed(2)).bfloat16()
+    w[5, 100] = float("inf")
+    for fmt in FORMATS:
+        for rows in (40, 9):
+            y = torch.zeros(rows, 24, dtype=torch.float32, device="cuda")
+            ops.gemm_fp4(ops.weight_quant_fp4(cu(w), fmt), ops.quant_fp4(cu(x[:rows]), None, fmt), y)
+            check_status()
+            bad = torch.isnan(y).cpu()
+            want = torch.zeros(rows, 24, dtype=torch.bool)
+            want[7], want[:, 5] = True, True
+            assert torch.equal(bad, want)
+
+
+# ----------------------------------------------------------------------------- the layer
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lead", [(1,), (2, 9), (3, 70)])
+def test_layer_is_quantize_then_product(ops, fmt, dtype, lead):
+    from lyradiff_b200 import layers
+    g = torch.Generator().manual_seed(7)
+    w, b = (torch.randn(160, 352, generator=g) * 0.05).to(dtype), torch.randn(160, generator=g).to(dtype)
+    x, r = torch.randn(*lead, 352, generator=g).to(dtype), torch.randn(*lead, 160, generator=g).to(dtype)
+    layer = layers.Fp4Linear(cu(w), cu(b), torch.tensor(0.011), gelu=True, fmt=fmt)
+    if fmt == "nvfp4":
+        assert float(layer.input_scale) == 2.0 ** -6 and layer.weight.tensor_scale is not None
+    got = layer.forward(cu(x), residual=cu(r), beta=0.5)
+    check_status()
+    assert got.shape == (*lead, 160)
+    rows = got.numel() // 160
+    gx, gw = (2.0 ** -6, fp4.tensor_scale(w)) if fmt == "nvfp4" else (1.0, 1.0)
+    assert_product(got.reshape(rows, 160), (*fp4.encode(x.reshape(rows, 352), fmt, gx), gx), (*fp4.encode(w, fmt, gw), gw), fmt, b, r.reshape(rows, 160), 0.5, True)
+    q = layer.empty_input(rows)
+    ops.quant_fp4(cu(x).reshape(rows, 352), out=q)
+    again = layer.forward_quantized(q, dtype, cu(r), 0.5)
+    assert torch.equal(again, got.reshape(rows, 160))
+    with pytest.raises(ValueError):
+        layer.forward(cu(x)[..., :320])
+    with pytest.raises(ValueError):
+        layer.forward(cu(x), residual=cu(r).float())
+
+
+def test_layer_in_two_captured_graphs_and_on_two_streams(ops):
+    """Nothing is shared between calls: graphs captured from one layer replay at the same time and with new inputs."""
+    from lyradiff_b200 import layers
+    g = torch.Generator().manual_seed(8)
+    layer = layers.Fp4Linear(cu((torch.randn(512, 1024, generator=g) * 0.05).bfloat16()), None, torch.tensor([0.01]))
+    xs = [torch.randn(m, 1024, generator=g).bfloat16().cuda() for m in (3, 200)]
+    graphs, outs = [], []
+    side = [torch.cuda.Stream() for _ in xs]
+    for x, s in zip(xs, side):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            layer.forward(x)
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=s):
+            outs.append(layer.forward(x))
+        graphs.append(gr)
+    for x in xs:
+        x.copy_(torch.randn(x.shape, generator=g))
+    want = [layer.forward(x) for x in xs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for gr, s in zip(graphs, side):
+            with torch.cuda.stream(s):
+                gr.replay()
+    torch.cuda.synchronize()
+    check_status()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
