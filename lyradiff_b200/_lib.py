@@ -3,6 +3,7 @@ missing or lacks a symbol the import of the ops fails with a clear error."""
 
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("LYRAQ_LIB_PATH", os.path.join(_HERE, "liblyraq.so"))
@@ -25,6 +26,10 @@ class GatedNormArgs(ctypes.Structure):
                 + [("residual_scale", c_float), ("eps", c_float), ("dtype", c_int)] + [(n, c_size_t) for n in ("batch", "seq_len", "dim")])
 
 
+# the same as one format: a call packs its arguments at once, a tenth of the time of filling the structure field by field
+GATED_NORM = struct.Struct("@2P4Q2P4Q5Pi3P3Q2P2i2fi3Q")
+
+
 class RopeAxesArgs(ctypes.Structure):
     """lyraq_rope_axes_t."""
     _fields_ = ([(n, c_void_p) for n in ("q", "k")] + [(a + n, c_size_t) for a in ("q_", "k_") for n in ("batch", "token", "head")]
@@ -34,6 +39,8 @@ class RopeAxesArgs(ctypes.Structure):
                 + [(n, c_int) for n in ("pos_dtype", "dtype", "q_heads", "k_heads", "head_dim", "pairs", "interleaved")] + [("eps", c_float)]
                 + [(n, c_size_t) for n in ("batch", "seq_len")])
 
+
+ROPE_AXES = struct.Struct("@2P6Q2P6Q3P3Q2P7if2Q")
 
 # name -> (restype, argtypes); mirrors include/lyraq.h declaration by declaration
 SIGNATURES = {
@@ -92,8 +99,8 @@ SIGNATURES = {
     "lyraq_quant_fp8_2d": (c_int, [c_void_p, c_size_t, c_void_p, c_int, c_void_p, c_size_t, c_size_t, c_void_p]),
     "lyraq_load_lora": (c_int, [c_void_p, c_void_p, c_int, c_float, c_size_t, c_void_p]),
     "lyraq_gate_residual": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_size_t, c_size_t, c_size_t, c_void_p]),
-    "lyraq_rope_axes": (c_int, [ctypes.POINTER(RopeAxesArgs), c_void_p]),
-    "lyraq_gated_residual_norm": (c_int, [ctypes.POINTER(GatedNormArgs), c_void_p]),
+    "lyraq_rope_axes": (c_int, [c_void_p, c_void_p]),
+    "lyraq_gated_residual_norm": (c_int, [c_void_p, c_void_p]),
     "lyraq_gemm_w4a4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p,
                                 c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "lyraq_gemm_fp4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p,

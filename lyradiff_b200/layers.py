@@ -6,6 +6,8 @@ calls by the FP8 and INT8 layers and taken per call by W4A4Gemm.  torch supplies
 torch.
 """
 
+import functools
+
 import torch
 
 from . import _lib, ops
@@ -18,6 +20,11 @@ def _workspace(op, m, n, k, device, current):
     if current is None or current.numel() < need or current.device != device:
         current = torch.empty(max(need, 256), dtype=torch.uint8, device=device)
     return current
+
+
+@functools.lru_cache(maxsize=4096)
+def _fp4_workspace(m, k):
+    return _lib.lib().lyraq_workspace_bytes(OP_LINEAR_FP4, m, 1, k)
 
 
 class Fp8Linear:
@@ -60,6 +67,7 @@ class Fp4Linear:
         n, k = weight.shape
         dev = weight.device
         self.n, self.k, self.gelu, self.fmt = n, k, gelu, fmt
+        self.format, self.epilogue = ops._fp4_format(fmt), ops.EPI_GELU_TANH if gelu else ops.EPI_NONE
         self.weight = ops.weight_quant_fp4(weight.contiguous(), fmt)
         self.bias = None if bias is None else bias.contiguous()
         if input_scale is None or fmt != "nvfp4":
@@ -71,34 +79,33 @@ class Fp4Linear:
                 raise ValueError("input_scale must be positive and finite")
             self.input_scale = torch.ldexp(torch.ones_like(s), torch.where(m == 0.5, e - 1, e)).to(device=dev, dtype=torch.float32)
 
-    def _out(self, shape, dtype, device, out):
-        m = 1
-        for d in shape:
-            m *= d
-        if out is None:
-            return m, torch.empty(m, self.n, dtype=dtype, device=device)
+    def forward(self, x, residual=None, beta=1.0, out=None):
+        shape, k, n = x.shape, self.k, self.n
+        if shape[-1] != k:
+            raise ValueError("expected [..., %d], got %s" % (k, tuple(shape)))
+        m = x.numel() // k
+        here, stream = ops._here()
+        if x.get_device() != here:
+            raise ValueError("x is on %s, but the current device is cuda:%d" % (x.device, here))
+        ldx = k
+        if not x.is_contiguous():
+            x = x.reshape(m, k)
+            ldx = ops._rows_of(x)
+        y = torch.empty(*shape[:-1], n, dtype=x.dtype, device=x.device) if out is None else self._into(out, x.dtype, m)
+        ops.check_epilogue(x.dtype, self.bias, residual, m, n)
+        need = _fp4_workspace(m, k)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        w, at = self.weight, ops._at
+        st = _lib.lib().lyraq_linear_fp4_forward(
+            at(y, here, "out"), x.data_ptr(), ops._dt(x), ldx, at(self.input_scale, here), at(w.codes, here), at(w.scales, here), at(w.tensor_scale, here),
+            self.format, at(self.bias, here), at(residual, here, "residual"), beta, self.epilogue, m, n, k, ws.data_ptr(), need, stream)
+        _lib.check(st, "lyraq_linear_fp4_forward")
+        return y if out is None else y.view(*shape[:-1], n)
+
+    def _into(self, out, dtype, m):
         if out.dtype != dtype or out.numel() != m * self.n or out.shape[-1] != self.n:
             raise ValueError("out must be [..., %d] of x's dtype" % self.n)
-        return m, out.view(m, self.n)
-
-    def forward(self, x, residual=None, beta=1.0, out=None):
-        lead = x.shape[:-1]
-        if x.shape[-1] != self.k:
-            raise ValueError("expected [..., %d], got %s" % (self.k, tuple(x.shape)))
-        m, y = self._out(lead, x.dtype, x.device, out)
-        x2 = x.reshape(m, self.k)
-        ldx = ops._rows_of(x2)
-        ops._check_epilogue(y, self.bias, residual, m, self.n)
-        ops._same_device(x, y, residual, self.weight.codes)
-        need = _lib.lib().lyraq_workspace_bytes(OP_LINEAR_FP4, m, self.n, self.k)
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-        w = self.weight
-        st = _lib.lib().lyraq_linear_fp4_forward(
-            ops._p(y), x2.data_ptr(), ops._dt(x2), ldx, ops._p(self.input_scale), ops._p(w.codes), ops._p(w.scales), ops._p(w.tensor_scale),
-            ops.FP4_FORMATS[self.fmt], ops._p(self.bias), ops._p(residual), float(beta), ops.EPI_GELU_TANH if self.gelu else ops.EPI_NONE,
-            m, self.n, self.k, ops._p(ws), need, ops._stream())
-        _lib.check(st, "lyraq_linear_fp4_forward")
-        return y.reshape(*lead, self.n)
+        return out
 
     def empty_input(self, rows):
         """An Fp4Tensor for `rows` rows of this layer's input, for producers that write FP4 themselves (ops.gated_residual_norm)."""
@@ -108,7 +115,7 @@ class Fp4Linear:
         """The product alone, for an input that is FP4 already (empty_input): [rows, n] of `dtype`."""
         if x.tensor_scale is not self.input_scale:
             raise ValueError("the input was not quantized for this layer (empty_input)")
-        y = self._out((x.rows,), dtype, x.codes.device, out)[1]
+        y = torch.empty(x.rows, self.n, dtype=dtype, device=x.codes.device) if out is None else self._into(out, dtype, x.rows).view(x.rows, self.n)
         return ops.gemm_fp4(self.weight, x, y, self.bias, residual, beta, self.gelu)
 
 

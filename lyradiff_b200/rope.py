@@ -11,25 +11,21 @@ position axis it follows.
 """
 
 import decimal
-import fractions
-import math
 
 import torch
 
-_PI = "3.14159265358979323846264338327950288419716939937510582097494459230781640628620899"
+_EXACT = decimal.Context(prec=60)
+_TWO_PI = _EXACT.multiply(2, decimal.Decimal("3.14159265358979323846264338327950288419716939937510582097494459230781640628620899"))
+_TURN = _EXACT.divide(decimal.Decimal(2 ** 64), _TWO_PI)
 
 
 def _turns(freq):
     """Frequency in radians per position, at least 0 and below a whole turn -> turns per position times 2^64, rounded, its bits as a signed
     64-bit number."""
-    with decimal.localcontext() as ctx:
-        ctx.prec = 60
-        if not isinstance(freq, decimal.Decimal) and not math.isfinite(freq):
-            raise ValueError("rope: a frequency must be finite, got %s" % freq)
-        f = freq if isinstance(freq, decimal.Decimal) else decimal.Decimal(fractions.Fraction(freq).numerator) / fractions.Fraction(freq).denominator
-        if not 0 <= f < 2 * decimal.Decimal(_PI):
-            raise ValueError("rope: a frequency must be at least 0 and below 2 pi radians per position, got %s" % freq)
-        t = int((f / (2 * decimal.Decimal(_PI)) * 2 ** 64).to_integral_value()) % 2 ** 64
+    f = freq if isinstance(freq, decimal.Decimal) else decimal.Decimal(freq)      # a float's value, exactly
+    if not (f.is_finite() and 0 <= f < _TWO_PI):
+        raise ValueError("rope: a frequency must be at least 0 and below 2 pi radians per position, got %s" % freq)
+    t = min(int(_EXACT.multiply(f, _TURN).to_integral_value()), 2 ** 64 - 1)
     return t - 2 ** 64 if t >= 2 ** 63 else t
 
 
@@ -55,12 +51,15 @@ class AxisRope:
 
     @staticmethod
     def _ladder(dim, theta):
-        with decimal.localcontext() as ctx:
-            ctx.prec = 60
-            base = decimal.Decimal(fractions.Fraction(theta).numerator) / fractions.Fraction(theta).denominator
-            if not base > 0:
-                raise ValueError("rope: theta must be positive, got %s" % theta)
-            return [base ** (decimal.Decimal(-2 * i) / dim) for i in range(dim // 2)]
+        base = decimal.Decimal(theta)
+        if not (base.is_finite() and base > 0):
+            raise ValueError("rope: theta must be positive, got %s" % theta)
+        step = _EXACT.power(base, _EXACT.divide(decimal.Decimal(-2), dim)) if dim else 0
+        f, ladder = decimal.Decimal(1), []
+        for _ in range(dim // 2):
+            ladder.append(f)
+            f = _EXACT.multiply(f, step)
+        return ladder
 
     def _set(self, freq, axis, axes, interleaved, device):
         if len(freq) != len(axis) or axes > 255 or any(not 0 <= a < axes for a in axis):

@@ -1,5 +1,6 @@
 """CPU checks of the rotary plan and of what the C entry points of the norm and the rotary embedding refuse."""
 
+import ctypes
 import math
 
 import pytest
@@ -58,7 +59,7 @@ def test_c_entry_points_refuse_without_a_device(lib):
 
     def norm(**k):
         a = _lib.GatedNormArgs(**{**dict(y=p, x=p, x_out=p, h=p, dtype=1, post=1, pre=2, batch=1, seq_len=4, dim=64, y_row=64, x_row=64, x_out_row=64, h_row=64), **k})
-        return lib.lyraq_gated_residual_norm(a, None)
+        return lib.lyraq_gated_residual_norm(ctypes.byref(a), None)
     assert lib.lyraq_gated_residual_norm(None, None) == INVALID
     assert norm(seq_len=0) == ok and norm(dim=60) == UNSUPPORTED and norm(dim=16392) == UNSUPPORTED and norm(dtype=2) == UNSUPPORTED
     assert norm(y=None) == INVALID and norm(x=p + 2) == INVALID and norm(pre=0) == INVALID and norm(post=3) == INVALID and norm(x_row=60) == INVALID
@@ -68,9 +69,17 @@ def test_c_entry_points_refuse_without_a_device(lib):
 
     def turn(**k):
         a = _lib.RopeAxesArgs(**{**dict(q=p, q_out=p, positions=p, turns=p, axis=p, pos_dtype=3, dtype=1, q_heads=2, head_dim=64, pairs=32, batch=1, seq_len=3), **k})
-        return lib.lyraq_rope_axes(a, None)
+        return lib.lyraq_rope_axes(ctypes.byref(a), None)
     assert lib.lyraq_rope_axes(None, None) == INVALID
     assert turn(seq_len=0) == ok and turn(q_heads=0) == ok and turn(dtype=2) == UNSUPPORTED and turn(pos_dtype=1) == INVALID and turn(q=None) == INVALID
     assert turn(k_heads=1) == INVALID and turn(head_dim=258, pairs=4) == UNSUPPORTED and turn(head_dim=63, pairs=4) == UNSUPPORTED and turn(pairs=33) == UNSUPPORTED
     assert turn(turns=None) == INVALID and turn(positions=p + 2) == INVALID and turn(q=p + 1) == INVALID and turn(q_heads=-1) == INVALID
     assert turn(pos_dtype=5, positions=p + 4) == INVALID
+
+
+def test_packed_arguments_are_the_structures():
+    for fmt, cls in ((_lib.GATED_NORM, _lib.GatedNormArgs), (_lib.ROPE_AXES, _lib.RopeAxesArgs)):
+        assert fmt.size == ctypes.sizeof(cls)
+        values = [float(i) if cls._fields_[i][1] is ctypes.c_float else i + 1 for i in range(len(cls._fields_))]
+        back = cls.from_buffer_copy(fmt.pack(*values))
+        assert [getattr(back, n) for n, _ in cls._fields_] == values
