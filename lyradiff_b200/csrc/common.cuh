@@ -228,6 +228,17 @@ template<> __device__ __forceinline__ void unpack8<__nv_bfloat16>(const Vec16& v
     }
 }
 
+// The same as four packed pairs.
+template<typename T> __device__ __forceinline__ void unpack4x2(const Vec16& v, float2* out)
+{
+    float f[8];
+    unpack8<T>(v, f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        out[i] = make_float2(f[2 * i], f[2 * i + 1]);
+    }
+}
+
 template<typename T> __device__ __forceinline__ Vec16 pack8(const float* in);
 template<> __device__ __forceinline__ Vec16 pack8<__half>(const float* in)
 {

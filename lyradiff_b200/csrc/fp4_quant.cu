@@ -12,21 +12,21 @@ int device_sm_count();  // gemm_dense.cu
 template<typename T, int FORMAT>
 __global__ void __launch_bounds__(256)
 fp4_quant_kernel(uint8_t* q, uint8_t* sf, const T* x, size_t ldx, const float* tensor_scale, size_t rows, size_t k, unsigned chunks,
-                 unsigned octets, size_t tasks)
+                 unsigned octets, unsigned tasks)
 {
     constexpr int kGroup  = fp4_group(FORMAT);
     constexpr int kBlocks = 32 / kGroup;            // of one thread
     constexpr int kPer    = 16 / (int)sizeof(T);    // values of a 16-byte vector
     constexpr int kVecs   = 32 / kPer;
     grid_launch_dependents();
-    const size_t   task  = (size_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    const unsigned task  = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);   // 32 bits: a 64-bit division costs more than a block of values
     const unsigned lane  = threadIdx.x & 31;
-    const size_t   rest  = task / chunks;
-    const unsigned chunk = (unsigned)(task - rest * chunks);
-    const size_t   rb    = rest / octets;
-    const unsigned octet = (unsigned)(rest - rb * octets);
+    const unsigned rest  = task / chunks;
+    const unsigned chunk = task - rest * chunks;
+    const unsigned rb    = rest / octets;
+    const unsigned octet = rest - rb * octets;
     const unsigned i     = lane >> 2, j = lane & 3;
-    const size_t   row   = rb * 128 + 2 * octet + (i >> 2) + 32 * (i & 3);
+    const size_t   row   = (size_t)rb * 128 + 2 * octet + (i >> 2) + 32 * (i & 3);
     const size_t   col   = (size_t)chunk * 128 + (size_t)j * 32;
     const bool     in    = task < tasks && row < rows && col < k;   // k is a multiple of 32: a thread's values are there or not
     grid_dependency_wait();
@@ -167,13 +167,13 @@ static int run_quant(uint8_t* q, uint8_t* sf, const void* x, int dtype, size_t l
     const size_t octets  = rows >= 32 ? 16 : (rows + 1) / 2;     // fewer than 32 rows lie in the first quarter of their 128
     const size_t tasks   = (rows + 127) / 128 * octets * chunks;  // one warp each
     const size_t blocks  = (tasks + 7) / 8;
-    if (blocks > 0x7fffffffu) {
+    if (blocks > 0x0fffffffu) {   // the number of a warp stays within 32 bits
         return LYRAQ_ERR_UNSUPPORTED;
     }
     auto launch = [&](auto* kernel, auto type) {
         using T = decltype(type);
         return launch_kernel(kernel, (unsigned)blocks, 256u, (size_t)0, s, 1u, q, sf, (const T*)x, ldx, tensor_scale, rows, k, (unsigned)chunks,
-                             (unsigned)octets, tasks);
+                             (unsigned)octets, (unsigned)tasks);
     };
     auto pick = [&](auto type) {
         using T = decltype(type);

@@ -40,7 +40,7 @@ constexpr int kThreads   = 384;
 constexpr int kEpiWarp0  = 4;
 constexpr int kEpiWarps  = 8;
 constexpr int kBox       = 32 * 64;      // one warp's staging box: 32 rows x 32 columns of a 16-bit type
-constexpr int kBiasBytes = 128 * 4;      // one warp's bias: up to 128 columns in fp32
+constexpr int kBiasBytes = 128 * 2;      // one warp's bias: up to 128 columns of a 16-bit type (fp32, which uses no box, keeps its there)
 constexpr int kBarBytes  = 256;
 constexpr int kOtherRegs = 72;
 constexpr int kEpiRegs   = 216;
@@ -81,9 +81,11 @@ __device__ __forceinline__ void tile_coords(int tile, int m_tiles, int n_tiles, 
     n_blk               = in_group / rows;
 }
 
-// 32 columns of one row: accumulators -> fp32 results, in the order beta R, bias, GELU.  bias: the columns' own in shared memory.
+// 32 columns of one row: accumulators -> fp32 results, in the order beta R, bias, GELU.  bias: the columns' own in shared memory;
+// staged: the row's residual in the warp's box, or null (then it is fetched here).
 template<typename T, bool RES>
-__device__ __forceinline__ void finish32(const Fp4GemmParams& p, const uint32_t* acc, const float* bias, float scale, int row, int col0, int valid, bool vec_ok, float* v)
+__device__ __forceinline__ void finish32(const Fp4GemmParams& p, const uint32_t* acc, const uint8_t* bias, const uint8_t* staged, int swizzle, float scale, int row,
+                                         int col0, int valid, bool vec_ok, float* v)
 {
     constexpr int kPer = 16 / (int)sizeof(T);
     const float2  s2 = make_float2(scale, scale);
@@ -93,7 +95,22 @@ __device__ __forceinline__ void finish32(const Fp4GemmParams& p, const uint32_t*
         v[2 * i]       = t.x;
         v[2 * i + 1]   = t.y;
     }
-    if (RES && p.residual != nullptr && row < p.M) {
+    if (RES && staged != nullptr) {
+        if constexpr (sizeof(T) == 2) {
+            const float2 b2 = make_float2(p.beta, p.beta);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float2 f[4];
+                unpack4x2<T>(*reinterpret_cast<const Vec16*>(staged + ((q ^ swizzle) << 4)), f);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 a = fma_f32x2(b2, f[j], make_float2(v[8 * q + 2 * j], v[8 * q + 2 * j + 1]));
+                    v[8 * q + 2 * j]     = a.x;
+                    v[8 * q + 2 * j + 1] = a.y;
+                }
+            }
+        }
+    } else if (RES && p.residual != nullptr && row < p.M) {
         const T* r = reinterpret_cast<const T*>(p.residual) + (size_t)row * (size_t)p.N + (size_t)col0;
         if (vec_ok && valid >= 32) {
 #pragma unroll
@@ -122,13 +139,25 @@ __device__ __forceinline__ void finish32(const Fp4GemmParams& p, const uint32_t*
             }
         }
     }
-    if (p.bias != nullptr) {
+    if (p.bias != nullptr) {   // every lane reads the same 16 bytes
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {   // every lane reads the same 16 bytes
-            const float4 b = *reinterpret_cast<const float4*>(bias + 4 * q);
-            const float2 a0 = add_f32x2(make_float2(v[4 * q], v[4 * q + 1]), make_float2(b.x, b.y));
-            const float2 a1 = add_f32x2(make_float2(v[4 * q + 2], v[4 * q + 3]), make_float2(b.z, b.w));
-            v[4 * q] = a0.x; v[4 * q + 1] = a0.y; v[4 * q + 2] = a1.x; v[4 * q + 3] = a1.y;
+        for (int q = 0; q < 32 / kPer; ++q) {
+            const Vec16 x = *reinterpret_cast<const Vec16*>(bias + 16 * q);
+            float       f[8];
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    f[j] = __uint_as_float(x.w[j]);
+                }
+            } else {
+                unpack8<T>(x, f);
+            }
+#pragma unroll
+            for (int j = 0; j < kPer; j += 2) {
+                const float2 a = add_f32x2(make_float2(v[q * kPer + j], v[q * kPer + j + 1]), make_float2(f[j], f[j + 1]));
+                v[q * kPer + j]     = a.x;
+                v[q * kPer + j + 1] = a.y;
+            }
         }
     }
     if (p.gelu) {
@@ -197,7 +226,6 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     const int      unit    = (CTAS == 2) ? (int)(blockIdx.x >> 1) : (int)blockIdx.x;
     const int      n_units = (CTAS == 2) ? (int)(gridDim.x >> 1) : (int)gridDim.x;
 
-    grid_launch_dependents();
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(full_bar(s), 1);
@@ -383,8 +411,8 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         const int      half      = (warp - kEpiWarp0) >> 2;  // which half of the tile's columns
         const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
         uint8_t*       box       = gen_base + S::kEpiOffset + (warp - kEpiWarp0) * kBox;
-        const uint32_t box_addr  = smem_base + S::kEpiOffset + (warp - kEpiWarp0) * kBox;
-        float*         bias      = reinterpret_cast<float*>(gen_base + S::kEpiOffset + kEpiWarps * kBox + (warp - kEpiWarp0) * kBiasBytes);
+        const uint32_t box_at    = smem_base + S::kEpiOffset + (warp - kEpiWarp0) * kBox;
+        uint8_t*       bias      = p.c_dtype == LYRAQ_F32 ? box : gen_base + S::kEpiOffset + kEpiWarps * kBox + (warp - kEpiWarp0) * kBiasBytes;
         const float    scale     = fp4_tensor_scale(p);
         const bool     vec_ok    = p.c_dtype == LYRAQ_F32 ? (p.N & 3) == 0 : (p.N & 7) == 0;
         int            local     = 0;
@@ -398,42 +426,35 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             const int ncol0 = n_blk * BLOCK_N + half * kHalfN;
             if (p.bias != nullptr) {
                 // staged while the main loop of the tile still runs; the warp's own piece, so no other warp is waited for
-                float b[kHalfN / 32];
+                uint32_t b[kHalfN / 32];
 #pragma unroll
                 for (int i = 0; i < kHalfN / 32; ++i) {
                     const int col = ncol0 + lane + 32 * i;
-                    b[i]          = 0.0f;
+                    b[i]          = 0;
                     if (col < p.N) {
-                        b[i] = p.c_dtype == LYRAQ_F32    ? reinterpret_cast<const float*>(p.bias)[col]
-                               : p.c_dtype == LYRAQ_BF16 ? to_f32(reinterpret_cast<const __nv_bfloat16*>(p.bias)[col])
-                                                         : to_f32(reinterpret_cast<const __half*>(p.bias)[col]);
+                        b[i] = p.c_dtype == LYRAQ_F32 ? reinterpret_cast<const uint32_t*>(p.bias)[col] : (uint32_t)reinterpret_cast<const uint16_t*>(p.bias)[col];
                     }
                 }
                 __syncwarp();
 #pragma unroll
                 for (int i = 0; i < kHalfN / 32; ++i) {
-                    bias[lane + 32 * i] = b[i];
+                    if (p.c_dtype == LYRAQ_F32) {
+                        reinterpret_cast<uint32_t*>(bias)[lane + 32 * i] = b[i];
+                    } else {
+                        reinterpret_cast<uint16_t*>(bias)[lane + 32 * i] = (uint16_t)b[i];
+                    }
                 }
                 __syncwarp();
             }
             if (RES && p.residual != nullptr && row < p.M) {
                 // the row's share of the residual is asked into L2 while the main loop of the tile still runs
-                const int      esz = p.c_dtype == LYRAQ_F32 ? 4 : 2;
-                const uint8_t* seg = reinterpret_cast<const uint8_t*>(p.residual) + ((size_t)row * (size_t)p.N + (size_t)ncol0) * esz;
-                for (int b = 0; b < kHalfN * esz; b += 128) {
-                    if (ncol0 + b / esz < p.N) {
-                        prefetch_l2(seg + b);
-                    }
+                const int      esz   = p.c_dtype == LYRAQ_F32 ? 4 : 2;
+                const uint8_t* seg   = reinterpret_cast<const uint8_t*>(p.residual) + ((size_t)row * (size_t)p.N + (size_t)ncol0) * esz;
+                const int      bytes = min(kHalfN, p.N - ncol0) * esz;
+                if (vec_ok && bytes > 0) {   // whole 16-byte pieces on 16-byte addresses
+                    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(seg), "r"(bytes) : "memory");
                 }
             }
-            if (!mbar_wait_warp(tmem_full_bar(buf), acc_phase, abort_flag)) {
-                if (lane == 0) {
-                    report_timeout(p.status, 0x5400u | (unsigned)buf);
-                }
-                *abort_flag = 1;
-                break;
-            }
-            tc_fence_after_sync();
             const uint32_t t_addr = tmem_base + lane_addr + (uint32_t)(buf * BLOCK_N + half * kHalfN);
             auto release = [&]() {   // this warp's share of the accumulator is in registers: the next tile may have its columns
                 tc_fence_before_sync();
@@ -447,8 +468,36 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                 }
             };
             constexpr int kChunks = kHalfN / 32;
+            // Residual of a 16-bit output: a lane that fetched its own row would touch 32 lines an instruction and use half a sector of each
+            // ([4608, 12288, 3072]: 191 us against 72 without a residual).  Instead four lanes fetch the 64 bytes of a row, eight rows an instruction, two chunks
+            // ahead, and hand them over through the box that the result leaves by.
+            const bool staged = RES && p.residual != nullptr && p.tma_store;
+            Vec16      rr[2][RES ? 4 : 1];
+            auto fetch = [&](int c, Vec16* dst) {
+                const int col = ncol0 + c * 32 + (lane & 3) * 8;
+#pragma unroll
+                for (int i = 0; i < (RES ? 4 : 1); ++i) {
+                    const int rw = row0 + i * 8 + (lane >> 2);
+                    dst[i]       = Vec16{};
+                    if (rw < p.M && col < p.N) {   // N is a multiple of 8
+                        dst[i] = ld_16(reinterpret_cast<const uint16_t*>(p.residual) + (size_t)rw * (size_t)p.N + (size_t)col);
+                    }
+                }
+            };
+            if (staged) {
+                fetch(0, rr[0]);
+                fetch(1, rr[1]);
+            }
             constexpr int kAhead  = S::kAccBufs == 1 ? kChunks : 2;   // chunks in registers: all of a lone accumulator
             uint32_t acc[kAhead][32];
+            if (!mbar_wait_warp(tmem_full_bar(buf), acc_phase, abort_flag)) {
+                if (lane == 0) {
+                    report_timeout(p.status, 0x5400u | (unsigned)buf);
+                }
+                *abort_flag = 1;
+                break;
+            }
+            tc_fence_after_sync();
             if (S::kAccBufs == 1) {
 #pragma unroll
                 for (int c = 0; c < kChunks; ++c) {
@@ -474,19 +523,38 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                 if (valid <= 0) {
                     continue;
                 }
-                float v[32];
+                float     v[32];
+                uint8_t*  brow = box + lane * 64;
+                const int sw   = (lane >> 1) & 3;
+                if (p.tma_store) {
+                    if (lane == 0) {
+                        tma_store_wait_read();  // the store before has drained the box
+                    }
+                    __syncwarp();
+                }
+                if (staged) {
+#pragma unroll
+                    for (int i = 0; i < (RES ? 4 : 1); ++i) {
+                        const int r = i * 8 + (lane >> 2);
+                        *reinterpret_cast<Vec16*>(box + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4)) = rr[c & 1][i];
+                    }
+                    __syncwarp();
+                    if (c + 2 < kChunks) {
+                        fetch(c + 2, rr[c & 1]);
+                    }
+                }
                 if (p.c_dtype == LYRAQ_F32) {
                     if (row < p.M) {
-                        finish32<float, RES>(p, acc[c % kAhead], bias + c * 32, scale, row, col0, valid, vec_ok, v);
+                        finish32<float, RES>(p, acc[c % kAhead], bias + c * 128, nullptr, 0, scale, row, col0, valid, vec_ok, v);
                         store32<float>(reinterpret_cast<float*>(p.C) + (size_t)row * (size_t)p.N + (size_t)col0, valid, vec_ok, v);
                     }
                     continue;
                 }
                 const bool bf16 = p.c_dtype == LYRAQ_BF16;
                 if (bf16) {
-                    finish32<__nv_bfloat16, RES>(p, acc[c % kAhead], bias + c * 32, scale, row, col0, valid, vec_ok, v);
+                    finish32<__nv_bfloat16, RES>(p, acc[c % kAhead], bias + c * 64, RES && staged ? brow : nullptr, sw, scale, row, col0, valid, vec_ok, v);
                 } else {
-                    finish32<__half, RES>(p, acc[c % kAhead], bias + c * 32, scale, row, col0, valid, vec_ok, v);
+                    finish32<__half, RES>(p, acc[c % kAhead], bias + c * 64, RES && staged ? brow : nullptr, sw, scale, row, col0, valid, vec_ok, v);
                 }
                 if (!p.tma_store) {
                     if (row < p.M) {
@@ -500,12 +568,6 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                     continue;
                 }
                 // 32 rows x 64 bytes through this warp's box in the 64-byte swizzle, one TMA store; rows and columns beyond the matrix are clipped
-                if (lane == 0) {
-                    tma_store_wait_read();  // the previous store has drained the box
-                }
-                __syncwarp();
-                uint8_t*  brow = box + lane * 64;
-                const int sw   = (lane >> 1) & 3;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     *reinterpret_cast<Vec16*>(brow + ((q ^ sw) << 4)) = bf16 ? pack8<__nv_bfloat16>(v + 8 * q) : pack8<__half>(v + 8 * q);
@@ -513,7 +575,7 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0 && row0 < p.M) {
-                    tma_store_2d(&tmap_c, box_addr, col0, row0);
+                    tma_store_2d(&tmap_c, box_at, col0, row0);
                     tma_store_commit();
                 }
             }
@@ -530,6 +592,9 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     } else {
         __syncthreads();
     }
+    // The kernel behind may begin only now: quantizers that were let in at the start and waited beside the GEMM made a chain of
+    // linears 10 to 25 % slower ([1317, 3072, 12288] 40 us a linear against 31, [4608, 12288, 3072] 86 against 81).
+    grid_launch_dependents();
     if (warp == 2) {
         tc_fence_after_sync();
         if (CTAS == 2) {
@@ -590,7 +655,6 @@ static int run(const uint8_t* X, const uint8_t* xs, const uint8_t* W, const uint
 {
     const long m128 = ((long)p.M + 127) / 128, n128 = ((long)p.N + 127) / 128, m256 = ((long)p.M + 255) / 256, n256 = ((long)p.N + 255) / 256;
     const long pairs = sms / 2;
-    const long c1 = (m128 * n128 + sms - 1) / sms, c2 = 2 * ((m256 * n256 + pairs - 1) / pairs);
     // The few-row kernel's time grows with the rows (their partial sums cross shared memory and leave row by row), the other's does not; what it
     // gains grows with K.  Dense against few-row, us: 4 rows of [256, 256] 2.8 / 3.1, of [1280, 1280] 4.3 / 4.1, 8 rows of it 4.3 / 5.2; 16
     // rows of [1280, 2048] 5.1 / 4.7, of [3072, 3072] 6.4 / 5.6, of [3072, 12288] 17.4 / 8.2; one row of [9216, 3072] 8.3 / 5.4.
@@ -598,7 +662,11 @@ static int run(const uint8_t* X, const uint8_t* xs, const uint8_t* W, const uint
     if (p.M <= kFp4SkinnyRows && (g_forced_tile == 16 || (g_forced_tile == 0 && (num_kb >= 8 || p.M <= 2 + num_kb / 2)))) {
         return launch_skinny(X, xs, W, ws, format, p, sms, stream);
     }
-    const int  tile = g_forced_tile > 16 ? g_forced_tile : c2 <= c1 ? 2562 : 1281;
+    // Rounds of each tile times what one takes, us: 0.2 + 0.323 a K block for 128 x 128, 1.3 + 0.39 for a pair's 256 x 256, from [4608, 12288, 3072]
+    // (98 / 72), [4608, 3072, 12288] (94 / 60), [4608, 3072, 3072] (29 / 19), [1155, 9216, 3072] (24 / 18), [512, 3072, 3072] (7.8 / 9.7).
+    const double c1   = (double)((m128 * n128 + sms - 1) / sms) * (0.2 + 0.323 * num_kb);
+    const double c2   = pairs > 0 ? (double)((m256 * n256 + pairs - 1) / pairs) * (1.3 + 0.39 * num_kb) : 1e30;
+    const int    tile = g_forced_tile > 16 ? g_forced_tile : c2 <= c1 ? 2562 : 1281;
     auto pick = [&](auto fmt, auto res) {
         constexpr int  kFmt = decltype(fmt)::value;
         constexpr bool kRes = decltype(res)::value;

@@ -35,7 +35,8 @@ struct NormParams {
     const float* q4_scale;
     size_t       y_batch, y_row, x_batch, x_row, xo_batch, xo_row, h_batch, h_row;   // strides in elements
     size_t       gate_batch, scale_batch, shift_batch;
-    size_t       rows, seq, atoms;
+    size_t       atoms;
+    unsigned     rows, seq;      // batch * seq_len and seq_len
     int          dim, post, pre;
     float        r, eps;
 };
@@ -53,13 +54,14 @@ norm_residual_kernel(const NormParams p)
     grid_launch_dependents();
     grid_dependency_wait();
 
-    const size_t row = WARP ? (size_t)blockIdx.x * 8 + (threadIdx.x >> 5) : (size_t)blockIdx.x;
+    const unsigned row = WARP ? blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
     if (row >= p.rows) {
         return;   // whole warps, and never part of a block that meets at a barrier
     }
-    const size_t b = row / p.seq, s = row - b * p.seq;
+    const unsigned b = row / p.seq, s = row - b * p.seq;
     // slot: which exchange of the row this is; every exchange has its own words, so one barrier each is enough
-    auto total = [&](float v, int slot) {
+    auto total = [&](float2 v2, int slot) {
+        float v = v2.x + v2.y;
 #pragma unroll
         for (int m = 16; m > 0; m >>= 1) {
             v += __shfl_xor_sync(0xffffffffu, v, m);
@@ -82,91 +84,98 @@ norm_residual_kernel(const NormParams p)
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
         const int vi = t + i * threads;
+        yv[i] = Vec16{};
+        xv[i] = Vec16{};
         if (vi < nvec) {
-            yv[i] = ld_16(yr + (size_t)vi * 8);
-            xv[i] = ld_16(xr + (size_t)vi * 8);
-        } else {
-            yv[i] = Vec16{};
-            xv[i] = Vec16{};
+            yv[i] = ld_16(yr + vi * 8);
+            xv[i] = ld_16(xr + vi * 8);
         }
     }
 
-    float v[VPT][8];
+    // u = (y - mean) * inv as one fma: y * inv + (-mean * inv).  Vectors beyond the row are zeros that no sum takes in.
+    float2 v[VPT][4];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        unpack4x2<T>(yv[i], v[i]);
+    }
     float mean = 0.0f, inv = 1.0f;
     if (p.post == LYRAQ_NORM_LAYER) {
-        float a = 0.0f;
+        float2 a = make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            unpack8<T>(yv[i], v[i]);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                a += v[i][j];
+            for (int j = 0; j < 4; ++j) {
+                a = add_f32x2(a, v[i][j]);
             }
         }
         mean = total(a, 0) * inv_d;
     }
     if (p.post != LYRAQ_NORM_NONE) {
-        float a = 0.0f;
+        const float2 m2 = make_float2(-mean, -mean);
+        float2       a  = make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            unpack8<T>(yv[i], v[i]);
             if (t + i * threads < nvec) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float d = v[i][j] - mean;
-                    a             = fmaf(d, d, a);
+                for (int j = 0; j < 4; ++j) {
+                    v[i][j] = add_f32x2(v[i][j], m2);
+                    a       = fma_f32x2(v[i][j], v[i][j], a);
                 }
             }
         }
         inv = rsqrtf(total(a, 1) * inv_d + p.eps);
     }
-    const T* gate = reinterpret_cast<const T*>(p.gate) + b * p.gate_batch;
-    T*       xo   = reinterpret_cast<T*>(p.x_out) + b * p.xo_batch + s * p.xo_row;
-    float    sum  = 0.0f;
+    const T*     gate = reinterpret_cast<const T*>(p.gate) + b * p.gate_batch;
+    T*           xo   = reinterpret_cast<T*>(p.x_out) + b * p.xo_batch + s * p.xo_row;
+    const float2 r2   = make_float2(p.r, p.r);
+    float2       sum  = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
         const int vi = t + i * threads;
-        float     f[8];
-        unpack8<T>(yv[i], v[i]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            v[i][j] = (v[i][j] - mean) * inv;
-        }
         if (vi < nvec) {
-            if (p.w1 != nullptr) {
-                unpack8<T>(ld_nc_16_keep(reinterpret_cast<const T*>(p.w1) + (size_t)vi * 8), f);
+            float2 f[4], c[4];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    v[i][j] *= f[j];
+            for (int j = 0; j < 4; ++j) {
+                c[j] = make_float2(inv, inv);
+            }
+            if (p.w1 != nullptr) {
+                unpack4x2<T>(ld_nc_16_keep(reinterpret_cast<const T*>(p.w1) + vi * 8), f);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    c[j] = mul_f32x2(c[j], f[j]);
                 }
             }
             if (p.gate != nullptr) {
-                unpack8<T>(ld_nc_16_keep(gate + (size_t)vi * 8), f);
+                unpack4x2<T>(ld_nc_16_keep(gate + vi * 8), f);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    v[i][j] *= f[j];
+                for (int j = 0; j < 4; ++j) {
+                    c[j] = mul_f32x2(c[j], f[j]);
                 }
             }
-            unpack8<T>(xv[i], f);
+            unpack4x2<T>(xv[i], f);
+            float o[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v[i][j] = fmaf(p.r, f[j], v[i][j]);
-                sum += v[i][j];
+            for (int j = 0; j < 4; ++j) {
+                v[i][j]      = fma_f32x2(v[i][j], c[j], mul_f32x2(r2, f[j]));
+                sum          = add_f32x2(sum, v[i][j]);
+                o[2 * j]     = v[i][j].x;
+                o[2 * j + 1] = v[i][j].y;
             }
             if (p.x_out != nullptr) {
-                st_16(xo + (size_t)vi * 8, pack8<T>(v[i]));
+                st_16(xo + vi * 8, pack8<T>(o));
             }
         }
     }
     mean = p.pre == LYRAQ_NORM_LAYER ? total(sum, 2) * inv_d : 0.0f;
-    float sq = 0.0f;
+    const float2 m2 = make_float2(-mean, -mean);
+    float2       sq = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
         if (t + i * threads < nvec) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v[i][j] -= mean;
-                sq = fmaf(v[i][j], v[i][j], sq);
+            for (int j = 0; j < 4; ++j) {
+                v[i][j] = add_f32x2(v[i][j], m2);
+                sq      = fma_f32x2(v[i][j], v[i][j], sq);
             }
         }
     }
@@ -184,40 +193,47 @@ norm_residual_kernel(const NormParams p)
         const bool in = vi < nvec;
         Vec16      o{};
         if (in) {
-            float f[8];
+            float2 f[4], c[4];
+            float  h[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v[i][j] *= inv;
+            for (int j = 0; j < 4; ++j) {
+                c[j] = make_float2(inv, inv);
             }
             if (p.w2 != nullptr) {
-                unpack8<T>(ld_nc_16_keep(reinterpret_cast<const T*>(p.w2) + (size_t)vi * 8), f);
+                unpack4x2<T>(ld_nc_16_keep(reinterpret_cast<const T*>(p.w2) + vi * 8), f);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    v[i][j] *= f[j];
+                for (int j = 0; j < 4; ++j) {
+                    c[j] = mul_f32x2(c[j], f[j]);
                 }
             }
             if (p.scale != nullptr) {
-                unpack8<T>(ld_nc_16_keep(scale + (size_t)vi * 8), f);
+                unpack4x2<T>(ld_nc_16_keep(scale + vi * 8), f);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    v[i][j] *= 1.0f + f[j];
+                for (int j = 0; j < 4; ++j) {
+                    c[j] = fma_f32x2(c[j], f[j], c[j]);
                 }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                f[j] = make_float2(0.0f, 0.0f);
             }
             if (p.shift != nullptr) {
-                unpack8<T>(ld_nc_16_keep(shift + (size_t)vi * 8), f);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    v[i][j] += f[j];
-                }
+                unpack4x2<T>(ld_nc_16_keep(shift + vi * 8), f);
             }
-            o = pack8<T>(v[i]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 w = fma_f32x2(v[i][j], c[j], f[j]);
+                h[2 * j]       = w.x;
+                h[2 * j + 1]   = w.y;
+            }
+            o = pack8<T>(h);
             if (p.h != nullptr) {
-                st_16(hr + (size_t)vi * 8, o);
+                st_16(hr + vi * 8, o);
             }
             if (p.qf8 != nullptr) {
-                unpack8<T>(o, f);
-                st_8(p.qf8 + row * (size_t)p.dim + (size_t)vi * 8, f32x2_to_e4m3x2(f[0] * r8, f[1] * r8) | (f32x2_to_e4m3x2(f[2] * r8, f[3] * r8) << 16),
-                     f32x2_to_e4m3x2(f[4] * r8, f[5] * r8) | (f32x2_to_e4m3x2(f[6] * r8, f[7] * r8) << 16));
+                unpack8<T>(o, h);
+                st_8(p.qf8 + (size_t)row * (size_t)p.dim + vi * 8, f32x2_to_e4m3x2(h[0] * r8, h[1] * r8) | (f32x2_to_e4m3x2(h[2] * r8, h[3] * r8) << 16),
+                     f32x2_to_e4m3x2(h[4] * r8, h[5] * r8) | (f32x2_to_e4m3x2(h[6] * r8, h[7] * r8) << 16));
             }
         }
         if (FORMAT >= 0) {
@@ -236,7 +252,7 @@ norm_residual_kernel(const NormParams p)
             if (in) {
                 float f[8];
                 unpack8<T>(o, f);
-                *reinterpret_cast<uint32_t*>(p.q4 + row * (size_t)(p.dim >> 1) + (size_t)vi * 4) = fp4_encode8<kFmt>(f, blk);
+                *reinterpret_cast<uint32_t*>(p.q4 + (size_t)row * (size_t)(p.dim >> 1) + vi * 4) = fp4_encode8<kFmt>(f, blk);
                 if (vi % (4 * kLanes) == 0) {
                     *reinterpret_cast<uint32_t*>(p.q4_sf + fp4_scale_offset(row, p.atoms, (size_t)(vi / (4 * kLanes)))) = word;
                 }
@@ -312,11 +328,11 @@ extern "C" int lyraq_gated_residual_norm(const lyraq_gated_norm_t* a, void* stre
     p.y_batch = a->y_batch; p.y_row = a->y_row; p.x_batch = a->x_batch; p.x_row = a->x_row;
     p.xo_batch = a->x_out_batch; p.xo_row = a->x_out_row; p.h_batch = a->h_batch; p.h_row = a->h_row;
     p.gate_batch = a->gate_batch; p.scale_batch = a->scale_batch; p.shift_batch = a->shift_batch;
-    p.rows = a->batch * a->seq_len; p.seq = a->seq_len; p.dim = (int)a->dim; p.post = a->post; p.pre = a->pre;
+    p.rows = (unsigned)(a->batch * a->seq_len); p.seq = (unsigned)a->seq_len; p.dim = (int)a->dim; p.post = a->post; p.pre = a->pre;
     p.r = a->residual_scale; p.eps = a->eps;
     p.atoms = a->q4 != nullptr ? fp4_atoms(a->dim, a->q4_format) : 0;
     const NormSplit split = norm_split(p.rows, p.dim, sms);
-    const unsigned  grid  = (unsigned)(split.warp ? (p.rows + 7) / 8 : p.rows);
+    const unsigned  grid  = split.warp ? (p.rows + 7) / 8 : p.rows;
     auto launch = [&](auto* kernel) {
         return launch_kernel(kernel, grid, (unsigned)split.threads, (size_t)0, (cudaStream_t)stream, 1u, p);
     };

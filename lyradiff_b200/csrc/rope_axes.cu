@@ -28,9 +28,9 @@ struct RopeAxesParams {
     const unsigned char* axis;        // [pairs]
     int                  pos_dtype;
     int                  heads[2];
-    int                  head_dim, pairs, lanes_log2, groups, chunks, tokens_per_block;
-    size_t               tokens, seq;
-    float                eps;
+    int                  head_dim, pairs, lanes_log2, groups, chunks, share, tokens_per_block;
+    unsigned             tokens, seq;
+    float                eps, inv_dim;
 };
 
 // Angle of one pair as a fraction of a turn, in 1 / 2^64.
@@ -87,6 +87,17 @@ template<typename T> struct Piece<T, 4> {
         b = Pair<T>::from_f32(f[2], f[3]);
     }
 };
+template<typename T> struct Piece<T, 2> {
+    uint32_t a;
+    __device__ __forceinline__ void load(const T* p) { asm volatile("ld.global.u32 %0, [%1];" : "=r"(a) : "l"(p)); }
+    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint32_t*>(p) = a; }
+    __device__ __forceinline__ void get(float* f) const
+    {
+        const float2 x = Pair<T>::to_f32(a);
+        f[0] = x.x; f[1] = x.y;
+    }
+    __device__ __forceinline__ void set(const float* f) { a = Pair<T>::from_f32(f[0], f[1]); }
+};
 template<typename T> struct Piece<T, 1> {
     T v;
     __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const volatile T*>(p); }
@@ -97,38 +108,36 @@ template<typename T> struct Piece<T, 1> {
 template<> __device__ __forceinline__ void Piece<__half, 1>::load(const __half* p) { v = __ushort_as_half((unsigned short)ld_u16(p)); }
 template<> __device__ __forceinline__ void Piece<__nv_bfloat16, 1>::load(const __nv_bfloat16* p) { v = __ushort_as_bfloat16((unsigned short)ld_u16(p)); }
 
-// VEC: pairs of a lane's unit; NU: units of a lane (more than one only for single pairs of long heads); HALVES: pair i is (x[i], x[i + pairs]), else
+// VEC: pairs of a lane's unit; NU: units of a lane (more than one only where 32 lanes of small units do not span a head); HALVES: pair i is (x[i], x[i + pairs]), else
 // (x[2 i], x[2 i + 1]); NORM: q or k is normalised.
 template<typename T, int VEC, int NU, bool HALVES, bool NORM>
 __global__ void __launch_bounds__(256) rope_axes_kernel(const RopeAxesParams p)
 {
-    extern __shared__ float2 turn[];      // [tokens_per_block][pairs]: cosine, sine
+    extern __shared__ __align__(16) float turn_c[];      // [2][tokens_per_block][pairs]: cosines, then sines
     grid_launch_dependents();
     grid_dependency_wait();
-    const int    chunk = (int)(blockIdx.x % (unsigned)p.chunks);
-    const size_t t0    = (size_t)(blockIdx.x / (unsigned)p.chunks) * (size_t)p.tokens_per_block;
-    const int    n_tok = (int)min((size_t)p.tokens_per_block, p.tokens - t0);
+    const unsigned at    = blockIdx.x / (unsigned)p.chunks, chunk = blockIdx.x - at * (unsigned)p.chunks;
+    const unsigned t0    = at * (unsigned)p.tokens_per_block;
+    const int      n_tok = (int)min((unsigned)p.tokens_per_block, p.tokens - t0);
     for (int i = threadIdx.x; i < n_tok * p.pairs; i += blockDim.x) {
-        const int    tk = i / p.pairs, pair = i - tk * p.pairs;
-        const size_t token = t0 + tk, b = token / p.seq, s = token - b * p.seq;
-        uint64_t     phase = 0;
-        float2       cs;
+        const int      tk = i / p.pairs, pair = i - tk * p.pairs;
+        const unsigned token = t0 + tk, b = token / p.seq, s = token - b * p.seq;
+        uint64_t       phase = 0;
+        float2         cs    = make_float2(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
         if (angle_of(p, b * p.pos_batch + s * p.pos_token + (size_t)p.axis[pair] * p.pos_axis, p.turns[pair], phase)) {
             // half turns in [-1, 1)
             sincospif((float)(int)(uint32_t)(phase >> 32) * 4.656612873077393e-10f, &cs.y, &cs.x);
-        } else {
-            cs = make_float2(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
         }
-        turn[i] = cs;
+        turn_c[i]                            = cs.x;
+        turn_c[p.tokens_per_block * p.pairs + i] = cs.y;
     }
     __syncthreads();
 
     const int lanes = 1 << p.lanes_log2;
     const int lane = (int)threadIdx.x & (lanes - 1), group = (int)threadIdx.x >> p.lanes_log2;
     const int units = p.head_dim / (2 * VEC), turning = p.pairs / VEC;     // units of a head, those of them that turn
-    const int heads = p.heads[0] + p.heads[1];
     // this block's share of the heads, dealt to groups
-    const int h0 = (int)((long long)heads * chunk / p.chunks), h1 = (int)((long long)heads * (chunk + 1) / p.chunks);
+    const int h0 = (int)chunk * p.share, h1 = min(h0 + p.share, p.heads[0] + p.heads[1]);
     int  at_a[NU], at_b[NU];
     bool there[NU], turns[NU];
 #pragma unroll
@@ -140,14 +149,35 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(const RopeAxesParams p)
         at_b[u]  = HALVES && turns[u] ? p.pairs + unit * VEC : unit * 2 * VEC + VEC;
     }
     for (int tk = 0; tk < n_tok; ++tk) {
-        const size_t token = t0 + tk, b = token / p.seq, s = token - b * p.seq;
-        float2       cs[NU][VEC];
+        const unsigned token = t0 + tk, b = token / p.seq, s = token - b * p.seq;
+        float          cosine[NU][VEC], sine[NU][VEC];
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
+            if (turns[u]) {
+                const float* c = turn_c + tk * p.pairs + (lane + u * lanes) * VEC;
+                const float* n = c + p.tokens_per_block * p.pairs;
+                if constexpr (VEC >= 4) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                cs[u][j] = turns[u] ? turn[tk * p.pairs + (lane + u * lanes) * VEC + j] : make_float2(1.0f, 0.0f);
+                    for (int j = 0; j < VEC; j += 4) {
+                        const float4 c4 = *reinterpret_cast<const float4*>(c + j), n4 = *reinterpret_cast<const float4*>(n + j);
+                        cosine[u][j] = c4.x; cosine[u][j + 1] = c4.y; cosine[u][j + 2] = c4.z; cosine[u][j + 3] = c4.w;
+                        sine[u][j] = n4.x; sine[u][j + 1] = n4.y; sine[u][j + 2] = n4.z; sine[u][j + 3] = n4.w;
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) {
+                        cosine[u][j] = c[j];
+                        sine[u][j]   = n[j];
+                    }
+                }
             }
+        }
+        const T* base_in[2];
+        T*       base_out[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            base_in[k]  = reinterpret_cast<const T*>(p.src[k]) + b * p.src_batch[k] + s * p.src_token[k];
+            base_out[k] = reinterpret_cast<T*>(p.dst[k]) + b * p.dst_batch[k] + s * p.dst_token[k];
         }
         for (int hb = h0; hb < h1; hb += 2 * p.groups) {
             Piece<T, VEC> a[2][NU], c[2][NU];
@@ -158,11 +188,10 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(const RopeAxesParams p)
             for (int i = 0; i < 2; ++i) {
                 const int  head = hb + group + i * p.groups;
                 const bool is_k = head >= p.heads[0];
-                const int  k    = is_k ? 1 : 0, h = is_k ? head - p.heads[0] : head;
                 on[i]           = group < p.groups && head < h1;
-                const T* in     = reinterpret_cast<const T*>(p.src[k]) + b * p.src_batch[k] + s * p.src_token[k] + (size_t)h * p.src_head[k];
-                out[i]          = reinterpret_cast<T*>(p.dst[k]) + b * p.dst_batch[k] + s * p.dst_token[k] + (size_t)h * p.dst_head[k];
-                w[i]            = reinterpret_cast<const T*>(p.norm[k]);
+                const T* in     = is_k ? base_in[1] + (size_t)(head - p.heads[0]) * p.src_head[1] : base_in[0] + (size_t)head * p.src_head[0];
+                out[i]          = is_k ? base_out[1] + (size_t)(head - p.heads[0]) * p.dst_head[1] : base_out[0] + (size_t)head * p.dst_head[0];
+                w[i]            = reinterpret_cast<const T*>(is_k ? p.norm[1] : p.norm[0]);
 #pragma unroll
                 for (int u = 0; u < NU; ++u) {
                     if (on[i] && there[u]) {
@@ -173,8 +202,10 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(const RopeAxesParams p)
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
+                if (!NORM && !on[i]) {
+                    continue;
+                }
                 float x[NU][2 * VEC];
-                float sq = 0.0f;
 #pragma unroll
                 for (int u = 0; u < NU; ++u) {
 #pragma unroll
@@ -185,17 +216,24 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(const RopeAxesParams p)
                         a[i][u].get(x[u]);
                         c[i][u].get(x[u] + VEC);
                     }
-#pragma unroll
-                    for (int j = 0; j < 2 * VEC; ++j) {
-                        sq = fmaf(x[u][j], x[u][j], sq);
-                    }
                 }
                 if (NORM) {
+                    float2 sq2 = make_float2(0.0f, 0.0f);
+#pragma unroll
+                    for (int u = 0; u < NU; ++u) {
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j) {
+                            const float2 e = make_float2(x[u][2 * j], x[u][2 * j + 1]);
+                            sq2            = fma_f32x2(e, e, sq2);
+                        }
+                    }
+                    float sq = sq2.x + sq2.y;
                     for (int m = lanes >> 1; m > 0; m >>= 1) {
                         sq += __shfl_xor_sync(0xffffffffu, sq, m);
                     }
-                    const float inv = rsqrtf(sq / (float)p.head_dim + p.eps);
                     if (w[i] != nullptr) {
+                        const float  inv = rsqrtf(sq * p.inv_dim + p.eps);
+                        const float2 in2 = make_float2(inv, inv);
 #pragma unroll
                         for (int u = 0; u < NU; ++u) {
                             if (on[i] && there[u]) {
@@ -206,8 +244,10 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(const RopeAxesParams p)
                                 wa.get(f);
                                 wc.get(f + VEC);
 #pragma unroll
-                                for (int j = 0; j < 2 * VEC; ++j) {
-                                    x[u][j] *= inv * f[j];
+                                for (int j = 0; j < VEC; ++j) {
+                                    const float2 e  = mul_f32x2(make_float2(x[u][2 * j], x[u][2 * j + 1]), mul_f32x2(in2, make_float2(f[2 * j], f[2 * j + 1])));
+                                    x[u][2 * j]     = e.x;
+                                    x[u][2 * j + 1] = e.y;
                                 }
                             }
                         }
@@ -216,17 +256,17 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(const RopeAxesParams p)
 #pragma unroll
                 for (int u = 0; u < NU; ++u) {
                     if (on[i] && there[u]) {
-                        float y[2 * VEC];
+                        if (turns[u]) {
 #pragma unroll
-                        for (int j = 0; j < VEC; ++j) {
-                            // a pair beyond the turning part has cosine 1 and sine 0, but its partner may be anything: it is copied
-                            const int   p0 = HALVES ? j : 2 * j, p1 = HALVES ? VEC + j : 2 * j + 1;
-                            const float v0 = x[u][p0], v1 = x[u][p1];
-                            y[p0] = turns[u] ? fmaf(v0, cs[u][j].x, -v1 * cs[u][j].y) : v0;
-                            y[p1] = turns[u] ? fmaf(v0, cs[u][j].y, v1 * cs[u][j].x) : v1;
+                            for (int j = 0; j < VEC; ++j) {
+                                const int   p0 = HALVES ? j : 2 * j, p1 = HALVES ? VEC + j : 2 * j + 1;
+                                const float v0 = x[u][p0], v1 = x[u][p1];
+                                x[u][p0]       = fmaf(v0, cosine[u][j], -v1 * sine[u][j]);
+                                x[u][p1]       = fmaf(v0, sine[u][j], v1 * cosine[u][j]);
+                            }
                         }
-                        a[i][u].set(y);
-                        c[i][u].set(y + VEC);
+                        a[i][u].set(x[u]);
+                        c[i][u].set(x[u] + VEC);
                         a[i][u].store(out[i] + at_a[u]);
                         c[i][u].store(out[i] + at_b[u]);
                     }
@@ -283,7 +323,7 @@ extern "C" int lyraq_rope_axes(const lyraq_rope_axes_t* a, void* stream)
     p.dst_batch[1] = a->k_out_batch; p.dst_token[1] = a->k_out_token; p.dst_head[1] = a->k_out_head;
     p.pos = a->positions; p.pos_batch = a->pos_batch; p.pos_token = a->pos_token; p.pos_axis = a->pos_axis; p.pos_dtype = a->pos_dtype;
     p.turns = a->turns; p.axis = a->axis; p.heads[0] = a->q_heads; p.heads[1] = a->k_heads; p.head_dim = a->head_dim; p.pairs = a->pairs;
-    p.tokens = a->batch * a->seq_len; p.seq = a->seq_len; p.eps = a->eps;
+    p.tokens = (unsigned)(a->batch * a->seq_len); p.seq = (unsigned)a->seq_len; p.eps = a->eps; p.inv_dim = 1.0f / (float)a->head_dim;
     // the widest pieces that sizes, strides and addresses allow
     auto fits = [&](int vec) {
         const int  rest = a->head_dim - 2 * a->pairs;
@@ -294,7 +334,7 @@ extern "C" int lyraq_rope_axes(const lyraq_rope_axes_t* a, void* stream)
                                            even_strides(a->k_out, a->k_out_batch, a->k_out_token, a->k_out_head, vec) && even_strides(a->k_norm, 0, 0, 0, vec));
         return size && q && k;
     };
-    const int vec   = fits(8) ? 8 : fits(4) ? 4 : 1;
+    const int vec   = fits(8) ? 8 : fits(4) ? 4 : fits(2) ? 2 : 1;
     const int units = a->head_dim / (2 * vec);
     while ((1 << p.lanes_log2) < units && p.lanes_log2 < 5) {
         ++p.lanes_log2;
@@ -303,16 +343,17 @@ extern "C" int lyraq_rope_axes(const lyraq_rope_axes_t* a, void* stream)
     // cosines' cost, few enough to fill the chip; where there are few, a token's heads are dealt to several blocks.
     const int lanes  = 1 << p.lanes_log2;
     const int most   = 256 / lanes;
-    p.chunks         = p.tokens >= (size_t)sms * 2 ? 1 : (heads + most - 1) / most;
-    const int share  = (heads + p.chunks - 1) / p.chunks;
-    const int rounds = (share + most - 1) / most;
-    p.groups         = (share + rounds - 1) / rounds;
-    p.tokens_per_block = p.tokens >= (size_t)sms * 32 ? 4 : p.tokens >= (size_t)sms * 16 ? 2 : 1;
+    p.chunks         = p.tokens >= (unsigned)sms * 2 ? 1 : (heads + most - 1) / most;
+    p.share          = (heads + p.chunks - 1) / p.chunks;
+    const int rounds = (p.share + most - 1) / most;
+    p.groups         = (p.share + rounds - 1) / rounds;
+    p.tokens_per_block = p.tokens >= (unsigned)sms * 32 ? 4 : p.tokens >= (unsigned)sms * 16 ? 2 : 1;
     const unsigned threads = (unsigned)((p.groups * lanes + 31) / 32 * 32);
-    const unsigned grid    = (unsigned)((p.tokens + p.tokens_per_block - 1) / p.tokens_per_block) * (unsigned)p.chunks;
-    if (((p.tokens + p.tokens_per_block - 1) / p.tokens_per_block) * (size_t)p.chunks > 0x7fffffffu) {
+    const size_t   blocks  = ((size_t)p.tokens + p.tokens_per_block - 1) / p.tokens_per_block * (size_t)p.chunks;
+    if (blocks > 0x7fffffffu) {
         return LYRAQ_ERR_UNSUPPORTED;
     }
+    const unsigned grid = (unsigned)blocks;
     const size_t smem = sizeof(float2) * (size_t)p.tokens_per_block * (size_t)(p.pairs > 0 ? p.pairs : 1);
     const bool   norm = a->q_norm != nullptr || a->k_norm != nullptr;
     auto launch = [&](auto* kernel) { return launch_kernel(kernel, grid, threads, smem, (cudaStream_t)stream, 1u, p); };
@@ -321,6 +362,7 @@ extern "C" int lyraq_rope_axes(const lyraq_rope_axes_t* a, void* stream)
         constexpr bool kH = decltype(halves)::value, kN = decltype(normed)::value;
         return vec == 8   ? launch(rope_axes_kernel<T, 8, 1, kH, kN>)
                : vec == 4 ? launch(rope_axes_kernel<T, 4, 1, kH, kN>)
+               : vec == 2 ? launch(rope_axes_kernel<T, 2, 2, kH, kN>)
                           : launch(rope_axes_kernel<T, 1, 4, kH, kN>);
     };
     auto pick_norm = [&](auto type, auto halves) {
