@@ -40,7 +40,8 @@ constexpr int kThreads   = 384;
 constexpr int kEpiWarp0  = 4;
 constexpr int kEpiWarps  = 8;
 constexpr int kBox       = 32 * 64;      // one warp's staging box: 32 rows x 32 columns of a 16-bit type
-constexpr int kBiasBytes = 128 * 2;      // one warp's bias: up to 128 columns of a 16-bit type (fp32, which uses no box, keeps its there)
+constexpr int kBoxes     = 2;            // the store of one chunk drains its box while the next chunk is computed and fills the other
+constexpr int kBiasBytes = 128 * 2;      // one warp's bias: up to 128 columns of a 16-bit type (fp32, which uses no boxes, keeps its there)
 constexpr int kBarBytes  = 256;
 constexpr int kOtherRegs = 72;
 constexpr int kEpiRegs   = 216;
@@ -54,7 +55,7 @@ template<int FORMAT, int BLOCK_N, int CTAS> struct Smem {
     static constexpr int kSfaBytes   = kAtoms * 512;
     static constexpr int kSfbBytes   = kSbBlocks * kAtoms * 512;
     static constexpr int kStageBytes = kABytes + kBBytes + kSfaBytes + kSfbBytes;
-    static constexpr int kEpiBytes   = kEpiWarps * (kBox + kBiasBytes);
+    static constexpr int kEpiBytes   = kEpiWarps * (kBoxes * kBox + kBiasBytes);
     static constexpr int kStages     = (227 * 1024 - 1024 - kBarBytes - kEpiBytes) / kStageBytes;
     static constexpr int kEpiOffset  = kStages * kStageBytes;
     static constexpr int kBarOffset  = kEpiOffset + kEpiBytes;
@@ -410,9 +411,27 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         const int      quad      = warp & 3;                 // the TMEM lane quadrant this warp may read
         const int      half      = (warp - kEpiWarp0) >> 2;  // which half of the tile's columns
         const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
-        uint8_t*       box       = gen_base + S::kEpiOffset + (warp - kEpiWarp0) * kBox;
-        const uint32_t box_at    = smem_base + S::kEpiOffset + (warp - kEpiWarp0) * kBox;
-        uint8_t*       bias      = p.c_dtype == LYRAQ_F32 ? box : gen_base + S::kEpiOffset + kEpiWarps * kBox + (warp - kEpiWarp0) * kBiasBytes;
+        uint8_t*       boxes     = gen_base + S::kEpiOffset + (warp - kEpiWarp0) * kBoxes * kBox;
+        const uint32_t boxes_at  = smem_base + S::kEpiOffset + (warp - kEpiWarp0) * kBoxes * kBox;
+        uint8_t*       bias      = p.c_dtype == LYRAQ_F32 ? boxes : gen_base + S::kEpiOffset + kEpiWarps * kBoxes * kBox + (warp - kEpiWarp0) * kBiasBytes;
+        // the bias of this warp's columns of a tile, one column in 32 per lane; fetched a tile ahead
+        uint32_t bias_ahead[kHalfN / 32];
+        auto fetch_bias = [&](int tile) {
+            int m_blk, n_blk;
+            tile_coords(tile, p.m_tiles, p.n_tiles, m_blk, n_blk);
+#pragma unroll
+            for (int i = 0; i < kHalfN / 32; ++i) {
+                const int col = n_blk * BLOCK_N + half * kHalfN + lane + 32 * i;
+                bias_ahead[i] = 0;
+                if (p.bias != nullptr && col < p.N) {
+                    bias_ahead[i] = p.c_dtype == LYRAQ_F32 ? reinterpret_cast<const uint32_t*>(p.bias)[col]
+                                                           : (uint32_t)reinterpret_cast<const uint16_t*>(p.bias)[col];
+                }
+            }
+        };
+        if (unit < num_tiles) {
+            fetch_bias(unit);
+        }
         const float    scale     = fp4_tensor_scale(p);
         const bool     vec_ok    = p.c_dtype == LYRAQ_F32 ? (p.N & 3) == 0 : (p.N & 7) == 0;
         int            local     = 0;
@@ -425,34 +444,19 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             const int row   = row0 + lane;
             const int ncol0 = n_blk * BLOCK_N + half * kHalfN;
             if (p.bias != nullptr) {
-                // staged while the main loop of the tile still runs; the warp's own piece, so no other warp is waited for
-                uint32_t b[kHalfN / 32];
-#pragma unroll
-                for (int i = 0; i < kHalfN / 32; ++i) {
-                    const int col = ncol0 + lane + 32 * i;
-                    b[i]          = 0;
-                    if (col < p.N) {
-                        b[i] = p.c_dtype == LYRAQ_F32 ? reinterpret_cast<const uint32_t*>(p.bias)[col] : (uint32_t)reinterpret_cast<const uint16_t*>(p.bias)[col];
-                    }
-                }
+                // the warp's own piece of shared memory, so no other warp is waited for
                 __syncwarp();
 #pragma unroll
                 for (int i = 0; i < kHalfN / 32; ++i) {
                     if (p.c_dtype == LYRAQ_F32) {
-                        reinterpret_cast<uint32_t*>(bias)[lane + 32 * i] = b[i];
+                        reinterpret_cast<uint32_t*>(bias)[lane + 32 * i] = bias_ahead[i];
                     } else {
-                        reinterpret_cast<uint16_t*>(bias)[lane + 32 * i] = (uint16_t)b[i];
+                        reinterpret_cast<uint16_t*>(bias)[lane + 32 * i] = (uint16_t)bias_ahead[i];
                     }
                 }
                 __syncwarp();
-            }
-            if (RES && p.residual != nullptr && row < p.M) {
-                // the row's share of the residual is asked into L2 while the main loop of the tile still runs
-                const int      esz   = p.c_dtype == LYRAQ_F32 ? 4 : 2;
-                const uint8_t* seg   = reinterpret_cast<const uint8_t*>(p.residual) + ((size_t)row * (size_t)p.N + (size_t)ncol0) * esz;
-                const int      bytes = min(kHalfN, p.N - ncol0) * esz;
-                if (vec_ok && bytes > 0) {   // whole 16-byte pieces on 16-byte addresses
-                    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(seg), "r"(bytes) : "memory");
+                if (tile + n_units < num_tiles) {
+                    fetch_bias(tile + n_units);
                 }
             }
             const uint32_t t_addr = tmem_base + lane_addr + (uint32_t)(buf * BLOCK_N + half * kHalfN);
@@ -468,9 +472,10 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                 }
             };
             constexpr int kChunks = kHalfN / 32;
+            static_assert(kChunks % kBoxes == 0, "the boxes alternate from tile to tile too");
             // Residual of a 16-bit output: a lane that fetched its own row would touch 32 lines an instruction and use half a sector of each
             // ([4608, 12288, 3072]: 191 us against 72 without a residual).  Instead four lanes fetch the 64 bytes of a row, eight rows an instruction, two chunks
-            // ahead, and hand them over through the box that the result leaves by.
+            // ahead (the first brings all 256 bytes of the row's share into L2), and hand them over through the box that the result leaves by.
             const bool staged = RES && p.residual != nullptr && p.tma_store;
             Vec16      rr[2][RES ? 4 : 1];
             auto fetch = [&](int c, Vec16* dst) {
@@ -480,7 +485,7 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                     const int rw = row0 + i * 8 + (lane >> 2);
                     dst[i]       = Vec16{};
                     if (rw < p.M && col < p.N) {   // N is a multiple of 8
-                        dst[i] = ld_16(reinterpret_cast<const uint16_t*>(p.residual) + (size_t)rw * (size_t)p.N + (size_t)col);
+                        dst[i] = ld_16_l2_256(reinterpret_cast<const uint16_t*>(p.residual) + (size_t)rw * (size_t)p.N + (size_t)col);
                     }
                 }
             };
@@ -524,11 +529,12 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                     continue;
                 }
                 float     v[32];
+                uint8_t*  box  = boxes + (c % kBoxes) * kBox;
                 uint8_t*  brow = box + lane * 64;
                 const int sw   = (lane >> 1) & 3;
                 if (p.tma_store) {
                     if (lane == 0) {
-                        tma_store_wait_read();  // the store before has drained the box
+                        tma_store_wait_read_but_one();  // the store before the last has drained this box
                     }
                     __syncwarp();
                 }
@@ -575,7 +581,7 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0 && row0 < p.M) {
-                    tma_store_2d(&tmap_c, box_at, col0, row0);
+                    tma_store_2d(&tmap_c, boxes_at + (uint32_t)((c % kBoxes) * kBox), col0, row0);
                     tma_store_commit();
                 }
             }

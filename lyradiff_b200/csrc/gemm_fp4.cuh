@@ -50,6 +50,17 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t smem_dst, const CUtens
         : "memory");
 }
 
+// all of this thread's committed stores but the last have finished reading shared memory
+__device__ __forceinline__ void tma_store_wait_read_but_one() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
+
+// 16 bytes, on a miss the 256 around them into L2
+__device__ __forceinline__ Vec16 ld_16_l2_256(const void* p)
+{
+    Vec16 v;
+    asm volatile("ld.global.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]) : "l"(p));
+    return v;
+}
+
 // Arrive on another CTA's barrier when all that has to be ordered before it is complete already (tensor-memory loads behind their wait).  The
 // releasing form makes the warp's earlier memory accesses visible first, which took a pair's second CTA 900 ns per tile.
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr)
