@@ -3,7 +3,6 @@ missing or lacks a symbol the import of the ops fails with a clear error."""
 
 import ctypes
 import os
-import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("LYRAQ_LIB_PATH", os.path.join(_HERE, "liblyraq.so"))
@@ -26,10 +25,6 @@ class GatedNormArgs(ctypes.Structure):
                 + [("residual_scale", c_float), ("eps", c_float), ("dtype", c_int)] + [(n, c_size_t) for n in ("batch", "seq_len", "dim")])
 
 
-# the same as one format: a call packs its arguments at once, a tenth of the time of filling the structure field by field
-GATED_NORM = struct.Struct("@2P4Q2P4Q5Pi3P3Q2P2i2fi3Q")
-
-
 class RopeAxesArgs(ctypes.Structure):
     """lyraq_rope_axes_t."""
     _fields_ = ([(n, c_void_p) for n in ("q", "k")] + [(a + n, c_size_t) for a in ("q_", "k_") for n in ("batch", "token", "head")]
@@ -39,8 +34,6 @@ class RopeAxesArgs(ctypes.Structure):
                 + [(n, c_int) for n in ("pos_dtype", "dtype", "q_heads", "k_heads", "head_dim", "pairs", "interleaved")] + [("eps", c_float)]
                 + [(n, c_size_t) for n in ("batch", "seq_len")])
 
-
-ROPE_AXES = struct.Struct("@2P6Q2P6Q3P3Q2P7if2Q")
 
 # name -> (restype, argtypes); mirrors include/lyraq.h declaration by declaration
 SIGNATURES = {
@@ -121,6 +114,7 @@ SIGNATURES = {
 }
 
 _lib = None
+_host = None
 
 
 class LyraqError(RuntimeError):
@@ -147,6 +141,23 @@ def lib():
             fn.argtypes = args
         _lib = handle
     return _lib
+
+
+def host():
+    """The extension module _host.so (csrc/host_calls.cpp), bound to the loaded library's functions."""
+    global _host
+    if _host is None:
+        path = os.path.join(_HERE, "_host.so")
+        if not os.path.exists(path):
+            raise ImportError("%s is not built: run `python -m lyradiff_b200.build` (there is no fallback)" % path)
+        import torch  # noqa: F401  (its libraries are what the module links to)
+        from . import _host as module
+        handle = lib()
+        names = ("lyraq_gated_residual_norm", "lyraq_rope_axes", "lyraq_linear_fp4_forward", "lyraq_gemm_fp4", "lyraq_quant_fp4",
+                 "lyraq_workspace_bytes", "lyraq_fp4_scale_bytes")
+        module.bind({n: ctypes.cast(getattr(handle, n), c_void_p).value for n in names}, LyraqError)
+        _host = module
+    return _host
 
 
 def check(status, where):

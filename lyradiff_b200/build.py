@@ -1,5 +1,5 @@
 """Builds liblyraq.so (the C-ABI CUDA library) in-tree with nvcc for sm_100a, and liblyradiff_classes.so (host C++ that
-registers the torch custom classes over that C ABI) with g++.
+registers the torch custom classes over that C ABI) and _host.so (the extension module behind some of ops.py) with g++.
 
 Usage: python -m lyradiff_b200.build [--force] [--verbose]
 """
@@ -7,12 +7,15 @@ Usage: python -m lyradiff_b200.build [--force] [--verbose]
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "liblyraq.so")
 CLASSES_LIB = os.path.join(HERE, "liblyradiff_classes.so")
 CLASSES_SRC = os.path.join(CSRC, "torch_classes.cpp")
+HOST_LIB = os.path.join(HERE, "_host.so")
+HOST_SRC = os.path.join(CSRC, "host_calls.cpp")
 
 SOURCES = ["api.cu", "quant_kernels.cu", "gemm_dense.cu", "gemm_skinny.cu", "gemm_w4a4.cu", "gemm_w4a4_wide.cu", "fp4_quant.cu", "gemm_fp4.cu", "gemm_fp4_skinny.cu", "norm_residual.cu", "rope_axes.cu", "lora_down.cu", "block_kernels.cu", "attention.cu", "linear_layers.cu", "noalloc.cu"]
 
@@ -65,22 +68,33 @@ def build(force=False, verbose=False):
     return LIB
 
 
-def build_classes(force=False):
-    """Compile csrc/torch_classes.cpp (no device code) against torch's headers and link it to liblyraq.so, found at load time
-    beside it ($ORIGIN).  Returns the library path."""
-    build(force=force)
-    deps = [CLASSES_SRC, LIB, os.path.join(HERE, "..", "include", "lyraq.h")]
-    if not force and os.path.exists(CLASSES_LIB) and all(os.path.getmtime(d) <= os.path.getmtime(CLASSES_LIB) for d in deps):
-        return CLASSES_LIB
+def _torch_command(src, out):
     import torch
     from torch.utils import cpp_extension
     cuda_inc = os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "include")
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
     cmd += ["-I" + p for p in cpp_extension.include_paths()] + ["-I" + cuda_inc]
-    cmd += [CLASSES_SRC, "-o", CLASSES_LIB, "-L" + HERE, "-llyraq", "-L" + torch_lib,
-            "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
-    subprocess.check_call(cmd)
+    return cmd + [src, "-o", out, "-L" + torch_lib, "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
+
+
+def _current(lib, src):
+    deps = [src, LIB, os.path.join(HERE, "..", "include", "lyraq.h")]
+    return os.path.exists(lib) and all(os.path.getmtime(d) <= os.path.getmtime(lib) for d in deps)
+
+
+def build_classes(force=False):
+    """Compile csrc/torch_classes.cpp (no device code) against torch's headers and link it to liblyraq.so, found at load time
+    beside it ($ORIGIN), and csrc/host_calls.cpp, the extension module behind some of ops.py, which is given liblyraq.so's functions at run
+    time.  Returns the path of the first."""
+    build(force=force)
+    procs = []
+    if force or not _current(HOST_LIB, HOST_SRC):
+        procs.append(subprocess.Popen(_torch_command(HOST_SRC, HOST_LIB) + ["-I" + sysconfig.get_paths()["include"], "-ltorch_python"]))
+    if force or not _current(CLASSES_LIB, CLASSES_SRC):
+        procs.append(subprocess.Popen(_torch_command(CLASSES_SRC, CLASSES_LIB) + ["-L" + HERE, "-llyraq", "-Wl,-rpath,$ORIGIN"]))
+    if any([p.wait() for p in procs]):
+        raise RuntimeError("g++ failed")
     return CLASSES_LIB
 
 

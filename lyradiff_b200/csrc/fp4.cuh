@@ -74,8 +74,8 @@ template<int FORMAT> __device__ __forceinline__ Fp4Tensor fp4_tensor(const float
 struct Fp4Block {
     uint32_t code;
     float    t;      // 0: every code is 0
-    float    r;      // 1 / t: exact for mxfp4, about so for nvfp4
-    bool     plain;  // nothing over- or underflows on the way of the values' quotients
+    float    r;      // 1 / t: exact for mxfp4, about so for nvfp4; 0 where t is
+    bool     plain;  // finite, and nothing over- or underflows on the way of the values' quotients
 };
 
 // amax_bits: the largest |x| of the block as fp32 bits, taken as an integer maximum, so that a NaN beats an infinity and both beat every
@@ -88,7 +88,7 @@ template<int FORMAT> __device__ __forceinline__ Fp4Block fp4_block(uint32_t amax
         b.code  = FORMAT == LYRAQ_NVFP4 ? 0x7fu : 0xffu;
         b.t     = 0.0f;
         b.r     = 0.0f;
-        b.plain = true;
+        b.plain = false;
         return b;
     }
     if (FORMAT == LYRAQ_NVFP4) {
@@ -101,8 +101,8 @@ template<int FORMAT> __device__ __forceinline__ Fp4Block fp4_block(uint32_t amax
         b.code = f32x2_to_e4m3x2(ratio, 0.0f) & 0xffu;
         // e4m3 -> fp32: the code's seven bits under fp16's exponent read 2^-8 times its value, subnormals included
         b.t     = __half2float(__ushort_as_half((unsigned short)(b.code << 7))) * 256.0f * s.g;
-        b.r     = rcp_approx(b.t);
-        b.plain = b.t >= 7.9e-31f && b.t <= 1.2e30f && amax <= b.t * 1048576.0f;
+        b.r     = b.t > 0.0f ? rcp_approx(b.t) : 0.0f;
+        b.plain = b.t == 0.0f || (b.t >= 7.9e-31f && b.t <= 1.2e30f && amax <= b.t * 1048576.0f);
     } else {
         const uint32_t e = amax_bits >> 23;                                  // biased; 0 for subnormals
         b.code           = e > 2u ? e - 2u : 0u;
@@ -117,32 +117,24 @@ template<int FORMAT> __device__ __forceinline__ Fp4Block fp4_block(uint32_t amax
 // The codes of eight values of a block.  A quotient that over- or underflows saturates or rounds to zero like any other.
 template<int FORMAT> __device__ __forceinline__ uint32_t fp4_encode8(const float* x, const Fp4Block& b)
 {
-    float        q[8];
-    const float2 r2 = make_float2(b.r, b.r);
-    if (b.t == 0.0f) {
-        return 0u;
-    }
-    if (FORMAT != LYRAQ_NVFP4) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 p = mul_f32x2(make_float2(x[2 * j], x[2 * j + 1]), r2);
-            q[2 * j]       = p.x;
-            q[2 * j + 1]   = p.y;
-        }
-    } else if (b.plain) {
+    float q[8];
+    if (b.plain) {   // with t = r = 0 every quotient comes out as 0
+        const float2 r2 = make_float2(b.r, b.r);
         const float2 m2 = make_float2(-b.t, -b.t);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float2 v  = make_float2(x[2 * j], x[2 * j + 1]);
-            const float2 q0 = mul_f32x2(v, r2);
-            const float2 q1 = fma_f32x2(fma_f32x2(q0, m2, v), r2, q0);
-            q[2 * j]        = q1.x;
-            q[2 * j + 1]    = q1.y;
+            const float2 v = make_float2(x[2 * j], x[2 * j + 1]);
+            float2       p = mul_f32x2(v, r2);
+            if (FORMAT == LYRAQ_NVFP4) {
+                p = fma_f32x2(fma_f32x2(p, m2, v), r2, p);
+            }
+            q[2 * j]     = p.x;
+            q[2 * j + 1] = p.y;
         }
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            q[j] = x[j] / b.t;
+            q[j] = b.t > 0.0f ? x[j] / b.t : 0.0f;
         }
     }
     return f32x8_to_e2m1x8(q);
@@ -159,17 +151,30 @@ template<> __device__ __forceinline__ uint32_t amax_bits_of<float>(const Vec16& 
     }
     return m;
 }
-__device__ __forceinline__ uint32_t amax16_of(const Vec16& v)
+// Of two 16-bit pairs the larger magnitudes, NaN before all (the sign is of no use).
+template<typename T> __device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b);
+template<> __device__ __forceinline__ uint32_t max_abs2<__nv_bfloat16>(uint32_t a, uint32_t b)
 {
-    uint32_t m = __vmaxu2(__vmaxu2(v.w[0] & 0x7fff7fffu, v.w[1] & 0x7fff7fffu), __vmaxu2(v.w[2] & 0x7fff7fffu, v.w[3] & 0x7fff7fffu));
+    uint32_t r;
+    asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template<> __device__ __forceinline__ uint32_t max_abs2<__half>(uint32_t a, uint32_t b)
+{
+    uint32_t r;
+    asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template<typename T> __device__ __forceinline__ uint32_t amax16_of(const Vec16& v)
+{
+    const uint32_t m = max_abs2<T>(max_abs2<T>(v.w[0], v.w[1]), max_abs2<T>(v.w[2], v.w[3])) & 0x7fff7fffu;
     return max(m & 0xffffu, m >> 16);
 }
-template<> __device__ __forceinline__ uint32_t amax_bits_of<__nv_bfloat16>(const Vec16& v) { return amax16_of(v) << 16; }
+template<> __device__ __forceinline__ uint32_t amax_bits_of<__nv_bfloat16>(const Vec16& v) { return amax16_of<__nv_bfloat16>(v) << 16; }
 template<> __device__ __forceinline__ uint32_t amax_bits_of<__half>(const Vec16& v)
 {
-    const uint32_t m = amax16_of(v);
     // half -> float keeps order, infinities and NaN
-    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m))) & 0x7fffffffu;
+    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)amax16_of<__half>(v)))) & 0x7fffffffu;
 }
 
 }  // namespace lyraq

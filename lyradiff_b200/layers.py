@@ -6,13 +6,11 @@ calls by the FP8 and INT8 layers and taken per call by W4A4Gemm.  torch supplies
 torch.
 """
 
-import functools
-
 import torch
 
 from . import _lib, ops
 
-OP_LINEAR_INT8, OP_LINEAR_FP8, OP_LINEAR_W4A4, OP_LINEAR_W4A4_LORA, OP_LINEAR_FP4 = 3, 4, 5, 6, 8
+OP_LINEAR_INT8, OP_LINEAR_FP8, OP_LINEAR_W4A4, OP_LINEAR_W4A4_LORA = 3, 4, 5, 6
 
 
 def _workspace(op, m, n, k, device, current):
@@ -20,11 +18,6 @@ def _workspace(op, m, n, k, device, current):
     if current is None or current.numel() < need or current.device != device:
         current = torch.empty(max(need, 256), dtype=torch.uint8, device=device)
     return current
-
-
-@functools.lru_cache(maxsize=4096)
-def _fp4_workspace(m, k):
-    return _lib.lib().lyraq_workspace_bytes(OP_LINEAR_FP4, m, 1, k)
 
 
 class Fp8Linear:
@@ -80,32 +73,9 @@ class Fp4Linear:
             self.input_scale = torch.ldexp(torch.ones_like(s), torch.where(m == 0.5, e - 1, e)).to(device=dev, dtype=torch.float32)
 
     def forward(self, x, residual=None, beta=1.0, out=None):
-        shape, k, n = x.shape, self.k, self.n
-        if shape[-1] != k:
-            raise ValueError("expected [..., %d], got %s" % (k, tuple(shape)))
-        m = x.numel() // k
-        here, stream = ops._here()
-        if x.get_device() != here:
-            raise ValueError("x is on %s, but the current device is cuda:%d" % (x.device, here))
-        ldx = k
-        if not x.is_contiguous():
-            x = x.reshape(m, k)
-            ldx = ops._rows_of(x)
-        y = torch.empty(*shape[:-1], n, dtype=x.dtype, device=x.device) if out is None else self._into(out, x.dtype, m)
-        ops.check_epilogue(x.dtype, self.bias, residual, m, n)
-        need = _fp4_workspace(m, k)
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-        w, at = self.weight, ops._at
-        st = _lib.lib().lyraq_linear_fp4_forward(
-            at(y, here, "out"), x.data_ptr(), ops._dt(x), ldx, at(self.input_scale, here), at(w.codes, here), at(w.scales, here), at(w.tensor_scale, here),
-            self.format, at(self.bias, here), at(residual, here, "residual"), beta, self.epilogue, m, n, k, ws.data_ptr(), need, stream)
-        _lib.check(st, "lyraq_linear_fp4_forward")
-        return y if out is None else y.view(*shape[:-1], n)
-
-    def _into(self, out, dtype, m):
-        if out.dtype != dtype or out.numel() != m * self.n or out.shape[-1] != self.n:
-            raise ValueError("out must be [..., %d] of x's dtype" % self.n)
-        return out
+        w = self.weight
+        return _lib.host().linear_fp4(x, w.codes, w.scales, w.tensor_scale, self.n, self.k, self.format, self.input_scale, self.bias, residual, beta,
+                                      self.epilogue, out)
 
     def empty_input(self, rows):
         """An Fp4Tensor for `rows` rows of this layer's input, for producers that write FP4 themselves (ops.gated_residual_norm)."""
@@ -115,7 +85,9 @@ class Fp4Linear:
         """The product alone, for an input that is FP4 already (empty_input): [rows, n] of `dtype`."""
         if x.tensor_scale is not self.input_scale:
             raise ValueError("the input was not quantized for this layer (empty_input)")
-        y = torch.empty(x.rows, self.n, dtype=dtype, device=x.codes.device) if out is None else self._into(out, dtype, x.rows).view(x.rows, self.n)
+        y = torch.empty(x.rows, self.n, dtype=dtype, device=x.codes.device) if out is None else out.view(x.rows, self.n)
+        if y.dtype != dtype:
+            raise ValueError("out must be %s" % dtype)
         return ops.gemm_fp4(self.weight, x, y, self.bias, residual, beta, self.gelu)
 
 

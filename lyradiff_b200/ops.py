@@ -118,23 +118,6 @@ def weight_quant_int4_g64(qw, w_scale, w):
     return qw, w_scale
 
 
-def _here():
-    """(the current device, torch's current stream on it): a call runs there, and its tensors have to be there."""
-    here = torch.cuda.current_device()
-    return here, torch.cuda.current_stream().cuda_stream if _raw_stream is None else _raw_stream(here)
-
-
-def _at(t, here, what="tensor"):
-    """Address of a contiguous tensor on the current device, or of none."""
-    if t is None:
-        return None
-    if t.get_device() != here:
-        raise ValueError("%s is on %s, but the current device is cuda:%d" % (what, t.device, here))
-    if not t.is_contiguous():
-        raise ValueError("%s must be contiguous" % what)
-    return t.data_ptr()
-
-
 def _fp4_format(fmt):
     try:
         return FP4_FORMATS[fmt]
@@ -163,50 +146,29 @@ class Fp4Tensor:
             raise ValueError("FP4 codes must be uint8 [%d, %d / 2], k a multiple of 32" % (self.rows, self.k))
         if self.scales.dtype != torch.uint8 or self.scales.numel() != _lib.lib().lyraq_fp4_scale_bytes(self.rows, self.k, _fp4_format(self.fmt)):
             raise ValueError("FP4 block scales do not fit [%d, %d] in %s" % (self.rows, self.k, self.fmt))
-        _fp4_tensor_scale(self.tensor_scale)
+        if self.tensor_scale is not None and (self.tensor_scale.dtype != torch.float32 or self.tensor_scale.numel() != 1):
+            raise ValueError("an FP4 tensor scale is one fp32 number")
         return self
-
-
-def _fp4_tensor_scale(t):
-    if t is not None and (t.dtype != torch.float32 or t.numel() != 1):
-        raise ValueError("an FP4 tensor scale is one fp32 number")
-
-
-def _rows_of(x):
-    """x [rows, k] with contiguous rows -> its row pitch in elements."""
-    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
-        raise ValueError("expected a matrix with contiguous rows that do not overlap")
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
 def quant_fp4(x, tensor_scale=None, fmt="nvfp4", out=None):
     """Microscaled FP4 quantize (lyraq_quant_fp4) of x [rows, k], whose rows may lie further apart than k.  Returns an Fp4Tensor; `out`
     reuses one (its tensor scale is the one that counts then)."""
-    ldx = _rows_of(x)
-    if x.get_device() < 0:
-        raise ValueError("expected a CUDA tensor")
     if out is None:
         out = Fp4Tensor.empty(x.shape[0], x.shape[1], fmt, tensor_scale, x.device)
     elif tensor_scale is not None or (out.rows, out.k) != tuple(x.shape):
         raise ValueError("out must have x's shape and carries its own tensor scale")
-    out.check()
-    here, stream = _here()
-    if x.get_device() != here:
-        raise ValueError("x is on %s, but the current device is cuda:%d" % (x.device, here))
-    st = _lib.lib().lyraq_quant_fp4(_at(out.codes, here), _at(out.scales, here), x.data_ptr(), _dt(x), ldx, _at(out.tensor_scale, here),
-                                    FP4_FORMATS[out.fmt], out.rows, out.k, stream)
-    _lib.check(st, "lyraq_quant_fp4")
+    _lib.host().quant_fp4(x, out.codes, out.scales, out.tensor_scale, _fp4_format(out.fmt))
     return out
 
 
 def weight_quant_fp4(w, fmt="nvfp4"):
     """FP4 weight quantize (lyraq_weight_quant_fp4): w [n, k] -> Fp4Tensor, with the weight's own tensor scale for nvfp4."""
     n, k = w.shape
-    here, stream = _here()
-    at = _at(w, here, "the weight")
+    if w.get_device() != torch.cuda.current_device():
+        raise ValueError("the weight is on %s, but the current device is cuda:%d" % (w.device, torch.cuda.current_device()))
     out = Fp4Tensor.empty(n, k, fmt, torch.empty(1, dtype=torch.float32, device=w.device) if fmt == "nvfp4" else None, w.device).check()
-    st = _lib.lib().lyraq_weight_quant_fp4(_at(out.codes, here), _at(out.scales, here), _at(out.tensor_scale, here), at, _dt(w), _fp4_format(fmt), n,
-                                           k, stream)
+    st = _lib.lib().lyraq_weight_quant_fp4(_p(out.codes), _p(out.scales), _p(out.tensor_scale), _p(w), _dt(w), _fp4_format(fmt), n, k, _stream())
     _lib.check(st, "lyraq_weight_quant_fp4")
     return out
 
@@ -300,25 +262,10 @@ def gemm_with_residual_and_bias_fp8(W, w_scale, X, x_scale, Y, bias=None, residu
 def gemm_fp4(W, X, Y, bias=None, residual=None, beta=1.0, is_gelu=False):
     """Microscaled FP4 GEMM (lyraq_gemm_fp4), weight first as in gemm_with_residual_and_bias_fp8: Y[m,n] = epi(X W^T + beta * R + bias) for
     two Fp4Tensors of one format."""
-    m, n = X.rows, W.rows
-    if X.fmt != W.fmt or X.k != W.k or tuple(Y.shape) != (m, n):
+    if X.fmt != W.fmt or X.k != W.k:
         raise ValueError("shape or format mismatch")
-    X.check()
-    W.check()
-    check_epilogue(Y.dtype, bias, residual, m, n)
-    here, stream = _here()
-    st = _lib.lib().lyraq_gemm_fp4(_at(X.codes, here), _at(X.scales, here), _at(X.tensor_scale, here), _at(W.codes, here), _at(W.scales, here),
-                                   _at(W.tensor_scale, here), FP4_FORMATS[X.fmt], _at(Y, here), _dt(Y), _at(bias, here), _at(residual, here), beta,
-                                   EPI_GELU_TANH if is_gelu else EPI_NONE, m, n, X.k, stream)
-    _lib.check(st, "lyraq_gemm_fp4")
-    return Y
-
-
-def check_epilogue(dtype, bias, residual, m, n):
-    if bias is not None and (bias.dtype != dtype or bias.numel() != n):
-        raise ValueError("bias must be [%d] of %s" % (n, dtype))
-    if residual is not None and (residual.dtype != dtype or residual.numel() != m * n or residual.shape[-1] != n):
-        raise ValueError("residual must be [%d, %d] of %s" % (m, n, dtype))
+    return _lib.host().gemm_fp4(X.codes, X.scales, X.tensor_scale, X.rows, W.codes, W.scales, W.tensor_scale, W.rows, X.k, _fp4_format(X.fmt), bias,
+                                residual, beta, EPI_GELU_TANH if is_gelu else EPI_NONE, Y)
 
 
 def gemm_fp8_qk_rope(W, w_scale, X, x_scale, Y, qk_scale, rope_emb, heads, head_dim, bias=None, eps=1e-6):
@@ -389,86 +336,15 @@ def invoke_fused_gate_and_residual(out, y, gate, residual):
     return out
 
 
-_POSITIONS = {torch.int32: S32, torch.int64: 5, torch.float32: F32}
-
-
-def _overlaps(t):
-    """Whether a view may hold one element of memory twice (dimensions ordered by stride, each must step past what lies inside it)."""
-    span = 1
-    for stride, size in sorted((t.stride(d), t.shape[d]) for d in range(t.dim()) if t.shape[d] > 1):
-        if stride < span:
-            return True
-        span = stride * (size - 1) + span
-    return False
-
-
 def rope_axes(plan, positions, q, k=None, q_norm=None, k_norm=None, eps=1e-6, q_out=None, k_out=None):
     """Rotary embedding over several position axes (lyraq_rope_axes).  plan: a rope.AxisRope; q [batch, seq, heads, head_dim] and optionally k
     (its own number of heads), any strides with contiguous heads (views of a packed projection, heads before tokens by transpose);
     positions [batch, seq, axes] or [seq, axes], int32, int64 or fp32, any strides.  q_norm / k_norm [head_dim]: RMS norm weights.  Returns
     (q_out, k_out), created when omitted; they may be q and k."""
-    shape = q.shape
-    if len(shape) != 4:
-        raise ValueError("expected q [batch, seq, heads, head_dim]")
-    batch, seq, hq, d = shape
-    dt = q.dtype
-    here, stream = _here()
-
-    def heads(t, out, norm, name):
-        """Addresses and strides of one of q and k: (in, strides, out, strides, norm, number of heads, out tensor)."""
-        if t is None:
-            if out is not None or norm is not None:
-                raise ValueError("%s_out or %s_norm without %s" % (name, name, name))
-            return None, (0, 0, 0), None, (0, 0, 0), None, 0, None
-        own = out is None
-        if own:
-            out = torch.empty(t.shape, dtype=dt, device=t.device)
-        s, o = t.shape, out.shape
-        if len(s) != 4 or s[0] != batch or s[1] != seq or s[3] != d or o != s or t.dtype != dt or out.dtype != dt:
-            raise ValueError("%s and its output must be [%d, %d, heads, %d] of %s" % (name, batch, seq, d, dt))
-        if t.get_device() != here or out.get_device() != here:
-            raise ValueError("%s is on %s, but the current device is cuda:%d" % (name, t.device, here))
-        ts, os = t.stride(), out.stride()
-        if d > 1 and (ts[3] != 1 or os[3] != 1):
-            raise ValueError("%s: heads must be contiguous" % name)
-        if not own and not out.is_contiguous() and _overlaps(out):
-            raise ValueError("%s_out has overlapping elements" % name)
-        if norm is not None and (norm.dtype != dt or norm.shape != (d,)):
-            raise ValueError("%s_norm must be [%d] of %s" % (name, d, dt))
-        if batch == 1 or seq == 1 or s[2] == 1:     # the stride of a dimension of one is anything
-            ts, os = ([v[i] if s[i] > 1 else 0 for i in range(3)] for v in (ts, os))
-        return t.data_ptr(), ts[:3], out.data_ptr(), os[:3], _at(norm, here, "%s_norm" % name), s[2], out
-
-    qp, qs, qo, qos, qn, hq, q_out = heads(q, q_out, q_norm, "q")
-    kp, ks, ko, kos, kn, hk, k_out = heads(k, k_out, k_norm, "k")
-    kind = _POSITIONS.get(positions.dtype)
-    if kind is None:
-        raise TypeError("positions must be int32, int64 or fp32")
-    ps, pt = positions.shape, positions.stride()
-    if positions.get_device() != here or ps[-1] != plan.axes or ps[-2] != seq or len(ps) not in (2, 3) or (len(ps) == 3 and ps[0] != batch):
-        raise ValueError("positions must be [%d, %d, %d] or [%d, %d] on cuda:%d" % (batch, seq, plan.axes, seq, plan.axes, here))
-    args = _lib.ROPE_AXES.pack(qp or 0, kp or 0, *qs, *ks, qo or 0, ko or 0, *qos, *kos, qn or 0, kn or 0, positions.data_ptr(), pt[0] if len(ps) == 3 else 0,
-                               pt[-2], pt[-1], _at(plan.turns, here, "the plan"), _at(plan.axis, here, "the plan"), kind, _dt(q), hq, hk, d, plan.pairs,
-                               1 if plan.interleaved else 0, eps, batch, seq)
-    _lib.check(_lib.lib().lyraq_rope_axes(args, stream), "lyraq_rope_axes")
-    return q_out, k_out
+    return _lib.host().rope_axes(plan.turns, plan.axis, plan.pairs, plan.axes, plan.interleaved, positions, q, k, q_norm, k_norm, eps, q_out, k_out)
 
 
 _NORMS = {"none": 0, "rms": 1, "layer": 2}
-
-
-def _row_strides(t, what, shape, dtype, here):
-    """(address, batch stride, row stride) of a [batch, seq, dim] view whose rows are contiguous."""
-    if t.shape != shape or t.dtype != dtype:
-        raise ValueError("%s must be %s of %s" % (what, list(shape), dtype))
-    if t.get_device() != here:
-        raise ValueError("%s is on %s, but the current device is cuda:%d" % (what, t.device, here))
-    if t.is_contiguous():
-        return t.data_ptr(), shape[1] * shape[2], shape[2]
-    b, r, e = t.stride()
-    if e != 1 and shape[2] > 1:
-        raise ValueError("%s: rows must be contiguous" % what)
-    return t.data_ptr(), b if shape[0] > 1 else 0, r if shape[1] > 1 else 0
 
 
 def gated_residual_norm(y, x, gate=None, scale=None, shift=None, post_weight=None, pre_weight=None, post="rms", pre="rms", residual_scale=1.0,
@@ -478,62 +354,18 @@ def gated_residual_norm(y, x, gate=None, scale=None, shift=None, post_weight=Non
     Returns (x_out, h).  gate, scale, shift: [batch, dim] (rows may lie apart, as chunks of one modulation tensor do) or [dim]; post: "none",
     "rms" or "layer", pre: "rms" or "layer".  x_out is created when omitted, h when no other form of it is asked for.  qf8 (uint8, contiguous,
     with f8_scale) takes e4m3 codes of h, q4 (an Fp4Tensor of [batch * seq, dim]) its FP4 form.  x_out may be x itself, h may be y."""
-    shape, dt = y.shape, y.dtype
-    if len(shape) != 3:
-        raise ValueError("expected [batch, seq, dim]")
-    batch, seq, dim = shape
     if post not in _NORMS or pre not in _NORMS or pre == "none":
         raise ValueError("unknown norm %r / %r" % (post, pre))
-    here, stream = _here()
-    rows_y = _row_strides(y, "y", shape, dt, here)
-    rows_x = _row_strides(x, "x", shape, dt, here)
-    rows_h = (0, 0, 0)
-    if x_out is None:
-        x_out = torch.empty(shape, dtype=dt, device=y.device)
-        rows_o = x_out.data_ptr(), seq * dim, dim
+    if q4 is None:
+        codes = scales = tensor_scale = None
+        fmt = 0
     else:
-        rows_o = _output_rows(x_out, "x_out", shape, dt, here)
-    if h is not None:
-        rows_h = _output_rows(h, "h", shape, dt, here)
-    elif qf8 is None and q4 is None:
-        h = torch.empty(shape, dtype=dt, device=y.device)
-        rows_h = h.data_ptr(), seq * dim, dim
-
-    def per_batch(t, what):
-        if t is None:
-            return 0, 0
-        s = t.shape
-        if t.dtype != dt or t.get_device() != here or s[-1] != dim or len(s) > 2 or (len(s) == 2 and s[0] != batch) or (dim > 1 and t.stride(-1) != 1):
-            raise ValueError("%s must be [%d, %d] or [%d] of %s on cuda:%d" % (what, batch, dim, dim, dt, here))
-        return t.data_ptr(), t.stride(0) if len(s) == 2 and batch > 1 else 0
-
-    def weight(t, what):
-        if t is not None and (t.dtype != dt or t.shape != (dim,)):
-            raise ValueError("%s must be [%d] of %s" % (what, dim, dt))
-        return _at(t, here, what) or 0
-
-    (gp, gs), (sp, ss), (hp, hs) = per_batch(gate, "gate"), per_batch(scale, "scale"), per_batch(shift, "shift")
-    if qf8 is not None and (f8_scale is None or f8_scale.dtype != torch.float32 or qf8.dtype != torch.uint8 or qf8.numel() != batch * seq * dim):
-        raise ValueError("qf8 must be uint8 of y's size, with an fp32 f8_scale")
-    codes = scales = tensor_scale = fmt = 0
-    if q4 is not None:
-        if q4.rows != batch * seq or q4.k != dim:
-            raise ValueError("q4 must be [%d, %d]" % (batch * seq, dim))
+        if q4.k != y.shape[-1] or q4.rows * q4.k != y.numel():
+            raise ValueError("q4 must be [batch * seq, dim]")
         q4.check()
-        codes, scales, tensor_scale, fmt = _at(q4.codes, here), _at(q4.scales, here), _at(q4.tensor_scale, here) or 0, FP4_FORMATS[q4.fmt]
-    args = _lib.GATED_NORM.pack(rows_y[0], rows_x[0], rows_y[1], rows_y[2], rows_x[1], rows_x[2], rows_o[0], rows_h[0], rows_o[1], rows_o[2], rows_h[1],
-                                rows_h[2], _at(qf8, here, "qf8") or 0, _at(f8_scale, here, "f8_scale") or 0, codes, scales, tensor_scale, fmt, gp, sp, hp, gs,
-                                ss, hs, weight(post_weight, "post_weight"), weight(pre_weight, "pre_weight"), _NORMS[post], _NORMS[pre], residual_scale,
-                                eps, _dt(y), batch, seq, dim)
-    _lib.check(_lib.lib().lyraq_gated_residual_norm(args, stream), "lyraq_gated_residual_norm")
-    return x_out, h
-
-
-def _output_rows(t, what, shape, dtype, here):
-    rows = _row_strides(t, what, shape, dtype, here)
-    if (shape[1] > 1 and rows[2] < shape[2]) or (shape[0] > 1 and rows[1] < shape[2]):
-        raise ValueError("%s has overlapping rows" % what)
-    return rows
+        codes, scales, tensor_scale, fmt = q4.codes, q4.scales, q4.tensor_scale, FP4_FORMATS[q4.fmt]
+    return _lib.host().gated_residual_norm(y, x, gate, scale, shift, post_weight, pre_weight, _NORMS[post], _NORMS[pre], residual_scale, eps, x_out, h,
+                                           qf8, f8_scale, codes, scales, tensor_scale, fmt)
 
 
 def invoke_load_lora(weight, lora, alpha):

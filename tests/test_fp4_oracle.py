@@ -101,7 +101,3 @@ def test_python_side_refuses_parts_that_do_not_fit(lib):
             bad.check()
     with pytest.raises(ValueError):
         ops.Fp4Tensor.empty(4, 64, "int4", device="cpu")
-    with pytest.raises(ValueError):
-        ops._rows_of(torch.empty(64, 4).t())
-    with pytest.raises(ValueError):
-        ops.quant_fp4(torch.empty(4, 64))                            # not on a GPU
