@@ -118,7 +118,7 @@ template<int FORMAT> __device__ __forceinline__ Fp4Block fp4_block(uint32_t amax
 template<int FORMAT> __device__ __forceinline__ uint32_t fp4_encode8(const float* x, const Fp4Block& b)
 {
     float q[8];
-    if (b.plain) {   // with t = r = 0 every quotient comes out as 0
+    if (FORMAT != LYRAQ_NVFP4 || b.plain) {   // with t = r = 0 every quotient comes out as 0
         const float2 r2 = make_float2(b.r, b.r);
         const float2 m2 = make_float2(-b.t, -b.t);
 #pragma unroll
@@ -137,7 +137,8 @@ template<int FORMAT> __device__ __forceinline__ uint32_t fp4_encode8(const float
             q[j] = b.t > 0.0f ? x[j] / b.t : 0.0f;
         }
     }
-    return f32x8_to_e2m1x8(q);
+    const uint32_t codes = f32x8_to_e2m1x8(q);
+    return FORMAT == LYRAQ_NVFP4 || b.plain ? codes : 0u;   // mxfp4: not plain is not finite
 }
 
 // Largest magnitude of a 16-byte vector of T, as fp32 bits (see fp4_block).

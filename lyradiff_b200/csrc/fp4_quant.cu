@@ -11,24 +11,22 @@ int device_sm_count();  // gemm_dense.cu
 // each quarter of the 128: whole lines of every row, and scale words that fill 32-byte sectors.
 template<typename T, int FORMAT>
 __global__ void __launch_bounds__(256)
-fp4_quant_kernel(uint8_t* q, uint8_t* sf, const T* x, size_t ldx, const float* tensor_scale, size_t rows, size_t k, unsigned chunks,
-                 unsigned octets, unsigned tasks)
+fp4_quant_kernel(uint8_t* q, uint8_t* sf, const T* x, size_t ldx, const float* tensor_scale, size_t rows, size_t k, unsigned blocks_k, int warps_k_log2)
 {
     constexpr int kGroup  = fp4_group(FORMAT);
     constexpr int kBlocks = 32 / kGroup;            // of one thread
     constexpr int kPer    = 16 / (int)sizeof(T);    // values of a 16-byte vector
     constexpr int kVecs   = 32 / kPer;
     grid_launch_dependents();
-    const unsigned task  = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);   // 32 bits: a 64-bit division costs more than a block of values
-    const unsigned lane  = threadIdx.x & 31;
-    const unsigned rest  = task / chunks;
-    const unsigned chunk = task - rest * chunks;
-    const unsigned rb    = rest / octets;
-    const unsigned octet = rest - rb * octets;
+    // a block's eight warps: 2^warps_k_log2 neighbouring pieces of 128 columns, the rest of them further rows
+    const unsigned by = blockIdx.x / blocks_k, bx = blockIdx.x - by * blocks_k;
+    const unsigned warp  = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const unsigned chunk = (bx << warps_k_log2) + (warp & ((1u << warps_k_log2) - 1u));
+    const unsigned octet = (by << (3 - warps_k_log2)) + (warp >> warps_k_log2);      // 16 to 128 rows
     const unsigned i     = lane >> 2, j = lane & 3;
-    const size_t   row   = (size_t)rb * 128 + 2 * octet + (i >> 2) + 32 * (i & 3);
+    const size_t   row   = (size_t)(octet >> 4) * 128 + 2 * (octet & 15) + (i >> 2) + 32 * (i & 3);
     const size_t   col   = (size_t)chunk * 128 + (size_t)j * 32;
-    const bool     in    = task < tasks && row < rows && col < k;   // k is a multiple of 32: a thread's values are there or not
+    const bool     in    = row < rows && col < k;   // k is a multiple of 32: a thread's values are there or not
     grid_dependency_wait();
 
     Vec16 v[kVecs];
@@ -77,7 +75,7 @@ fp4_quant_kernel(uint8_t* q, uint8_t* sf, const T* x, size_t ldx, const float* t
         word |= __shfl_xor_sync(0xffffffffu, word, 2);
     }
     const size_t atom = (size_t)chunk * (4 / kLanes) + j / kLanes, atoms = fp4_atoms(k, FORMAT);
-    if (j % kLanes == 0 && task < tasks && row < rows && atom < atoms) {
+    if (j % kLanes == 0 && row < rows && atom < atoms) {
         *reinterpret_cast<uint32_t*>(sf + fp4_scale_offset(row, atoms, atom)) = word;
     }
 }
@@ -164,16 +162,20 @@ static int run_quant(uint8_t* q, uint8_t* sf, const void* x, int dtype, size_t l
                      size_t k, cudaStream_t s)
 {
     const size_t chunks  = (k + 127) / 128;
-    const size_t octets  = rows >= 32 ? 16 : (rows + 1) / 2;     // fewer than 32 rows lie in the first quarter of their 128
-    const size_t tasks   = (rows + 127) / 128 * octets * chunks;  // one warp each
-    const size_t blocks  = (tasks + 7) / 8;
-    if (blocks > 0x0fffffffu) {   // the number of a warp stays within 32 bits
+    const size_t octets  = rows >= 32 ? (rows + 127) / 128 * 16 : (rows + 1) / 2;   // fewer than 32 rows lie in the first quarter of their 128
+    int          warps_k = 0;
+    while (warps_k < 3 && (size_t)1 << warps_k < chunks) {
+        ++warps_k;
+    }
+    const size_t blocks_k = (chunks + ((size_t)1 << warps_k) - 1) >> warps_k;
+    const size_t blocks   = blocks_k * ((octets + ((size_t)8 >> warps_k) - 1) >> (3 - warps_k));
+    if (blocks > 0x7fffffffu) {
         return LYRAQ_ERR_UNSUPPORTED;
     }
     auto launch = [&](auto* kernel, auto type) {
         using T = decltype(type);
-        return launch_kernel(kernel, (unsigned)blocks, 256u, (size_t)0, s, 1u, q, sf, (const T*)x, ldx, tensor_scale, rows, k, (unsigned)chunks,
-                             (unsigned)octets, (unsigned)tasks);
+        return launch_kernel(kernel, (unsigned)blocks, 256u, (size_t)0, s, 1u, q, sf, (const T*)x, ldx, tensor_scale, rows, k, (unsigned)blocks_k,
+                             warps_k);
     };
     auto pick = [&](auto type) {
         using T = decltype(type);

@@ -41,8 +41,9 @@ struct NormParams {
     float        r, eps;
 };
 
-// FORMAT: -1 without an FP4 output.
-template<typename T, int VPT, int FORMAT, bool WARP>
+// FORMAT: -1 without an FP4 output.  ALL: every parameter and the new stream are there.  FULL: every vector of every thread is.  The kernel is bound by
+// the instructions it issues, and asking took a sixth of them: [4608, 3072] 25.1 us without, 22.3 with ALL, 21.5 with both.
+template<typename T, int VPT, int FORMAT, bool WARP, bool ALL, bool FULL>
 __global__ void __launch_bounds__(WARP ? 256 : 512)
 norm_residual_kernel(const NormParams p)
 {
@@ -86,7 +87,7 @@ norm_residual_kernel(const NormParams p)
         const int vi = t + i * threads;
         yv[i] = Vec16{};
         xv[i] = Vec16{};
-        if (vi < nvec) {
+        if (FULL || vi < nvec) {
             yv[i] = ld_16(yr + vi * 8);
             xv[i] = ld_16(xr + vi * 8);
         }
@@ -115,7 +116,7 @@ norm_residual_kernel(const NormParams p)
         float2       a  = make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            if (t + i * threads < nvec) {
+            if (FULL || t + i * threads < nvec) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     v[i][j] = add_f32x2(v[i][j], m2);
@@ -132,20 +133,20 @@ norm_residual_kernel(const NormParams p)
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
         const int vi = t + i * threads;
-        if (vi < nvec) {
+        if (FULL || vi < nvec) {
             float2 f[4], c[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 c[j] = make_float2(inv, inv);
             }
-            if (p.w1 != nullptr) {
+            if (ALL || p.w1 != nullptr) {
                 unpack4x2<T>(ld_nc_16_keep(reinterpret_cast<const T*>(p.w1) + vi * 8), f);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     c[j] = mul_f32x2(c[j], f[j]);
                 }
             }
-            if (p.gate != nullptr) {
+            if (ALL || p.gate != nullptr) {
                 unpack4x2<T>(ld_nc_16_keep(gate + vi * 8), f);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -161,7 +162,7 @@ norm_residual_kernel(const NormParams p)
                 o[2 * j]     = v[i][j].x;
                 o[2 * j + 1] = v[i][j].y;
             }
-            if (p.x_out != nullptr) {
+            if (ALL || p.x_out != nullptr) {
                 st_16(xo + vi * 8, pack8<T>(o));
             }
         }
@@ -171,7 +172,7 @@ norm_residual_kernel(const NormParams p)
     float2       sq = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-        if (t + i * threads < nvec) {
+        if (FULL || t + i * threads < nvec) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 v[i][j] = add_f32x2(v[i][j], m2);
@@ -190,7 +191,7 @@ norm_residual_kernel(const NormParams p)
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
         const int  vi = t + i * threads;
-        const bool in = vi < nvec;
+        const bool in = FULL || vi < nvec;
         Vec16      o{};
         if (in) {
             float2 f[4], c[4];
@@ -199,14 +200,14 @@ norm_residual_kernel(const NormParams p)
             for (int j = 0; j < 4; ++j) {
                 c[j] = make_float2(inv, inv);
             }
-            if (p.w2 != nullptr) {
+            if (ALL || p.w2 != nullptr) {
                 unpack4x2<T>(ld_nc_16_keep(reinterpret_cast<const T*>(p.w2) + vi * 8), f);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     c[j] = mul_f32x2(c[j], f[j]);
                 }
             }
-            if (p.scale != nullptr) {
+            if (ALL || p.scale != nullptr) {
                 unpack4x2<T>(ld_nc_16_keep(scale + vi * 8), f);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -217,7 +218,7 @@ norm_residual_kernel(const NormParams p)
             for (int j = 0; j < 4; ++j) {
                 f[j] = make_float2(0.0f, 0.0f);
             }
-            if (p.shift != nullptr) {
+            if (ALL || p.shift != nullptr) {
                 unpack4x2<T>(ld_nc_16_keep(shift + vi * 8), f);
             }
 #pragma unroll
@@ -261,8 +262,9 @@ norm_residual_kernel(const NormParams p)
     }
 }
 
-// Threads of a row.  Up to 1024 elements a warp has it (up to four vectors a lane) and no barrier; longer rows have a block, with three or
-// four vectors a thread where there are rows enough to fill the chip, and one or two where a call is latency.
+// Threads of a row.  Up to 1024 elements a warp has it (up to four vectors a lane) and no barrier; longer rows have a block, with three
+// vectors a thread where there are rows enough to fill the chip ([4608, 3072], us: one 34.8, two 28.8, three 25.4, four 28.5; a thread's part of the
+// three sums weighs more the fewer it has), and one where a call is latency; more only where 512 threads cannot have the row otherwise.
 struct NormSplit {
     int  vpt, threads;
     bool warp;
@@ -273,10 +275,9 @@ static NormSplit norm_split(size_t rows, int dim, int sms)
     if (nvec <= 128 && (nvec <= 32 || rows > (size_t)sms * 2)) {
         return NormSplit{nvec <= 32 ? 1 : nvec <= 64 ? 2 : 4, 256, true};
     }
-    const int want = rows > (size_t)sms * 2 ? 3 : 1;
-    int       vpt  = want;
+    int vpt = rows > (size_t)sms * 2 ? 3 : 1;
     while ((nvec + vpt - 1) / vpt > 512) {
-        vpt = vpt < 3 ? vpt + 1 : 4;
+        ++vpt;
     }
     return NormSplit{vpt, ((nvec + vpt - 1) / vpt + 31) / 32 * 32, false};
 }
@@ -336,23 +337,30 @@ extern "C" int lyraq_gated_residual_norm(const lyraq_gated_norm_t* a, void* stre
     auto launch = [&](auto* kernel) {
         return launch_kernel(kernel, grid, (unsigned)split.threads, (size_t)0, (cudaStream_t)stream, 1u, p);
     };
-    auto pick_split = [&](auto type, auto fmt) {
-        using T              = decltype(type);
-        constexpr int kFmt   = decltype(fmt)::value;
+    const bool all  = p.w1 != nullptr && p.gate != nullptr && p.w2 != nullptr && p.scale != nullptr && p.shift != nullptr && p.x_out != nullptr;
+    const bool full = !split.warp && p.dim == 8 * split.vpt * split.threads;
+    auto pick_split = [&](auto type, auto fmt, auto every) {
+        using T             = decltype(type);
+        constexpr int  kFmt = decltype(fmt)::value;
+        constexpr bool kAll = decltype(every)::value;
         if (split.warp) {
-            return split.vpt == 1   ? launch(norm_residual_kernel<T, 1, kFmt, true>)
-                   : split.vpt == 2 ? launch(norm_residual_kernel<T, 2, kFmt, true>)
-                                    : launch(norm_residual_kernel<T, 4, kFmt, true>);
+            return split.vpt == 1   ? launch(norm_residual_kernel<T, 1, kFmt, true, kAll, false>)
+                   : split.vpt == 2 ? launch(norm_residual_kernel<T, 2, kFmt, true, kAll, false>)
+                                    : launch(norm_residual_kernel<T, 4, kFmt, true, kAll, false>);
         }
-        return split.vpt == 1   ? launch(norm_residual_kernel<T, 1, kFmt, false>)
-               : split.vpt == 2 ? launch(norm_residual_kernel<T, 2, kFmt, false>)
-               : split.vpt == 3 ? launch(norm_residual_kernel<T, 3, kFmt, false>)
-                                : launch(norm_residual_kernel<T, 4, kFmt, false>);
+        return split.vpt == 3 && kAll && full ? launch(norm_residual_kernel<T, 3, kFmt, false, true, true>)
+               : split.vpt == 1               ? launch(norm_residual_kernel<T, 1, kFmt, false, kAll, false>)
+               : split.vpt == 2               ? launch(norm_residual_kernel<T, 2, kFmt, false, kAll, false>)
+               : split.vpt == 3               ? launch(norm_residual_kernel<T, 3, kFmt, false, kAll, false>)
+                                              : launch(norm_residual_kernel<T, 4, kFmt, false, kAll, false>);
+    };
+    auto pick_all = [&](auto type, auto fmt) {
+        return all ? pick_split(type, fmt, std::integral_constant<bool, true>{}) : pick_split(type, fmt, std::integral_constant<bool, false>{});
     };
     auto pick_fmt = [&](auto type) {
-        return a->q4 == nullptr                ? pick_split(type, std::integral_constant<int, -1>{})
-               : a->q4_format == LYRAQ_NVFP4   ? pick_split(type, std::integral_constant<int, LYRAQ_NVFP4>{})
-                                               : pick_split(type, std::integral_constant<int, LYRAQ_MXFP4>{});
+        return a->q4 == nullptr                ? pick_all(type, std::integral_constant<int, -1>{})
+               : a->q4_format == LYRAQ_NVFP4   ? pick_all(type, std::integral_constant<int, LYRAQ_NVFP4>{})
+                                               : pick_all(type, std::integral_constant<int, LYRAQ_MXFP4>{});
     };
     const cudaError_t e = a->dtype == LYRAQ_BF16 ? pick_fmt(__nv_bfloat16{}) : pick_fmt(__half{});
     return cuda_status(e, "cudaLaunchKernelEx(norm_residual_kernel)");

@@ -108,6 +108,23 @@ template<typename T> struct Piece<T, 1> {
 template<> __device__ __forceinline__ void Piece<__half, 1>::load(const __half* p) { v = __ushort_as_half((unsigned short)ld_u16(p)); }
 template<> __device__ __forceinline__ void Piece<__nv_bfloat16, 1>::load(const __nv_bfloat16* p) { v = __ushort_as_bfloat16((unsigned short)ld_u16(p)); }
 
+// VEC floats of shared memory, on 16 bytes where VEC is a multiple of four
+template<int VEC> __device__ __forceinline__ void load_floats(const float* p, float* f)
+{
+    if constexpr (VEC % 4 == 0) {
+#pragma unroll
+        for (int j = 0; j < VEC; j += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(p + j);
+            f[j] = v.x; f[j + 1] = v.y; f[j + 2] = v.z; f[j + 3] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            f[j] = p[j];
+        }
+    }
+}
+
 // VEC: pairs of a lane's unit; NU: units of a lane (more than one only where 32 lanes of small units do not span a head); HALVES: pair i is (x[i], x[i + pairs]), else
 // (x[2 i], x[2 i + 1]); NORM: q or k is normalised.
 template<typename T, int VEC, int NU, bool HALVES, bool NORM>
@@ -128,7 +145,7 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(const RopeAxesParams p)
             // half turns in [-1, 1)
             sincospif((float)(int)(uint32_t)(phase >> 32) * 4.656612873077393e-10f, &cs.y, &cs.x);
         }
-        turn_c[i]                            = cs.x;
+        turn_c[i]                                = cs.x;
         turn_c[p.tokens_per_block * p.pairs + i] = cs.y;
     }
     __syncthreads();
@@ -155,21 +172,8 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(const RopeAxesParams p)
         for (int u = 0; u < NU; ++u) {
             if (turns[u]) {
                 const float* c = turn_c + tk * p.pairs + (lane + u * lanes) * VEC;
-                const float* n = c + p.tokens_per_block * p.pairs;
-                if constexpr (VEC >= 4) {
-#pragma unroll
-                    for (int j = 0; j < VEC; j += 4) {
-                        const float4 c4 = *reinterpret_cast<const float4*>(c + j), n4 = *reinterpret_cast<const float4*>(n + j);
-                        cosine[u][j] = c4.x; cosine[u][j + 1] = c4.y; cosine[u][j + 2] = c4.z; cosine[u][j + 3] = c4.w;
-                        sine[u][j] = n4.x; sine[u][j + 1] = n4.y; sine[u][j + 2] = n4.z; sine[u][j + 3] = n4.w;
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        cosine[u][j] = c[j];
-                        sine[u][j]   = n[j];
-                    }
-                }
+                load_floats<VEC>(c, cosine[u]);
+                load_floats<VEC>(c + p.tokens_per_block * p.pairs, sine[u]);
             }
         }
         const T* base_in[2];
@@ -237,7 +241,7 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(const RopeAxesParams p)
 #pragma unroll
                         for (int u = 0; u < NU; ++u) {
                             if (on[i] && there[u]) {
-                                Piece<T, VEC> wa, wc;
+                                Piece<T, VEC> wa, wc;   // from L1; in shared memory as fp32 their bank conflicts cost 5 us of 26
                                 float         f[2 * VEC];
                                 wa.load(w[i] + at_a[u]);
                                 wc.load(w[i] + at_b[u]);
@@ -339,14 +343,15 @@ extern "C" int lyraq_rope_axes(const lyraq_rope_axes_t* a, void* stream)
     while ((1 << p.lanes_log2) < units && p.lanes_log2 < 5) {
         ++p.lanes_log2;
     }
-    // Groups: all heads of a token in as few rounds as 256 threads make of them, the rounds equally full.  Tokens: enough to share the
-    // cosines' cost, few enough to fill the chip; where there are few, a token's heads are dealt to several blocks.
+    // Groups: two heads each at a time (24 heads as 12 groups of two take 65 us for 32760 tokens of 128, as 24 of one 83), all of a token in as few
+    // rounds as 128 threads make of them, the rounds equally full (48 normalised heads with 192 threads 26.5 us, with 96 23.7).  Tokens: enough to share the cosines' cost, few enough to fill the chip;
+    // where there are few, a token's heads are dealt to several blocks.
     const int lanes  = 1 << p.lanes_log2;
-    const int most   = 256 / lanes;
+    const int most   = 128 / lanes;
     p.chunks         = p.tokens >= (unsigned)sms * 2 ? 1 : (heads + most - 1) / most;
     p.share          = (heads + p.chunks - 1) / p.chunks;
-    const int rounds = (p.share + most - 1) / most;
-    p.groups         = (p.share + rounds - 1) / rounds;
+    const int rounds = (p.share + 2 * most - 1) / (2 * most);
+    p.groups         = (p.share + 2 * rounds - 1) / (2 * rounds);
     p.tokens_per_block = p.tokens >= (unsigned)sms * 32 ? 4 : p.tokens >= (unsigned)sms * 16 ? 2 : 1;
     const unsigned threads = (unsigned)((p.groups * lanes + 31) / 32 * 32);
     const size_t   blocks  = ((size_t)p.tokens + p.tokens_per_block - 1) / p.tokens_per_block * (size_t)p.chunks;
@@ -354,8 +359,8 @@ extern "C" int lyraq_rope_axes(const lyraq_rope_axes_t* a, void* stream)
         return LYRAQ_ERR_UNSUPPORTED;
     }
     const unsigned grid = (unsigned)blocks;
-    const size_t smem = sizeof(float2) * (size_t)p.tokens_per_block * (size_t)(p.pairs > 0 ? p.pairs : 1);
     const bool   norm = a->q_norm != nullptr || a->k_norm != nullptr;
+    const size_t smem = 2 * sizeof(float) * (size_t)p.tokens_per_block * (size_t)p.pairs;
     auto launch = [&](auto* kernel) { return launch_kernel(kernel, grid, threads, smem, (cudaStream_t)stream, 1u, p); };
     auto pick = [&](auto type, auto halves, auto normed) {
         using T           = decltype(type);
