@@ -205,7 +205,7 @@ int lyraq_quant_fp4(uint8_t* q, uint8_t* q_scale, const void* x, int x_dtype, si
     if (format != LYRAQ_NVFP4 && format != LYRAQ_MXFP4) {
         return LYRAQ_ERR_INVALID_ARG;
     }
-    if (rows * k == 0) {
+    if (rows == 0 || k == 0) {
         return LYRAQ_OK;
     }
     const int st = check_fp4(q, q_scale, x, x_dtype, ldx, format, rows, k);
@@ -221,7 +221,7 @@ int lyraq_weight_quant_fp4(uint8_t* qw, uint8_t* w_scale, float* tensor_scale, c
     if (format != LYRAQ_NVFP4 && format != LYRAQ_MXFP4) {
         return LYRAQ_ERR_INVALID_ARG;
     }
-    if (n * k == 0) {
+    if (n == 0 || k == 0) {
         return LYRAQ_OK;
     }
     const int st = check_fp4(qw, w_scale, w, w_dtype, k, format, n, k);

@@ -294,11 +294,12 @@ extern "C" int lyraq_gated_residual_norm(const lyraq_gated_norm_t* a, void* stre
         (a->pre != LYRAQ_NORM_RMS && a->pre != LYRAQ_NORM_LAYER)) {
         return LYRAQ_ERR_INVALID_ARG;
     }
+    if ((a->dtype != LYRAQ_F16 && a->dtype != LYRAQ_BF16) || (a->dim & 7u) != 0 || a->dim > 16384 || a->batch > 0x7fffffffu ||
+        a->seq_len > 0x7fffffffu || a->batch * a->seq_len > 0x7fffffffu) {
+        return LYRAQ_ERR_UNSUPPORTED;
+    }
     if (a->batch * a->seq_len * a->dim == 0) {
         return LYRAQ_OK;
-    }
-    if ((a->dtype != LYRAQ_F16 && a->dtype != LYRAQ_BF16) || (a->dim & 7u) != 0 || a->dim > 16384 || a->batch > 0x7fffffffu || a->seq_len > 0x7fffffffu || a->batch * a->seq_len > 0x7fffffffu) {
-        return LYRAQ_ERR_UNSUPPORTED;
     }
     if (a->y == nullptr || a->x == nullptr || (a->x_out == nullptr && a->h == nullptr && a->qf8 == nullptr && a->q4 == nullptr) ||
         (a->qf8 != nullptr && a->f8_scale == nullptr) || (a->q4 != nullptr && a->q4_scales == nullptr)) {

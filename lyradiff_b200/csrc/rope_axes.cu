@@ -295,13 +295,13 @@ extern "C" int lyraq_rope_axes(const lyraq_rope_axes_t* a, void* stream)
         a->head_dim <= 0 || a->pairs < 0) {
         return LYRAQ_ERR_INVALID_ARG;
     }
+    if ((a->dtype != LYRAQ_F16 && a->dtype != LYRAQ_BF16) || a->head_dim > 256 || (a->head_dim & 1) != 0 || a->pairs > a->head_dim / 2 ||
+        a->q_heads > 65536 || a->k_heads > 65536 || a->batch > 0x7fffffffu || a->seq_len > 0x7fffffffu || a->batch * a->seq_len > 0x7fffffffu) {
+        return LYRAQ_ERR_UNSUPPORTED;
+    }
     const int heads = a->q_heads + a->k_heads;
     if (a->batch * a->seq_len == 0 || heads == 0) {
         return LYRAQ_OK;
-    }
-    if ((a->dtype != LYRAQ_F16 && a->dtype != LYRAQ_BF16) || a->head_dim > 256 || (a->head_dim & 1) != 0 || 2 * a->pairs > a->head_dim || heads > 65536 || a->q_heads > 65536 || a->k_heads > 65536 ||
-        a->batch > 0x7fffffffu || a->seq_len > 0x7fffffffu || a->batch * a->seq_len > 0x7fffffffu) {
-        return LYRAQ_ERR_UNSUPPORTED;
     }
     if ((a->q_heads > 0 && (a->q == nullptr || a->q_out == nullptr)) || (a->k_heads > 0 && (a->k == nullptr || a->k_out == nullptr)) ||
         (a->pairs > 0 && (a->positions == nullptr || a->turns == nullptr || a->axis == nullptr))) {
