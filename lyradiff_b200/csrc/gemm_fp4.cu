@@ -341,12 +341,6 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             for (int tile = unit; ok && tile < num_tiles; tile += n_units, ++local) {
                 const int      buf       = S::kAccBufs == 2 ? (local & 1) : 0;
                 const uint32_t acc_phase = (uint32_t)(S::kAccBufs == 2 ? local >> 1 : local) & 1u;
-                if (!mbar_wait_warp(tmem_empty_bar(buf), acc_phase ^ 1u, abort_flag)) {
-                    report_timeout(p.status, 0x5200u | (unsigned)buf);
-                    *abort_flag = 1;
-                    break;
-                }
-                tc_fence_after_sync();
                 const uint32_t d_tmem = tmem_base + (uint32_t)(buf * BLOCK_N);
                 for (int kb = 0; kb < num_kb; ++kb) {
                     if (!mbar_wait_warp(full_bar(stage), phase, abort_flag)) {
@@ -365,25 +359,41 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                     const uint32_t sfb    = sfa + S::kAtoms * 4;
                     const int      steps  = min(kBlockK, p.K - kb * kBlockK + 63) / 64;   // MMAs of this K block
                     const bool     last   = kb + 1 == num_kb;
-                    if (elect_one()) {
+                    auto copy_scales = [&]() {
 #pragma unroll
                         for (int a = 0; a < S::kAtoms; ++a) {
-                            if (a * (4 / S::kAtoms) < steps) {
-                                // in tensor memory the row blocks of an atom stand side by side
-                                tmem_copy_scales<CTAS>(sfa + a * 4, sadesc + (uint64_t)(a * 32));
+                            tmem_copy_scales<CTAS>(sfa + a * 4, sadesc + (uint64_t)(a * 32));
+                            // in tensor memory the row blocks of an atom stand side by side
 #pragma unroll
-                                for (int rb = 0; rb < S::kSbBlocks; ++rb) {
-                                    tmem_copy_scales<CTAS>(sfb + a * (4 * S::kSbBlocks) + rb * 4, sbdesc + (uint64_t)((rb * S::kAtoms + a) * 32));
-                                }
+                            for (int rb = 0; rb < S::kSbBlocks; ++rb) {
+                                tmem_copy_scales<CTAS>(sfb + a * (4 * S::kSbBlocks) + rb * 4, sbdesc + (uint64_t)((rb * S::kAtoms + a) * 32));
+                            }
+                        }
+                    };
+                    if (kb == 0) {
+                        // the scales of a tile's first K block are on their way while the epilogue still has the accumulator
+                        if (elect_one()) {
+                            copy_scales();
+                        }
+                        if (!mbar_wait_warp(tmem_empty_bar(buf), acc_phase ^ 1u, abort_flag)) {
+                            report_timeout(p.status, 0x5200u | (unsigned)buf);
+                            *abort_flag = 1;
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after_sync();
+                    }
+                    if (elect_one()) {
+                        if (kb > 0) {
+                            copy_scales();
+                        }
 #pragma unroll
-                                for (int h = 0; h < 4 / S::kAtoms; ++h) {
-                                    const int k = a * (4 / S::kAtoms) + h;
-                                    if (k < steps) {
-                                        mma_fp4<FORMAT, CTAS>(d_tmem, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k),
-                                                              umma_idesc_fp4(FORMAT, kTileM, BLOCK_N, 2u * h), sfa + a * 4,
-                                                              sfb + a * (4 * S::kSbBlocks), (kb > 0 || k > 0) ? 1u : 0u);
-                                    }
-                                }
+                        for (int k = 0; k < 4; ++k) {
+                            constexpr int kPer = 4 / S::kAtoms;   // MMAs of one atom
+                            if (k < steps) {
+                                mma_fp4<FORMAT, CTAS>(d_tmem, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k),
+                                                      umma_idesc_fp4(FORMAT, kTileM, BLOCK_N, 2u * (k % kPer)), sfa + k / kPer * 4,
+                                                      sfb + k / kPer * (4 * S::kSbBlocks), (kb > 0 || k > 0) ? 1u : 0u);
                             }
                         }
                         if (CTAS == 2) {
