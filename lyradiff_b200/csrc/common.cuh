@@ -137,6 +137,27 @@ __device__ __forceinline__ Vec16 ld_nc_16(const void* p)
     return v;
 }
 
+// 32 bytes on a 32-byte address by one lane.  Where a lane owns 32 bytes or more in a row, two 16-byte loads (or stores) of the warp touch every sector
+// twice; one of 32 asks for each once.
+__device__ __forceinline__ void ld_nc_32(const void* p, Vec16& a, Vec16& b)
+{
+    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(a.w[0]), "=r"(a.w[1]), "=r"(a.w[2]), "=r"(a.w[3]), "=r"(b.w[0]), "=r"(b.w[1]), "=r"(b.w[2]), "=r"(b.w[3])
+                 : "l"(p));
+}
+__device__ __forceinline__ void ld_32(const void* p, Vec16& a, Vec16& b)   // memory that the kernel itself writes
+{
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(a.w[0]), "=r"(a.w[1]), "=r"(a.w[2]), "=r"(a.w[3]), "=r"(b.w[0]), "=r"(b.w[1]), "=r"(b.w[2]), "=r"(b.w[3])
+                 : "l"(p));
+}
+__device__ __forceinline__ void st_32(void* p, const Vec16& a, const Vec16& b)
+{
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.w[0]), "r"(a.w[1]), "r"(a.w[2]), "r"(a.w[3]),
+                 "r"(b.w[0]), "r"(b.w[1]), "r"(b.w[2]), "r"(b.w[3])
+                 : "memory");
+}
+
 // Same, for vectors that every row re-reads (modulation scale / shift, gamma / beta, bias): kept in L1.
 // A 16-byte load that stays where it is written (the compiler may not sink it towards its first use), for loads that
 // are issued ahead of time on purpose; and a prefetch of one 128-byte line into L2.

@@ -11,7 +11,8 @@ int device_sm_count();  // gemm_dense.cu
 // each quarter of the 128: whole lines of every row, and scale words that fill 32-byte sectors.
 template<typename T, int FORMAT>
 __global__ void __launch_bounds__(256)
-fp4_quant_kernel(uint8_t* q, uint8_t* sf, const T* x, size_t ldx, const float* tensor_scale, size_t rows, size_t k, unsigned blocks_k, int warps_k_log2)
+fp4_quant_kernel(uint8_t* q, uint8_t* sf, const T* x, size_t ldx, const float* tensor_scale, size_t rows, size_t k, unsigned blocks_k, int warps_k_log2,
+                 int wide)
 {
     constexpr int kGroup  = fp4_group(FORMAT);
     constexpr int kBlocks = 32 / kGroup;            // of one thread
@@ -32,9 +33,16 @@ fp4_quant_kernel(uint8_t* q, uint8_t* sf, const T* x, size_t ldx, const float* t
     Vec16 v[kVecs];
     if (in) {
         const T* src = x + row * ldx + col;
+        if (wide) {   // [4608, 3072]: nvfp4 8.7 -> 7.2 us, mxfp4 7.3 -> 5.0
 #pragma unroll
-        for (int a = 0; a < kVecs; ++a) {
-            v[a] = ld_nc_16(src + a * kPer);
+            for (int a = 0; a < kVecs; a += 2) {
+                ld_nc_32(src + a * kPer, v[a], v[a + 1]);
+            }
+        } else {
+#pragma unroll
+            for (int a = 0; a < kVecs; ++a) {
+                v[a] = ld_nc_16(src + a * kPer);
+            }
         }
     }
     const Fp4Tensor tensor = fp4_tensor<FORMAT>(tensor_scale);
@@ -172,10 +180,11 @@ static int run_quant(uint8_t* q, uint8_t* sf, const void* x, int dtype, size_t l
     if (blocks > 0x7fffffffu) {
         return LYRAQ_ERR_UNSUPPORTED;
     }
+    const int wide = ((reinterpret_cast<uintptr_t>(x) | ldx * (dtype == LYRAQ_F32 ? 4u : 2u)) & 31u) == 0;   // rows on 32 bytes
     auto launch = [&](auto* kernel, auto type) {
         using T = decltype(type);
         return launch_kernel(kernel, (unsigned)blocks, 256u, (size_t)0, s, 1u, q, sf, (const T*)x, ldx, tensor_scale, rows, k, (unsigned)blocks_k,
-                             warps_k);
+                             warps_k, wide);
     };
     auto pick = [&](auto type) {
         using T = decltype(type);

@@ -29,6 +29,7 @@ struct RopeAxesParams {
     int                  pos_dtype;
     int                  heads[2];
     int                  head_dim, pairs, lanes_log2, groups, chunks, share, tokens_per_block;
+    int                  wide;        // interleaved pairs whose 16 neighbours lie on 32 bytes, in and out
     unsigned             tokens, seq;
     float                eps, inv_dim;
 };
@@ -199,6 +200,12 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(const RopeAxesParams p)
 #pragma unroll
                 for (int u = 0; u < NU; ++u) {
                     if (on[i] && there[u]) {
+                        if constexpr (VEC == 8 && !HALVES) {
+                            if (p.wide) {
+                                ld_32(in + at_a[u], a[i][u].v, c[i][u].v);
+                                continue;
+                            }
+                        }
                         a[i][u].load(in + at_a[u]);
                         c[i][u].load(in + at_b[u]);
                     }
@@ -271,6 +278,12 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(const RopeAxesParams p)
                         }
                         a[i][u].set(x[u]);
                         c[i][u].set(x[u] + VEC);
+                        if constexpr (VEC == 8 && !HALVES) {
+                            if (p.wide) {
+                                st_32(out[i] + at_a[u], a[i][u].v, c[i][u].v);
+                                continue;
+                            }
+                        }
                         a[i][u].store(out[i] + at_a[u]);
                         c[i][u].store(out[i] + at_b[u]);
                     }
@@ -340,6 +353,10 @@ extern "C" int lyraq_rope_axes(const lyraq_rope_axes_t* a, void* stream)
     };
     const int vec   = fits(8) ? 8 : fits(4) ? 4 : fits(2) ? 2 : 1;
     const int units = a->head_dim / (2 * vec);
+    auto on_32 = [](const void* x, size_t batch, size_t token, size_t head) { return even_strides(x, batch, token, head, 16); };
+    p.wide = vec == 8 && a->interleaved != 0 &&
+             (a->q_heads == 0 || (on_32(a->q, a->q_batch, a->q_token, a->q_head) && on_32(a->q_out, a->q_out_batch, a->q_out_token, a->q_out_head))) &&
+             (a->k_heads == 0 || (on_32(a->k, a->k_batch, a->k_token, a->k_head) && on_32(a->k_out, a->k_out_batch, a->k_out_token, a->k_out_head)));
     while ((1 << p.lanes_log2) < units && p.lanes_log2 < 5) {
         ++p.lanes_log2;
     }
