@@ -11,6 +11,7 @@ position axis it follows.
 """
 
 import decimal
+import functools
 
 import torch
 
@@ -22,11 +23,25 @@ _TURN = _EXACT.divide(decimal.Decimal(2 ** 64), _TWO_PI)
 def _turns(freq):
     """Frequency in radians per position, at least 0 and below a whole turn -> turns per position times 2^64, rounded, its bits as a signed
     64-bit number."""
-    f = freq if isinstance(freq, decimal.Decimal) else decimal.Decimal(freq)      # a float's value, exactly
+    f = decimal.Decimal(freq)      # a float's value, exactly
     if not (f.is_finite() and 0 <= f < _TWO_PI):
         raise ValueError("rope: a frequency must be at least 0 and below 2 pi radians per position, got %s" % freq)
     t = min(int(_EXACT.multiply(f, _TURN).to_integral_value()), 2 ** 64 - 1)
     return t - 2 ** 64 if t >= 2 ** 63 else t
+
+
+@functools.lru_cache(maxsize=256)
+def _ladder(dim, theta):
+    """theta^(-2 i / dim), i below dim / 2, to 60 digits, and their turns."""
+    base = decimal.Decimal(theta)
+    if not (base.is_finite() and base > 0):
+        raise ValueError("rope: theta must be positive, got %s" % theta)
+    step = _EXACT.power(base, _EXACT.divide(decimal.Decimal(-2), dim)) if dim else 0
+    f, ladder = decimal.Decimal(1), []
+    for _ in range(dim // 2):
+        ladder.append(_turns(f))
+        f = _EXACT.multiply(f, step)
+    return tuple(ladder)
 
 
 class AxisRope:
@@ -41,43 +56,33 @@ class AxisRope:
         thetas = list(theta) if isinstance(theta, (list, tuple)) else [theta] * len(axes_dim)
         if len(thetas) != len(axes_dim):
             raise ValueError("rope: %d axes and %d thetas" % (len(axes_dim), len(thetas)))
-        freq, axis = [], []
+        turns, axis = [], []
         for a, (dim, th) in enumerate(zip(axes_dim, thetas)):
             if dim % 2 or dim < 0:
                 raise ValueError("rope: the axis dimension must be even, got %d" % dim)
-            freq += self._ladder(dim, th)
+            turns += _ladder(dim, float(th))
             axis += [a] * (dim // 2)
-        self._set(freq, axis, len(axes_dim), interleaved, device)
+        self._set(turns, axis, len(axes_dim), interleaved, device)
 
-    @staticmethod
-    def _ladder(dim, theta):
-        base = decimal.Decimal(theta)
-        if not (base.is_finite() and base > 0):
-            raise ValueError("rope: theta must be positive, got %s" % theta)
-        step = _EXACT.power(base, _EXACT.divide(decimal.Decimal(-2), dim)) if dim else 0
-        f, ladder = decimal.Decimal(1), []
-        for _ in range(dim // 2):
-            ladder.append(f)
-            f = _EXACT.multiply(f, step)
-        return ladder
-
-    def _set(self, freq, axis, axes, interleaved, device):
-        if len(freq) != len(axis) or axes > 255 or any(not 0 <= a < axes for a in axis):
-            raise ValueError("rope: one axis below %d for each of %d pairs" % (min(axes, 255), len(freq)))
-        self.pairs, self.axes, self.interleaved = len(freq), axes, bool(interleaved)
-        self.turns = torch.tensor([_turns(f) for f in freq], dtype=torch.int64, device=device)
+    def _set(self, turns, axis, axes, interleaved, device):
+        if len(turns) != len(axis) or axes > 255 or any(not 0 <= a < axes for a in axis):
+            raise ValueError("rope: one axis below %d for each of %d pairs" % (min(axes, 255), len(turns)))
+        self.pairs, self.axes, self.interleaved = len(turns), axes, bool(interleaved)
+        self.turns = torch.tensor(turns, dtype=torch.int64, device=device)
         self.axis = torch.tensor(axis, dtype=torch.uint8, device=device)
 
     @classmethod
     def sections(cls, sections, theta=10000.0, interleaved=False, device="cuda"):
         """sections: pairs per axis; pair i of all has frequency theta^(-i / pairs)."""
-        return cls.from_pairs(cls._ladder(2 * sum(sections), theta), [a for a, n in enumerate(sections) for _ in range(n)], len(sections), interleaved, device)
+        plan = cls.__new__(cls)
+        plan._set(list(_ladder(2 * sum(sections), float(theta))), [a for a, n in enumerate(sections) for _ in range(n)], len(sections), interleaved, device)
+        return plan
 
     @classmethod
     def from_pairs(cls, freq, axis, axes, interleaved=False, device="cuda"):
         """freq: radians per position of each pair (floats), axis: its position axis, below `axes`."""
         plan = cls.__new__(cls)
-        plan._set([f if isinstance(f, decimal.Decimal) else float(f) for f in freq], [int(a) for a in axis], axes, interleaved, device)
+        plan._set([_turns(float(f)) for f in freq], [int(a) for a in axis], axes, interleaved, device)
         return plan
 
 
