@@ -116,7 +116,7 @@ __device__ __forceinline__ void finish32(const Fp4GemmParams& p, const uint32_t*
         if (vec_ok && valid >= 32) {
 #pragma unroll
             for (int q = 0; q < 32 / kPer; ++q) {
-                const Vec16 x = ld_nc_16(r + q * kPer);
+                const Vec16 x = ld_16(r + q * kPer);   // Y may be R
                 float       f[8];
                 if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -482,7 +482,6 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                 }
             };
             constexpr int kChunks = kHalfN / 32;
-            static_assert(kChunks % kBoxes == 0, "the boxes alternate from tile to tile too");
             // Residual of a 16-bit output: a lane that fetched its own row would touch 32 lines an instruction and use half a sector of each
             // ([4608, 12288, 3072]: 191 us against 72 without a residual).  Instead four lanes fetch the 64 bytes of a row, eight rows an instruction, two chunks
             // ahead (the first brings all 256 bytes of the row's share into L2), and hand them over through the box that the result leaves by.
@@ -544,7 +543,12 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                 const int sw   = (lane >> 1) & 3;
                 if (p.tma_store) {
                     if (lane == 0) {
-                        tma_store_wait_read_but_one();  // the store before the last has drained this box
+                        // the store before the last has drained this box; the tile before may have ended with either box
+                        if (c == 0) {
+                            tma_store_wait_read();
+                        } else {
+                            tma_store_wait_read_but_one();
+                        }
                     }
                     __syncwarp();
                 }

@@ -102,6 +102,11 @@ def test_quantize_takes_rows_apart_and_leaves_absent_rows_alone(ops, fmt):
     ops.quant_fp4(wide[:, 128:320], out=out)
     check_status()
     assert_quantized(out, x, fmt)
+    wide[:, 136:328] = x.cuda()
+    assert_quantized(ops.quant_fp4(wide[:, 136:328], None, fmt), x, fmt)      # rows on 16 bytes, not on 32
+    odd = torch.empty(70, 200, dtype=torch.bfloat16, device="cuda")[:, :192]  # a pitch of 400 bytes
+    odd.copy_(x)
+    assert_quantized(ops.quant_fp4(odd, None, fmt), x, fmt)
     blocks = 192 // fp4.GROUP[fmt]
     rest = torch.ones(out.scales.numel(), dtype=torch.bool)
     rest[fp4.scale_offsets(70, (blocks + 3) // 4 * 4).flatten()] = False
@@ -281,6 +286,46 @@ def test_large_product_is_exact_and_the_same_with_every_tile(ops, tile):
             h = torch.full((m, n), float("nan"), dtype=torch.bfloat16, device="cuda")
             ops.gemm_fp4(parts[0][0], parts[1][0], h)
             assert torch.equal(h, want.bfloat16()), (fmt, code)
+
+
+@pytest.mark.parametrize("code", [1281, 2562])
+@pytest.mark.parametrize("m,n", [(60001, 32), (25000, 224), (30000, 72)])
+def test_many_tiles_whose_last_columns_fill_one_store_box(ops, tile, code, m, n):
+    """Tile after tile in which a warp stores an odd number of 32-column pieces, with a short K: integer operands, exact."""
+    tile(code)
+    g = torch.Generator(device="cuda").manual_seed(n)
+    codes = torch.tensor([0, 2, 10, 4], dtype=torch.uint8, device="cuda")
+    values = torch.tensor([0.0, 1.0, -1.0, 2.0], dtype=torch.float32, device="cuda")
+    parts = []
+    for rows in (n, m):
+        i = torch.randint(0, 4, (rows, 32), generator=g, device="cuda")
+        t = ops.Fp4Tensor.empty(rows, 32)
+        t.codes.copy_(codes[i][:, 0::2] | (codes[i][:, 1::2] << 4))
+        t.scales.zero_()
+        t.scales[fp4.scale_offsets(rows, 2).flatten().cuda()] = 0x38
+        parts.append((t, values[i]))
+    want = (parts[1][1].double() @ parts[0][1].double().t()).bfloat16()
+    y = torch.full((m, n), float("nan"), dtype=torch.bfloat16, device="cuda")
+    r = torch.full((m, n), 3.0, dtype=torch.bfloat16, device="cuda")
+    for _ in range(3):
+        ops.gemm_fp4(parts[0][0], parts[1][0], y)
+        check_status()
+        assert torch.equal(y, want)
+    ops.gemm_fp4(parts[0][0], parts[1][0], r, residual=r, beta=2.0)   # |sum| + 6 <= 134: exact
+    check_status()
+    assert torch.equal(r, want + 6.0)
+
+
+@pytest.mark.parametrize("code", [0, 1281, 2562])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n", [(7, 72), (300, 264), (200, 131)])
+def test_result_in_the_residuals_place(ops, tile, code, dtype, m, n):
+    tile(code)
+    x, w, b, r = problem(m, n, 320, "mxfp4", dtype, 21, True, True)
+    y = cu(r).clone()
+    ops.gemm_fp4(to_device(ops, w, "mxfp4"), to_device(ops, x, "mxfp4"), y, cu(b), y, -1.25)
+    check_status()
+    assert_product(y, x, w, "mxfp4", b, r, -1.25)
 
 
 @pytest.mark.parametrize("stalled", [0, 1])
