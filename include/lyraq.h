@@ -415,7 +415,7 @@ LYRAQ_API int lyraq_gate_residual(void* out, const void* y, const void* gate, co
 typedef struct {
     const void *q, *k;                       /* [batch, seq_len, heads, head_dim] by strides */
     size_t q_batch, q_token, q_head, k_batch, k_token, k_head;
-    void *q_out, *k_out;                     /* may be q and k */
+    void *q_out, *k_out;                     /* may be q and k (same strides); not each other, nor the other's input */
     size_t q_out_batch, q_out_token, q_out_head, k_out_batch, k_out_token, k_out_head;
     const void *q_norm, *k_norm;             /* RMS norm weights [head_dim], or NULL: not normalised */
     const void* positions;
@@ -464,7 +464,7 @@ typedef struct {
 /* Norms before and after a block with its gate and residual in one pass:
  *   u = post(y) * post_weight;  v = residual_scale * x + gate_b * u;  x_out = T(v);  h = T( pre(v) * pre_weight * (1 + scale_b) + shift_b )
  * RMS: v / sqrt(mean(v^2) + eps); LAYER: the mean subtracted first.  fp32 throughout, each output rounded once; pre sees v before its rounding.
- * qf8 and q4 hold the codes that lyraq_quant_fp8 and lyraq_quant_fp4 make of T(h).  x_out may be x and h may be y (same strides).  dim a
+ * qf8 and q4 hold the codes that lyraq_quant_fp8 and lyraq_quant_fp4 make of T(h).  x_out and h may each be x or y (same strides), but not the same.  dim a
  * multiple of 8 (32 with q4), at most 16384; pointers 16-byte aligned (qf8: 8).  The fused form of what the reference runs as
  * invokeFusedGateAndResidual (src/lyradiff/kernels/flux_single_transformer_block/flux_single_transformer_kernels.cu:43-65) and
  * invokeLayerNormWithShiftAndScale (src/lyradiff/kernels/norms/layer_norm.h:19); the norm after a block has no counterpart there. */

@@ -130,7 +130,39 @@ PyObject* result(PyObject* given, const Tensor& made)
     return made.defined() ? THPVariable_Wrap(made) : Py_NewRef(Py_None);
 }
 
+// A launch may wait for room in the stream, and what holds the stream may be a callback that wants the interpreter.
+struct NoGil {
+    PyThreadState* state = PyEval_SaveThread();
+    ~NoGil() { PyEval_RestoreThread(state); }
+};
+template<typename F, typename... A> int run(F* f, A... args)
+{
+    NoGil free;
+    return f(args...);
+}
+
 void* current_stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
+
+// Whether a view may hold one element of memory twice: dimensions by stride, each must step past what lies inside it.
+bool overlaps(const Tensor& t)
+{
+    std::pair<int64_t, int64_t> d[8];
+    int                         n = 0;
+    for (int64_t i = 0; i < t.dim() && i < 8; ++i) {
+        if (t.size(i) > 1) {
+            d[n++] = {t.stride(i), t.size(i)};
+        }
+    }
+    std::sort(d, d + n);
+    int64_t span = 1;
+    for (int i = 0; i < n; ++i) {
+        if (d[i].first < span) {
+            return true;
+        }
+        span += d[i].first * (d[i].second - 1);
+    }
+    return false;
+}
 
 struct Rows {
     void*  p     = nullptr;
@@ -146,7 +178,7 @@ Rows rows_of(const Tensor& t, const char* what, at::IntArrayRef shape, at::Scala
     if (shape[2] > 1 && t.stride(2) != 1) {
         refuse(PyExc_ValueError, "%s: rows must be contiguous", what);
     }
-    if (output && ((shape[1] > 1 && t.stride(1) < shape[2]) || (shape[0] > 1 && t.stride(0) < shape[2]))) {
+    if (output && !t.is_contiguous() && overlaps(t)) {
         refuse(PyExc_ValueError, "%s has overlapping rows", what);
     }
     return Rows{t.data_ptr(), shape[0] > 1 ? (size_t)t.stride(0) : 0, shape[1] > 1 ? (size_t)t.stride(1) : 0};
@@ -230,29 +262,8 @@ PyObject* gated_residual_norm(PyObject* const* a)
     if (h != nullptr || (q8 == nullptr && q4 == nullptr)) {
         output(h, "h", h_new, n.h, n.h_batch, n.h_row);
     }
-    check_status(g_norm(&n, current_stream()), "lyraq_gated_residual_norm");
+    check_status(run(g_norm, &n, current_stream()), "lyraq_gated_residual_norm");
     return Py_BuildValue("(NN)", result(a[11], x_new), result(a[12], h_new));
-}
-
-// Whether a view may hold one element of memory twice: dimensions by stride, each must step past what lies inside it.
-bool overlaps(const Tensor& t)
-{
-    std::pair<int64_t, int64_t> d[8];
-    int                         n = 0;
-    for (int64_t i = 0; i < t.dim() && i < 8; ++i) {
-        if (t.size(i) > 1) {
-            d[n++] = {t.stride(i), t.size(i)};
-        }
-    }
-    std::sort(d, d + n);
-    int64_t span = 1;
-    for (int i = 0; i < n; ++i) {
-        if (d[i].first < span) {
-            return true;
-        }
-        span += d[i].first * (d[i].second - 1);
-    }
-    return false;
 }
 
 // (turns, axis, pairs, axes, interleaved, positions, q, k, q_norm, k_norm, eps, q_out, k_out) -> (q_out, k_out)
@@ -336,7 +347,7 @@ PyObject* rope_axes(PyObject* const* a)
     };
     heads(a[6], a[11], a[8], 0, r.q, r.q_batch, r.q_token, r.q_head, r.q_out, r.q_out_batch, r.q_out_token, r.q_out_head, r.q_norm, r.q_heads);
     heads(a[7], a[12], a[9], 1, r.k, r.k_batch, r.k_token, r.k_head, r.k_out, r.k_out_batch, r.k_out_token, r.k_out_head, r.k_norm, r.k_heads);
-    check_status(g_rope(&r, current_stream()), "lyraq_rope_axes");
+    check_status(run(g_rope, &r, current_stream()), "lyraq_rope_axes");
     return Py_BuildValue("(NN)", result(a[11], made[0]), result(a[12], made[1]));
 }
 
@@ -424,9 +435,11 @@ PyObject* linear_fp4(PyObject* const* a)
     }
     const size_t need = g_workspace(LYRAQ_OP_LINEAR_FP4, m, n, k);
     const Tensor ws   = empty_like_cuda({(int64_t)need}, at::kByte, dev);
-    check_status(g_linear_fp4(at_contiguous(out, "out"), (flat.defined() ? flat : x).data_ptr(), dtype_code(x, "x"), ldx,
-                              g == nullptr ? nullptr : (const float*)g->data_ptr(), w.codes, w.scales, w.scale, format, at_contiguous(bias, "bias"),
-                              at_contiguous(residual, "residual"), as_float(a[10]), (int)as_long(a[11]), m, n, k, ws.data_ptr(), need, current_stream()),
+    void* const  yp   = at_contiguous(out, "out");
+    const void*  bp   = at_contiguous(bias, "bias");
+    const void*  rp   = at_contiguous(residual, "residual");
+    check_status(run(g_linear_fp4, yp, (flat.defined() ? flat : x).data_ptr(), dtype_code(x, "x"), ldx, g == nullptr ? nullptr : (const float*)g->data_ptr(),
+                     w.codes, w.scales, w.scale, format, bp, rp, as_float(a[10]), (int)as_long(a[11]), m, n, k, ws.data_ptr(), need, current_stream()),
                  "lyraq_linear_fp4_forward");
     return result(a[12], y);
 }
@@ -444,8 +457,11 @@ PyObject* gemm_fp4(PyObject* const* a)
     const Tensor* bias     = tensor(a[10], "bias", dev);
     const Tensor* residual = tensor(a[11], "residual", dev);
     check_epilogue(bias, residual, y.scalar_type(), m, n);
-    check_status(g_gemm_fp4(x.codes, x.scales, x.scale, w.codes, w.scales, w.scale, format, at_contiguous(&y, "Y"), dtype_code(y, "Y"), at_contiguous(bias, "bias"),
-                            at_contiguous(residual, "residual"), as_float(a[12]), (int)as_long(a[13]), m, n, k, current_stream()),
+    void* const yp = at_contiguous(&y, "Y");
+    const void* bp = at_contiguous(bias, "bias");
+    const void* rp = at_contiguous(residual, "residual");
+    check_status(run(g_gemm_fp4, x.codes, x.scales, x.scale, w.codes, w.scales, w.scale, format, yp, dtype_code(y, "Y"), bp, rp, as_float(a[12]),
+                     (int)as_long(a[13]), m, n, k, current_stream()),
                  "lyraq_gemm_fp4");
     return Py_NewRef(a[14]);
 }
@@ -460,8 +476,8 @@ PyObject* quant_fp4(PyObject* const* a)
     }
     const int format = (int)as_long(a[4]);
     const Fp4 q      = fp4_of(a[1], a[2], a[3], x.size(0), x.size(1), format, dev);
-    check_status(g_quant_fp4(q.codes, q.scales, x.data_ptr(), dtype_code(x, "x"), x.size(0) > 1 ? (size_t)x.stride(0) : (size_t)x.size(1), q.scale, format,
-                             (size_t)x.size(0), (size_t)x.size(1), current_stream()),
+    check_status(run(g_quant_fp4, q.codes, q.scales, x.data_ptr(), dtype_code(x, "x"), x.size(0) > 1 ? (size_t)x.stride(0) : (size_t)x.size(1), q.scale,
+                     format, (size_t)x.size(0), (size_t)x.size(1), current_stream()),
                  "lyraq_quant_fp4");
     Py_RETURN_NONE;
 }

@@ -319,6 +319,9 @@ extern "C" int lyraq_gated_residual_norm(const lyraq_gated_norm_t* a, void* stre
             return LYRAQ_ERR_UNSUPPORTED;
         }
     }
+    if (a->x_out != nullptr && a->x_out == a->h) {
+        return LYRAQ_ERR_INVALID_ARG;
+    }
     const int sms = device_sm_count();
     if (sms <= 0) {
         return LYRAQ_ERR_CUDA;

@@ -320,6 +320,10 @@ extern "C" int lyraq_rope_axes(const lyraq_rope_axes_t* a, void* stream)
         (a->pairs > 0 && (a->positions == nullptr || a->turns == nullptr || a->axis == nullptr))) {
         return LYRAQ_ERR_INVALID_ARG;
     }
+    // q's heads are written while k's are read
+    if (a->q_heads > 0 && a->k_heads > 0 && (a->q_out == a->k_out || a->q_out == a->k || a->k_out == a->q)) {
+        return LYRAQ_ERR_INVALID_ARG;
+    }
     const uintptr_t pos_align = a->pos_dtype == LYRAQ_S64 ? 7u : 3u;
     if ((reinterpret_cast<uintptr_t>(a->positions) & pos_align) != 0 || (reinterpret_cast<uintptr_t>(a->turns) & 7u) != 0) {
         return LYRAQ_ERR_INVALID_ARG;

@@ -340,7 +340,7 @@ def rope_axes(plan, positions, q, k=None, q_norm=None, k_norm=None, eps=1e-6, q_
     """Rotary embedding over several position axes (lyraq_rope_axes).  plan: a rope.AxisRope; q [batch, seq, heads, head_dim] and optionally k
     (its own number of heads), any strides with contiguous heads (views of a packed projection, heads before tokens by transpose);
     positions [batch, seq, axes] or [seq, axes], int32, int64 or fp32, any strides.  q_norm / k_norm [head_dim]: RMS norm weights.  Returns
-    (q_out, k_out), created when omitted; they may be q and k."""
+    (q_out, k_out), created when omitted; they may be q and k, but neither each other nor the other's input."""
     return _lib.host().rope_axes(plan.turns, plan.axis, plan.pairs, plan.axes, plan.interleaved, positions, q, k, q_norm, k_norm, eps, q_out, k_out)
 
 
@@ -353,7 +353,7 @@ def gated_residual_norm(y, x, gate=None, scale=None, shift=None, post_weight=Non
         v = residual_scale * x + gate[b] * (post(y) * post_weight);  x_out = v;  h = pre(v) * pre_weight * (1 + scale[b]) + shift[b]
     Returns (x_out, h).  gate, scale, shift: [batch, dim] (rows may lie apart, as chunks of one modulation tensor do) or [dim]; post: "none",
     "rms" or "layer", pre: "rms" or "layer".  x_out is created when omitted, h when no other form of it is asked for.  qf8 (uint8, contiguous,
-    with f8_scale) takes e4m3 codes of h, q4 (an Fp4Tensor of [batch * seq, dim]) its FP4 form.  x_out may be x itself, h may be y."""
+    with f8_scale) takes e4m3 codes of h, q4 (an Fp4Tensor of [batch * seq, dim]) its FP4 form.  x_out and h may each be x or y, but not the same tensor."""
     if post not in _NORMS or pre not in _NORMS or pre == "none":
         raise ValueError("unknown norm %r / %r" % (post, pre))
     if q4 is None:

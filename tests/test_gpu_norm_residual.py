@@ -152,7 +152,8 @@ def test_python_side_refuses(ops):
     t = {k: cu(a) for k, a in make(2, 4, 64, torch.bfloat16, 5).items()}
     bad = [dict(t, x=t["x"][:, :3]), dict(t, gate=t["gate"].float()), dict(t, post_weight=t["post_weight"][:32]), dict(t, post="l2"), dict(t, pre="none"),
            dict(t, qf8=torch.empty(2, 4, 64, dtype=torch.uint8, device="cuda")), dict(t, q4=ops.Fp4Tensor.empty(7, 64)), dict(t, y=t["y"].cpu()),
-           dict(t, x_out=t["x"][:1].expand(2, 4, 64)), dict(t, y=t["y"].transpose(1, 2))]
+           dict(t, x_out=t["x"][:1].expand(2, 4, 64)), dict(t, y=t["y"].transpose(1, 2)),
+           dict(t, h=torch.zeros(512, dtype=torch.bfloat16, device="cuda").as_strided((2, 4, 64), (64, 64, 1)))]
     for b in bad:
         with pytest.raises((ValueError, TypeError)):
             ops.gated_residual_norm(**b)
@@ -164,3 +165,17 @@ def test_python_side_refuses(ops):
         ops.gated_residual_norm(wide[..., :60].contiguous(), wide[..., :60].contiguous())
     with pytest.raises(LyraqError):
         ops.gated_residual_norm(wide.float(), wide.float())
+    both = torch.zeros_like(wide)
+    with pytest.raises(LyraqError):
+        ops.gated_residual_norm(wide, wide, x_out=both, h=both)
+
+
+@pytest.mark.parametrize("dim", [640, 1288])
+def test_outputs_in_the_inputs_places(ops, dim):
+    t = {k: cu(a) for k, a in make(2, 200, dim, torch.bfloat16, 11).items()}
+    want = ops.gated_residual_norm(post="layer", pre="rms", **t)
+    for first, second in (("x", "y"), ("y", "x")):
+        own = dict(t, x=t["x"].clone(), y=t["y"].clone())
+        ops.gated_residual_norm(post="layer", pre="rms", x_out=own[first], h=own[second], **own)
+        check_status()
+        assert torch.equal(own[first], want[0]) and torch.equal(own[second], want[1])

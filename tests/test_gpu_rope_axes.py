@@ -123,6 +123,10 @@ def test_layouts_and_in_place(ops, rope, d, dims):
     odd = torch.empty(2, 11, 4, d + 3, dtype=torch.bfloat16, device="cuda")[..., 1:d + 1]
     odd.copy_(q)
     assert torch.equal(ops.rope_axes(plan, pos, odd)[0], want[0])
+    by_16 = torch.empty(2, 11, 4, d + 8, dtype=torch.bfloat16, device="cuda")[..., 8:]          # on 16 bytes, not on 32
+    by_16.copy_(q)
+    assert torch.equal(ops.rope_axes(plan, pos, by_16)[0], want[0])
+    assert torch.equal(ops.rope_axes(plan, pos, q, q_out=q.new_zeros(2, 11, 4, d + 8)[..., 8:])[0], want[0])
     out = torch.zeros(2, 4, 11, d, dtype=torch.bfloat16, device="cuda")
     ops.rope_axes(plan, pos, q, q_out=out.transpose(1, 2))
     assert torch.equal(out.transpose(1, 2), want[0])
@@ -179,6 +183,11 @@ def test_refusals(ops, rope):
         ops.rope_axes(rope.AxisRope((66,)), pos, q)                   # more pairs than the head has
     with pytest.raises(LyraqError):
         ops.rope_axes(plan, pos, torch.zeros(1, 4, 1, 258, dtype=torch.bfloat16, device="cuda"))
+    k = torch.zeros_like(q)
+    for kw in ({"q_out": k}, {"k_out": q}, {"q_out": torch.empty_like(q)}):
+        kw.setdefault("k_out", kw.get("q_out") if kw.get("q_out") is not k else None)
+        with pytest.raises(LyraqError):
+            ops.rope_axes(plan, pos, q, k, **kw)
 
 
 def test_empty_calls(ops, rope):

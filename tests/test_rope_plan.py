@@ -52,14 +52,14 @@ def test_c_entry_points_refuse_without_a_device(lib):
     INVALID, UNSUPPORTED = 1, 2
 
     def norm(**k):
-        a = _lib.GatedNormArgs(**{**dict(y=p, x=p, x_out=p, h=p, dtype=1, post=1, pre=2, batch=1, seq_len=4, dim=64, y_row=64, x_row=64, x_out_row=64, h_row=64), **k})
+        a = _lib.GatedNormArgs(**{**dict(y=p, x=p, x_out=p, h=2 * p, dtype=1, post=1, pre=2, batch=1, seq_len=4, dim=64, y_row=64, x_row=64, x_out_row=64, h_row=64), **k})
         return lib.lyraq_gated_residual_norm(ctypes.byref(a), None)
     assert lib.lyraq_gated_residual_norm(None, None) == INVALID
     assert norm(seq_len=0) == ok and norm(dim=60) == UNSUPPORTED and norm(dim=16392) == UNSUPPORTED and norm(dtype=2) == UNSUPPORTED
     assert norm(y=None) == INVALID and norm(x=p + 2) == INVALID and norm(pre=0) == INVALID and norm(post=3) == INVALID and norm(x_row=60) == INVALID
     assert norm(x_out=None, h=None) == INVALID and norm(qf8=p) == INVALID and norm(qf8=p + 4, f8_scale=p) == INVALID and norm(q4=p) == INVALID
     assert norm(q4=p, q4_scales=p, q4_format=5) == INVALID and norm(q4=p, q4_scales=p, dim=72) == UNSUPPORTED and norm(gate=p, gate_batch=4) == INVALID
-    assert norm(post_weight=p + 8) == INVALID
+    assert norm(post_weight=p + 8) == INVALID and norm(h=p) == INVALID
 
     def turn(**k):
         a = _lib.RopeAxesArgs(**{**dict(q=p, q_out=p, positions=p, turns=p, axis=p, pos_dtype=3, dtype=1, q_heads=2, head_dim=64, pairs=32, batch=1, seq_len=3), **k})
