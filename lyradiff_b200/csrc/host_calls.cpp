@@ -8,6 +8,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -164,6 +165,29 @@ bool overlaps(const Tensor& t)
     return false;
 }
 
+// One FP4 matrix: codes uint8 [rows, k / 2], block scales, tensor scale (fp32 [1] or None).  A kernel would read past parts that do not fit.
+struct Fp4 {
+    uint8_t* codes;
+    uint8_t* scales;
+    float*   scale;
+};
+Fp4 fp4_of(PyObject* codes, PyObject* scales, PyObject* scale, int64_t rows, int64_t k, int format, int dev)
+{
+    const Tensor& c = needed(codes, "FP4 codes", dev);
+    const Tensor& s = needed(scales, "FP4 block scales", dev);
+    const Tensor* g = tensor(scale, "an FP4 tensor scale", dev);
+    if (k % 32 != 0 || c.scalar_type() != at::kByte || c.dim() != 2 || c.size(0) != rows || c.size(1) != k / 2) {
+        refuse(PyExc_ValueError, "FP4 codes must be uint8 [%lld, %lld / 2], k a multiple of 32", (long long)rows, (long long)k);
+    }
+    if (s.scalar_type() != at::kByte || (size_t)s.numel() != g_scale_bytes((size_t)rows, (size_t)k, format)) {
+        refuse(PyExc_ValueError, "FP4 block scales do not fit [%lld, %lld]", (long long)rows, (long long)k);
+    }
+    if (g != nullptr && (g->scalar_type() != at::kFloat || g->numel() != 1)) {
+        refuse(PyExc_ValueError, "an FP4 tensor scale is one fp32 number");
+    }
+    return Fp4{(uint8_t*)at_contiguous(&c, "FP4 codes"), (uint8_t*)at_contiguous(&s, "FP4 block scales"), g == nullptr ? nullptr : (float*)g->data_ptr()};
+}
+
 struct Rows {
     void*  p     = nullptr;
     size_t batch = 0, row = 0;
@@ -213,7 +237,6 @@ PyObject* gated_residual_norm(PyObject* const* a)
     const Tensor* h  = tensor(a[12], "h", dev);
     const Tensor* q8 = tensor(a[13], "qf8", dev);
     const Tensor* s8 = tensor(a[14], "f8_scale", dev);
-    const Tensor* q4 = tensor(a[15], "q4", dev);
     if (q8 != nullptr && (s8 == nullptr || s8->scalar_type() != at::kFloat || s8->numel() != 1 || q8->scalar_type() != at::kByte || q8->numel() != y.numel())) {
         refuse(PyExc_ValueError, "qf8 must be uint8 of y's size, with an fp32 f8_scale");
     }
@@ -244,11 +267,12 @@ PyObject* gated_residual_norm(PyObject* const* a)
     n.pre_weight  = weight(a[6], "pre_weight");
     n.qf8         = (uint8_t*)at_contiguous(q8, "qf8");
     n.f8_scale    = q8 == nullptr ? nullptr : (const float*)s8->data_ptr();
-    if (q4 != nullptr) {
-        n.q4              = (uint8_t*)at_contiguous(q4, "q4");
-        n.q4_scales       = (uint8_t*)at_contiguous(&needed(a[16], "the scales of q4", dev), "the scales of q4");
-        n.q4_tensor_scale = (const float*)at_contiguous(tensor(a[17], "the tensor scale of q4", dev), "the tensor scale of q4");
+    if (a[15] != Py_None) {
         n.q4_format       = (int)as_long(a[18]);
+        const Fp4 q4      = fp4_of(a[15], a[16], a[17], shape[0] * shape[1], shape[2], n.q4_format, dev);
+        n.q4              = q4.codes;
+        n.q4_scales       = q4.scales;
+        n.q4_tensor_scale = q4.scale;
     }
     // rows of a new output are contiguous
     auto output = [&](const Tensor* given, const char* what, Tensor& made, void*& p, size_t& batch, size_t& row) {
@@ -259,7 +283,7 @@ PyObject* gated_residual_norm(PyObject* const* a)
         p = r.p; batch = r.batch; row = r.row;
     };
     output(xo, "x_out", x_new, n.x_out, n.x_out_batch, n.x_out_row);
-    if (h != nullptr || (q8 == nullptr && q4 == nullptr)) {
+    if (h != nullptr || (q8 == nullptr && n.q4 == nullptr)) {
         output(h, "h", h_new, n.h, n.h_batch, n.h_row);
     }
     check_status(run(g_norm, &n, current_stream()), "lyraq_gated_residual_norm");
@@ -369,29 +393,6 @@ int as_size(int64_t v, const char* what)
     return (int)v;
 }
 
-// One FP4 matrix: codes uint8 [rows, k / 2], block scales, tensor scale (fp32 [1] or None).  A kernel would read past parts that do not fit.
-struct Fp4 {
-    uint8_t* codes;
-    uint8_t* scales;
-    float*   scale;
-};
-Fp4 fp4_of(PyObject* codes, PyObject* scales, PyObject* scale, int64_t rows, int64_t k, int format, int dev)
-{
-    const Tensor& c = needed(codes, "FP4 codes", dev);
-    const Tensor& s = needed(scales, "FP4 block scales", dev);
-    const Tensor* g = tensor(scale, "an FP4 tensor scale", dev);
-    if (k % 32 != 0 || c.scalar_type() != at::kByte || c.dim() != 2 || c.size(0) != rows || c.size(1) != k / 2) {
-        refuse(PyExc_ValueError, "FP4 codes must be uint8 [%lld, %lld / 2], k a multiple of 32", (long long)rows, (long long)k);
-    }
-    if (s.scalar_type() != at::kByte || (size_t)s.numel() != g_scale_bytes((size_t)rows, (size_t)k, format)) {
-        refuse(PyExc_ValueError, "FP4 block scales do not fit [%lld, %lld]", (long long)rows, (long long)k);
-    }
-    if (g != nullptr && (g->scalar_type() != at::kFloat || g->numel() != 1)) {
-        refuse(PyExc_ValueError, "an FP4 tensor scale is one fp32 number");
-    }
-    return Fp4{(uint8_t*)at_contiguous(&c, "FP4 codes"), (uint8_t*)at_contiguous(&s, "FP4 block scales"), g == nullptr ? nullptr : (float*)g->data_ptr()};
-}
-
 // (x, codes, scales, tensor scale of the weight, n, k, format, input scale, bias, residual, beta, epilogue, out) -> y
 PyObject* linear_fp4(PyObject* const* a)
 {
@@ -444,13 +445,21 @@ PyObject* linear_fp4(PyObject* const* a)
     return result(a[12], y);
 }
 
-// (codes, scales, tensor scale of X, rows, the same of W, k, format, bias, residual, beta, epilogue, Y) -> Y
+// (codes, scales, tensor scale of X, rows, the same of W, k, format, bias, residual, beta, epilogue, Y or the dtype of a new one) -> Y
 PyObject* gemm_fp4(PyObject* const* a)
 {
     const int     dev = c10::cuda::current_device();
     const int     m = as_size(as_long(a[3]), "m"), n = as_size(as_long(a[7]), "n"), k = as_size(as_long(a[8]), "k"), format = (int)as_long(a[9]);
     const Fp4     x = fp4_of(a[0], a[1], a[2], m, k, format, dev), w = fp4_of(a[4], a[5], a[6], n, k, format, dev);
-    const Tensor& y = needed(a[14], "Y", dev);
+    Tensor        made;
+    if (THPDtype_Check(a[14])) {
+        const at::ScalarType type = reinterpret_cast<THPDtype*>(a[14])->scalar_type;
+        if (type != at::kHalf && type != at::kBFloat16 && type != at::kFloat) {
+            refuse(PyExc_TypeError, "Y: unsupported dtype %s", c10::toString(type));
+        }
+        made = empty_like_cuda({m, n}, type, dev);
+    }
+    const Tensor& y = made.defined() ? made : needed(a[14], "Y", dev);
     if (y.dim() != 2 || y.size(0) != m || y.size(1) != n) {
         refuse(PyExc_ValueError, "Y must be [%d, %d]", m, n);
     }
@@ -463,7 +472,16 @@ PyObject* gemm_fp4(PyObject* const* a)
     check_status(run(g_gemm_fp4, x.codes, x.scales, x.scale, w.codes, w.scales, w.scale, format, yp, dtype_code(y, "Y"), bp, rp, as_float(a[12]),
                      (int)as_long(a[13]), m, n, k, current_stream()),
                  "lyraq_gemm_fp4");
-    return Py_NewRef(a[14]);
+    return made.defined() ? THPVariable_Wrap(made) : Py_NewRef(a[14]);
+}
+
+// (rows, k, format, device) -> (codes, scales) of an FP4 matrix
+PyObject* fp4_empty(PyObject* const* a)
+{
+    const int rows = as_size(as_long(a[0]), "rows"), k = as_size(as_long(a[1]), "k"), format = (int)as_long(a[2]), dev = as_size(as_long(a[3]), "the device");
+    const Tensor codes  = empty_like_cuda({rows, k / 2}, at::kByte, dev);
+    const Tensor scales = empty_like_cuda({(int64_t)g_scale_bytes((size_t)rows, (size_t)k, format)}, at::kByte, dev);
+    return Py_BuildValue("(NN)", THPVariable_Wrap(codes), THPVariable_Wrap(scales));
 }
 
 // (x, codes, scales, tensor scale, format)
@@ -532,6 +550,7 @@ PyMethodDef g_methods[] = {
     {"rope_axes", (PyCFunction)(void (*)())call<rope_axes, 13>, METH_FASTCALL, nullptr},
     {"linear_fp4", (PyCFunction)(void (*)())call<linear_fp4, 13>, METH_FASTCALL, nullptr},
     {"gemm_fp4", (PyCFunction)(void (*)())call<gemm_fp4, 15>, METH_FASTCALL, nullptr},
+    {"fp4_empty", (PyCFunction)(void (*)())call<fp4_empty, 4>, METH_FASTCALL, nullptr},
     {"quant_fp4", (PyCFunction)(void (*)())call<quant_fp4, 5>, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

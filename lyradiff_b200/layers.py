@@ -79,16 +79,20 @@ class Fp4Linear:
 
     def empty_input(self, rows):
         """An Fp4Tensor for `rows` rows of this layer's input, for producers that write FP4 themselves (ops.gated_residual_norm)."""
-        return ops.Fp4Tensor.empty(rows, self.k, self.fmt, self.input_scale, self.weight.codes.device)
+        codes, scales = _lib.host().fp4_empty(rows, self.k, self.format, self.weight.codes.get_device())
+        return ops.Fp4Tensor(rows, self.k, self.fmt, codes, scales, self.input_scale)
 
     def forward_quantized(self, x, dtype, residual=None, beta=1.0, out=None):
         """The product alone, for an input that is FP4 already (empty_input): [rows, n] of `dtype`."""
-        if x.tensor_scale is not self.input_scale:
+        if x.tensor_scale is not self.input_scale or x.fmt != self.fmt:
             raise ValueError("the input was not quantized for this layer (empty_input)")
-        y = torch.empty(x.rows, self.n, dtype=dtype, device=x.codes.device) if out is None else out.view(x.rows, self.n)
-        if y.dtype != dtype:
-            raise ValueError("out must be %s" % dtype)
-        return ops.gemm_fp4(self.weight, x, y, self.bias, residual, beta, self.gelu)
+        if out is not None:
+            if out.dtype != dtype:
+                raise ValueError("out must be %s" % dtype)
+            dtype = out.view(x.rows, self.n)
+        w = self.weight
+        return _lib.host().gemm_fp4(x.codes, x.scales, x.tensor_scale, x.rows, w.codes, w.scales, w.tensor_scale, self.n, self.k, self.format, self.bias,
+                                    residual, beta, self.epilogue, dtype)
 
 
 class SmoothQuantLinear:

@@ -360,10 +360,7 @@ def gated_residual_norm(y, x, gate=None, scale=None, shift=None, post_weight=Non
         codes = scales = tensor_scale = None
         fmt = 0
     else:
-        if q4.k != y.shape[-1] or q4.rows * q4.k != y.numel():
-            raise ValueError("q4 must be [batch * seq, dim]")
-        q4.check()
-        codes, scales, tensor_scale, fmt = q4.codes, q4.scales, q4.tensor_scale, FP4_FORMATS[q4.fmt]
+        codes, scales, tensor_scale, fmt = q4.codes, q4.scales, q4.tensor_scale, _fp4_format(q4.fmt)
     return _lib.host().gated_residual_norm(y, x, gate, scale, shift, post_weight, pre_weight, _NORMS[post], _NORMS[pre], residual_scale, eps, x_out, h,
                                            qf8, f8_scale, codes, scales, tensor_scale, fmt)
 
