@@ -48,19 +48,22 @@ __device__ __forceinline__ float rcp_approx(float v)
     return r;
 }
 
-// What the blocks of a tensor share: its scale g, 6 g and about 1 / (6 g).
+// A power of two that brings a divisor to where neither its reciprocal nor a remainder over- or underflows.  Dividends are multiplied by it too; what
+// that over- or underflows has a quotient that saturates or rounds to zero.
+__device__ __forceinline__ float fp4_range(float v) { return v < 7.9e-31f ? 1.2089258e24f : v > 1.2e30f ? 8.271806e-25f : 1.0f; }   // 2^-100, 2^80, 2^100, 2^-80
+
+// What the blocks of a tensor share: its scale g, and with c = fp4_range(g): c, 6 g c and about 1 / (6 g c).
 struct Fp4Tensor {
-    float g, g6, r6;
-    bool  plain;    // 6 g is far from where its reciprocal or a remainder over- or underflows
+    float g, c, g6, r6;
 };
 template<int FORMAT> __device__ __forceinline__ Fp4Tensor fp4_tensor(const float* tensor_scale)
 {
-    Fp4Tensor t{1.0f, 6.0f, 0.0f, true};
+    Fp4Tensor t{1.0f, 1.0f, 6.0f, 0.0f};
     if (FORMAT == LYRAQ_NVFP4) {
-        t.g     = tensor_scale != nullptr ? ld_f32(tensor_scale) : 1.0f;
-        t.g6    = 6.0f * t.g;
-        t.r6    = rcp_approx(t.g6);
-        t.plain = t.g6 >= 7.9e-31f && t.g6 <= 1.2e30f;
+        t.g  = tensor_scale != nullptr ? ld_f32(tensor_scale) : 1.0f;
+        t.c  = fp4_range(t.g);
+        t.g6 = 6.0f * (t.g * t.c);
+        t.r6 = t.g6 > 0.0f ? rcp_approx(t.g6) : 0.0f;
     }
     return t;
 }
@@ -93,11 +96,9 @@ template<int FORMAT> __device__ __forceinline__ Fp4Block fp4_block(uint32_t amax
     }
     if (FORMAT == LYRAQ_NVFP4) {
         const float amax  = __uint_as_float(amax_bits);
-        const float q0    = amax * s.r6;
-        float       ratio = fmaf(fmaf(-q0, s.g6, amax), s.r6, q0);
-        if (!s.plain || amax > s.g6 * 1024.0f) {   // the second saturates
-            ratio = amax_bits == 0u ? 0.0f : amax / s.g6;
-        }
+        const float a     = fminf(amax * s.c, s.g6 * 1024.0f);   // saturates at 448
+        const float q0    = a * s.r6;
+        const float ratio = fmaf(fmaf(-q0, s.g6, a), s.r6, q0);
         b.code = f32x2_to_e4m3x2(ratio, 0.0f) & 0xffu;
         // e4m3 -> fp32: the code's seven bits under fp16's exponent read 2^-8 times its value, subnormals included
         b.t     = __half2float(__ushort_as_half((unsigned short)(b.code << 7))) * 256.0f * s.g;
@@ -114,28 +115,35 @@ template<int FORMAT> __device__ __forceinline__ Fp4Block fp4_block(uint32_t amax
     return b;
 }
 
-// The codes of eight values of a block.  A quotient that over- or underflows saturates or rounds to zero like any other.
+// The codes of eight values of a block.
 template<int FORMAT> __device__ __forceinline__ uint32_t fp4_encode8(const float* x, const Fp4Block& b)
 {
-    float q[8];
-    if (FORMAT != LYRAQ_NVFP4 || b.plain) {   // with t = r = 0 every quotient comes out as 0
-        const float2 r2 = make_float2(b.r, b.r);
-        const float2 m2 = make_float2(-b.t, -b.t);
+    float q[8], t = b.t, r = b.r;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 v = make_float2(x[2 * j], x[2 * j + 1]);
-            float2       p = mul_f32x2(v, r2);
-            if (FORMAT == LYRAQ_NVFP4) {
-                p = fma_f32x2(fma_f32x2(p, m2, v), r2, p);
-            }
-            q[2 * j]     = p.x;
-            q[2 * j + 1] = p.y;
-        }
-    } else {
+    for (int j = 0; j < 8; ++j) {
+        q[j] = x[j];
+    }
+    if (FORMAT == LYRAQ_NVFP4 && !b.plain) {   // no divisions here either: they are long, and every launch would fetch them on its way past
+        const float c = fp4_range(t);
+        t *= c;
+        r = t > 0.0f ? rcp_approx(t) : 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            q[j] = b.t > 0.0f ? x[j] / b.t : 0.0f;
+            q[j] = t > 0.0f ? fminf(fmaxf(q[j] * c, t * -1048576.0f), t * 1048576.0f) : 0.0f;
         }
+    }
+    // with t = r = 0 every quotient comes out as 0
+    const float2 r2 = make_float2(r, r);
+    const float2 m2 = make_float2(-t, -t);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float2 v = make_float2(q[2 * j], q[2 * j + 1]);
+        float2       p = mul_f32x2(v, r2);
+        if (FORMAT == LYRAQ_NVFP4) {
+            p = fma_f32x2(fma_f32x2(p, m2, v), r2, p);
+        }
+        q[2 * j]     = p.x;
+        q[2 * j + 1] = p.y;
     }
     const uint32_t codes = f32x8_to_e2m1x8(q);
     return FORMAT == LYRAQ_NVFP4 || b.plain ? codes : 0u;   // mxfp4: not plain is not finite
@@ -177,5 +185,41 @@ template<> __device__ __forceinline__ uint32_t amax_bits_of<__half>(const Vec16&
     // half -> float keeps order, infinities and NaN
     return __float_as_uint(__half2float(__ushort_as_half((unsigned short)amax16_of<__half>(v)))) & 0x7fffffffu;
 }
+
+// 32 consecutive values of a row, two blocks or one: their codes, and their scale bytes from the lowest on.
+template<typename T, int FORMAT> __device__ __forceinline__ uint32_t fp4_encode32(const Vec16* v, const Fp4Tensor& tensor, Vec16& o)
+{
+    constexpr int kGroup  = fp4_group(FORMAT);
+    constexpr int kBlocks = 32 / kGroup;
+    constexpr int kV      = 2 * (int)sizeof(T) / kBlocks;   // vectors of a block
+    uint32_t      code    = 0;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+        uint32_t amax = 0;
+#pragma unroll
+        for (int a = 0; a < kV; ++a) {
+            amax = max(amax, amax_bits_of<T>(v[b * kV + a]));
+        }
+        const Fp4Block blk = fp4_block<FORMAT>(amax, tensor);
+        code |= blk.code << (8 * b);
+#pragma unroll
+        for (int a = 0; a < kGroup / 8; ++a) {
+            float f[8];
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    f[e] = __uint_as_float(v[b * kV + 2 * a + (e >> 2)].w[e & 3]);
+                }
+            } else {
+                unpack8<T>(v[b * kV + a], f);
+            }
+            o.w[b * (kGroup / 8) + a] = fp4_encode8<FORMAT>(f, blk);
+        }
+    }
+    return code;
+}
+
+// What lyraq_quant_fp4 asks of its arguments (fp4_quant.cu).
+int check_fp4(const void* q, const void* sf, const void* x, int dtype, size_t ldx, int format, size_t rows, size_t k);
 
 }  // namespace lyraq

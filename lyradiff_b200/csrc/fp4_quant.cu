@@ -49,30 +49,7 @@ fp4_quant_kernel(uint8_t* q, uint8_t* sf, const T* x, size_t ldx, const float* t
     uint32_t        code   = 0;
     if (in) {
         Vec16 o;
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-            constexpr int kV = kVecs / kBlocks;
-            uint32_t      amax = 0;
-#pragma unroll
-            for (int a = 0; a < kV; ++a) {
-                amax = max(amax, amax_bits_of<T>(v[b * kV + a]));
-            }
-            const Fp4Block blk = fp4_block<FORMAT>(amax, tensor);
-            code |= blk.code << (8 * b);
-#pragma unroll
-            for (int a = 0; a < kGroup / 8; ++a) {
-                float f[8];
-                if constexpr (sizeof(T) == 4) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        f[e] = __uint_as_float(v[b * kV + 2 * a + (e >> 2)].w[e & 3]);
-                    }
-                } else {
-                    unpack8<T>(v[b * kV + a], f);
-                }
-                o.w[b * (kGroup / 8) + a] = fp4_encode8<FORMAT>(f, blk);
-            }
-        }
+        code = fp4_encode32<T, FORMAT>(v, tensor, o);
         st_16(q + row * (k >> 1) + (col >> 1), o);
     }
     // blocks beyond k have scale 0, so the word of an existing row is always written whole
@@ -146,7 +123,7 @@ __global__ void __launch_bounds__(256) fp4_tensor_scale_kernel(float* tensor_sca
     }
 }
 
-static int check_fp4(const void* q, const void* sf, const void* x, int dtype, size_t ldx, int format, size_t rows, size_t k)
+int check_fp4(const void* q, const void* sf, const void* x, int dtype, size_t ldx, int format, size_t rows, size_t k)
 {
     if (format != LYRAQ_NVFP4 && format != LYRAQ_MXFP4) {
         return LYRAQ_ERR_INVALID_ARG;

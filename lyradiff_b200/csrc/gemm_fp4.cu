@@ -670,17 +670,22 @@ static int launch(const uint8_t* X, const uint8_t* xs, const uint8_t* W, const u
 // forced kernel for tests and sweeps: 0 = automatic, 16 = the few-row kernel (up to 16 rows), 2562 = CTA pair with 256 x 256, 1281 = one CTA with 128 x 128
 static int g_forced_tile = 0;
 
-static int run(const uint8_t* X, const uint8_t* xs, const uint8_t* W, const uint8_t* ws, int format, const Fp4GemmParams& p, int sms,
-               cudaStream_t stream)
+bool few_rows(int m, int k)
 {
-    const long m128 = ((long)p.M + 127) / 128, n128 = ((long)p.N + 127) / 128, m256 = ((long)p.M + 255) / 256, n256 = ((long)p.N + 255) / 256;
-    const long pairs = sms / 2;
     // The few-row kernel's time grows with the rows (their partial sums cross shared memory and leave row by row), the other's does not; what it
     // gains grows with K.  Dense against few-row, us: 4 rows of [256, 256] 2.8 / 3.1, of [1280, 1280] 4.3 / 4.1, 8 rows of it 4.3 / 5.2; 16
     // rows of [1280, 2048] 5.1 / 4.7, of [3072, 3072] 6.4 / 5.6, of [3072, 12288] 17.4 / 8.2; one row of [9216, 3072] 8.3 / 5.4.
+    const int num_kb = (k + kBlockK - 1) / kBlockK;
+    return m <= kFp4SkinnyRows && (g_forced_tile == 16 || (g_forced_tile == 0 && (num_kb >= 8 || m <= 2 + num_kb / 2)));
+}
+
+static int run(const Fp4Input& X, const uint8_t* W, const uint8_t* ws, int format, const Fp4GemmParams& p, int sms, cudaStream_t stream)
+{
+    const long m128 = ((long)p.M + 127) / 128, n128 = ((long)p.N + 127) / 128, m256 = ((long)p.M + 255) / 256, n256 = ((long)p.N + 255) / 256;
+    const long pairs = sms / 2;
     const int num_kb = (p.K + kBlockK - 1) / kBlockK;
-    if (p.M <= kFp4SkinnyRows && (g_forced_tile == 16 || (g_forced_tile == 0 && (num_kb >= 8 || p.M <= 2 + num_kb / 2)))) {
-        return launch_skinny(X, xs, W, ws, format, p, sms, stream);
+    if (few_rows(p.M, p.K)) {
+        return launch_skinny(X, W, ws, format, p, sms, stream);
     }
     // Rounds of each tile times what one takes, us: 0.2 + 0.323 a K block for 128 x 128, 1.3 + 0.39 for a pair's 256 x 256, from [4608, 12288, 3072]
     // (98 / 72), [4608, 3072, 12288] (94 / 60), [4608, 3072, 3072] (29 / 19), [1155, 9216, 3072] (24 / 18), [512, 3072, 3072] (7.8 / 9.7).
@@ -690,13 +695,36 @@ static int run(const uint8_t* X, const uint8_t* xs, const uint8_t* W, const uint
     auto pick = [&](auto fmt, auto res) {
         constexpr int  kFmt = decltype(fmt)::value;
         constexpr bool kRes = decltype(res)::value;
-        return tile == 2562 ? launch<kFmt, 256, 2, kRes>(X, xs, W, ws, p, sms, stream)
-                            : launch<kFmt, 128, 1, kRes>(X, xs, W, ws, p, sms, stream);
+        return tile == 2562 ? launch<kFmt, 256, 2, kRes>(X.codes, X.scales, W, ws, p, sms, stream)
+                            : launch<kFmt, 128, 1, kRes>(X.codes, X.scales, W, ws, p, sms, stream);
     };
     auto pick_res = [&](auto fmt) {
         return p.residual != nullptr ? pick(fmt, std::integral_constant<bool, true>{}) : pick(fmt, std::integral_constant<bool, false>{});
     };
     return format == LYRAQ_NVFP4 ? pick_res(std::integral_constant<int, LYRAQ_NVFP4>{}) : pick_res(std::integral_constant<int, LYRAQ_MXFP4>{});
+}
+
+int product(const Fp4Input& X, const float* g_x, const uint8_t* W, const uint8_t* ws, const float* g_w, int format, void* Y, int c_dtype, const void* bias,
+            const void* residual, float beta, int epilogue, int m, int n, int k, cudaStream_t stream)
+{
+    Fp4GemmParams p{};
+    p.M        = m;
+    p.N        = n;
+    p.K        = k;
+    p.C        = Y;
+    p.c_dtype  = c_dtype;
+    p.s_x      = g_x;
+    p.s_w      = g_w;
+    p.bias     = bias;
+    p.residual = residual;
+    p.beta     = beta;
+    p.gelu     = epilogue == LYRAQ_EPI_GELU_TANH;
+    p.status   = status_word_ptr();
+    const int sms = device_sm_count();
+    if (p.status == nullptr || sms <= 0) {
+        return LYRAQ_ERR_CUDA;
+    }
+    return run(X, W, ws, format, p, sms, stream);
 }
 
 }  // namespace fp4
@@ -735,24 +763,8 @@ int lyraq_gemm_fp4(const uint8_t* X, const uint8_t* x_scale, const float* x_tens
         (residual != nullptr && !aligned16(residual))) {
         return LYRAQ_ERR_INVALID_ARG;
     }
-    Fp4GemmParams p{};
-    p.M        = m;
-    p.N        = n;
-    p.K        = k;
-    p.C        = Y;
-    p.c_dtype  = c_dtype;
-    p.s_x      = x_tensor_scale;
-    p.s_w      = w_tensor_scale;
-    p.bias     = bias;
-    p.residual = residual;
-    p.beta     = beta;
-    p.gelu     = epilogue == LYRAQ_EPI_GELU_TANH;
-    p.status   = status_word_ptr();
-    const int sms = device_sm_count();
-    if (p.status == nullptr || sms <= 0) {
-        return LYRAQ_ERR_CUDA;
-    }
-    return fp4::run(X, x_scale, W, w_scale, format, p, sms, (cudaStream_t)stream);
+    return fp4::product({X, x_scale, nullptr, 0, 0}, x_tensor_scale, W, w_scale, w_tensor_scale, format, Y, c_dtype, bias, residual, beta, epilogue, m, n, k,
+                        (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -23,8 +23,21 @@ struct Fp4GemmParams {
 
 namespace fp4 {
 constexpr int kFp4SkinnyRows = 16;   // most rows of X that gemm_fp4_skinny.cu takes
-int launch_skinny(const uint8_t* X, const uint8_t* xs, const uint8_t* W, const uint8_t* ws, int format, const Fp4GemmParams& p, int sms,
-                  cudaStream_t stream);
+
+// The left operand: FP4 codes with their block scales, or (codes null) rows of a 16- or 32-bit type that the few-row kernel quantizes itself.
+struct Fp4Input {
+    const uint8_t* codes;
+    const uint8_t* scales;
+    const void*    x;
+    int            dtype;
+    size_t         ldx;
+};
+
+int  launch_skinny(const Fp4Input& X, const uint8_t* W, const uint8_t* ws, int format, const Fp4GemmParams& p, int sms, cudaStream_t stream);
+bool few_rows(int m, int k);   // whether a product takes the few-row kernel
+// lyraq_gemm_fp4 behind its checks; rows that are not FP4 yet only where few_rows
+int product(const Fp4Input& X, const float* g_x, const uint8_t* W, const uint8_t* ws, const float* g_w, int format, void* Y, int c_dtype, const void* bias,
+            const void* residual, float beta, int epilogue, int m, int n, int k, cudaStream_t stream);
 }  // namespace fp4
 
 __device__ __forceinline__ float fp4_tensor_scale(const Fp4GemmParams& p)

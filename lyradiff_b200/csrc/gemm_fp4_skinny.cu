@@ -10,7 +10,9 @@
 //              kernels in front of it, it asks its share of W into L2: the weight stream starts while the quantize of X still runs.  A
 //              prefetch is not a read: whatever that kernel writes is what the loads behind the wait see.
 //   warp 1   : scales to tensor memory, MMAs; the warp owns tensor memory
-//   warps 2-5: accumulator -> shared memory of the owning CTA -> sum, epilogue, store
+//   warps 2-5: accumulator -> shared memory of the owning CTA -> sum, epilogue, store.  For rows of X that are not FP4 yet they fill the stages' X and its
+//              scales before that, 32 values a thread: every CTA quantizes what it reads, behind the weight stream, which saves a launch
+//              and the way through memory
 // All waits are bounded.  A timeout sets the status word and the abort flag of every CTA of the cluster: the sums a CTA stores need the partial
 // products of all of them, so when one gives up none of the cluster stores anything.
 #include "gemm_fp4.cuh"
@@ -86,13 +88,15 @@ template<typename T> __device__ __forceinline__ void finish(const Fp4GemmParams&
     reinterpret_cast<T*>(p.C)[at] = from_f32<T>(t);
 }
 
-template<int FORMAT>
+// X: the type of the rows, or void where they are FP4
+template<int FORMAT, typename X>
 __global__ void __launch_bounds__(kThreads, 2)
 gemm_fp4_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_sw,
-                       const __grid_constant__ CUtensorMap tmap_sx, const Fp4GemmParams p, const int num_kb, const int splits, const int stalled_rank,
-                       const unsigned wait_limit_ms)
+                       const __grid_constant__ CUtensorMap tmap_sx, const Fp4GemmParams p, const void* rows, const size_t ldx, const int num_kb,
+                       const int splits, const int stalled_rank, const unsigned wait_limit_ms)
 {
     using S = Smem<FORMAT>;
+    constexpr bool kQuantize = !std::is_void_v<X>;
     extern __shared__ uint8_t smem_raw[];
     // the dynamic shared window starts at the same offset in every CTA of the kernel, so the layout is that of the peers too
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -112,6 +116,11 @@ gemm_fp4_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
     const int      kb0  = (int)((long long)num_kb * rank / splits);
     const int      kb1  = (int)((long long)num_kb * (rank + 1) / splits);
     const uint64_t wait_limit_ns = (uint64_t)wait_limit_ms * 1000000u;
+    // Quantizing warps: a quarter of a warp has a row's 256 values of a K block.  Up to four rows, a warp takes all of them for one K block or for the
+    // few that fill it; more rows are dealt to two or four warps, each with one K block after the other.
+    const int rows_log2    = p.M <= 1 ? 0 : 32 - __clz(p.M - 1);
+    const int kbs_per_warp = rows_log2 <= 2 ? 4 >> rows_log2 : 1;
+    const int warps_per_kb = rows_log2 <= 2 ? 1 : 1 << (rows_log2 - 2);
     // records a wait that ran out and stops the whole cluster; its writes are visible to the peers behind the barrier in front of the sums
     auto give_up = [&](unsigned code) {
         report_timeout(p.status, code);
@@ -123,7 +132,7 @@ gemm_fp4_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
     grid_launch_dependents();
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
-            mbar_init(full_bar(s), 1);
+            mbar_init(full_bar(s), 1u + (kQuantize ? (uint32_t)warps_per_kb : 0u));
             mbar_init(empty_bar(s), 1);
         }
         mbar_init(acc_bar, 1);
@@ -158,11 +167,13 @@ gemm_fp4_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
             }
             if (elect_one()) {
                 const uint32_t w = smem_base + stage * S::kStage, x = w + S::kW, sw = x + S::kX, sx = sw + S::kSw;
-                mbar_arrive_expect_tx(full_bar(stage), (uint32_t)S::kBytes);
+                mbar_arrive_expect_tx(full_bar(stage), (uint32_t)(kQuantize ? S::kW + S::kSw : S::kBytes));
                 tma_load_2d(w, &tmap_w, full_bar(stage), kb * kRowBytes, n0);
                 tma_load_3d(sw, &tmap_sw, full_bar(stage), 0, kb * S::kAtoms, tile);
-                tma_load_2d(x, &tmap_x, full_bar(stage), kb * kRowBytes, 0);
-                tma_load_3d(sx, &tmap_sx, full_bar(stage), 0, kb * S::kAtoms, 0);
+                if (!kQuantize) {
+                    tma_load_2d(x, &tmap_x, full_bar(stage), kb * kRowBytes, 0);
+                    tma_load_3d(sx, &tmap_sx, full_bar(stage), 0, kb * S::kAtoms, 0);
+                }
             }
             ++issued;
             if (++stage == kStages) {
@@ -232,6 +243,67 @@ gemm_fp4_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
             }
         }
         (void)ok;
+    } else if constexpr (kQuantize) {
+        constexpr int kPer  = 16 / (int)sizeof(X);
+        constexpr int kVecs = 32 / kPer;
+        const int     qw = warp - 2, j = lane & 7, quarter = lane >> 3;
+        const int     row   = rows_log2 <= 2 ? quarter & ((1 << rows_log2) - 1) : (qw & (warps_per_kb - 1)) * 4 + quarter;
+        const int     sub   = rows_log2 <= 2 ? quarter >> rows_log2 : 0;
+        const int     round = kbs_per_warp * (4 / warps_per_kb);      // K blocks that the four warps take at a time
+        const X*      src = reinterpret_cast<const X*>(rows) + (size_t)row * ldx;
+        auto load = [&](int kb, Vec16* v) {
+#pragma unroll
+            for (int a = 0; a < kVecs; ++a) {
+                v[a] = Vec16{};
+                if (row < p.M && kb < kb1 && kb * kBlockK + j * 32 < p.K) {   // K is a multiple of 32; zeros have zero codes and scales
+                    v[a] = ld_nc_16(src + (size_t)kb * kBlockK + j * 32 + a * kPer);
+                }
+            }
+        };
+        Vec16 v[kVecs], ahead[kVecs];
+        int   base = kb0 + qw / warps_per_kb * kbs_per_warp;
+        load(base + sub, v);
+        const Fp4Tensor tensor = fp4_tensor<FORMAT>(p.s_x);
+        for (bool ok = true; ok && base < kb1; base += round) {
+            load(base + round + sub, ahead);
+            for (int s = 0; ok && s < kbs_per_warp && base + s < kb1; ++s) {
+                const int i = base + s - kb0;
+                ok = mbar_wait_warp(empty_bar(i % kStages), (uint32_t)(i / kStages & 1) ^ 1u, abort_flag, wait_limit_ns);
+            }
+            if (!ok) {
+                if (lane == 0) {
+                    give_up(0x6400u);
+                }
+                break;
+            }
+            Vec16          o;
+            const uint32_t code = fp4_encode32<X, FORMAT>(v, tensor, o);
+            if (base + sub < kb1 && row < p.M) {
+                uint8_t* x  = gen_base + (base + sub - kb0) % kStages * S::kStage + S::kW;
+                uint8_t* sx = x + S::kX + S::kSw;
+                *reinterpret_cast<Vec16*>(x + row * kRowBytes + ((j ^ (row & 7)) << 4)) = o;    // the 128-byte swizzle
+                if (FORMAT == LYRAQ_NVFP4) {
+                    *reinterpret_cast<uint16_t*>(sx + (j >> 1) * 256 + row * 16 + (j & 1) * 2) = (uint16_t)code;
+                } else {
+                    sx[(j >> 2) * 256 + row * 16 + (j & 3)] = (uint8_t)code;
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                for (int s = 0; s < kbs_per_warp && base + s < kb1; ++s) {
+                    mbar_arrive(full_bar((base + s - kb0) % kStages));
+                }
+            }
+#pragma unroll
+            for (int a = 0; a < kVecs; ++a) {
+                v[a] = ahead[a];
+            }
+        }
+    }
+    float scale = 0.0f;
+    if (warp >= 2) {
+        scale = fp4_tensor_scale(p);   // asked for before the accumulator is waited for
     }
     // ---- accumulator lane = row of W; the CTA of rank r owns the token columns [r kRows / S, (r + 1) kRows / S)
     const int slice = kRows / splits;
@@ -263,8 +335,7 @@ gemm_fp4_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
         tmem_dealloc(tmem_base, 256);
     }
     if (warp >= 2 && *abort_flag == 0 && n0 + wrow < p.N) {
-        const float* red   = reinterpret_cast<const float*>(gen_base + S::kRedOffset);
-        const float  scale = fp4_tensor_scale(p);
+        const float* red = reinterpret_cast<const float*>(gen_base + S::kRedOffset);
         for (int c = 0; c < slice; ++c) {
             const int m = rank * slice + c;
             if (m >= p.M) {
@@ -303,8 +374,8 @@ static int pick_splits(long tiles, int num_kb, int sms)
 static int          g_stalled_rank  = -1;
 static unsigned int g_wait_limit_ms = kWaitLimitNs / 1000000;
 
-template<int FORMAT>
-static int launch(const uint8_t* X, const uint8_t* xs, const uint8_t* W, const uint8_t* ws, const Fp4GemmParams& p, int sms, cudaStream_t stream)
+template<int FORMAT, typename X>
+static int launch(const Fp4Input& in, const uint8_t* W, const uint8_t* ws, const Fp4GemmParams& p, int sms, cudaStream_t stream)
 {
     using S = Smem<FORMAT>;
     const int      n_tiles = (int)(((long)p.N + kWRows - 1) / kWRows);
@@ -314,33 +385,45 @@ static int launch(const uint8_t* X, const uint8_t* xs, const uint8_t* W, const u
     CUtensorMap    tw, tx, tsw, tsx;
     int            st = make_tmap_bytes_2d(&tw, W, (uint64_t)p.N, kb, kb, kWRows, kRowBytes, true);
     if (st == LYRAQ_OK) {
-        st = make_tmap_bytes_2d(&tx, X, (uint64_t)p.M, kb, kb, kRows, kRowBytes, true);
-    }
-    if (st == LYRAQ_OK) {
         st = make_tmap_atoms(&tsw, ws, ((uint64_t)p.N + 127) / 128, atoms, 1, S::kAtoms, 128);
     }
-    if (st == LYRAQ_OK) {
-        st = make_tmap_atoms(&tsx, xs, 1, atoms, 1, S::kAtoms, 64);
+    if (!std::is_void_v<X>) {
+        tx  = tw;    // never used
+        tsx = tsw;
+    } else {
+        if (st == LYRAQ_OK) {
+            st = make_tmap_bytes_2d(&tx, in.codes, (uint64_t)p.M, kb, kb, kRows, kRowBytes, true);
+        }
+        if (st == LYRAQ_OK) {
+            st = make_tmap_atoms(&tsx, in.scales, 1, atoms, 1, S::kAtoms, 64);
+        }
     }
     static bool smem_raised[64] = {};
     if (st == LYRAQ_OK) {
-        st = raise_dynamic_smem_once(gemm_fp4_skinny_kernel<FORMAT>, S::kTotal, smem_raised, "cudaFuncSetAttribute(gemm_fp4_skinny_kernel)");
+        st = raise_dynamic_smem_once(gemm_fp4_skinny_kernel<FORMAT, X>, S::kTotal, smem_raised, "cudaFuncSetAttribute(gemm_fp4_skinny_kernel)");
     }
     if (st != LYRAQ_OK) {
         return st;
     }
-    return cuda_status(launch_kernel(gemm_fp4_skinny_kernel<FORMAT>, (unsigned)(n_tiles * splits), (unsigned)kThreads, (size_t)S::kTotal, stream,
-                                     (unsigned)splits, tw, tx, tsw, tsx, p, num_kb, splits, g_stalled_rank, g_wait_limit_ms),
+    return cuda_status(launch_kernel(gemm_fp4_skinny_kernel<FORMAT, X>, (unsigned)(n_tiles * splits), (unsigned)kThreads, (size_t)S::kTotal, stream,
+                                     (unsigned)splits, tw, tx, tsw, tsx, p, in.x, in.ldx, num_kb, splits, g_stalled_rank, g_wait_limit_ms),
                        "cudaLaunchKernelEx(gemm_fp4_skinny_kernel)");
+}
+
+template<int FORMAT>
+static int launch_of(const Fp4Input& in, const uint8_t* W, const uint8_t* ws, const Fp4GemmParams& p, int sms, cudaStream_t stream)
+{
+    return in.codes != nullptr        ? launch<FORMAT, void>(in, W, ws, p, sms, stream)
+           : in.dtype == LYRAQ_BF16   ? launch<FORMAT, __nv_bfloat16>(in, W, ws, p, sms, stream)
+           : in.dtype == LYRAQ_F16    ? launch<FORMAT, __half>(in, W, ws, p, sms, stream)
+                                      : launch<FORMAT, float>(in, W, ws, p, sms, stream);
 }
 
 }  // namespace skinny
 
-int launch_skinny(const uint8_t* X, const uint8_t* xs, const uint8_t* W, const uint8_t* ws, int format, const Fp4GemmParams& p, int sms,
-                  cudaStream_t stream)
+int launch_skinny(const Fp4Input& X, const uint8_t* W, const uint8_t* ws, int format, const Fp4GemmParams& p, int sms, cudaStream_t stream)
 {
-    return format == LYRAQ_NVFP4 ? skinny::launch<LYRAQ_NVFP4>(X, xs, W, ws, p, sms, stream)
-                                 : skinny::launch<LYRAQ_MXFP4>(X, xs, W, ws, p, sms, stream);
+    return format == LYRAQ_NVFP4 ? skinny::launch_of<LYRAQ_NVFP4>(X, W, ws, p, sms, stream) : skinny::launch_of<LYRAQ_MXFP4>(X, W, ws, p, sms, stream);
 }
 
 }  // namespace fp4

@@ -2,7 +2,7 @@
 // the quantized activation (and its scales) held in caller-provided workspace.  These are what the reference's layers
 // do around every quantized linear with buffers from their allocator; here the caller owns the buffer.
 #include "common.cuh"
-#include "fp4.cuh"
+#include "gemm_fp4.cuh"
 #include "gemm_w4a4.cuh"
 
 namespace lyraq {
@@ -106,11 +106,23 @@ int lyraq_linear_fp4_forward(void* Y, const void* x, int dtype, size_t ldx, cons
     }
     uint8_t* qx = static_cast<uint8_t*>(workspace);
     uint8_t* sx = qx + align_up((size_t)m * (size_t)k / 2, 256);
-    int      st = lyraq_quant_fp4(qx, sx, x, dtype, ldx, x_tensor_scale, format, (size_t)m, (size_t)k, stream);
+    const float* g = format == LYRAQ_NVFP4 ? x_tensor_scale : nullptr;
+    int          st;
+    // One launch, which quantizes the rows on their way.  Every CTA reads all rows, so a result in their place needs them quantized before.
+    const size_t   bytes = dtype == LYRAQ_F32 ? 4 : 2;
+    const uint8_t *x0 = static_cast<const uint8_t*>(x), *y0 = static_cast<const uint8_t*>(Y);
+    const bool     apart = y0 + (size_t)m * (size_t)n * bytes <= x0 || x0 + ((size_t)(m - 1) * ldx + (size_t)k) * bytes <= y0;
+    if (apart && fp4::few_rows(m, k)) {
+        st = check_fp4(qx, sx, x, dtype, ldx, format, (size_t)m, (size_t)k);
+        return st != LYRAQ_OK ? st
+                              : fp4::product({nullptr, nullptr, x, dtype, ldx}, g, W, w_scale, w_tensor_scale, format, Y, dtype, bias, residual, beta, epilogue,
+                                             m, n, k, (cudaStream_t)stream);
+    }
+    st = lyraq_quant_fp4(qx, sx, x, dtype, ldx, g, format, (size_t)m, (size_t)k, stream);
     if (st != LYRAQ_OK) {
         return st;
     }
-    return lyraq_gemm_fp4(qx, sx, x_tensor_scale, W, w_scale, w_tensor_scale, format, Y, dtype, bias, residual, beta, epilogue, m, n, k, stream);
+    return lyraq_gemm_fp4(qx, sx, g, W, w_scale, w_tensor_scale, format, Y, dtype, bias, residual, beta, epilogue, m, n, k, stream);
 }
 
 int lyraq_linear_int8_forward(void* Y, const void* x, int dtype, const float* pre_quant_scale, const float* input_scale,

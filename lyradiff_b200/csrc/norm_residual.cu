@@ -44,7 +44,7 @@ struct NormParams {
 // FORMAT: -1 without an FP4 output.  ALL: every parameter and the new stream are there.  FULL: every vector of every thread is.  The kernel is bound by
 // the instructions it issues, and asking took a sixth of them: [4608, 3072] 25.1 us without, 22.3 with ALL, 21.5 with both.
 template<typename T, int VPT, int FORMAT, bool WARP, bool ALL, bool FULL>
-__global__ void __launch_bounds__(WARP ? 256 : 512)
+__global__ void __launch_bounds__(WARP ? 256 : 512, 2)
 norm_residual_kernel(const NormParams p)
 {
     __shared__ float part[4][16];

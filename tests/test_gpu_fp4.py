@@ -396,6 +396,62 @@ def test_layer_is_quantize_then_product(ops, fmt, dtype, lead):
         layer.forward(cu(x), residual=cu(r).float())
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("n,k", [(136, 32), (520, 96), (264, 1312), (4224, 2048), (72, 12320), (9216, 3072)])
+def test_few_rows_quantized_on_their_way(ops, tile, fmt, dtype, n, k):
+    """The layer's one launch gives the bits of the quantizer and the product in turn, for every number of rows and way of dealing them to warps."""
+    from lyradiff_b200 import layers
+    g = torch.Generator().manual_seed(n + k)
+    w, b = (torch.randn(n, k, generator=g) * 0.05).to(dtype), torch.randn(n, generator=g).to(dtype)
+    layer = layers.Fp4Linear(cu(w), cu(b), torch.tensor(2.0 ** -7), fmt=fmt)
+    wide = torch.full((16, k + 40), float("nan"), dtype=dtype, device="cuda")
+    wide[:, :k] = torch.randn(16, k, generator=g).to(dtype).cuda()
+    wide[3, k // 2] = float("inf")
+    for m in (1, 2, 3, 4, 5, 8, 9, 16):
+        x = wide[:m, :k]
+        tile(1281)          # two launches
+        q = layer.empty_input(m)
+        ops.quant_fp4(x, out=q)
+        tile(16)
+        want = layer.forward_quantized(q, dtype)
+        got = layer.forward(x)
+        check_status()
+        assert torch.equal(torch.nan_to_num(got, 7.0), torch.nan_to_num(want, 7.0)) and bool(torch.isnan(got).any()) == (m > 3)
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+
+
+def test_few_rows_with_the_result_in_their_place(ops):
+    from lyradiff_b200 import layers
+    g = torch.Generator().manual_seed(5)
+    w, x = (torch.randn(2048, 2048, generator=g) * 0.05).bfloat16(), torch.randn(9, 2048, generator=g).bfloat16()
+    layer = layers.Fp4Linear(cu(w), None, torch.tensor(2.0 ** -7))
+    y = cu(x).clone()
+    assert torch.equal(layer.forward(y, out=y), layer.forward(cu(x)))
+    check_status()
+
+
+@pytest.mark.parametrize("stalled", [0, 1])
+def test_few_rows_quantized_on_their_way_wait_that_runs_out_stores_nothing(ops, stalled):
+    from lyradiff_b200 import _lib, layers
+    g = torch.Generator().manual_seed(6)
+    layer = layers.Fp4Linear(cu((torch.randn(512, 2048, generator=g) * 0.05).bfloat16()), None, torch.tensor(2.0 ** -7))
+    x, out = cu(torch.randn(4, 2048, generator=g).bfloat16()), torch.full((4, 512), 7.0, dtype=torch.bfloat16, device="cuda")
+    good = layer.forward(x)
+    check_status()
+    assert _lib.lib().lyraq_debug_fp4_skinny_wait_test(stalled, 50) == 0
+    try:
+        layer.forward(x, out=out)
+        torch.cuda.synchronize()
+        status, detail = ops.last_status()
+    finally:
+        assert _lib.lib().lyraq_debug_fp4_skinny_wait_test(-1, 0) == 0
+    assert status == 4 and 0x6000 <= detail < 0x7000, (status, hex(detail))
+    assert bool((out == 7.0).all())
+    assert torch.equal(layer.forward(x, out=out), good)
+    check_status()
+
+
 def test_layer_in_two_captured_graphs_and_on_two_streams(ops):
     """Nothing is shared between calls: graphs captured from one layer replay at the same time and with new inputs."""
     from lyradiff_b200 import layers
