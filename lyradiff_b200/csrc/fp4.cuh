@@ -123,7 +123,7 @@ template<int FORMAT> __device__ __forceinline__ uint32_t fp4_encode8(const float
     for (int j = 0; j < 8; ++j) {
         q[j] = x[j];
     }
-    if (FORMAT == LYRAQ_NVFP4 && !b.plain) {   // no divisions here either: they are long, and every launch would fetch them on its way past
+    if (FORMAT == LYRAQ_NVFP4 && __builtin_expect(!b.plain, 0)) {   // no divisions here either: they are long, and every launch would fetch them on its way past
         const float c = fp4_range(t);
         t *= c;
         r = t > 0.0f ? rcp_approx(t) : 0.0f;

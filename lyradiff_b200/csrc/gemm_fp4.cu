@@ -679,6 +679,8 @@ bool few_rows(int m, int k)
     return m <= kFp4SkinnyRows && (g_forced_tile == 16 || (g_forced_tile == 0 && (num_kb >= 8 || m <= 2 + num_kb / 2)));
 }
 
+bool few_rows_quantize(int m, int n, int k) { return few_rows(m, k) && (g_forced_tile == 16 || skinny_quantize_pays(m, n, k, device_sm_count())); }
+
 static int run(const Fp4Input& X, const uint8_t* W, const uint8_t* ws, int format, const Fp4GemmParams& p, int sms, cudaStream_t stream)
 {
     const long m128 = ((long)p.M + 127) / 128, n128 = ((long)p.N + 127) / 128, m256 = ((long)p.M + 255) / 256, n256 = ((long)p.N + 255) / 256;

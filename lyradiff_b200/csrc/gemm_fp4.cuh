@@ -34,7 +34,9 @@ struct Fp4Input {
 };
 
 int  launch_skinny(const Fp4Input& X, const uint8_t* W, const uint8_t* ws, int format, const Fp4GemmParams& p, int sms, cudaStream_t stream);
-bool few_rows(int m, int k);   // whether a product takes the few-row kernel
+bool skinny_quantize_pays(int m, int n, int k, int sms);
+bool few_rows(int m, int k);                  // whether a product takes the few-row kernel,
+bool few_rows_quantize(int m, int n, int k);  // and whether a linear leaves the quantize to it
 // lyraq_gemm_fp4 behind its checks; rows that are not FP4 yet only where few_rows
 int product(const Fp4Input& X, const float* g_x, const uint8_t* W, const uint8_t* ws, const float* g_w, int format, void* Y, int c_dtype, const void* bias,
             const void* residual, float beta, int epilogue, int m, int n, int k, cudaStream_t stream);

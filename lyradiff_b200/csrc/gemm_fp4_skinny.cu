@@ -1,7 +1,7 @@
 // FP4 linear for few tokens: Y[m,n] = T(epi(g_x g_w (X W^T) + beta R + bias)) with so few rows of X that the tiles of gemm_fp4_kernel leave
 // most of the chip idle.
 //
-// What bounds it is the weight: every byte of it is read once (16 MB for [9216, 3072], 2.4 us of HBM), the arithmetic is negligible.  So the
+// What bounds it is the weight: every byte of it is read once (16 MB for [9216, 3072], 2.4 us of HBM; measured 5.1), the arithmetic is negligible.  So the
 // operands change places, 128 rows of W on the M side of the MMA, the rows of X (padded to 16 by TMA) on its N side, and K is split over the
 // CTAs of a cluster until all SMs stream.  The partial products meet through distributed shared memory: each CTA of the cluster owns a share of
 // the token columns, receives the others' partials for them and adds them in rank order, so the result does not depend on timing.
@@ -370,6 +370,20 @@ static int pick_splits(long tiles, int num_kb, int sms)
     return s;
 }
 
+// Quantizing in the kernel saves a launch, and every CTA does it for the K blocks it reads: it pays up to 64 rows times K blocks of a CTA, rows in powers of
+// two.  In the kernel against a launch of its own, nvfp4 / mxfp4, us: 1 row of [1280, 1280] 3.8 and 4.7 / 3.3 and 4.2, of [9216, 3072] (6) 6.2 and 6.4 / 5.3 and
+// 5.8, 16 rows of [1280, 2048] (32) 6.1 and 6.6 / 5.3 and 6.2, of [3072, 3072] (48) 7.1 and 7.2 / 6.2 and 6.8, of [9216, 3072] (96) 11.1 and
+// 9.6 / 9.6 and 8.8, of [3072, 12288] (96) 11.4 and 9.7 / 9.8 and 9.1.
+static bool quantize_pays(int m, int n, int k, int sms)
+{
+    const int num_kb = (k + kBlockK - 1) / kBlockK, splits = pick_splits(((long)n + kWRows - 1) / kWRows, num_kb, sms);
+    int       rows   = 1;
+    while (rows < m) {
+        rows *= 2;
+    }
+    return (long long)rows * ((num_kb + splits - 1) / splits) <= 64;
+}
+
 // Test hook (lyraq_debug_fp4_skinny_wait_test)
 static int          g_stalled_rank  = -1;
 static unsigned int g_wait_limit_ms = kWaitLimitNs / 1000000;
@@ -420,6 +434,8 @@ static int launch_of(const Fp4Input& in, const uint8_t* W, const uint8_t* ws, co
 }
 
 }  // namespace skinny
+
+bool skinny_quantize_pays(int m, int n, int k, int sms) { return skinny::quantize_pays(m, n, k, sms); }
 
 int launch_skinny(const Fp4Input& X, const uint8_t* W, const uint8_t* ws, int format, const Fp4GemmParams& p, int sms, cudaStream_t stream)
 {

@@ -112,7 +112,7 @@ int lyraq_linear_fp4_forward(void* Y, const void* x, int dtype, size_t ldx, cons
     const size_t   bytes = dtype == LYRAQ_F32 ? 4 : 2;
     const uint8_t *x0 = static_cast<const uint8_t*>(x), *y0 = static_cast<const uint8_t*>(Y);
     const bool     apart = y0 + (size_t)m * (size_t)n * bytes <= x0 || x0 + ((size_t)(m - 1) * ldx + (size_t)k) * bytes <= y0;
-    if (apart && fp4::few_rows(m, k)) {
+    if (apart && fp4::few_rows_quantize(m, n, k)) {
         st = check_fp4(qx, sx, x, dtype, ldx, format, (size_t)m, (size_t)k);
         return st != LYRAQ_OK ? st
                               : fp4::product({nullptr, nullptr, x, dtype, ldx}, g, W, w_scale, w_tensor_scale, format, Y, dtype, bias, residual, beta, epilogue,
