@@ -49,7 +49,7 @@ fp4_quant_kernel(uint8_t* q, uint8_t* sf, const T* x, size_t ldx, const float* t
     uint32_t        code   = 0;
     if (in) {
         Vec16 o;
-        code = fp4_encode32<T, FORMAT>(v, tensor, o);
+        code = fp4_encode32<T, FORMAT, false>(v, tensor, o);
         st_16(q + row * (k >> 1) + (col >> 1), o);
     }
     // blocks beyond k have scale 0, so the word of an existing row is always written whole

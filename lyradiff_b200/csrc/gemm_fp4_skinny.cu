@@ -276,8 +276,8 @@ gemm_fp4_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
                 }
                 break;
             }
-            Vec16          o;
-            const uint32_t code = fp4_encode32<X, FORMAT>(v, tensor, o);
+            Vec16          o{};
+            const uint32_t code = fp4_encode32<X, FORMAT, true>(v, tensor, o);
             if (base + sub < kb1 && row < p.M) {
                 uint8_t* x  = gen_base + (base + sub - kb0) % kStages * S::kStage + S::kW;
                 uint8_t* sx = x + S::kX + S::kSw;
