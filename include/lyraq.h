@@ -489,7 +489,7 @@ LYRAQ_API int lyraq_linear_fp8_forward(void* Y, const void* x, int dtype, const 
                                        int m, int n, int k, void* workspace, size_t workspace_bytes, void* stream);
 
 /* FP4 linear: x [m, k] (row pitch ldx elements) -> FP4 with the tensor scale x_tensor_scale[0], then lyraq_gemm_fp4.  The workspace of
- * LYRAQ_OP_LINEAR_FP4 suffices for either format.  The FP4 form of lyraq_linear_fp8_forward; no counterpart in the reference. */
+ * LYRAQ_OP_LINEAR_FP4 suffices for either format (calls of few rows ask for it too, and use it only where Y overlaps x).  The FP4 form of lyraq_linear_fp8_forward; no counterpart in the reference. */
 LYRAQ_API int lyraq_linear_fp4_forward(void* Y, const void* x, int dtype, size_t ldx, const float* x_tensor_scale, const uint8_t* W,
                                        const uint8_t* w_scale, const float* w_tensor_scale, int format, const void* bias,
                                        const void* residual, float beta, int epilogue, int m, int n, int k, void* workspace,
