@@ -1,6 +1,8 @@
 """The FP4 linear, the fused norms and the rotary embedding over axes as they follow one another in a transformer block, with this library's attention
 between them; captured in a graph; and where their offsets pass 32 bits."""
 
+import threading
+
 import pytest
 import torch
 
@@ -121,6 +123,73 @@ def test_a_captured_block_replays_with_new_inputs_beside_an_eager_one(lib):
     for a, b, c in zip(got, want, again):
         if isinstance(a, torch.Tensor):
             assert torch.equal(a, b) and torch.equal(c, b)
+
+
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("rows", [1, 6])
+def test_a_chain_of_few_row_linears_replays(lib, fmt, rows):
+    """Launches that begin before their predecessors end, each of which reads what the one before wrote."""
+    layers, ops, _ = lib
+    g = torch.Generator().manual_seed(rows)
+    chain = [layers.Fp4Linear(cu((torch.randn(1024, 1024, generator=g) * 0.06).bfloat16()), None, torch.tensor(2.0 ** -6), fmt=fmt) for _ in range(6)]
+
+    def by_steps(x):
+        for layer in chain:
+            q = layer.empty_input(x.shape[0])
+            ops.quant_fp4(x, out=q)
+            torch.cuda.synchronize()
+            x = layer.forward_quantized(q, x.dtype)
+            torch.cuda.synchronize()
+        return x
+
+    def run(x):
+        for layer in chain:
+            x = layer.forward(x)
+        return x
+    x = torch.randn(rows, 1024, generator=g).bfloat16().cuda()
+    run(x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(x)
+    for seed in range(8):
+        x.copy_(torch.randn(rows, 1024, generator=g).bfloat16())
+        want = by_steps(x)
+        graph.replay()
+        assert torch.equal(run(x), want) and torch.equal(got, want)
+    check_status()
+
+
+def test_calls_from_several_threads(lib):
+    """Each thread on a stream of its own; the calls leave the interpreter lock while they launch."""
+    layers, ops, rope = lib
+    g = torch.Generator().manual_seed(9)
+    layer = layers.Fp4Linear(cu((torch.randn(512, 512, generator=g) * 0.05).bfloat16()), None, torch.tensor(2.0 ** -6))
+    plan, pos = rope.AxisRope((16, 24, 24)), torch.randint(0, 50, (40, 3), generator=g).cuda()
+    xs = [torch.randn(1, n, 512, generator=g).bfloat16().cuda() for n in (1, 40, 7, 40)]
+
+    def once(x):
+        y = layer.forward(x)
+        x1, h = ops.gated_residual_norm(y, x, post="layer")
+        n = x.shape[1]
+        return y, x1, h, ops.rope_axes(plan, pos[:n], h.view(1, n, 8, 64))[0]
+    want = [once(x) for x in xs]
+    torch.cuda.synchronize()
+    wrong, streams = [], [torch.cuda.Stream() for _ in xs]
+
+    def work(i):
+        with torch.cuda.stream(streams[i]):
+            for _ in range(60):
+                if not all(torch.equal(a, b) for a, b in zip(once(xs[i]), want[i])):
+                    wrong.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(xs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    check_status()
+    assert not wrong
 
 
 def test_offsets_beyond_32_bits(lib):
