@@ -262,7 +262,10 @@ norm_residual_kernel(const NormParams p)
     }
 }
 
-// Threads of a row.  Up to 1024 elements a warp has it (up to four vectors a lane) and no barrier; longer rows have a block, with three
+// Threads of a row.  Up to 1280 elements a warp may have it (up to five vectors a lane) and no barrier; whether it does depends on how many rows there are to
+// fill the chip with.  A warp against a block, us: 640 elements, 300 rows 3.6 / 3.6, 2400 4.6 / 6.0, 16384 16.9 / 20.1; 1024 elements, 450 rows 4.4 / 3.6, 900
+// 4.7 / 4.7, 16384 27.1 / 29.2; 1280 elements, 600 rows 5.0 / 4.5, 900 5.2 / 5.6, 4608 9.7 / 10.7, 8192 16.4 / 17.5, 12288 29.0 / 27.2 (two blocks of five
+// vectors a lane are all an SM holds).  Longer rows have a block, with three
 // vectors a thread where there are rows enough to fill the chip ([4608, 3072], us: one 34.8, two 28.8, three 25.4, four 28.5; a thread's part of the
 // three sums weighs more the fewer it has), and one where a call is latency; more only where 512 threads cannot have the row otherwise.
 struct NormSplit {
@@ -272,8 +275,9 @@ struct NormSplit {
 static NormSplit norm_split(size_t rows, int dim, int sms)
 {
     const int nvec = dim / 8;
-    if (nvec <= 128 && (nvec <= 32 || rows > (size_t)sms * 2)) {
-        return NormSplit{nvec <= 32 ? 1 : nvec <= 64 ? 2 : 4, 256, true};
+    const size_t fill = (size_t)sms * (nvec <= 80 ? 2 : 6);
+    if (nvec <= 32 || (nvec <= 128 && rows > fill) || (nvec <= 160 && rows > fill && rows <= (size_t)sms * 64)) {
+        return NormSplit{nvec <= 32 ? 1 : nvec <= 64 ? 2 : nvec <= 96 ? 3 : nvec <= 128 ? 4 : 5, 256, true};
     }
     int vpt = rows > (size_t)sms * 2 ? 3 : 1;
     while ((nvec + vpt - 1) / vpt > 512) {
@@ -350,7 +354,9 @@ extern "C" int lyraq_gated_residual_norm(const lyraq_gated_norm_t* a, void* stre
         if (split.warp) {
             return split.vpt == 1   ? launch(norm_residual_kernel<T, 1, kFmt, true, kAll, false>)
                    : split.vpt == 2 ? launch(norm_residual_kernel<T, 2, kFmt, true, kAll, false>)
-                                    : launch(norm_residual_kernel<T, 4, kFmt, true, kAll, false>);
+                   : split.vpt == 3 ? launch(norm_residual_kernel<T, 3, kFmt, true, kAll, false>)
+                   : split.vpt == 4 ? launch(norm_residual_kernel<T, 4, kFmt, true, kAll, false>)
+                                    : launch(norm_residual_kernel<T, 5, kFmt, true, kAll, false>);
         }
         return split.vpt == 3 && kAll && full ? launch(norm_residual_kernel<T, 3, kFmt, false, true, true>)
                : split.vpt == 1               ? launch(norm_residual_kernel<T, 1, kFmt, false, kAll, false>)

@@ -77,6 +77,26 @@ def test_against_the_formula(ops, dtype, post, pre, batch, seq, dim):
     assert_close(ho, h, dh)
 
 
+@pytest.mark.parametrize("post,pre", [("rms", "layer"), ("layer", "rms")])
+@pytest.mark.parametrize("rows,dim", [(889, 768), (901, 1000), (890, 1280), (1201, 1096), (9473, 1280)])
+def test_every_way_of_dealing_a_row_to_threads(ops, post, pre, rows, dim):
+    """Three, four and five vectors a lane of a warp, whole and in part, and a block where there are more rows than warps with five pay for; the quantized
+    outputs are those of the separate calls."""
+    t = make(1, rows, dim, torch.bfloat16, rows)
+    v, dv, h, dh = reference(t, post, pre, 0.75, 1e-5)
+    dev = {k: cu(a) for k, a in t.items()}
+    xo, ho = ops.gated_residual_norm(post=post, pre=pre, residual_scale=0.75, eps=1e-5, **dev)
+    check_status()
+    assert_close(xo, v, dv)
+    assert_close(ho, h, dh)
+    if dim % 32 == 0:
+        for fmt in ("nvfp4", "mxfp4"):
+            q = ops.Fp4Tensor.empty(rows, dim, fmt)
+            ops.gated_residual_norm(post=post, pre=pre, residual_scale=0.75, eps=1e-5, q4=q, **dev)
+            want = ops.quant_fp4(ho[0], None, fmt, ops.Fp4Tensor(rows, dim, fmt, torch.empty_like(q.codes), q.scales.clone()))
+            assert torch.equal(q.codes, want.codes) and torch.equal(q.scales, want.scales)
+
+
 @pytest.mark.parametrize("post,pre", CASES)
 def test_without_modulation_and_weights(ops, post, pre):
     t = make(2, 9, 320, torch.float16, 1, mod=False, weights=False)
