@@ -263,11 +263,13 @@ norm_residual_kernel(const NormParams p)
 }
 
 // Threads of a row.  Up to 1280 elements a warp may have it (up to five vectors a lane) and no barrier; whether it does depends on how many rows there are to
-// fill the chip with.  A warp against a block, us: 640 elements, 300 rows 3.6 / 3.6, 2400 4.6 / 6.0, 16384 16.9 / 20.1; 1024 elements, 450 rows 4.4 / 3.6, 900
+// fill the chip with.  A warp against a block, us: 640 elements, 300 rows 3.6 / 3.6, 2400 4.6 / 6.0, 16384 16.9 / 20.1; 1024 elements, 450 rows 4.4 / 3.1, 900
 // 4.7 / 4.7, 16384 27.1 / 29.2; 1280 elements, 600 rows 5.0 / 4.5, 900 5.2 / 5.6, 4608 9.7 / 10.7, 8192 16.4 / 17.5, 12288 29.0 / 27.2 (two blocks of five
-// vectors a lane are all an SM holds).  Longer rows have a block, with three
-// vectors a thread where there are rows enough to fill the chip ([4608, 3072], us: one 34.8, two 28.8, three 25.4, four 28.5; a thread's part of the
-// three sums weighs more the fewer it has), and one where a call is latency; more only where 512 threads cannot have the row otherwise.
+// vectors a lane are all an SM holds).
+// Longer rows have a block, best one without absent vectors (FULL): as many threads as let all rows run at once (1024 threads an SM), since a thread's part of
+// the sums weighs more the fewer vectors it has, and three or four vectors a thread where rows take turns.  Vectors a thread, us: 2048 elements, 1000 rows two
+// 4.5, three (not FULL) 6.1, four 6.9, 4608 rows 14.0 / 15.2 / 13.0; 3072 elements, 4608 rows 26.2 / 21.3 / 22.9; 8192 elements, 4608 rows 73 / 75 / 55; 2560
+// elements, 4608 rows 20.3 (FULL) / 18.8 / 19.4.
 struct NormSplit {
     int  vpt, threads;
     bool warp;
@@ -279,7 +281,13 @@ static NormSplit norm_split(size_t rows, int dim, int sms)
     if (nvec <= 32 || (nvec <= 128 && rows > fill) || (nvec <= 160 && rows > fill && rows <= (size_t)sms * 64)) {
         return NormSplit{nvec <= 32 ? 1 : nvec <= 64 ? 2 : nvec <= 96 ? 3 : nvec <= 128 ? 4 : 5, 256, true};
     }
-    int vpt = rows > (size_t)sms * 2 ? 3 : 1;
+    auto whole = [&](int vpt) { return nvec % (32 * vpt) == 0 && nvec / vpt <= 512; };
+    for (int vpt = rows <= (size_t)sms * 2 ? 1 : 2; vpt <= 4; ++vpt) {
+        if (whole(vpt) && rows <= (size_t)sms * (size_t)(1024 * vpt / nvec)) {
+            return NormSplit{vpt, nvec / vpt, false};
+        }
+    }
+    int vpt = rows <= (size_t)sms * 2 ? 1 : !whole(3) && whole(4) ? 4 : 3;
     while ((nvec + vpt - 1) / vpt > 512) {
         ++vpt;
     }
@@ -358,8 +366,13 @@ extern "C" int lyraq_gated_residual_norm(const lyraq_gated_norm_t* a, void* stre
                    : split.vpt == 4 ? launch(norm_residual_kernel<T, 4, kFmt, true, kAll, false>)
                                     : launch(norm_residual_kernel<T, 5, kFmt, true, kAll, false>);
         }
-        return split.vpt == 3 && kAll && full ? launch(norm_residual_kernel<T, 3, kFmt, false, true, true>)
-               : split.vpt == 1               ? launch(norm_residual_kernel<T, 1, kFmt, false, kAll, false>)
+        if (kAll && full) {
+            return split.vpt == 1   ? launch(norm_residual_kernel<T, 1, kFmt, false, true, true>)
+                   : split.vpt == 2 ? launch(norm_residual_kernel<T, 2, kFmt, false, true, true>)
+                   : split.vpt == 3 ? launch(norm_residual_kernel<T, 3, kFmt, false, true, true>)
+                                    : launch(norm_residual_kernel<T, 4, kFmt, false, true, true>);
+        }
+        return split.vpt == 1               ? launch(norm_residual_kernel<T, 1, kFmt, false, kAll, false>)
                : split.vpt == 2               ? launch(norm_residual_kernel<T, 2, kFmt, false, kAll, false>)
                : split.vpt == 3               ? launch(norm_residual_kernel<T, 3, kFmt, false, kAll, false>)
                                               : launch(norm_residual_kernel<T, 4, kFmt, false, kAll, false>);

@@ -78,10 +78,11 @@ def test_against_the_formula(ops, dtype, post, pre, batch, seq, dim):
 
 
 @pytest.mark.parametrize("post,pre", [("rms", "layer"), ("layer", "rms")])
-@pytest.mark.parametrize("rows,dim", [(889, 768), (901, 1000), (890, 1280), (1201, 1096), (9473, 1280)])
+@pytest.mark.parametrize("rows,dim", [(889, 768), (901, 1000), (890, 1280), (1201, 1096), (9473, 1280), (3, 1536), (320, 1536), (1200, 2048),
+                                      (1200, 4096), (300, 2560)])
 def test_every_way_of_dealing_a_row_to_threads(ops, post, pre, rows, dim):
-    """Three, four and five vectors a lane of a warp, whole and in part, and a block where there are more rows than warps with five pay for; the quantized
-    outputs are those of the separate calls."""
+    """Three, four and five vectors a lane of a warp, whole and in part, a block where there are more rows than warps with five pay for, blocks of one to
+    four vectors a thread without absent ones; the quantized outputs are those of the separate calls."""
     t = make(1, rows, dim, torch.bfloat16, rows)
     v, dv, h, dh = reference(t, post, pre, 0.75, 1e-5)
     dev = {k: cu(a) for k, a in t.items()}
@@ -190,7 +191,7 @@ def test_python_side_refuses(ops):
         ops.gated_residual_norm(wide, wide, x_out=both, h=both)
 
 
-@pytest.mark.parametrize("dim", [640, 1288])
+@pytest.mark.parametrize("dim", [640, 1288, 1536])
 def test_outputs_in_the_inputs_places(ops, dim):
     t = {k: cu(a) for k, a in make(2, 200, dim, torch.bfloat16, 11).items()}
     want = ops.gated_residual_norm(post="layer", pre="rms", **t)
