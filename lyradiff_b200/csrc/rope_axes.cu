@@ -29,6 +29,7 @@ struct RopeAxesParams {
     int                  pos_dtype;
     int                  heads[2];
     int                  head_dim, pairs, lanes_log2, groups, chunks, share, tokens_per_block;
+    int                  beside;      // tokens that a block's groups take at a time
     int                  wide;        // interleaved pairs whose 16 neighbours lie on 32 bytes, in and out
     unsigned             tokens, seq;
     float                eps, inv_dim;
@@ -127,8 +128,9 @@ template<int VEC> __device__ __forceinline__ void load_floats(const float* p, fl
 }
 
 // VEC: pairs of a lane's unit; NU: units of a lane (more than one only where 32 lanes of small units do not span a head); HALVES: pair i is (x[i], x[i + pairs]), else
-// (x[2 i], x[2 i + 1]); NORM: q or k is normalised.
-template<typename T, int VEC, int NU, bool HALVES, bool NORM>
+// (x[2 i], x[2 i + 1]); NORM: q or k is normalised; BESIDE: several tokens at a time (asking
+// for it took a block of many heads 23.6 -> 29.5 us).
+template<typename T, int VEC, int NU, bool HALVES, bool NORM, bool BESIDE>
 __global__ void __launch_bounds__(256) rope_axes_kernel(const RopeAxesParams p)
 {
     extern __shared__ __align__(16) float turn_c[];      // [2][tokens_per_block][pairs]: cosines, then sines
@@ -152,7 +154,8 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(const RopeAxesParams p)
     __syncthreads();
 
     const int lanes = 1 << p.lanes_log2;
-    const int lane = (int)threadIdx.x & (lanes - 1), group = (int)threadIdx.x >> p.lanes_log2;
+    const int lane = (int)threadIdx.x & (lanes - 1), any_group = (int)threadIdx.x >> p.lanes_log2;
+    const int next = BESIDE ? any_group / p.groups : 0, group = any_group - next * p.groups;     // which of the tokens beside each other, group of it
     const int units = p.head_dim / (2 * VEC), turning = p.pairs / VEC;     // units of a head, those of them that turn
     // this block's share of the heads, dealt to groups
     const int h0 = (int)chunk * p.share, h1 = min(h0 + p.share, p.heads[0] + p.heads[1]);
@@ -166,7 +169,9 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(const RopeAxesParams p)
         at_a[u]  = HALVES && turns[u] ? unit * VEC : unit * 2 * VEC;
         at_b[u]  = HALVES && turns[u] ? p.pairs + unit * VEC : unit * 2 * VEC + VEC;
     }
-    for (int tk = 0; tk < n_tok; ++tk) {
+    for (int t = 0; t < n_tok; t += BESIDE ? p.beside : 1) {
+        const bool     here  = !BESIDE || (next < p.beside && t + next < n_tok);
+        const int      tk    = BESIDE && here ? t + next : t;
         const unsigned token = t0 + tk, b = token / p.seq, s = token - b * p.seq;
         float          cosine[NU][VEC], sine[NU][VEC];
 #pragma unroll
@@ -193,7 +198,7 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(const RopeAxesParams p)
             for (int i = 0; i < 2; ++i) {
                 const int  head = hb + group + i * p.groups;
                 const bool is_k = head >= p.heads[0];
-                on[i]           = group < p.groups && head < h1;
+                on[i]           = (BESIDE ? here : group < p.groups) && head < h1;
                 const T* in     = is_k ? base_in[1] + (size_t)(head - p.heads[0]) * p.src_head[1] : base_in[0] + (size_t)head * p.src_head[0];
                 out[i]          = is_k ? base_out[1] + (size_t)(head - p.heads[0]) * p.dst_head[1] : base_out[0] + (size_t)head * p.dst_head[0];
                 w[i]            = reinterpret_cast<const T*>(is_k ? p.norm[1] : p.norm[0]);
@@ -374,7 +379,16 @@ extern "C" int lyraq_rope_axes(const lyraq_rope_axes_t* a, void* stream)
     const int rounds = (p.share + 2 * most - 1) / (2 * most);
     p.groups         = (p.share + 2 * rounds - 1) / (2 * rounds);
     p.tokens_per_block = p.tokens >= (unsigned)sms * 32 ? 4 : p.tokens >= (unsigned)sms * 16 ? 2 : 1;
-    const unsigned threads = (unsigned)((p.groups * lanes + 31) / 32 * 32);
+    // Heads that leave most of 128 threads idle: several tokens beside each other, as long as two blocks an SM are left.  One after the other / beside, us:
+    // 8000 tokens of 1 + 1 heads of 128 11.2 / 6.6, of 4 + 4 11.2 / 7.8, of 8 + 2 11.6 / 9.9; 30000 tokens of 1 + 1 20.6 / 13.2, but of 4 + 4 24.8 / 29.7:
+    // where there are many of both, a token a block at a time keeps more loads in flight.
+    p.beside = 1;
+    const bool few = p.groups * lanes <= 16 || p.tokens < (unsigned)sms * 100u;
+    while (p.chunks == 1 && few && 2 * p.beside * p.groups * lanes <= 128 && (unsigned)(2 * p.beside) * (unsigned)sms * 2u <= p.tokens) {
+        p.beside *= 2;
+    }
+    p.tokens_per_block     = p.tokens_per_block > p.beside ? p.tokens_per_block : p.beside;
+    const unsigned threads = (unsigned)((p.beside * p.groups * lanes + 31) / 32 * 32);
     const size_t   blocks  = ((size_t)p.tokens + p.tokens_per_block - 1) / p.tokens_per_block * (size_t)p.chunks;
     if (blocks > 0x7fffffffu) {
         return LYRAQ_ERR_UNSUPPORTED;
@@ -386,10 +400,14 @@ extern "C" int lyraq_rope_axes(const lyraq_rope_axes_t* a, void* stream)
     auto pick = [&](auto type, auto halves, auto normed) {
         using T           = decltype(type);
         constexpr bool kH = decltype(halves)::value, kN = decltype(normed)::value;
-        return vec == 8   ? launch(rope_axes_kernel<T, 8, 1, kH, kN>)
-               : vec == 4 ? launch(rope_axes_kernel<T, 4, 1, kH, kN>)
-               : vec == 2 ? launch(rope_axes_kernel<T, 2, 2, kH, kN>)
-                          : launch(rope_axes_kernel<T, 1, 4, kH, kN>);
+        auto by_tokens = [&](auto many) {
+            constexpr bool kB = decltype(many)::value;
+            return vec == 8   ? launch(rope_axes_kernel<T, 8, 1, kH, kN, kB>)
+                   : vec == 4 ? launch(rope_axes_kernel<T, 4, 1, kH, kN, kB>)
+                   : vec == 2 ? launch(rope_axes_kernel<T, 2, 2, kH, kN, kB>)
+                              : launch(rope_axes_kernel<T, 1, 4, kH, kN, kB>);
+        };
+        return p.beside > 1 ? by_tokens(std::integral_constant<bool, true>{}) : by_tokens(std::integral_constant<bool, false>{});
     };
     auto pick_norm = [&](auto type, auto halves) {
         return norm ? pick(type, halves, std::integral_constant<bool, true>{}) : pick(type, halves, std::integral_constant<bool, false>{});

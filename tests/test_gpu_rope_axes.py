@@ -65,7 +65,10 @@ def positions(batch, seq, axes, dtype, start=0):
 @pytest.mark.parametrize("norm", [True, False])
 @pytest.mark.parametrize("batch,seq,hq,hk,d,dims", [(1, 1, 1, 1, 64, (64,)), (2, 7, 24, 24, 128, (16, 56, 56)), (1, 33, 24, 8, 128, (16, 24, 24)), (3, 5, 5, 2, 72, (24, 24, 24)),
                                                     (1, 9, 3, 3, 80, (80,)), (1, 300, 12, 12, 128, (44, 42, 42)), (1, 4, 40, 1, 256, (128, 128)), (2, 3, 2, 1, 72, (36,)),
-                                                    (1, 2, 3, 2, 34, (10, 6)), (1, 5, 2, 2, 254, (84, 84, 84)), (1, 3, 2, 0, 128, ()), (1, 4800, 2, 1, 64, (32, 32))])
+                                                    (1, 2, 3, 2, 34, (10, 6)), (1, 5, 2, 2, 254, (84, 84, 84)), (1, 3, 2, 0, 128, ()), (1, 4800, 2, 1, 64, (32, 32)),
+                                                    # few heads: tokens beside each other, the last block's in part
+                                                    (3, 401, 1, 1, 128, (64,)), (1, 700, 3, 1, 80, (80,)), (1, 2503, 1, 0, 256, (128, 128)), (1, 4801, 1, 1, 2, (2,)),
+                                                    (2, 5001, 1, 1, 72, (36,))])
 def test_against_the_formula(ops, rope, dtype, interleaved, norm, batch, seq, hq, hk, d, dims):
     g = torch.Generator().manual_seed(d + seq)
     q, k = (torch.randn(batch, seq, h, d, generator=g).to(dtype) for h in (hq, hk))
