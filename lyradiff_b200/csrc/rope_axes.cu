@@ -370,8 +370,8 @@ extern "C" int lyraq_rope_axes(const lyraq_rope_axes_t* a, void* stream)
         ++p.lanes_log2;
     }
     // Groups: two heads each at a time (24 heads as 12 groups of two take 65 us for 32760 tokens of 128, as 24 of one 83), all of a token in as few
-    // rounds as 128 threads make of them, the rounds equally full (48 normalised heads with 192 threads 26.5 us, with 96 23.7).  Tokens: enough to share the cosines' cost, few enough to fill the chip;
-    // where there are few, a token's heads are dealt to several blocks.
+    // rounds as 128 threads make of them, the rounds equally full (48 normalised heads with 192 threads 26.5 us, with 96 23.7).
+    // Tokens: enough to share the cosines' cost, few enough to fill the chip; where there are few, a token's heads are dealt to several blocks.
     const int lanes  = 1 << p.lanes_log2;
     const int most   = 128 / lanes;
     p.chunks         = p.tokens >= (unsigned)sms * 2 ? 1 : (heads + most - 1) / most;
