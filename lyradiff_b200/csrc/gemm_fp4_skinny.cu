@@ -15,6 +15,7 @@
 //              and the way through memory
 // All waits are bounded.  A timeout sets the status word and the abort flag of every CTA of the cluster: the sums a CTA stores need the partial
 // products of all of them, so when one gives up none of the cluster stores anything.
+#include "fp4_deal.h"
 #include "gemm_fp4.cuh"
 
 namespace lyraq {
@@ -34,7 +35,7 @@ constexpr int kRows     = kFp4SkinnyRows;
 constexpr int kRowBytes = 128;
 constexpr int kBlockK   = 256;
 constexpr int kThreads  = 192;
-constexpr int kStages   = 4;      // two CTAs share an SM
+constexpr int kStages   = kDealStages;   // two CTAs share an SM
 
 template<int FORMAT> struct Smem {
     static constexpr int kAtoms     = kBlockK / fp4_atom_k(FORMAT);
@@ -116,11 +117,7 @@ gemm_fp4_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
     const int      kb0  = (int)((long long)num_kb * rank / splits);
     const int      kb1  = (int)((long long)num_kb * (rank + 1) / splits);
     const uint64_t wait_limit_ns = (uint64_t)wait_limit_ms * 1000000u;
-    // Quantizing warps: a quarter of a warp has a row's 256 values of a K block.  Up to four rows, a warp takes all of them for one K block or for the
-    // few that fill it; more rows are dealt to two or four warps, each with one K block after the other.
-    const int rows_log2    = p.M <= 1 ? 0 : 32 - __clz(p.M - 1);
-    const int kbs_per_warp = rows_log2 <= 2 ? 4 >> rows_log2 : 1;
-    const int warps_per_kb = rows_log2 <= 2 ? 1 : 1 << (rows_log2 - 2);
+    const FewRowsDeal deal = few_rows_deal(p.M);   // which K blocks a quantizing warp takes
     // records a wait that ran out and stops the whole cluster; its writes are visible to the peers behind the barrier in front of the sums
     auto give_up = [&](unsigned code) {
         report_timeout(p.status, code);
@@ -132,7 +129,7 @@ gemm_fp4_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
     grid_launch_dependents();
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
-            mbar_init(full_bar(s), 1u + (kQuantize ? (uint32_t)warps_per_kb : 0u));
+            mbar_init(full_bar(s), 1u + (kQuantize ? (uint32_t)deal.warps_per_kb : 0u));
             mbar_init(empty_bar(s), 1);
         }
         mbar_init(acc_bar, 1);
@@ -246,12 +243,13 @@ gemm_fp4_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
     } else if constexpr (kQuantize) {
         constexpr int kPer  = 16 / (int)sizeof(X);
         constexpr int kVecs = 32 / kPer;
-        const int     qw = warp - 2, j = lane & 7, quarter = lane >> 3;
-        const int     row   = rows_log2 <= 2 ? quarter & ((1 << rows_log2) - 1) : (qw & (warps_per_kb - 1)) * 4 + quarter;
-        const int     sub   = rows_log2 <= 2 ? quarter >> rows_log2 : 0;
-        const int     round = kbs_per_warp * (4 / warps_per_kb);      // K blocks that the four warps take at a time
-        const X*      src = reinterpret_cast<const X*>(rows) + (size_t)row * ldx;
-        auto load = [&](int kb, Vec16* v) {
+        // eight lanes have 256 values of a row; up to four rows, the quarters beyond them have further K blocks
+        const int qw = warp - 2, j = lane & 7, quarter = lane >> 3;
+        const int row   = deal.rows_log2 <= 2 ? quarter & ((1 << deal.rows_log2) - 1) : (qw & (deal.warps_per_kb - 1)) * 4 + quarter;
+        const int piece = deal.rows_log2 <= 2 ? quarter >> deal.rows_log2 : 0;
+        const X*  src   = reinterpret_cast<const X*>(rows) + (size_t)row * ldx;
+        auto load = [&](int visit, Vec16* v) {
+            const int kb = kb0 + few_rows_block(deal, qw, visit, piece);
 #pragma unroll
             for (int a = 0; a < kVecs; ++a) {
                 v[a] = Vec16{};
@@ -261,38 +259,41 @@ gemm_fp4_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
             }
         };
         Vec16 v[kVecs], ahead[kVecs];
-        int   base = kb0 + qw / warps_per_kb * kbs_per_warp;
-        load(base + sub, v);
+        load(0, v);
         const Fp4Tensor tensor = fp4_tensor<FORMAT>(p.s_x);
-        for (bool ok = true; ok && base < kb1; base += round) {
-            load(base + round + sub, ahead);
-            for (int s = 0; ok && s < kbs_per_warp && base + s < kb1; ++s) {
-                const int i = base + s - kb0;
-                ok = mbar_wait_warp(empty_bar(i % kStages), (uint32_t)(i / kStages & 1) ^ 1u, abort_flag, wait_limit_ns);
-            }
-            if (!ok) {
-                if (lane == 0) {
-                    give_up(0x6400u);
-                }
-                break;
-            }
+        bool            ok     = true;
+        for (int visit = 0; ok && few_rows_block(deal, qw, visit, 0) < kb1 - kb0; ++visit) {
+            load(visit + 1, ahead);
             Vec16          o{};
             const uint32_t code = fp4_encode32<X, FORMAT, true>(v, tensor, o);
-            if (base + sub < kb1 && row < p.M) {
-                uint8_t* x  = gen_base + (base + sub - kb0) % kStages * S::kStage + S::kW;
-                uint8_t* sx = x + S::kX + S::kSw;
-                *reinterpret_cast<Vec16*>(x + row * kRowBytes + ((j ^ (row & 7)) << 4)) = o;    // the 128-byte swizzle
-                if (FORMAT == LYRAQ_NVFP4) {
-                    *reinterpret_cast<uint16_t*>(sx + (j >> 1) * 256 + row * 16 + (j & 1) * 2) = (uint16_t)code;
-                } else {
-                    sx[(j >> 2) * 256 + row * 16 + (j & 3)] = (uint8_t)code;
+            // one K block after the other: each is written once its stage's last contents have been multiplied
+            for (int t = 0; t < deal.per_visit; ++t) {
+                const int i = few_rows_block(deal, qw, visit, t);
+                if (i >= kb1 - kb0) {
+                    break;
                 }
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-                for (int s = 0; s < kbs_per_warp && base + s < kb1; ++s) {
-                    mbar_arrive(full_bar((base + s - kb0) % kStages));
+                const int stage = i % kStages;
+                ok = mbar_wait_warp(empty_bar(stage), (uint32_t)(i / kStages & 1) ^ 1u, abort_flag, wait_limit_ns);
+                if (!ok) {
+                    if (lane == 0) {
+                        give_up(0x6400u | (unsigned)stage);
+                    }
+                    break;
+                }
+                if (piece == t && row < p.M) {
+                    uint8_t* x  = gen_base + stage * S::kStage + S::kW;
+                    uint8_t* sx = x + S::kX + S::kSw;
+                    *reinterpret_cast<Vec16*>(x + row * kRowBytes + ((j ^ (row & 7)) << 4)) = o;    // the 128-byte swizzle
+                    if (FORMAT == LYRAQ_NVFP4) {
+                        *reinterpret_cast<uint16_t*>(sx + (j >> 1) * 256 + row * 16 + (j & 1) * 2) = (uint16_t)code;
+                    } else {
+                        sx[(j >> 2) * 256 + row * 16 + (j & 3)] = (uint8_t)code;
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(full_bar(stage));
                 }
             }
 #pragma unroll
