@@ -415,7 +415,7 @@ LYRAQ_API int lyraq_gate_residual(void* out, const void* y, const void* gate, co
 typedef struct {
     const void *q, *k;                       /* [batch, seq_len, heads, head_dim] by strides */
     size_t q_batch, q_token, q_head, k_batch, k_token, k_head;
-    void *q_out, *k_out;                     /* may be q and k (same strides); not each other, nor the other's input */
+    void *q_out, *k_out;                     /* may be q and k (same strides); else apart from q, k and each other */
     size_t q_out_batch, q_out_token, q_out_head, k_out_batch, k_out_token, k_out_head;
     const void *q_norm, *k_norm;             /* RMS norm weights [head_dim], or NULL: not normalised */
     const void* positions;
@@ -433,7 +433,8 @@ typedef struct {
 /* Rotary embedding over several position axes (time, height, width), from the positions: pair i < pairs of every q and k head turns by
  * positions[b, s, axis[i]] * turns[i] / 2^64 turns, exact for any integer position; elements from 2 * pairs on pass through.  Heads with norm
  * weights are RMS-normalised first.  fp32, rounded once.  A position that is not finite gives NaN.  head_dim even, at most 256; either of q
- * and k may be absent (heads 0).  No alignment is required beyond the element; 16-byte aligned heads are faster.  What the reference does with a table
+ * and k may be absent (heads 0).  An output that shares memory with anything but its own input, or with that in part, is refused
+ * (LYRAQ_ERR_INVALID_ARG).  No alignment is required beyond the element; 16-byte aligned heads are faster.  What the reference does with a table
  * in invokeFusedRmsNormAndRope<T> (src/lyradiff/kernels/rope/flux_apply_rope.h:20-30), for other layouts, head counts and without the table. */
 LYRAQ_API int lyraq_rope_axes(const lyraq_rope_axes_t* args, void* stream);
 

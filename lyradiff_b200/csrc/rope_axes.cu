@@ -12,6 +12,7 @@
 // heads, then a group of L lanes takes a head, every lane VEC pairs (16 bytes of either half, or 32 in a row), two heads of every
 // thread in flight.  A lane's cosines stay in registers while it goes through the heads of a token.
 #include "common.cuh"
+#include "views.h"
 
 namespace lyraq {
 
@@ -303,6 +304,17 @@ static bool even_strides(const void* p, size_t batch, size_t token, size_t head,
     return (reinterpret_cast<uintptr_t>(p) & (2 * vec - 1)) == 0 && ((batch | token | head) & (vec - 1)) == 0;
 }
 
+// A head is written while others are read: an output is its input, element for element, or apart from it, and apart from the rest.
+static bool outputs_clash(const lyraq_rope_axes_t& a)
+{
+    auto view = [&](const void* p, int heads, size_t batch, size_t token, size_t head) {
+        return view_of(p, 2, a.batch, batch, a.seq_len, token, (size_t)heads, head, (size_t)a.head_dim);
+    };
+    const View q = view(a.q, a.q_heads, a.q_batch, a.q_token, a.q_head), qo = view(a.q_out, a.q_heads, a.q_out_batch, a.q_out_token, a.q_out_head);
+    const View k = view(a.k, a.k_heads, a.k_batch, a.k_token, a.k_head), ko = view(a.k_out, a.k_heads, a.k_out_batch, a.k_out_token, a.k_out_head);
+    return (!views_same(q, qo) && views_meet(q, qo)) || (!views_same(k, ko) && views_meet(k, ko)) || views_meet(qo, k) || views_meet(ko, q) || views_meet(qo, ko);
+}
+
 }  // namespace lyraq
 
 using namespace lyraq;
@@ -325,16 +337,15 @@ extern "C" int lyraq_rope_axes(const lyraq_rope_axes_t* a, void* stream)
         (a->pairs > 0 && (a->positions == nullptr || a->turns == nullptr || a->axis == nullptr))) {
         return LYRAQ_ERR_INVALID_ARG;
     }
-    // q's heads are written while k's are read
-    if (a->q_heads > 0 && a->k_heads > 0 && (a->q_out == a->k_out || a->q_out == a->k || a->k_out == a->q)) {
-        return LYRAQ_ERR_INVALID_ARG;
-    }
     const uintptr_t pos_align = a->pos_dtype == LYRAQ_S64 ? 7u : 3u;
     if ((reinterpret_cast<uintptr_t>(a->positions) & pos_align) != 0 || (reinterpret_cast<uintptr_t>(a->turns) & 7u) != 0) {
         return LYRAQ_ERR_INVALID_ARG;
     }
     if (((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->q_out) | reinterpret_cast<uintptr_t>(a->k) |
           reinterpret_cast<uintptr_t>(a->k_out) | reinterpret_cast<uintptr_t>(a->q_norm) | reinterpret_cast<uintptr_t>(a->k_norm)) & 1u) != 0) {
+        return LYRAQ_ERR_INVALID_ARG;
+    }
+    if (outputs_clash(*a)) {
         return LYRAQ_ERR_INVALID_ARG;
     }
     const int sms = device_sm_count();

@@ -340,7 +340,7 @@ def rope_axes(plan, positions, q, k=None, q_norm=None, k_norm=None, eps=1e-6, q_
     """Rotary embedding over several position axes (lyraq_rope_axes).  plan: a rope.AxisRope; q [batch, seq, heads, head_dim] and optionally k
     (its own number of heads), any strides with contiguous heads (views of a packed projection, heads before tokens by transpose);
     positions [batch, seq, axes] or [seq, axes], int32, int64 or fp32, any strides.  q_norm / k_norm [head_dim]: RMS norm weights.  Returns
-    (q_out, k_out), created when omitted; they may be q and k, but neither each other nor the other's input."""
+    (q_out, k_out), created when omitted; they may be q and k, but share memory with nothing else, not even with a part of them."""
     return _lib.host().rope_axes(plan.turns, plan.axis, plan.pairs, plan.axes, plan.interleaved, positions, q, k, q_norm, k_norm, eps, q_out, k_out)
 
 

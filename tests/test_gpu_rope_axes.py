@@ -199,3 +199,30 @@ def test_empty_calls(ops, rope):
     out, _ = ops.rope_axes(plan, torch.zeros(1, 0, 1, dtype=torch.int32, device="cuda"), q)
     assert out.shape == q.shape
     check_status()
+
+
+def test_outputs_that_share_memory_with_what_is_read_are_refused(ops, rope):
+    """Views one head or one token on, the other part of a packed projection, other strides at the same place; parts that nobody reads are taken."""
+    from lyradiff_b200._lib import LyraqError
+    g = torch.Generator().manual_seed(6)
+    plan = rope.AxisRope((64,))
+    pos = torch.arange(9, device="cuda").reshape(9, 1)
+    buf = torch.randn(2 * 10 * 4 * 4 * 64, generator=g).bfloat16().cuda()
+    qkv = buf[:2 * 9 * 4 * 4 * 64].view(2, 9, 4, 4, 64)        # q, k, v and a place
+    q, k, v, place = qkv.unbind(2)
+    want = ops.rope_axes(plan, pos, q.contiguous(), k.contiguous())
+    before = buf.clone()
+    by_head = qkv.view(-1)[:2 * 4 * 9 * 64].view(2, 4, 9, 64).transpose(1, 2)
+    moved = lambda n: buf.as_strided(q.shape, q.stride(), n)   # noqa: E731
+    for kw in ({"q_out": moved(64)}, {"q_out": moved(16 * 64)}, {"q_out": k}, {"k_out": q}, {"k_out": moved(5 * 64)}, {"q_out": by_head}, {"q_out": v, "k_out": v},
+               {"q_out": v, "k_out": moved(9 * 64)}):
+        with pytest.raises(LyraqError):
+            ops.rope_axes(plan, pos, q, k, **kw)
+    torch.cuda.synchronize()
+    assert torch.equal(buf, before)
+    got = ops.rope_axes(plan, pos, q, k, q_out=place, k_out=v)
+    check_status()
+    assert torch.equal(got[0], want[0]) and torch.equal(v, want[1]) and torch.equal(qkv[:, :, :2], before[:qkv.numel()].view_as(qkv)[:, :, :2])
+    ops.rope_axes(plan, pos, q, q_out=q)
+    ops.rope_axes(plan, pos, k, q_out=k)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
