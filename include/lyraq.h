@@ -465,8 +465,9 @@ typedef struct {
 /* Norms before and after a block with its gate and residual in one pass:
  *   u = post(y) * post_weight;  v = residual_scale * x + gate_b * u;  x_out = T(v);  h = T( pre(v) * pre_weight * (1 + scale_b) + shift_b )
  * RMS: v / sqrt(mean(v^2) + eps); LAYER: the mean subtracted first.  fp32 throughout, each output rounded once; pre sees v before its rounding.
- * qf8 and q4 hold the codes that lyraq_quant_fp8 and lyraq_quant_fp4 make of T(h).  x_out and h may each be x or y (same strides), but not the same.  dim a
- * multiple of 8 (32 with q4), at most 16384; pointers 16-byte aligned (qf8: 8).  The fused form of what the reference runs as
+ * qf8 and q4 hold the codes that lyraq_quant_fp8 and lyraq_quant_fp4 make of T(h).  x_out and h may each be x or y (same strides); else
+ * every output is apart from x, y and the other outputs, or the call is refused (LYRAQ_ERR_INVALID_ARG).  dim a multiple of 8 (32 with q4), at
+ * most 16384; pointers 16-byte aligned (qf8: 8).  The fused form of what the reference runs as
  * invokeFusedGateAndResidual (src/lyradiff/kernels/flux_single_transformer_block/flux_single_transformer_kernels.cu:43-65) and
  * invokeLayerNormWithShiftAndScale (src/lyradiff/kernels/norms/layer_norm.h:19); the norm after a block has no counterpart there. */
 LYRAQ_API int lyraq_gated_residual_norm(const lyraq_gated_norm_t* args, void* stream);

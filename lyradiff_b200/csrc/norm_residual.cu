@@ -13,6 +13,7 @@
 // mean (a difference of sums of squares would lose what a large mean covers).  The five parameter vectors are shared by a batch entry's rows and
 // come from L1.
 #include "fp4.cuh"
+#include "views.h"
 
 namespace lyraq {
 
@@ -294,6 +295,30 @@ static NormSplit norm_split(size_t rows, int dim, int sms)
     return NormSplit{vpt, ((nvec + vpt - 1) / vpt + 31) / 32 * 32, false};
 }
 
+// Rows are written while others are read: x_out and h are x or y, element for element, or apart from them; all outputs are apart from each other, the
+// quantized ones from x and y too.
+static bool outputs_clash(const lyraq_gated_norm_t& a)
+{
+    auto rows = [&](const void* p, size_t batch, size_t row) { return view_of(p, 2, a.batch, batch, a.seq_len, row, 1, 0, a.dim); };
+    const size_t n = a.batch * a.seq_len;
+    const View   in[2]  = {rows(a.y, a.y_batch, a.y_row), rows(a.x, a.x_batch, a.x_row)};
+    const View   out[5] = {rows(a.x_out, a.x_out_batch, a.x_out_row), rows(a.h, a.h_batch, a.h_row), view_of(a.qf8, n * a.dim), view_of(a.q4, n * a.dim / 2),
+                           view_of(a.q4 != nullptr ? a.q4_scales : nullptr, lyraq_fp4_scale_bytes(n, a.dim, a.q4_format))};
+    for (int i = 0; i < 5; ++i) {
+        for (const View& v : in) {
+            if (!(i < 2 && views_same(out[i], v)) && views_meet(out[i], v)) {
+                return true;
+            }
+        }
+        for (int j = 0; j < i; ++j) {
+            if (views_meet(out[i], out[j])) {
+                return true;
+            }
+        }
+    }
+    return false;
+}
+
 static bool rows_ok(const void* p, size_t batch, size_t row) { return aligned16(p) && (batch & 7u) == 0 && (row & 7u) == 0; }
 
 }  // namespace lyraq
@@ -331,7 +356,7 @@ extern "C" int lyraq_gated_residual_norm(const lyraq_gated_norm_t* a, void* stre
             return LYRAQ_ERR_UNSUPPORTED;
         }
     }
-    if (a->x_out != nullptr && a->x_out == a->h) {
+    if (outputs_clash(*a)) {
         return LYRAQ_ERR_INVALID_ARG;
     }
     const int sms = device_sm_count();

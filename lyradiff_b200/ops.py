@@ -353,7 +353,8 @@ def gated_residual_norm(y, x, gate=None, scale=None, shift=None, post_weight=Non
         v = residual_scale * x + gate[b] * (post(y) * post_weight);  x_out = v;  h = pre(v) * pre_weight * (1 + scale[b]) + shift[b]
     Returns (x_out, h).  gate, scale, shift: [batch, dim] (rows may lie apart, as chunks of one modulation tensor do) or [dim]; post: "none",
     "rms" or "layer", pre: "rms" or "layer".  x_out is created when omitted, h when no other form of it is asked for.  qf8 (uint8, contiguous,
-    with f8_scale) takes e4m3 codes of h, q4 (an Fp4Tensor of [batch * seq, dim]) its FP4 form.  x_out and h may each be x or y, but not the same tensor."""
+    with f8_scale) takes e4m3 codes of h, q4 (an Fp4Tensor of [batch * seq, dim]) its FP4 form.  x_out and h may each be x or y; otherwise no
+    output shares memory with them or with another output."""
     if post not in _NORMS or pre not in _NORMS or pre == "none":
         raise ValueError("unknown norm %r / %r" % (post, pre))
     if q4 is None:

@@ -200,3 +200,33 @@ def test_outputs_in_the_inputs_places(ops, dim):
         ops.gated_residual_norm(post="layer", pre="rms", x_out=own[first], h=own[second], **own)
         check_status()
         assert torch.equal(own[first], want[0]) and torch.equal(own[second], want[1])
+
+
+def test_outputs_that_share_memory_with_what_is_read_are_refused(ops):
+    """A row on, other strides at the same place, on another output, the quantized outputs on x; rows of a joint sequence that nobody reads are taken."""
+    from lyradiff_b200._lib import LyraqError
+    g = torch.Generator().manual_seed(9)
+    joint_y, joint_x = (torch.randn(2, 16, 640, generator=g).bfloat16().cuda() for _ in range(2))
+    y, x, below = joint_y[:, :7], joint_x[:, :7], joint_x[:, 8:15]
+    want = ops.gated_residual_norm(y.contiguous(), x.contiguous(), pre="layer")
+    before = joint_y.clone(), joint_x.clone()
+    dense = joint_x.flatten()[:14 * 640].view(2, 7, 640)                 # x's first row, other rows
+    fresh = torch.empty(2, 7, 640, dtype=torch.bfloat16, device="cuda")
+    s8, bytes_of_x = torch.ones(1, device="cuda"), joint_x.view(-1).view(torch.uint8)[:14 * 640].view(2, 7, 640)
+    q4 = ops.Fp4Tensor.empty(14, 640)
+    on_x = ops.Fp4Tensor(14, 640, "nvfp4", joint_x.view(-1).view(torch.uint8)[:14 * 320].view(14, 320), q4.scales)
+    scales_on_y = ops.Fp4Tensor(14, 640, "nvfp4", q4.codes, joint_y.view(-1).view(torch.uint8)[:q4.scales.numel()])
+    for kw in ({"x_out": joint_x[:, 1:8]}, {"h": joint_y[:, 1:8]}, {"x_out": dense}, {"x_out": fresh, "h": fresh}, {"x_out": below, "h": joint_x[:, 9:16]},
+               {"qf8": bytes_of_x, "f8_scale": s8}, {"q4": on_x}, {"q4": scales_on_y}):
+        with pytest.raises(LyraqError):
+            ops.gated_residual_norm(y, x, pre="layer", **kw)
+    torch.cuda.synchronize()
+    assert torch.equal(joint_y, before[0]) and torch.equal(joint_x, before[1])
+    got = ops.gated_residual_norm(y, x, pre="layer", x_out=below, h=joint_y[:, 8:15])
+    check_status()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(joint_y[:, :8], before[0][:, :8]) and torch.equal(joint_x[:, :8], before[1][:, :8])
+    # one stream with itself, the result in its place
+    twice = ops.gated_residual_norm(x.contiguous(), x.contiguous(), pre="layer")
+    own = x.contiguous().clone()
+    again = ops.gated_residual_norm(own, own, pre="layer", x_out=own)
+    assert torch.equal(own, twice[0]) and torch.equal(again[1], twice[1])

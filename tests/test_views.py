@@ -124,3 +124,37 @@ def test_rotary_embedding_refuses_outputs_on_what_it_reads():
     assert turn(q_out=p, batch=1, q_out_batch=7) == CUDA and turn(q_out=p, seq_len=1, q_out_token=7) == CUDA
     # without k its place is free
     assert turn(k=None, k_out=None, k_heads=0, q_out=p + 2 * H * D) == CUDA
+
+
+@needs_no_gpu
+def test_norms_refuse_outputs_on_what_they_read():
+    lib = _lib.lib()
+    B, S, D = 2, 5, 64
+    p, far = 1 << 30, [p << 20 for p in range(1, 9)]
+    joint = dict(zip(("batch", "row"), (8 * D, D)))       # 5 of 8 rows
+
+    def norm(**kw):
+        a = dict(y=p + far[0], x=p, x_out=p + far[1], h=p + far[2], batch=B, seq_len=S, dim=D, dtype=1, post=1, pre=2, residual_scale=1.0, eps=1e-6)
+        for t in ("y", "x", "x_out", "h"):
+            a.update({t + "_" + n: v for n, v in joint.items()})
+        return lib.lyraq_gated_residual_norm(ctypes.byref(_lib.GatedNormArgs(**{**a, **kw})), None)
+    assert norm() == CUDA
+    # either output in either input's place, and on rows that nobody reads
+    assert norm(x_out=p, h=p + far[0]) == CUDA and norm(x_out=p + far[0], h=p) == CUDA and norm(y=p, x_out=p) == CUDA
+    assert norm(x_out=p, h=p + 2 * 5 * D, seq_len=3) == CUDA
+    # a row on, within a row, with other strides, on each other, the two inputs a row apart
+    assert norm(x_out=p + 2 * D) == INVALID and norm(h=p + 2 * D) == INVALID and norm(x_out=p + far[0] - 16) == INVALID and norm(x_out=p, x_out_batch=5 * D) == INVALID
+    assert norm(x_out=p + far[2]) == INVALID and norm(x_out=p + far[2] + 2 * D) == INVALID and norm(y=p + 2 * D, x_out=p) == INVALID
+    assert norm(x_out=p, batch=1, x_out_batch=5 * D) == CUDA
+    # the quantized outputs: apart from everything
+    q = dict(f8_scale=p + far[7], q4_format=0)
+    for name, size in (("qf8", B * S * D), ("q4", B * S * D // 2)):
+        more = dict(q, q4_scales=p + far[6]) if name == "q4" else q
+        assert norm(**{name: p + far[3]}, **more) == CUDA
+        for at in (p, p + 2 * D, p + far[0], p + far[1], p + far[2], p + far[2] - size + 16):
+            assert norm(**{name: at}, **more) == INVALID
+        assert norm(**{name: p + far[0] - size}, **more) == CUDA
+    both = dict(q, qf8=p + far[3], q4=p + far[4], q4_scales=p + far[5])
+    assert norm(**both) == CUDA
+    for name, at in (("qf8", far[4]), ("q4", far[3]), ("q4_scales", far[3]), ("q4_scales", far[4]), ("q4_scales", 0), ("q4_scales", far[1])):
+        assert norm(**{**both, name: p + at}) == INVALID
