@@ -353,8 +353,8 @@ LYRAQ_API int lyraq_gemm_w4a4(const uint8_t* A, const uint8_t* B, const float* s
 
 /* Microscaled FP4: Y[m,n] = T( epi( g_x g_w * sum_k X[m,k] W[n,k] + beta * R[m,n] + bias[n] ) ), X and W codes with block scales as
  * lyraq_quant_fp4 lays them out, both of the same `format`, g_x and g_w fp32 [1] or NULL (= 1), exact products, fp32 accumulation, epi =
- * identity or tanh-GELU, T = c_dtype (F16, BF16, F32), bias and R of c_dtype or NULL; Y may alias R.  k a multiple of 32; all pointers
- * 16-byte aligned.  The FP4 form of lyraq_gemm_fp8; no counterpart in the reference. */
+ * identity or tanh-GELU, T = c_dtype (F16, BF16, F32), bias and R of c_dtype or NULL.  Y may be R; else it is apart from R and the other
+ * operands, or the call is refused (LYRAQ_ERR_INVALID_ARG).  k a multiple of 32; all pointers 16-byte aligned.  The FP4 form of lyraq_gemm_fp8; no counterpart in the reference. */
 LYRAQ_API int lyraq_gemm_fp4(const uint8_t* X, const uint8_t* x_scale, const float* x_tensor_scale, const uint8_t* W, const uint8_t* w_scale,
                              const float* w_tensor_scale, int format, void* Y, int c_dtype, const void* bias, const void* residual,
                              float beta, int epilogue, int m, int n, int k, void* stream);
@@ -491,7 +491,8 @@ LYRAQ_API int lyraq_linear_fp8_forward(void* Y, const void* x, int dtype, const 
                                        int m, int n, int k, void* workspace, size_t workspace_bytes, void* stream);
 
 /* FP4 linear: x [m, k] (row pitch ldx elements) -> FP4 with the tensor scale x_tensor_scale[0], then lyraq_gemm_fp4.  The workspace of
- * LYRAQ_OP_LINEAR_FP4 suffices for either format (calls of few rows ask for it too, and use it only where Y overlaps x).  The FP4 form of lyraq_linear_fp8_forward; no counterpart in the reference. */
+ * LYRAQ_OP_LINEAR_FP4 suffices for either format (calls of few rows ask for it too, and use it only where Y overlaps x).  Y may be R, and may lie on
+ * x; it and the workspace are apart from all else.  The FP4 form of lyraq_linear_fp8_forward; no counterpart in the reference. */
 LYRAQ_API int lyraq_linear_fp4_forward(void* Y, const void* x, int dtype, size_t ldx, const float* x_tensor_scale, const uint8_t* W,
                                        const uint8_t* w_scale, const float* w_tensor_scale, int format, const void* bias,
                                        const void* residual, float beta, int epilogue, int m, int n, int k, void* workspace,

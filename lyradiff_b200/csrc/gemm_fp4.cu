@@ -765,6 +765,12 @@ int lyraq_gemm_fp4(const uint8_t* X, const uint8_t* x_scale, const float* x_tens
         (residual != nullptr && !aligned16(residual))) {
         return LYRAQ_ERR_INVALID_ARG;
     }
+    const size_t rows = (size_t)m, cols = (size_t)n, depth = (size_t)k, bytes = c_dtype == LYRAQ_F32 ? 4 : 2;
+    if (fp4::result_clashes(view_of(Y, rows * cols * bytes), residual,
+                            {view_of(X, rows * depth / 2), view_of(x_scale, lyraq_fp4_scale_bytes(rows, depth, format)), view_of(W, cols * depth / 2),
+                             view_of(w_scale, lyraq_fp4_scale_bytes(cols, depth, format)), view_of(bias, cols * bytes)})) {
+        return LYRAQ_ERR_INVALID_ARG;
+    }
     return fp4::product({X, x_scale, nullptr, 0, 0}, x_tensor_scale, W, w_scale, w_tensor_scale, format, Y, c_dtype, bias, residual, beta, epilogue, m, n, k,
                         (cudaStream_t)stream);
 }

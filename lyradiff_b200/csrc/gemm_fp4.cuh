@@ -3,6 +3,9 @@
 
 #include "fp4.cuh"
 #include "sm100_ptx.cuh"
+#include "views.h"
+
+#include <initializer_list>
 
 namespace lyraq {
 
@@ -37,6 +40,16 @@ int  launch_skinny(const Fp4Input& X, const uint8_t* W, const uint8_t* ws, int f
 bool skinny_quantize_pays(int m, int n, int k, int sms);
 bool few_rows(int m, int k);                  // whether a product takes the few-row kernel,
 bool few_rows_quantize(int m, int n, int k);  // and whether a linear leaves the quantize to it
+// Whether a result lies on something that is still read while it is stored.  It may be the residual, element for element.
+inline bool result_clashes(const View& y, const void* residual, std::initializer_list<View> read)
+{
+    for (const View& v : read) {
+        if (views_meet(y, v)) {
+            return true;
+        }
+    }
+    return reinterpret_cast<uintptr_t>(residual) != y.base && views_meet(y, view_of(residual, y.count[3]));
+}
 // lyraq_gemm_fp4 behind its checks; rows that are not FP4 yet only where few_rows
 int product(const Fp4Input& X, const float* g_x, const uint8_t* W, const uint8_t* ws, const float* g_w, int format, void* Y, int c_dtype, const void* bias,
             const void* residual, float beta, int epilogue, int m, int n, int k, cudaStream_t stream);

@@ -104,15 +104,21 @@ int lyraq_linear_fp4_forward(void* Y, const void* x, int dtype, size_t ldx, cons
         (epilogue != LYRAQ_EPI_NONE && epilogue != LYRAQ_EPI_GELU_TANH)) {
         return LYRAQ_ERR_INVALID_ARG;
     }
+    const size_t bytes = dtype == LYRAQ_F32 ? 4 : 2, rows = (size_t)m, cols = (size_t)n, depth = (size_t)k;
+    const View   y     = view_of(Y, rows * cols * bytes);
+    const View   w = view_of(W, cols * depth / 2), ws = view_of(w_scale, lyraq_fp4_scale_bytes(cols, depth, format)), b = view_of(bias, cols * bytes);
+    const View   work = view_of(workspace, linear_workspace_bytes(LYRAQ_OP_LINEAR_FP4, rows, depth));
+    // the workspace is written before anything but x is read
+    if (fp4::result_clashes(y, residual, {w, ws, b, work}) ||
+        fp4::result_clashes(work, nullptr, {w, ws, b, view_of(residual, rows * cols * bytes), view_of(x, bytes, rows, ldx, 1, 0, 1, 0, depth)})) {
+        return LYRAQ_ERR_INVALID_ARG;
+    }
     uint8_t* qx = static_cast<uint8_t*>(workspace);
     uint8_t* sx = qx + align_up((size_t)m * (size_t)k / 2, 256);
     const float* g = format == LYRAQ_NVFP4 ? x_tensor_scale : nullptr;
     int          st;
     // One launch, which quantizes the rows on their way.  Every CTA reads all rows, so a result in their place needs them quantized before.
-    const size_t   bytes = dtype == LYRAQ_F32 ? 4 : 2;
-    const uint8_t *x0 = static_cast<const uint8_t*>(x), *y0 = static_cast<const uint8_t*>(Y);
-    const bool     apart = y0 + (size_t)m * (size_t)n * bytes <= x0 || x0 + ((size_t)(m - 1) * ldx + (size_t)k) * bytes <= y0;
-    if (apart && fp4::few_rows_quantize(m, n, k)) {
+    if (!views_meet(y, view_of(x, ((rows - 1) * ldx + depth) * bytes)) && fp4::few_rows_quantize(m, n, k)) {
         st = check_fp4(qx, sx, x, dtype, ldx, format, (size_t)m, (size_t)k);
         return st != LYRAQ_OK ? st
                               : fp4::product({nullptr, nullptr, x, dtype, ldx}, g, W, w_scale, w_tensor_scale, format, Y, dtype, bias, residual, beta, epilogue,

@@ -98,3 +98,23 @@ def test_a_captured_chain_of_one_and_two_rows(layers, m):
         torch.cuda.synchronize()
         check_status()
         assert torch.equal(out, want) and bool(torch.isfinite(out).all())
+
+
+@pytest.mark.parametrize("m", [2, 100])
+def test_a_result_on_the_weight_or_partly_on_the_residual_is_refused(layers, m):
+    from lyradiff_b200._lib import LyraqError
+    g = torch.Generator(device="cuda").manual_seed(4)
+    layer = layers.Fp4Linear((torch.randn(512, 512, generator=g, device="cuda") * 0.05).bfloat16(), None, torch.tensor(2.0 ** -7))
+    x = torch.randn(m, 512, generator=g, device="cuda").bfloat16()
+    both = torch.randn((m + 1) * 512, generator=g, device="cuda").bfloat16()
+    r, moved, before = both[:m * 512].view(m, 512), both[512:].view(m, 512), both.clone()
+    want = layer.forward(x, residual=r.clone())
+    with pytest.raises(LyraqError):
+        layer.forward(x, residual=r, out=moved)
+    with pytest.raises(LyraqError):
+        layer.forward(x, out=layer.weight.codes.view(-1).view(torch.bfloat16)[:m * 512].view(m, 512))
+    torch.cuda.synchronize()
+    assert torch.equal(both, before)
+    layer.forward(x, residual=r, out=r)
+    check_status()
+    assert torch.equal(r, want)

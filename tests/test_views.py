@@ -158,3 +158,29 @@ def test_norms_refuse_outputs_on_what_they_read():
     assert norm(**both) == CUDA
     for name, at in (("qf8", far[4]), ("q4", far[3]), ("q4_scales", far[3]), ("q4_scales", far[4]), ("q4_scales", 0), ("q4_scales", far[1])):
         assert norm(**{**both, name: p + at}) == INVALID
+
+
+@needs_no_gpu
+def test_fp4_products_refuse_a_result_on_what_they_read():
+    lib = _lib.lib()
+    m, n, k = 300, 256, 512
+    p = [(i + 1) << 30 for i in range(9)]
+    size = {"X": m * k // 2, "xs": lib.lyraq_fp4_scale_bytes(m, k, 0), "W": n * k // 2, "ws": lib.lyraq_fp4_scale_bytes(n, k, 0), "bias": 2 * n, "R": 2 * m * n}
+
+    def gemm(Y=p[0], X=p[1], xs=p[2], W=p[3], ws=p[4], bias=p[5], R=p[6]):
+        return lib.lyraq_gemm_fp4(X, xs, None, W, ws, None, 0, Y, 1, bias, R, 1.0, 0, m, n, k, None)
+
+    need = lib.lyraq_workspace_bytes(8, m, n, k)
+
+    def linear(Y=p[0], x=p[1], W=p[3], ws=p[4], bias=p[5], R=p[6], work=p[7]):
+        return lib.lyraq_linear_fp4_forward(Y, x, 1, k, None, W, ws, None, 0, bias, R, 1.0, 0, m, n, k, work, need, None)
+    assert gemm() == CUDA and linear() == CUDA and gemm(R=p[0]) == CUDA and linear(R=p[0]) == CUDA and gemm(bias=None, R=None) == CUDA
+    assert linear(x=p[0]) == CUDA and linear(x=p[0] + 2 * n) == CUDA           # the rows are quantized before
+    for call in (gemm, linear):
+        for name in ("X", "xs", "W", "ws", "bias", "R"):
+            if call is linear and name in ("X", "xs"):
+                continue
+            for at in (p[0] - size[name] + 16, p[0] + 16, p[0] + 2 * m * n - 16):
+                assert call(**{name: at}) == INVALID, (call, name)
+            assert call(**{name: p[0] - (size[name] + 15) // 16 * 16}) == CUDA and call(**{name: p[0] + 2 * m * n}) == CUDA
+    assert linear(work=p[0] - 16) == INVALID and linear(work=p[6] + 32) == INVALID and linear(work=p[1] - need + 16) == INVALID
