@@ -757,7 +757,7 @@ int lyraq_gemm_fp4(const uint8_t* X, const uint8_t* x_scale, const float* x_tens
     if (m == 0 || n == 0) {
         return LYRAQ_OK;
     }
-    if (k == 0 || (k & 31) != 0 || m > 0x7fffff00 || n > 0x7fffff00 || k > 0x7fffff00) {   // row and column numbers of a last tile stay within 31 bits
+    if (k == 0 || (k & 31) != 0 || m > fp4::kMaxSize || n > fp4::kMaxSize || k > fp4::kMaxSize) {
         return LYRAQ_ERR_UNSUPPORTED;
     }
     if (X == nullptr || x_scale == nullptr || W == nullptr || w_scale == nullptr || Y == nullptr || !aligned16(X) || !aligned16(x_scale) ||

@@ -26,6 +26,7 @@ struct Fp4GemmParams {
 
 namespace fp4 {
 constexpr int kFp4SkinnyRows = 16;   // most rows of X that gemm_fp4_skinny.cu takes
+constexpr int kMaxSize       = 0x7fffff00;   // of m, n and k: row, column and block numbers of a last tile stay within 31 bits
 
 // The left operand: FP4 codes with their block scales, or (codes null) rows of a 16- or 32-bit type that the few-row kernel quantizes itself.
 struct Fp4Input {

@@ -92,7 +92,7 @@ int lyraq_linear_fp4_forward(void* Y, const void* x, int dtype, size_t ldx, cons
     if (m == 0 || n == 0) {
         return LYRAQ_OK;
     }
-    if (k == 0 || (k & 31) != 0) {
+    if (k == 0 || (k & 31) != 0 || m > fp4::kMaxSize || n > fp4::kMaxSize || k > fp4::kMaxSize) {
         return LYRAQ_ERR_UNSUPPORTED;
     }
     if (workspace == nullptr || workspace_bytes < linear_workspace_bytes(LYRAQ_OP_LINEAR_FP4, (size_t)m, (size_t)k) || !aligned16(workspace)) {

@@ -101,3 +101,12 @@ def test_python_side_refuses_parts_that_do_not_fit(lib):
             bad.check()
     with pytest.raises(ValueError):
         ops.Fp4Tensor.empty(4, 64, "int4", device="cpu")
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="addresses that nothing lies at")
+def test_sizes_next_to_31_bits_are_refused_by_linear_and_product_alike(lib):
+    UNSUPPORTED, p = 2, [(i + 1) << 44 for i in range(5)]
+    for m, n, k in ((1, 1, 0x7fffffe0), (1, 0x7fffffff, 32), (0x7fffffff, 1, 32)):
+        assert lib.lyraq_gemm_fp4(p[0], p[1], None, p[2], p[3], None, 0, p[4], 1, None, None, 0.0, 0, m, n, k, None) == UNSUPPORTED
+        need = lib.lyraq_workspace_bytes(8, m, n, k)
+        assert lib.lyraq_linear_fp4_forward(p[0], p[1], 1, k, None, p[2], p[3], None, 0, None, None, 0.0, 0, m, n, k, p[4], need, None) == UNSUPPORTED
