@@ -8,6 +8,7 @@ import os
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -83,21 +84,41 @@ def _current(lib, src):
     return os.path.exists(lib) and all(os.path.getmtime(d) <= os.path.getmtime(lib) for d in deps)
 
 
+def _compile(src, lib, args, force):
+    if (force or not _current(lib, src)) and subprocess.Popen(_torch_command(src, lib) + args).wait():
+        raise RuntimeError("g++ failed for %s" % lib)
+    return lib
+
+
+def _compile_classes(force):
+    return _compile(CLASSES_SRC, CLASSES_LIB, ["-L" + HERE, "-llyraq", "-Wl,-rpath,$ORIGIN"], force)
+
+
+def _compile_host(force):
+    return _compile(HOST_SRC, HOST_LIB, ["-I" + sysconfig.get_paths()["include"], "-ltorch_python"], force)
+
+
 def build_classes(force=False):
     """Compile csrc/torch_classes.cpp (no device code) against torch's headers and link it to liblyraq.so, found at load time
-    beside it ($ORIGIN), and csrc/host_calls.cpp, the extension module behind some of ops.py, which is given liblyraq.so's functions at run
-    time.  Returns the path of the first."""
+    beside it ($ORIGIN).  Returns the library path."""
     build(force=force)
-    procs = []
-    if force or not _current(HOST_LIB, HOST_SRC):
-        procs.append(subprocess.Popen(_torch_command(HOST_SRC, HOST_LIB) + ["-I" + sysconfig.get_paths()["include"], "-ltorch_python"]))
-    if force or not _current(CLASSES_LIB, CLASSES_SRC):
-        procs.append(subprocess.Popen(_torch_command(CLASSES_SRC, CLASSES_LIB) + ["-L" + HERE, "-llyraq", "-Wl,-rpath,$ORIGIN"]))
-    if any([p.wait() for p in procs]):
-        raise RuntimeError("g++ failed")
-    return CLASSES_LIB
+    return _compile_classes(force)
+
+
+def build_host(force=False):
+    """Compile csrc/host_calls.cpp, the extension module behind some of ops.py, against torch's and this interpreter's headers; it is given
+    liblyraq.so's functions at run time.  Returns the module's path."""
+    build(force=force)
+    return _compile_host(force)
+
+
+def build_all(force=False, verbose=False):
+    """All three; the host code's two compile at the same time, and one that fails does not keep the other from being built."""
+    first = build(force=force, verbose=verbose)
+    with ThreadPoolExecutor(2) as pool:
+        jobs = [pool.submit(f, force) for f in (_compile_classes, _compile_host)]
+    return [first] + [j.result() for j in jobs]
 
 
 if __name__ == "__main__":
-    print(build(force="--force" in sys.argv, verbose="--verbose" in sys.argv))
-    print(build_classes(force="--force" in sys.argv))
+    print("\n".join(build_all(force="--force" in sys.argv, verbose="--verbose" in sys.argv)))
