@@ -3,6 +3,7 @@ missing or lacks a symbol the import of the ops fails with a clear error."""
 
 import ctypes
 import os
+import sysconfig
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("LYRAQ_LIB_PATH", os.path.join(_HERE, "liblyraq.so"))
@@ -144,10 +145,10 @@ def lib():
 
 
 def host():
-    """The extension module _host.so (csrc/host_calls.cpp), bound to the loaded library's functions."""
+    """The extension module _host (csrc/host_calls.cpp), bound to the loaded library's functions."""
     global _host
     if _host is None:
-        path = os.path.join(_HERE, "_host.so")
+        path = os.path.join(_HERE, "_host" + sysconfig.get_config_var("EXT_SUFFIX"))    # this interpreter's: another's would crash it
         if not os.path.exists(path):
             raise ImportError("%s is not built: run `python -m lyradiff_b200.build` (there is no fallback)" % path)
         import torch  # noqa: F401  (its libraries are what the module links to)

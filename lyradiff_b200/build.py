@@ -1,5 +1,5 @@
 """Builds liblyraq.so (the C-ABI CUDA library) in-tree with nvcc for sm_100a, and liblyradiff_classes.so (host C++ that
-registers the torch custom classes over that C ABI) and _host.so (the extension module behind some of ops.py) with g++.
+registers the torch custom classes over that C ABI) and _host.<interpreter>.so (the extension module behind some of ops.py) with g++.
 
 Usage: python -m lyradiff_b200.build [--force] [--verbose]
 """
@@ -15,7 +15,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "liblyraq.so")
 CLASSES_LIB = os.path.join(HERE, "liblyradiff_classes.so")
 CLASSES_SRC = os.path.join(CSRC, "torch_classes.cpp")
-HOST_LIB = os.path.join(HERE, "_host.so")
+HOST_LIB = os.path.join(HERE, "_host" + sysconfig.get_config_var("EXT_SUFFIX"))
 HOST_SRC = os.path.join(CSRC, "host_calls.cpp")
 
 SOURCES = ["api.cu", "quant_kernels.cu", "gemm_dense.cu", "gemm_skinny.cu", "gemm_w4a4.cu", "gemm_w4a4_wide.cu", "fp4_quant.cu", "gemm_fp4.cu", "gemm_fp4_skinny.cu", "norm_residual.cu", "rope_axes.cu", "lora_down.cu", "block_kernels.cu", "attention.cu", "linear_layers.cu", "noalloc.cu"]
@@ -107,7 +107,7 @@ def build_classes(force=False):
 
 def build_host(force=False):
     """Compile csrc/host_calls.cpp, the extension module behind some of ops.py, against torch's and this interpreter's headers; it is given
-    liblyraq.so's functions at run time.  Returns the module's path."""
+    liblyraq.so's functions at run time.  Returns the module's path, whose name carries the interpreter's tag."""
     build(force=force)
     return _compile_host(force)
 

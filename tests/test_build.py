@@ -1,8 +1,11 @@
-"""CPU tests of what is built for whom (lyradiff_b200/build.py)."""
+"""CPU tests of what is built for whom (lyradiff_b200/build.py) and of the loader of the extension module."""
+
+import os
+import sysconfig
 
 import pytest
 
-from lyradiff_b200 import build
+from lyradiff_b200 import _lib, build
 
 
 def test_the_classes_build_where_the_extension_module_cannot(monkeypatch, tmp_path):
@@ -27,3 +30,16 @@ def test_the_classes_build_where_the_extension_module_cannot(monkeypatch, tmp_pa
     with pytest.raises(RuntimeError, match="host.so"):
         build.build_all()
     assert sorted(started) == sorted([build.CLASSES_LIB, build.HOST_LIB])
+
+
+def test_the_extension_module_is_this_interpreters(monkeypatch, tmp_path):
+    """Its name carries the interpreter's tag, so that no other loads it; a file without one is not taken for it."""
+    build.build_host()
+    suffix = sysconfig.get_config_var("EXT_SUFFIX")
+    assert os.path.basename(build.HOST_LIB) == "_host" + suffix != "_host.so"
+    assert _lib.host().__file__ == build.HOST_LIB
+    (tmp_path / "_host.so").write_bytes(b"")
+    monkeypatch.setattr(_lib, "_host", None)
+    monkeypatch.setattr(_lib, "_HERE", str(tmp_path))
+    with pytest.raises(ImportError, match="not built"):
+        _lib.host()
