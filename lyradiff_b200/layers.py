@@ -49,6 +49,15 @@ class Fp8Linear:
         return y.reshape(*x.shape[:-1], self.n)
 
 
+def _power_of_two(scale):
+    """The least power of two that is not below `scale`, fp32 [1]; at least 2^-126, as a weight's tensor scale."""
+    s = scale.detach().reshape(1).double()
+    if not bool((s > 0).all() & (s <= 2.0 ** 127).all()):
+        raise ValueError("input_scale must be positive and at most 2^127")
+    m, e = torch.frexp(s)
+    return torch.ldexp(torch.ones_like(s), torch.where(m == 0.5, e - 1, e).clamp_min(-126)).float()
+
+
 class Fp4Linear:
     """Linear in microscaled FP4 (nvfp4 or mxfp4) on the tensor cores' 4-bit path: weight quantized on load, activations by the forward,
     bias / GELU-tanh / residual fused into the GEMM epilogue.  input_scale (nvfp4): the static tensor scale of the activations, the largest
@@ -66,11 +75,7 @@ class Fp4Linear:
         if input_scale is None or fmt != "nvfp4":
             self.input_scale = None
         else:
-            s = input_scale.detach().reshape(1).double()
-            m, e = torch.frexp(s)
-            if not bool((torch.isfinite(s) & (s > 0)).all()):
-                raise ValueError("input_scale must be positive and finite")
-            self.input_scale = torch.ldexp(torch.ones_like(s), torch.where(m == 0.5, e - 1, e)).to(device=dev, dtype=torch.float32)
+            self.input_scale = _power_of_two(input_scale).to(dev)
 
     def forward(self, x, residual=None, beta=1.0, out=None):
         w = self.weight

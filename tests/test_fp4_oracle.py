@@ -110,3 +110,14 @@ def test_sizes_next_to_31_bits_are_refused_by_linear_and_product_alike(lib):
         assert lib.lyraq_gemm_fp4(p[0], p[1], None, p[2], p[3], None, 0, p[4], 1, None, None, 0.0, 0, m, n, k, None) == UNSUPPORTED
         need = lib.lyraq_workspace_bytes(8, m, n, k)
         assert lib.lyraq_linear_fp4_forward(p[0], p[1], 1, k, None, p[2], p[3], None, 0, None, None, 0.0, 0, m, n, k, p[4], need, None) == UNSUPPORTED
+
+
+def test_input_scales_are_rounded_up_to_powers_of_two_of_fp32():
+    from lyradiff_b200 import layers
+    f = layers._power_of_two
+    for s, want in ((1.0, 1.0), (0.011, 2.0 ** -6), (2.0 ** -7, 2.0 ** -7), (1.0000001, 2.0), (2.0 ** 127, 2.0 ** 127), (1e-40, 2.0 ** -126), (1e-300, 2.0 ** -126)):
+        got = f(torch.tensor(s, dtype=torch.float64))
+        assert got.dtype == torch.float32 and got.shape == (1,) and float(got) == want
+    for s in (0.0, -1.0, float("nan"), float("inf"), 3e38, 1e300):
+        with pytest.raises(ValueError):
+            f(torch.tensor([s], dtype=torch.float64))
