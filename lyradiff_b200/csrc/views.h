@@ -9,20 +9,30 @@ namespace lyraq {
 
 // Up to three outer dimensions with strides in bytes, and a run of bytes in a row.  A dimension of one has no stride.
 struct View {
-    uintptr_t base;
+    uintptr_t base, last;  // its first and its last byte
     size_t    count[4];    // the last: the run
     size_t    stride[4];
+    bool      empty;
 };
 
 inline View view_of(const void* p, size_t elem_bytes, size_t n0, size_t s0, size_t n1, size_t s1, size_t n2, size_t s2, size_t run)
 {
-    return View{reinterpret_cast<uintptr_t>(p),
-                {n0, n1, n2, run * elem_bytes},
-                {n0 > 1 ? s0 * elem_bytes : 0, n1 > 1 ? s1 * elem_bytes : 0, n2 > 1 ? s2 * elem_bytes : 0, 1}};
+    View v{reinterpret_cast<uintptr_t>(p),
+           0,
+           {n0, n1, n2, run * elem_bytes},
+           {n0 > 1 ? s0 * elem_bytes : 0, n1 > 1 ? s1 * elem_bytes : 0, n2 > 1 ? s2 * elem_bytes : 0, 1},
+           p == nullptr || n0 == 0 || n1 == 0 || n2 == 0 || run == 0};
+    v.last = v.base;
+    for (int i = 0; i < 4 && !v.empty; ++i) {
+        size_t step;
+        if (__builtin_mul_overflow(v.count[i] - 1, v.stride[i], &step) || __builtin_add_overflow(v.last, step, &v.last)) {
+            v.last = UINTPTR_MAX;   // strides that lead out of memory
+            break;
+        }
+    }
+    return v;
 }
 inline View view_of(const void* p, size_t bytes) { return view_of(p, 1, 1, 0, 1, 0, 1, 0, bytes); }
-
-inline bool view_empty(const View& v) { return v.base == 0 || v.count[0] == 0 || v.count[1] == 0 || v.count[2] == 0 || v.count[3] == 0; }
 
 // Every element of one lies where the same element of the other does: a kernel whose threads write what they have read may have both.
 inline bool views_same(const View& a, const View& b)
@@ -73,20 +83,10 @@ inline bool reach(const Term* t, int n, __int128 sum, int& looks)
 inline bool views_meet(const View& a, const View& b)
 {
     using view_detail::Term;
-    if (view_empty(a) || view_empty(b)) {
+    if (a.empty || b.empty || a.last < b.base || b.last < a.base) {
         return false;
     }
-    auto span = [](const View& v) {
-        __int128 s = 0;
-        for (int i = 0; i < 4; ++i) {
-            s += (__int128)(v.count[i] - 1) * v.stride[i];
-        }
-        return s;
-    };
     const __int128 apart = (__int128)b.base - (__int128)a.base;     // what the steps within a, less those within b, have to make up
-    if (apart > span(a) || -apart > span(b)) {
-        return false;
-    }
     Term t[8];
     int  n = 0;
     auto add = [&](__int128 stride, __int128 lo, __int128 hi) {
