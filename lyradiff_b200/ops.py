@@ -127,11 +127,13 @@ def _fp4_format(fmt):
 
 class Fp4Tensor:
     """A matrix in microscaled FP4 (lyraq_quant_fp4): codes uint8 [rows, k / 2], the block scales in the tensor cores' order (scales, uint8),
-    the format, and for nvfp4 the tensor scale (fp32 [1], a power of two; None: 1)."""
+    the format, and for nvfp4 (mxfp4 has none) the tensor scale (fp32 [1], a power of two; None: 1)."""
 
     __slots__ = ("rows", "k", "fmt", "codes", "scales", "tensor_scale")
 
     def __init__(self, rows, k, fmt, codes, scales, tensor_scale=None):
+        if tensor_scale is not None and fmt == "mxfp4":
+            raise ValueError("mxfp4 has no tensor scale")
         self.rows, self.k, self.fmt, self.codes, self.scales, self.tensor_scale = rows, k, fmt, codes, scales, tensor_scale
 
     @classmethod

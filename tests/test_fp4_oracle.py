@@ -121,3 +121,15 @@ def test_input_scales_are_rounded_up_to_powers_of_two_of_fp32():
     for s in (0.0, -1.0, float("nan"), float("inf"), 3e38, 1e300):
         with pytest.raises(ValueError):
             f(torch.tensor([s], dtype=torch.float64))
+
+
+def test_mxfp4_has_no_tensor_scale():
+    """Its quantizer reads none, so a product that multiplied by one would be off by it."""
+    t, g = lambda *s: torch.empty(*s, dtype=torch.uint8), torch.ones(1)   # noqa: E731
+    with pytest.raises(ValueError, match="mxfp4"):
+        ops.Fp4Tensor(4, 64, "mxfp4", t(4, 32), t(512), g)
+    with pytest.raises(ValueError, match="mxfp4"):
+        ops.Fp4Tensor.empty(4, 64, "mxfp4", g, "cpu")
+    with pytest.raises(ValueError, match="mxfp4"):
+        ops.quant_fp4(torch.zeros(4, 64), g, "mxfp4")
+    assert ops.Fp4Tensor(4, 64, "nvfp4", t(4, 32), t(512), g).tensor_scale is g
