@@ -11,7 +11,7 @@
 //              prefetch is not a read: whatever that kernel writes is what the loads behind the wait see.
 //   warp 1   : scales to tensor memory, MMAs; the warp owns tensor memory
 //   warps 2-5: accumulator -> shared memory of the owning CTA -> sum, epilogue, store.  For rows of X that are not FP4 yet they fill the stages' X and its
-//              scales before that, 32 values a thread: every CTA quantizes what it reads, behind the weight stream, which saves a launch
+//              scales before that, 32 values a thread (fp4_deal.h has the order): every CTA quantizes what it reads, behind the weight stream, which saves a launch
 //              and the way through memory
 // All waits are bounded.  A timeout sets the status word and the abort flag of every CTA of the cluster: the sums a CTA stores need the partial
 // products of all of them, so when one gives up none of the cluster stores anything.
@@ -198,13 +198,11 @@ gemm_fp4_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
     } else if (warp == 1) {
         int      stage = 0;
         uint32_t phase = 0;
-        bool     ok    = true;
         for (int kb = kb0; kb < kb1; ++kb) {
             if (!mbar_wait_warp(full_bar(stage), phase, abort_flag, wait_limit_ns)) {
                 if (lane == 0) {
                     give_up(0x6200u | (unsigned)stage);
                 }
-                ok = false;
                 break;
             }
             tc_fence_after_sync();
@@ -239,7 +237,6 @@ gemm_fp4_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_
                 phase ^= 1u;
             }
         }
-        (void)ok;
     } else if constexpr (kQuantize) {
         constexpr int kPer  = 16 / (int)sizeof(X);
         constexpr int kVecs = 32 / kPer;
@@ -374,7 +371,8 @@ static int pick_splits(long tiles, int num_kb, int sms)
 // Quantizing in the kernel saves a launch, and every CTA does it for the K blocks it reads: it pays up to 64 rows times K blocks of a CTA, rows in powers of
 // two.  In the kernel against a launch of its own, nvfp4 / mxfp4, us: 1 row of [1280, 1280] 3.8 and 4.7 / 3.3 and 4.2, of [9216, 3072] (6) 6.2 and 6.4 / 5.3 and
 // 5.8, 16 rows of [1280, 2048] (32) 6.1 and 6.6 / 5.3 and 6.2, of [3072, 3072] (48) 7.1 and 7.2 / 6.2 and 6.8, of [9216, 3072] (96) 11.1 and
-// 9.6 / 9.6 and 8.8, of [3072, 12288] (96) 11.4 and 9.7 / 9.8 and 9.1.
+// 9.6 / 9.6 and 8.8, of [3072, 12288] (96) 11.4 and 9.7 / 9.8 and 9.1.  Few rows over deep K: 1 row of [21504, 3072] (12) 8.3 and 9.2 / 7.6 and
+// 8.2, of [28672, 8192] (32) 24.4 and 24.4 / 22.9 and 22.8, of [19072, 16128] (63) 35.3 and 34.8 / 32.3 and 32.5.
 static bool quantize_pays(int m, int n, int k, int sms)
 {
     const int num_kb = (k + kBlockK - 1) / kBlockK, splits = pick_splits(((long)n + kWRows - 1) / kWRows, num_kb, sms);

@@ -1,5 +1,6 @@
 // Calls of the FP4, norm and rotary operators over torch tensors: the argument checks, the outputs' allocation and the C-ABI call of one operator in one
-// step of host code.  In Python these took 14 to 18 us of a call whose kernel takes 2 to 6 (one token); here 6 to 9.  The module is bound to the
+// step of host code.  In Python these took 14 to 18 us of a call whose kernel takes 2 to 6 (one token); here 3 to 7, and 11 for a
+// norm that writes FP4, its buffers and the product behind it.  The module is bound to the
 // functions of the liblyraq.so that the ctypes loader has loaded (bind), so there is one library and one loader.  Functions return what
 // lyradiff_b200/ops.py documents; they raise ValueError or TypeError for arguments that do not fit and LyraqError for a status.
 #define PY_SSIZE_T_CLEAN
