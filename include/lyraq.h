@@ -115,6 +115,9 @@ LYRAQ_API int lyraq_debug_force_w4a4_wide(int on);
 /* Test / sweep hook: the kernel of lyraq_gemm_fp4.  0 = automatic (default); 2562 = CTA pair, 256 x 256 tile; 1281 = one CTA, 128 x 128; 16 = the few-row kernel wherever it can (16 rows), the automatic choice elsewhere.  Process-wide, not thread-safe.  It has no counterpart in the reference, which has no FP4 linears. */
 LYRAQ_API int lyraq_debug_force_fp4_tile(int code);
 
+/* Test / sweep hook: the kernel of lyraq_gemm_fp8_block.  0 = automatic (default); 2562 = CTA pair, 256 x 256 tile; 1281 = one CTA, 128 x 128; 16 = the few-row kernel wherever it can, the automatic choice elsewhere.  Process-wide, not thread-safe.  It has no counterpart in the reference. */
+LYRAQ_API int lyraq_debug_force_fp8_block_tile(int code);
+
 /* lyraq_debug_skinny_wait_test for the few-row FP4 kernel.  It has no counterpart in the reference. */
 LYRAQ_API int lyraq_debug_fp4_skinny_wait_test(int stalled_rank, unsigned int wait_limit_ms);
 
@@ -184,6 +187,19 @@ LYRAQ_API int lyraq_weight_quant_int8(float* w_scale, int8_t* qw, const void* w,
  * of scale_dtype (LYRAQ_F32 or LYRAQ_F16).  The reference has no device quantizer for this format. */
 LYRAQ_API int lyraq_weight_quant_int4_g64(uint8_t* qw, void* w_scale, int scale_dtype, const void* w, int w_dtype,
                                 size_t n, size_t k, void* stream);
+
+/* FP8 quantize of x [rows, k] (row pitch ldx elements; f16, bf16 or f32) with a scale for each 128 values of a row, k a multiple of 16 (the last block of a
+ * row may be shorter):
+ *   s = max(fl(max|x| / 448), 2^-100),  codes = e4m3(fl(x / s)), fl rounding to fp32, e4m3 to the nearest with ties to even
+ * A block that holds an infinity or a NaN gets the scale NaN and zero codes.  q: [rows, k] codes; scale of block b of row r at
+ * scale[r * scale_row + b * scale_block] (steps in elements, no two scales in one place).  q 16-byte aligned, x and its rows too.  Nothing
+ * shares memory.  lyraq_quant_fp8 without calibration; no counterpart in the reference. */
+LYRAQ_API int lyraq_quant_fp8_block(uint8_t* q, float* scale, size_t scale_row, size_t scale_block, const void* x, int x_dtype, size_t ldx,
+                                    size_t rows, size_t k, void* stream);
+
+/* The same for a weight [n, k] with a scale for each 128 x 128 values: w_scale [ceil(n / 128), ceil(k / 128)].  The block-scaled form of
+ * lyraq_weight_quant_fp8; no counterpart in the reference. */
+LYRAQ_API int lyraq_weight_quant_fp8_block(uint8_t* qw, float* w_scale, const void* w, int w_dtype, size_t n, size_t k, void* stream);
 
 /* Microscaled FP4 quantize of x [rows, k] (row pitch ldx elements; f16, bf16 or f32), k a multiple of 32.
  *   LYRAQ_NVFP4: a = max|x| of 16 values; s = e4m3(a / (6 g)), nearest, ties to even, at most 448; codes = e2m1(x / (s g)), nearest, ties to
@@ -256,7 +272,8 @@ enum {
     LYRAQ_OP_LINEAR_W4A4 = 5,
     LYRAQ_OP_LINEAR_W4A4_LORA = 6,
     LYRAQ_OP_GEMM_FP4 = 7,
-    LYRAQ_OP_LINEAR_FP4 = 8
+    LYRAQ_OP_LINEAR_FP4 = 8,
+    LYRAQ_OP_LINEAR_FP8_BLOCK = 9
 };
 
 /* Bytes of workspace an operation can use for (m, n, k).  0 for the INT8 and FP8 GEMMs (no split-K; the call is kept so that
@@ -350,6 +367,15 @@ LYRAQ_API int lyraq_gemm_w4a4(const uint8_t* A, const uint8_t* B, const float* s
                     void* D, int c_dtype, const void* lora_act, int lora_act_dtype, const void* lora_up,
                     const void* bias, const void* residual, int epilogue, int m, int n, int k,
                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* FP8 with a scale for each block of 128: Y[m,n] = T( epi( sum_b s_x[m,b] s_w[n/128,b] * sum_{k in block b} X[m,k] W[n,k] + beta * R[m,n] + bias[n] ) ),
+ * e4m3 codes X [m, k] and W [n, k], scales as lyraq_quant_fp8_block (element (row, block) of X's at row * x_scale_row + block * x_scale_block) and
+ * lyraq_weight_quant_fp8_block leave them, fp32 accumulation, epi = identity or GELU-tanh.  Y, R and bias have element type c_dtype (f16, bf16, f32).
+ * k a multiple of 16; code, result, bias and residual pointers 16-byte aligned.  Y may be R; otherwise it shares no memory with the operands, or the call
+ * is refused (LYRAQ_ERR_INVALID_ARG).  lyraq_gemm_fp8 for checkpoints with block scales; no counterpart in the reference. */
+LYRAQ_API int lyraq_gemm_fp8_block(const uint8_t* X, const float* x_scale, size_t x_scale_row, size_t x_scale_block, const uint8_t* W,
+                                   const float* w_scale, void* Y, int c_dtype, const void* bias, const void* residual, float beta, int epilogue,
+                                   int m, int n, int k, void* stream);
 
 /* Microscaled FP4: Y[m,n] = T( epi( g_x g_w * sum_k X[m,k] W[n,k] + beta * R[m,n] + bias[n] ) ), X and W codes with block scales as
  * lyraq_quant_fp4 lays them out, both of the same `format`, g_x and g_w fp32 [1] or NULL (= 1), exact products, fp32 accumulation, epi =
@@ -497,6 +523,12 @@ LYRAQ_API int lyraq_linear_fp4_forward(void* Y, const void* x, int dtype, size_t
                                        const uint8_t* w_scale, const float* w_tensor_scale, int format, const void* bias,
                                        const void* residual, float beta, int epilogue, int m, int n, int k, void* workspace,
                                        size_t workspace_bytes, void* stream);
+
+/* FP8 linear with block scales: x [m, k] (row pitch ldx elements) -> lyraq_quant_fp8_block, then lyraq_gemm_fp8_block.  Y may be R, and may lie on x; it
+ * and the workspace are apart from all else.  The dynamically scaled form of lyraq_linear_fp8_forward; no counterpart in the reference. */
+LYRAQ_API int lyraq_linear_fp8_block_forward(void* Y, const void* x, int dtype, size_t ldx, const uint8_t* W, const float* w_scale, const void* bias,
+                                             const void* residual, float beta, int epilogue, int m, int n, int k, void* workspace,
+                                             size_t workspace_bytes, void* stream);
 
 /* INT8 SmoothQuant linear: x -> int8 (scale_mode as in lyraq_quant_int8; PER_TOKEN_DYNAMIC keeps the computed scales in
  * the workspace), then lyraq_gemm_int8 with bias.  Replaces the invokeSqInputQuant + runGemmInt8 pair of the SDXL INT8

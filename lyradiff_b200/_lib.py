@@ -47,6 +47,7 @@ SIGNATURES = {
     "lyraq_debug_skinny_wait_test": (c_int, [c_int, ctypes.c_uint]),
     "lyraq_debug_force_w4a4_wide": (c_int, [c_int]),
     "lyraq_debug_force_fp4_tile": (c_int, [c_int]),
+    "lyraq_debug_force_fp8_block_tile": (c_int, [c_int]),
     "lyraq_debug_fp4_skinny_wait_test": (c_int, [c_int, ctypes.c_uint]),
     "lyraq_last_cuda_error": (ctypes.c_char_p, []),
     "lyraq_debug_set_row_vectors_per_thread": (c_int, [c_int]),
@@ -62,6 +63,8 @@ SIGNATURES = {
     "lyraq_quant_fp4": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_size_t, c_void_p, c_int, c_size_t, c_size_t, c_void_p]),
     "lyraq_fp4_scale_bytes": (c_size_t, [c_size_t, c_size_t, c_int]),
     "lyraq_weight_quant_fp4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_size_t, c_size_t, c_void_p]),
+    "lyraq_quant_fp8_block": (c_int, [c_void_p, c_void_p, c_size_t, c_size_t, c_void_p, c_int, c_size_t, c_size_t, c_size_t, c_void_p]),
+    "lyraq_weight_quant_fp8_block": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_size_t, c_size_t, c_void_p]),
     "lyraq_adaln_quant": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
                                   c_void_p, c_size_t, c_size_t, c_size_t, c_double, c_void_p]),
     "lyraq_adaln_quant_fp8x2": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
@@ -99,6 +102,10 @@ SIGNATURES = {
                                 c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "lyraq_gemm_fp4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p,
                                c_float, c_int, c_int, c_int, c_int, c_void_p]),
+    "lyraq_gemm_fp8_block": (c_int, [c_void_p, c_void_p, c_size_t, c_size_t, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_float,
+                                     c_int, c_int, c_int, c_int, c_void_p]),
+    "lyraq_linear_fp8_block_forward": (c_int, [c_void_p, c_void_p, c_int, c_size_t, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_int,
+                                               c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "lyraq_linear_fp4_forward": (c_int, [c_void_p, c_void_p, c_int, c_size_t, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
                                          c_void_p, c_float, c_int, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "lyraq_linear_fp8_forward": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float,
@@ -155,6 +162,7 @@ def host():
         from . import _host as module
         handle = lib()
         names = ("lyraq_gated_residual_norm", "lyraq_rope_axes", "lyraq_linear_fp4_forward", "lyraq_gemm_fp4", "lyraq_quant_fp4",
+                 "lyraq_linear_fp8_block_forward", "lyraq_gemm_fp8_block", "lyraq_quant_fp8_block",
                  "lyraq_workspace_bytes", "lyraq_fp4_scale_bytes")
         module.bind({n: ctypes.cast(getattr(handle, n), c_void_p).value for n in names}, LyraqError)
         _host = module

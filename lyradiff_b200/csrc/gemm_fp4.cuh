@@ -2,10 +2,9 @@
 #pragma once
 
 #include "fp4.cuh"
+#include "gemm_tiles.cuh"
 #include "sm100_ptx.cuh"
 #include "views.h"
-
-#include <initializer_list>
 
 namespace lyraq {
 
@@ -41,16 +40,6 @@ int  launch_skinny(const Fp4Input& X, const uint8_t* W, const uint8_t* ws, int f
 bool skinny_quantize_pays(int m, int n, int k, int sms);
 bool few_rows(int m, int k);                  // whether a product takes the few-row kernel,
 bool few_rows_quantize(int m, int n, int k);  // and whether a linear leaves the quantize to it
-// Whether a result lies on something that is still read while it is stored.  It may be the residual, element for element.
-inline bool result_clashes(const View& y, const void* residual, std::initializer_list<View> read)
-{
-    for (const View& v : read) {
-        if (views_meet(y, v)) {
-            return true;
-        }
-    }
-    return reinterpret_cast<uintptr_t>(residual) != y.base && views_meet(y, view_of(residual, y.count[3]));
-}
 // lyraq_gemm_fp4 behind its checks; rows that are not FP4 yet only where few_rows
 int product(const Fp4Input& X, const float* g_x, const uint8_t* W, const uint8_t* ws, const float* g_w, int format, void* Y, int c_dtype, const void* bias,
             const void* residual, float beta, int epilogue, int m, int n, int k, cudaStream_t stream);
@@ -77,31 +66,6 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t smem_dst, const CUtens
         "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
         ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(leader_bar), "r"(x), "r"(y), "r"(z)
         : "memory");
-}
-
-// all of this thread's committed stores but the last have finished reading shared memory
-__device__ __forceinline__ void tma_store_wait_read_but_one() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
-
-// 16 bytes, on a miss the 256 around them into L2
-__device__ __forceinline__ Vec16 ld_16_l2_256(const void* p)
-{
-    Vec16 v;
-    asm volatile("ld.global.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]) : "l"(p));
-    return v;
-}
-
-// Arrive on another CTA's barrier when all that has to be ordered before it is complete already (tensor-memory loads behind their wait).  The
-// releasing form makes the warp's earlier memory accesses visible first, which took a pair's second CTA 900 ns per tile.
-__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr)
-{
-    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-
-// Arrive on the barrier at this offset in both CTAs of a pair once all MMAs issued so far have completed.
-__device__ __forceinline__ void tc_commit_both(uint32_t bar)
-{
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3)
-                 : "memory");
 }
 
 // Shared memory -> tensor memory, 32 rows of 16 bytes, the same to each of the four lane quadrants: one atom of block scales, four columns.

@@ -29,6 +29,9 @@ decltype(&lyraq_rope_axes)           g_rope        = nullptr;
 decltype(&lyraq_linear_fp4_forward)  g_linear_fp4  = nullptr;
 decltype(&lyraq_gemm_fp4)            g_gemm_fp4    = nullptr;
 decltype(&lyraq_quant_fp4)           g_quant_fp4   = nullptr;
+decltype(&lyraq_linear_fp8_block_forward) g_linear_fp8_block = nullptr;
+decltype(&lyraq_gemm_fp8_block)      g_gemm_fp8_block  = nullptr;
+decltype(&lyraq_quant_fp8_block)     g_quant_fp8_block = nullptr;
 decltype(&lyraq_workspace_bytes)     g_workspace   = nullptr;
 decltype(&lyraq_fp4_scale_bytes)     g_scale_bytes = nullptr;
 PyObject*                            g_error       = nullptr;   // LyraqError(status, where)
@@ -394,6 +397,38 @@ int as_size(int64_t v, const char* what)
     return (int)v;
 }
 
+// The rows [m, k] of a linear's input: rows that lie one pitch apart stay where they are.
+const void* flat_rows(const Tensor& x, int m, int k, Tensor& flat, size_t& ldx)
+{
+    ldx = (size_t)k;
+    if (x.is_contiguous()) {
+        return x.data_ptr();
+    }
+    flat = x.reshape({m, k});
+    ldx  = m > 1 ? (size_t)flat.stride(0) : (size_t)k;
+    if ((k > 1 && flat.stride(1) != 1) || (m > 1 && flat.stride(0) < k)) {
+        flat = flat.contiguous();
+        ldx  = (size_t)k;
+    }
+    return flat.data_ptr();
+}
+
+// The result of a linear: the argument, or a new tensor.
+const Tensor& linear_out(PyObject* o, const Tensor& x, int m, int n, Tensor& made, int dev)
+{
+    const Tensor* out = tensor(o, "out", dev);
+    if (out != nullptr) {
+        if (out->scalar_type() != x.scalar_type() || out->dim() < 1 || out->numel() != (int64_t)m * n || out->size(out->dim() - 1) != n) {
+            refuse(PyExc_ValueError, "out must be [..., %d] of x's dtype", n);
+        }
+        return *out;
+    }
+    c10::SmallVector<int64_t, 6> sizes(x.sizes().begin(), x.sizes().end());
+    sizes.back() = n;
+    made         = empty_like_cuda(sizes, x.scalar_type(), dev);
+    return made;
+}
+
 // (x, codes, scales, tensor scale of the weight, n, k, format, input scale, bias, residual, beta, epilogue, out) -> y
 PyObject* linear_fp4(PyObject* const* a)
 {
@@ -413,37 +448,19 @@ PyObject* linear_fp4(PyObject* const* a)
     const Tensor* bias     = tensor(a[8], "bias", dev);
     const Tensor* residual = tensor(a[9], "residual", dev);
     check_epilogue(bias, residual, type, m, n);
-    // rows that lie one pitch apart stay where they are
-    Tensor flat;
-    size_t ldx = (size_t)k;
-    if (!x.is_contiguous()) {
-        flat = x.reshape({m, k});
-        ldx  = m > 1 ? (size_t)flat.stride(0) : (size_t)k;
-        if ((k > 1 && flat.stride(1) != 1) || (m > 1 && flat.stride(0) < k)) {
-            flat = flat.contiguous();
-            ldx  = (size_t)k;
-        }
-    }
-    const Tensor* out = tensor(a[12], "out", dev);
-    if (out != nullptr && (out->scalar_type() != type || out->dim() < 1 || out->numel() != (int64_t)m * n || out->size(out->dim() - 1) != n)) {
-        refuse(PyExc_ValueError, "out must be [..., %d] of x's dtype", n);
-    }
-    Tensor y;
-    if (out == nullptr) {
-        c10::SmallVector<int64_t, 6> sizes(x.sizes().begin(), x.sizes().end());
-        sizes.back() = n;
-        y            = empty_like_cuda(sizes, type, dev);
-        out          = &y;
-    }
+    Tensor        flat, made;
+    size_t        ldx;
+    const void*   xp  = flat_rows(x, m, k, flat, ldx);
+    const Tensor& out = linear_out(a[12], x, m, n, made, dev);
     const size_t need = g_workspace(LYRAQ_OP_LINEAR_FP4, m, n, k);
     const Tensor ws   = empty_like_cuda({(int64_t)need}, at::kByte, dev);
-    void* const  yp   = at_contiguous(out, "out");
+    void* const  yp   = at_contiguous(&out, "out");
     const void*  bp   = at_contiguous(bias, "bias");
     const void*  rp   = at_contiguous(residual, "residual");
-    check_status(run(g_linear_fp4, yp, (flat.defined() ? flat : x).data_ptr(), dtype_code(x, "x"), ldx, g == nullptr ? nullptr : (const float*)g->data_ptr(),
+    check_status(run(g_linear_fp4, yp, xp, dtype_code(x, "x"), ldx, g == nullptr ? nullptr : (const float*)g->data_ptr(),
                      w.codes, w.scales, w.scale, format, bp, rp, as_float(a[10]), (int)as_long(a[11]), m, n, k, ws.data_ptr(), need, current_stream()),
                  "lyraq_linear_fp4_forward");
-    return result(a[12], y);
+    return result(a[12], made);
 }
 
 // (codes, scales, tensor scale of X, rows, the same of W, k, format, bias, residual, beta, epilogue, Y or the dtype of a new one) -> Y
@@ -474,6 +491,119 @@ PyObject* gemm_fp4(PyObject* const* a)
                      (int)as_long(a[13]), m, n, k, current_stream()),
                  "lyraq_gemm_fp4");
     return made.defined() ? THPVariable_Wrap(made) : Py_NewRef(a[14]);
+}
+
+// A weight in FP8 with block scales: codes uint8 [n, k], scales fp32 [ceil(n / 128), ceil(k / 128)].
+std::pair<const uint8_t*, const float*> fp8_block_weight(PyObject* codes, PyObject* scales, int n, int k, int dev)
+{
+    const Tensor& c = needed(codes, "the weight's codes", dev);
+    const Tensor& s = needed(scales, "the weight's scales", dev);
+    if (c.scalar_type() != at::kByte || c.dim() != 2 || c.size(0) != n || c.size(1) != k) {
+        refuse(PyExc_ValueError, "the weight's codes must be uint8 [%d, %d]", n, k);
+    }
+    if (s.scalar_type() != at::kFloat || s.dim() != 2 || s.size(0) != ((int64_t)n + 127) / 128 || s.size(1) != ((int64_t)k + 127) / 128) {
+        refuse(PyExc_ValueError, "the weight's scales must be fp32, one for each 128 x 128 of [%d, %d]", n, k);
+    }
+    return {(const uint8_t*)at_contiguous(&c, "the weight's codes"), (const float*)at_contiguous(&s, "the weight's scales")};
+}
+
+// Scales of rows in FP8, fp32 [rows, ceil(k / 128)] of any steps; the step of a dimension of one is of no use.
+const Tensor& fp8_block_scales(PyObject* o, int64_t rows, int64_t k, int dev, size_t& row_step, size_t& block_step)
+{
+    const Tensor& s = needed(o, "the scales", dev);
+    if (s.scalar_type() != at::kFloat || s.dim() != 2 || s.size(0) != rows || s.size(1) != (k + 127) / 128) {
+        refuse(PyExc_ValueError, "the scales must be fp32, one for each 128 values of a row of [%lld, %lld]", (long long)rows, (long long)k);
+    }
+    row_step   = s.size(0) > 1 ? (size_t)s.stride(0) : 0;
+    block_step = s.size(1) > 1 ? (size_t)s.stride(1) : 0;
+    return s;
+}
+
+// (x, codes, scales of the weight, n, k, bias, residual, beta, epilogue, out) -> y
+PyObject* linear_fp8_block(PyObject* const* a)
+{
+    const int     dev = c10::cuda::current_device();
+    const Tensor& x   = needed(a[0], "x", dev);
+    const int     n = as_size(as_long(a[3]), "n"), k = as_size(as_long(a[4]), "k");
+    if (x.dim() < 1 || x.size(x.dim() - 1) != k || k == 0) {
+        refuse(PyExc_ValueError, "expected [..., %d]", k);
+    }
+    const int  m = as_size(x.numel() / k, "the number of rows");
+    const auto w = fp8_block_weight(a[1], a[2], n, k, dev);
+    const Tensor* bias     = tensor(a[5], "bias", dev);
+    const Tensor* residual = tensor(a[6], "residual", dev);
+    check_epilogue(bias, residual, x.scalar_type(), m, n);
+    Tensor        flat, made;
+    size_t        ldx;
+    const void*   xp   = flat_rows(x, m, k, flat, ldx);
+    const Tensor& out  = linear_out(a[9], x, m, n, made, dev);
+    const size_t  need = g_workspace(LYRAQ_OP_LINEAR_FP8_BLOCK, m, n, k);
+    const Tensor  ws   = empty_like_cuda({(int64_t)need}, at::kByte, dev);
+    void* const   yp   = at_contiguous(&out, "out");
+    const void*   bp   = at_contiguous(bias, "bias");
+    const void*   rp   = at_contiguous(residual, "residual");
+    check_status(run(g_linear_fp8_block, yp, xp, dtype_code(x, "x"), ldx, w.first, w.second, bp, rp, as_float(a[7]), (int)as_long(a[8]), m, n, k,
+                     ws.data_ptr(), need, current_stream()),
+                 "lyraq_linear_fp8_block_forward");
+    return result(a[9], made);
+}
+
+// (codes, scales of X, the same of W, bias, residual, beta, epilogue, Y or the dtype of a new one) -> Y
+PyObject* gemm_fp8_block(PyObject* const* a)
+{
+    const int     dev = c10::cuda::current_device();
+    const Tensor& x   = needed(a[0], "X", dev);
+    const Tensor& wc  = needed(a[2], "W", dev);
+    if (x.scalar_type() != at::kByte || x.dim() != 2 || wc.dim() != 2 || wc.size(1) != x.size(1)) {
+        refuse(PyExc_ValueError, "expected codes X uint8 [m, k] and W uint8 [n, k]");
+    }
+    const int m = as_size(x.size(0), "m"), n = as_size(wc.size(0), "n"), k = as_size(x.size(1), "k");
+    size_t        row_step, block_step;
+    const Tensor& xs = fp8_block_scales(a[1], m, k, dev, row_step, block_step);
+    const auto    w  = fp8_block_weight(a[2], a[3], n, k, dev);
+    Tensor        made;
+    if (THPDtype_Check(a[8])) {
+        const at::ScalarType type = reinterpret_cast<THPDtype*>(a[8])->scalar_type;
+        if (type != at::kHalf && type != at::kBFloat16 && type != at::kFloat) {
+            refuse(PyExc_TypeError, "Y: unsupported dtype %s", c10::toString(type));
+        }
+        made = empty_like_cuda({m, n}, type, dev);
+    }
+    const Tensor& y = made.defined() ? made : needed(a[8], "Y", dev);
+    if (y.dim() != 2 || y.size(0) != m || y.size(1) != n) {
+        refuse(PyExc_ValueError, "Y must be [%d, %d]", m, n);
+    }
+    const Tensor* bias     = tensor(a[4], "bias", dev);
+    const Tensor* residual = tensor(a[5], "residual", dev);
+    check_epilogue(bias, residual, y.scalar_type(), m, n);
+    const uint8_t* xp = (const uint8_t*)at_contiguous(&x, "X");
+    void* const    yp = at_contiguous(&y, "Y");
+    const void*    bp = at_contiguous(bias, "bias");
+    const void*    rp = at_contiguous(residual, "residual");
+    check_status(run(g_gemm_fp8_block, xp, (const float*)xs.data_ptr(), row_step, block_step, w.first, w.second, yp, dtype_code(y, "Y"), bp, rp,
+                     as_float(a[6]), (int)as_long(a[7]), m, n, k, current_stream()),
+                 "lyraq_gemm_fp8_block");
+    return made.defined() ? THPVariable_Wrap(made) : Py_NewRef(a[8]);
+}
+
+// (x, codes, scales)
+PyObject* quant_fp8_block(PyObject* const* a)
+{
+    const int     dev = c10::cuda::current_device();
+    const Tensor& x   = needed(a[0], "x", dev);
+    if (x.dim() != 2 || (x.size(1) > 1 && x.stride(1) != 1) || (x.size(0) > 1 && x.stride(0) < x.size(1))) {
+        refuse(PyExc_ValueError, "expected a matrix with contiguous rows that do not overlap");
+    }
+    const Tensor& q = needed(a[1], "codes", dev);
+    if (q.scalar_type() != at::kByte || q.sizes() != x.sizes()) {
+        refuse(PyExc_ValueError, "codes must be uint8 of x's shape");
+    }
+    size_t        row_step, block_step;
+    const Tensor& s = fp8_block_scales(a[2], x.size(0), x.size(1), dev, row_step, block_step);
+    check_status(run(g_quant_fp8_block, (uint8_t*)at_contiguous(&q, "codes"), (float*)s.data_ptr(), row_step, block_step, x.data_ptr(), dtype_code(x, "x"),
+                     x.size(0) > 1 ? (size_t)x.stride(0) : (size_t)x.size(1), (size_t)x.size(0), (size_t)x.size(1), current_stream()),
+                 "lyraq_quant_fp8_block");
+    Py_RETURN_NONE;
 }
 
 // (rows, k, format, device) -> (codes, scales) of an FP4 matrix
@@ -538,7 +668,8 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n)
     };
     if (!take("lyraq_gated_residual_norm", g_norm) || !take("lyraq_rope_axes", g_rope) || !take("lyraq_linear_fp4_forward", g_linear_fp4) ||
         !take("lyraq_gemm_fp4", g_gemm_fp4) || !take("lyraq_quant_fp4", g_quant_fp4) || !take("lyraq_workspace_bytes", g_workspace) ||
-        !take("lyraq_fp4_scale_bytes", g_scale_bytes)) {
+        !take("lyraq_linear_fp8_block_forward", g_linear_fp8_block) || !take("lyraq_gemm_fp8_block", g_gemm_fp8_block) ||
+        !take("lyraq_quant_fp8_block", g_quant_fp8_block) || !take("lyraq_fp4_scale_bytes", g_scale_bytes)) {
         return nullptr;
     }
     Py_XSETREF(g_error, Py_NewRef(args[1]));
@@ -551,6 +682,9 @@ PyMethodDef g_methods[] = {
     {"rope_axes", (PyCFunction)(void (*)())call<rope_axes, 13>, METH_FASTCALL, nullptr},
     {"linear_fp4", (PyCFunction)(void (*)())call<linear_fp4, 13>, METH_FASTCALL, nullptr},
     {"gemm_fp4", (PyCFunction)(void (*)())call<gemm_fp4, 15>, METH_FASTCALL, nullptr},
+    {"linear_fp8_block", (PyCFunction)(void (*)())call<linear_fp8_block, 10>, METH_FASTCALL, nullptr},
+    {"gemm_fp8_block", (PyCFunction)(void (*)())call<gemm_fp8_block, 9>, METH_FASTCALL, nullptr},
+    {"quant_fp8_block", (PyCFunction)(void (*)())call<quant_fp8_block, 3>, METH_FASTCALL, nullptr},
     {"fp4_empty", (PyCFunction)(void (*)())call<fp4_empty, 4>, METH_FASTCALL, nullptr},
     {"quant_fp4", (PyCFunction)(void (*)())call<quant_fp4, 5>, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},

@@ -2,6 +2,7 @@
 // the quantized activation (and its scales) held in caller-provided workspace.  These are what the reference's layers
 // do around every quantized linear with buffers from their allocator; here the caller owns the buffer.
 #include "common.cuh"
+#include "fp8_block.cuh"
 #include "gemm_fp4.cuh"
 #include "gemm_w4a4.cuh"
 
@@ -17,6 +18,7 @@ static inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; 
 //   LINEAR_W4A4 : packed int4 activation [m, k/2] | fp32 group scales [m, k/64]
 //   LINEAR_W4A4_LORA : the same, then the fp32 low-rank activation [m, 32]
 //   LINEAR_FP4  : e2m1 activation [m, k/2] | block scales (nvfp4's, the larger)
+//   LINEAR_FP8_BLOCK : e4m3 activation [m, k] | fp32 block scales [k/128][m rounded up to 4]
 // The W4A4 forwards hand what a larger workspace has left to the GEMM, for its wide form (gemm_w4a4_wide.cu): w4a4_wide_bytes.
 size_t linear_workspace_bytes(int op, size_t m, size_t k)
 {
@@ -27,6 +29,7 @@ size_t linear_workspace_bytes(int op, size_t m, size_t k)
         case LYRAQ_OP_LINEAR_W4A4_LORA:
             return align_up(m * k / 2, 256) + align_up(4 * m * (k / 64), 256) + align_up(4 * m * 32, 256);
         case LYRAQ_OP_LINEAR_FP4: return align_up(m * k / 2, 256) + lyraq_fp4_scale_bytes(m, k, LYRAQ_NVFP4);
+        case LYRAQ_OP_LINEAR_FP8_BLOCK: return align_up(m * k, 256) + align_up(4 * fp8b::scale_pitch(m) * fp8b::blocks_of(k), 256);
         default: return 0;
     }
 }
@@ -109,8 +112,8 @@ int lyraq_linear_fp4_forward(void* Y, const void* x, int dtype, size_t ldx, cons
     const View   w = view_of(W, cols * depth / 2), ws = view_of(w_scale, lyraq_fp4_scale_bytes(cols, depth, format)), b = view_of(bias, cols * bytes);
     const View   work = view_of(workspace, linear_workspace_bytes(LYRAQ_OP_LINEAR_FP4, rows, depth));
     // the workspace is written before anything but x is read
-    if (fp4::result_clashes(y, residual, {w, ws, b, work}) ||
-        fp4::result_clashes(work, nullptr, {w, ws, b, view_of(residual, rows * cols * bytes), view_of(x, bytes, rows, ldx, 1, 0, 1, 0, depth)})) {
+    if (result_clashes(y, residual, {w, ws, b, work}) ||
+        result_clashes(work, nullptr, {w, ws, b, view_of(residual, rows * cols * bytes), view_of(x, bytes, rows, ldx, 1, 0, 1, 0, depth)})) {
         return LYRAQ_ERR_INVALID_ARG;
     }
     uint8_t* qx = static_cast<uint8_t*>(workspace);
@@ -129,6 +132,50 @@ int lyraq_linear_fp4_forward(void* Y, const void* x, int dtype, size_t ldx, cons
         return st;
     }
     return lyraq_gemm_fp4(qx, sx, g, W, w_scale, w_tensor_scale, format, Y, dtype, bias, residual, beta, epilogue, m, n, k, stream);
+}
+
+int lyraq_linear_fp8_block_forward(void* Y, const void* x, int dtype, size_t ldx, const uint8_t* W, const float* w_scale, const void* bias,
+                                   const void* residual, float beta, int epilogue, int m, int n, int k, void* workspace, size_t workspace_bytes,
+                                   void* stream)
+{
+    if (m < 0 || n < 0 || k < 0 || (epilogue != LYRAQ_EPI_NONE && epilogue != LYRAQ_EPI_GELU_TANH)) {
+        return LYRAQ_ERR_INVALID_ARG;
+    }
+    if (m == 0 || n == 0) {
+        return LYRAQ_OK;
+    }
+    if (k == 0 || (k & 15) != 0 || m > fp8b::kMaxSize || n > fp8b::kMaxSize || k > fp8b::kMaxSize) {
+        return LYRAQ_ERR_UNSUPPORTED;
+    }
+    const size_t rows = (size_t)m, cols = (size_t)n, depth = (size_t)k, blocks = fp8b::blocks_of(depth), need = linear_workspace_bytes(LYRAQ_OP_LINEAR_FP8_BLOCK, rows, depth);
+    if (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)) {
+        return LYRAQ_ERR_WORKSPACE;
+    }
+    uint8_t* qx = static_cast<uint8_t*>(workspace);
+    float*   sx = reinterpret_cast<float*>(qx + align_up(rows * depth, 256));
+    // whatever the product would refuse is refused before the quantize runs
+    int st = fp8b::check_quant(qx, sx, x, dtype, ldx, rows, depth);
+    if (st != LYRAQ_OK) {
+        return st;
+    }
+    if (Y == nullptr || W == nullptr || w_scale == nullptr || !aligned16(Y) || !aligned16(W) || (reinterpret_cast<uintptr_t>(w_scale) & 3u) != 0 ||
+        (bias != nullptr && !aligned16(bias)) || (residual != nullptr && !aligned16(residual))) {
+        return LYRAQ_ERR_INVALID_ARG;
+    }
+    const size_t bytes = dtype == LYRAQ_F32 ? 4 : 2;
+    const View   y = view_of(Y, rows * cols * bytes), w = view_of(W, cols * depth), ws = view_of(w_scale, fp8b::blocks_of(cols) * blocks * 4);
+    const View   b = view_of(bias, cols * bytes), work = view_of(workspace, need);
+    // the workspace is written before anything but x is read
+    if (result_clashes(y, residual, {w, ws, b, work}) ||
+        result_clashes(work, nullptr, {w, ws, b, view_of(residual, rows * cols * bytes), view_of(x, bytes, rows, ldx, 1, 0, 1, 0, depth)})) {
+        return LYRAQ_ERR_INVALID_ARG;
+    }
+    const size_t pitch = fp8b::scale_pitch(rows);
+    st = lyraq_quant_fp8_block(qx, sx, 1, pitch, x, dtype, ldx, rows, depth, stream);
+    if (st != LYRAQ_OK) {
+        return st;
+    }
+    return fp8b::product({qx, {sx, 1, pitch}, nullptr, 0, 0}, W, w_scale, Y, dtype, bias, residual, beta, epilogue, m, n, k, (cudaStream_t)stream);
 }
 
 int lyraq_linear_int8_forward(void* Y, const void* x, int dtype, const float* pre_quant_scale, const float* input_scale,

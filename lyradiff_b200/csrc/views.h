@@ -4,6 +4,7 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <initializer_list>
 
 namespace lyraq {
 
@@ -114,6 +115,17 @@ inline bool views_meet(const View& a, const View& b)
     }
     int looks = 4096;
     return view_detail::reach(t, n, apart, looks);
+}
+
+// Whether a result lies on something that is still read while it is stored.  It may be the residual, element for element.
+inline bool result_clashes(const View& y, const void* residual, std::initializer_list<View> read)
+{
+    for (const View& v : read) {
+        if (views_meet(y, v)) {
+            return true;
+        }
+    }
+    return reinterpret_cast<uintptr_t>(residual) != y.base && views_meet(y, view_of(residual, y.count[3]));
 }
 
 }  // namespace lyraq

@@ -221,6 +221,32 @@ def invoke_fused_add_bias_geglu_int8o(dst, hidden_states, bias, pre_quant_scale,
     return dst
 
 
+def quant_fp8_block(x, codes=None, scales=None):
+    """FP8 quantize with a scale for each 128 values of a row (lyraq_quant_fp8_block) of x [rows, k], whose rows may lie further apart than k.
+    Returns (codes uint8 [rows, k], scales fp32 [rows, ceil(k / 128)]), created when omitted; scales may have any steps, those of a new one have the
+    rows of a block beside each other, which is how gemm_fp8_block reads them."""
+    rows, k = x.shape
+    if codes is None:
+        codes = torch.empty(rows, k, dtype=torch.uint8, device=x.device)
+    if scales is None:
+        scales = torch.empty((k + 127) // 128, (rows + 3) // 4 * 4, dtype=torch.float32, device=x.device).t()[:rows]
+    _lib.host().quant_fp8_block(x, codes, scales)
+    return codes, scales
+
+
+def weight_quant_fp8_block(w):
+    """FP8 weight quantize with a scale for each 128 x 128 values (lyraq_weight_quant_fp8_block): w [n, k], k a multiple of 16 -> codes uint8 [n, k],
+    scales fp32 [ceil(n / 128), ceil(k / 128)]."""
+    n, k = w.shape
+    if w.get_device() != torch.cuda.current_device():
+        raise ValueError("the weight is on %s, but the current device is cuda:%d" % (w.device, torch.cuda.current_device()))
+    codes = torch.empty(n, k, dtype=torch.uint8, device=w.device)
+    scales = torch.empty((n + 127) // 128, (k + 127) // 128, dtype=torch.float32, device=w.device)
+    st = _lib.lib().lyraq_weight_quant_fp8_block(_p(codes), _p(scales), _p(w), _dt(w), n, k, _stream())
+    _lib.check(st, "lyraq_weight_quant_fp8_block")
+    return codes, scales
+
+
 # ----------------------------------------------------------------------------- GEMMs
 def run_gemm_int8(A, B, alpha_col, alpha_row, C, bias=None, per_token=False, workspace=None, residual=None):
     """cublasMMWrapper::runGemmInt8 (src/lyradiff/utils/cublasMMWrapper.h:368-385): C[m,n] from A int8 [m,k], B int8 [n,k].
@@ -268,6 +294,12 @@ def gemm_fp4(W, X, Y, bias=None, residual=None, beta=1.0, is_gelu=False):
         raise ValueError("shape or format mismatch")
     return _lib.host().gemm_fp4(X.codes, X.scales, X.tensor_scale, X.rows, W.codes, W.scales, W.tensor_scale, W.rows, X.k, _fp4_format(X.fmt), bias,
                                 residual, beta, EPI_GELU_TANH if is_gelu else EPI_NONE, Y)
+
+
+def gemm_fp8_block(W, w_scale, X, x_scale, Y, bias=None, residual=None, beta=1.0, is_gelu=False):
+    """FP8 GEMM with a scale for each block of 128 (lyraq_gemm_fp8_block), weight first as in gemm_with_residual_and_bias_fp8: Y[m,n] = epi(X W^T + beta *
+    R + bias) for codes and scales as weight_quant_fp8_block and quant_fp8_block return them; Y a tensor, or the dtype of a new one."""
+    return _lib.host().gemm_fp8_block(X, x_scale, W, w_scale, bias, residual, beta, EPI_GELU_TANH if is_gelu else EPI_NONE, Y)
 
 
 def gemm_fp8_qk_rope(W, w_scale, X, x_scale, Y, qk_scale, rope_emb, heads, head_dim, bias=None, eps=1e-6):
