@@ -115,6 +115,9 @@ LYRAQ_API int lyraq_debug_force_w4a4_wide(int on);
 /* Test / sweep hook: the kernel of lyraq_gemm_fp4.  0 = automatic (default); 2562 = CTA pair, 256 x 256 tile; 1281 = one CTA, 128 x 128; 16 = the few-row kernel wherever it can (16 rows), the automatic choice elsewhere.  Process-wide, not thread-safe.  It has no counterpart in the reference, which has no FP4 linears. */
 LYRAQ_API int lyraq_debug_force_fp4_tile(int code);
 
+/* lyraq_debug_attention_wait_test for lyraq_sparse_attention.  It has no counterpart in the reference. */
+LYRAQ_API int lyraq_debug_sparse_attention_wait_test(int skip_loads, unsigned int wait_limit_ms);
+
 /* Test / sweep hook: the kernel of lyraq_gemm_fp8_block.  0 = automatic (default); 2562 = CTA pair, 256 x 256 tile; 1281 = one CTA, 128 x 128; 16 = the few-row kernel wherever it can, the automatic choice elsewhere.  Process-wide, not thread-safe.  It has no counterpart in the reference. */
 LYRAQ_API int lyraq_debug_force_fp8_block_tile(int code);
 
@@ -503,6 +506,66 @@ LYRAQ_API int lyraq_gated_residual_norm(const lyraq_gated_norm_t* args, void* st
  * (FP8LoraWeight<T>::load_lora, src/lyradiff/interface/IFLoraWeight.h:104-116).  Replaces invokeLoadLora<T>
  * (src/lyradiff/kernels/lora/load_lora.h; kernel load_lora.cu:6-14). */
 LYRAQ_API int lyraq_load_lora(void* weight, const void* lora, int dtype, float alpha, size_t n, void* stream);
+
+/* ------------------------------------------------------------------ attention over selected key blocks
+ * Queries in blocks of 128, keys in blocks of `block` tokens.  Every 128 queries of a head share a list of key blocks, chosen by the products of the
+ * blocks' means; lists belong to query heads, or one to all query heads of a key head ("lists" = q_heads or k_heads).  k_lens (int32 [batch], NULL: all)
+ * says how many keys of a sequence exist, values beyond 0 .. keys are taken as these; q_start (int32 [batch], NULL: keys - queries) at which key the
+ * first query stands, which causal order and the window go by. */
+
+/* Means of blocks of tokens: means fp32 [batch, heads, ceil(tokens / block), head_dim] of x (f16 or bf16, element (b, t, h, c) at b * batch_step + t *
+ * token_step + h * head_step + c, steps multiples of 8); sums in 64 bits, over the tokens below lens[b]; 0 for a block without any.  newest = n > 0
+ * takes only the blocks that hold one of a sequence's last n tokens and leaves the others as they are.  head_dim a multiple of 8 up to 256.  means
+ * shares no memory with what is read.  It has no counterpart in the reference, whose attention is dense. */
+LYRAQ_API int lyraq_block_means(float* means, const void* x, int dtype, size_t batch_step, size_t token_step, size_t head_step, const int* lens, int block,
+                                int newest, size_t batch, size_t tokens, int heads, int head_dim, void* stream);
+
+typedef struct {
+    const float* q_means;      /* [batch, q_heads, ceil(queries / 128), head_dim], lyraq_block_means with block 128 */
+    const float* k_means;      /* [batch, k_heads, ceil(keys / block), head_dim] */
+    int*         index;        /* [batch, lists, ceil(queries / 128), count]: the blocks taken in ascending order, then -1 */
+    int*         counts;       /* [batch, lists, ceil(queries / 128)]: how many */
+    const int*   k_lens;
+    const int*   q_start;
+    size_t       batch, queries, keys;
+    int          q_heads, k_heads, lists, head_dim;
+    int          block;        /* keys of a block */
+    int          count;        /* most blocks taken */
+    int          sink;         /* the first so many are taken in any case */
+    int          window;       /* n > 0: and those that hold the queries' own places, with n - 1 on either side */
+    int          causal;       /* only blocks with a key at or before the last query's place */
+} lyraq_select_blocks_t;
+
+/* The count key blocks with the largest fl(q_mean . k_mean) (sum in 64 bits; q_mean the sum over the list's query heads) among those that hold a key a query of
+ * the block may see, ties to the lowest index; blocks taken in any case come first, the lowest of them where they are more than count.  A score that
+ * is no number comes last.  Up to 32768 key blocks.  workspace: lyraq_select_blocks_workspace bytes, 16-byte aligned.  Outputs and workspace share no memory with anything
+ * else.  It has no counterpart in the reference. */
+LYRAQ_API int lyraq_select_blocks(const lyraq_select_blocks_t* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Workspace of lyraq_select_blocks (no counterpart in the reference). */
+LYRAQ_API size_t lyraq_select_blocks_workspace(size_t batch, int lists, size_t queries, size_t keys, int block);
+
+typedef struct {
+    const void *q, *k, *v;                            /* f16 or bf16 [batch, tokens, heads, head_dim], steps below */
+    void*       out;                                  /* like q */
+    size_t      q_batch, q_token, q_head, k_batch, k_token, k_head, v_batch, v_token, v_head, o_batch, o_token, o_head;   /* steps in elements */
+    const int*  index;                                /* as lyraq_select_blocks leaves them */
+    const int*  counts;
+    const int*  k_lens;
+    const int*  q_start;
+    size_t      batch, queries, keys;
+    int         q_heads, k_heads, lists, head_dim;    /* head_dim 64 or 128 */
+    int         block, count;                         /* block 64 or 128 */
+    int         causal;
+    float       softmax_scale;                        /* positive */
+    int         dtype;
+} lyraq_sparse_attention_t;
+
+/* out = softmax(q k^T * softmax_scale) v over the keys of the first counts[...] listed blocks that are below k_lens[b] and, if causal, not behind the
+ * query's place; a query without any gets zeros.  An index outside the keys adds nothing, a block listed twice counts twice.  Keys and values
+ * beyond k_lens may hold anything; in causal order the values within a listed block are finite.  All pointers of tensors 16-byte aligned, steps
+ * multiples of 8; out shares no memory with what is read.  lyraq_attention over a part of the keys; no counterpart in the reference. */
+LYRAQ_API int lyraq_sparse_attention(const lyraq_sparse_attention_t* args, void* stream);
 
 /* ------------------------------------------------------------------ quantized-Linear layer forwards
  * Activation quantize + GEMM of one linear on `stream`; the quantized activation lives in `workspace`

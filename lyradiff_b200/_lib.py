@@ -26,6 +26,20 @@ class GatedNormArgs(ctypes.Structure):
                 + [("residual_scale", c_float), ("eps", c_float), ("dtype", c_int)] + [(n, c_size_t) for n in ("batch", "seq_len", "dim")])
 
 
+class SelectBlocksArgs(ctypes.Structure):
+    """lyraq_select_blocks_t."""
+    _fields_ = ([(n, c_void_p) for n in ("q_means", "k_means", "index", "counts", "k_lens", "q_start")]
+                + [(n, c_size_t) for n in ("batch", "queries", "keys")]
+                + [(n, c_int) for n in ("q_heads", "k_heads", "lists", "head_dim", "block", "count", "sink", "window", "causal")])
+
+
+class SparseAttentionArgs(ctypes.Structure):
+    """lyraq_sparse_attention_t."""
+    _fields_ = ([(n, c_void_p) for n in ("q", "k", "v", "out")] + [(a + n, c_size_t) for a in ("q_", "k_", "v_", "o_") for n in ("batch", "token", "head")]
+                + [(n, c_void_p) for n in ("index", "counts", "k_lens", "q_start")] + [(n, c_size_t) for n in ("batch", "queries", "keys")]
+                + [(n, c_int) for n in ("q_heads", "k_heads", "lists", "head_dim", "block", "count", "causal")] + [("softmax_scale", c_float), ("dtype", c_int)])
+
+
 class RopeAxesArgs(ctypes.Structure):
     """lyraq_rope_axes_t."""
     _fields_ = ([(n, c_void_p) for n in ("q", "k")] + [(a + n, c_size_t) for a in ("q_", "k_") for n in ("batch", "token", "head")]
@@ -47,6 +61,7 @@ SIGNATURES = {
     "lyraq_debug_skinny_wait_test": (c_int, [c_int, ctypes.c_uint]),
     "lyraq_debug_force_w4a4_wide": (c_int, [c_int]),
     "lyraq_debug_force_fp4_tile": (c_int, [c_int]),
+    "lyraq_debug_sparse_attention_wait_test": (c_int, [c_int, ctypes.c_uint]),
     "lyraq_debug_force_fp8_block_tile": (c_int, [c_int]),
     "lyraq_debug_fp4_skinny_wait_test": (c_int, [c_int, ctypes.c_uint]),
     "lyraq_last_cuda_error": (ctypes.c_char_p, []),
@@ -96,6 +111,11 @@ SIGNATURES = {
     "lyraq_quant_fp8_2d": (c_int, [c_void_p, c_size_t, c_void_p, c_int, c_void_p, c_size_t, c_size_t, c_void_p]),
     "lyraq_load_lora": (c_int, [c_void_p, c_void_p, c_int, c_float, c_size_t, c_void_p]),
     "lyraq_gate_residual": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_size_t, c_size_t, c_size_t, c_void_p]),
+    "lyraq_block_means": (c_int, [c_void_p, c_void_p, c_int, c_size_t, c_size_t, c_size_t, c_void_p, c_int, c_int, c_size_t, c_size_t, c_int,
+                                  c_int, c_void_p]),
+    "lyraq_select_blocks": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
+    "lyraq_select_blocks_workspace": (c_size_t, [c_size_t, c_int, c_size_t, c_size_t, c_int]),
+    "lyraq_sparse_attention": (c_int, [c_void_p, c_void_p]),
     "lyraq_rope_axes": (c_int, [c_void_p, c_void_p]),
     "lyraq_gated_residual_norm": (c_int, [c_void_p, c_void_p]),
     "lyraq_gemm_w4a4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p,
@@ -163,6 +183,7 @@ def host():
         handle = lib()
         names = ("lyraq_gated_residual_norm", "lyraq_rope_axes", "lyraq_linear_fp4_forward", "lyraq_gemm_fp4", "lyraq_quant_fp4",
                  "lyraq_linear_fp8_block_forward", "lyraq_gemm_fp8_block", "lyraq_quant_fp8_block",
+                 "lyraq_block_means", "lyraq_select_blocks", "lyraq_select_blocks_workspace", "lyraq_sparse_attention",
                  "lyraq_workspace_bytes", "lyraq_fp4_scale_bytes")
         module.bind({n: ctypes.cast(getattr(handle, n), c_void_p).value for n in names}, LyraqError)
         _host = module

@@ -32,6 +32,10 @@ decltype(&lyraq_quant_fp4)           g_quant_fp4   = nullptr;
 decltype(&lyraq_linear_fp8_block_forward) g_linear_fp8_block = nullptr;
 decltype(&lyraq_gemm_fp8_block)      g_gemm_fp8_block  = nullptr;
 decltype(&lyraq_quant_fp8_block)     g_quant_fp8_block = nullptr;
+decltype(&lyraq_block_means)         g_block_means  = nullptr;
+decltype(&lyraq_select_blocks)       g_select       = nullptr;
+decltype(&lyraq_select_blocks_workspace) g_select_ws = nullptr;
+decltype(&lyraq_sparse_attention)    g_sparse       = nullptr;
 decltype(&lyraq_workspace_bytes)     g_workspace   = nullptr;
 decltype(&lyraq_fp4_scale_bytes)     g_scale_bytes = nullptr;
 PyObject*                            g_error       = nullptr;   // LyraqError(status, where)
@@ -631,6 +635,241 @@ PyObject* quant_fp4(PyObject* const* a)
     Py_RETURN_NONE;
 }
 
+// ------------------------------------------------------------------------------- attention over selected key blocks
+size_t step_of(const Tensor& t, int64_t d) { return t.size(d) > 1 ? (size_t)t.stride(d) : 0; }   // of a dimension of one: anything
+
+// int32 [batch] or None
+const int* per_sequence(PyObject* o, const char* what, int64_t batch, int dev)
+{
+    const Tensor* t = tensor(o, what, dev);
+    if (t != nullptr && (t->scalar_type() != at::kInt || t->dim() != 1 || t->size(0) != batch)) {
+        refuse(PyExc_ValueError, "%s must be int32 [%lld]", what, (long long)batch);
+    }
+    return (const int*)at_contiguous(t, what);
+}
+
+// q, k, v or out: [batch, tokens, heads, head_dim] with contiguous heads
+const Tensor& tokens_of(const Tensor& t, const char* what)
+{
+    if (t.dim() != 4) {
+        refuse(PyExc_ValueError, "%s must be [batch, tokens, heads, head_dim]", what);
+    }
+    if (t.scalar_type() != at::kHalf && t.scalar_type() != at::kBFloat16) {
+        refuse(PyExc_TypeError, "%s: unsupported dtype %s", what, c10::toString(t.scalar_type()));
+    }
+    if (t.size(3) > 1 && t.stride(3) != 1) {
+        refuse(PyExc_ValueError, "%s: heads must be contiguous", what);
+    }
+    return t;
+}
+
+int as_block(PyObject* o)
+{
+    const int block = as_size(as_long(o), "the block");
+    if (block == 0) {
+        refuse(PyExc_ValueError, "a block has one token or more");
+    }
+    return block;
+}
+
+int64_t blocks_of(int64_t n, int block) { return (n + block - 1) / block; }
+
+constexpr int kQueryBlock = 128;
+
+// Means of the blocks of x, into `out` or a new tensor.
+Tensor means_of(const Tensor& x, int block, const int* lens, const Tensor* out, int newest, int dev)
+{
+    const int64_t batch = x.size(0), tokens = x.size(1), heads = x.size(2), dim = x.size(3), blocks = blocks_of(tokens, block);
+    Tensor        made;
+    if (out == nullptr) {
+        made = empty_like_cuda({batch, heads, blocks, dim}, at::kFloat, dev);
+    } else {
+        if (out->scalar_type() != at::kFloat || out->sizes() != at::IntArrayRef({batch, heads, blocks, dim})) {
+            refuse(PyExc_ValueError, "the means must be fp32 [%lld, %lld, %lld, %lld]", (long long)batch, (long long)heads, (long long)blocks, (long long)dim);
+        }
+        made = *out;
+    }
+    float* p = (float*)at_contiguous(&made, "the means");
+    check_status(run(g_block_means, p, x.data_ptr(), dtype_code(x, "x"), step_of(x, 0), step_of(x, 1), step_of(x, 2), lens, block, newest, (size_t)batch,
+                     (size_t)tokens, as_size(heads, "the number of heads"), as_size(dim, "head_dim"), current_stream()),
+                 "lyraq_block_means");
+    return made;
+}
+
+// (x, block, lens, out, newest) -> means
+PyObject* block_means(PyObject* const* a)
+{
+    const int     dev  = c10::cuda::current_device();
+    const Tensor& x    = tokens_of(needed(a[0], "x", dev), "x");
+    const int*    lens = per_sequence(a[2], "lens", x.size(0), dev);
+    const Tensor* out  = tensor(a[3], "out", dev);
+    const int     n    = as_size(as_long(a[4]), "newest");
+    if (n > 0 && out == nullptr) {
+        refuse(PyExc_ValueError, "the newest tokens' blocks are written into means that are there (out)");
+    }
+    const Tensor means = means_of(x, as_block(a[1]), lens, out, n, dev);
+    return result(a[3], means);
+}
+
+struct Choice {
+    int  block, count, sink, window;
+    bool shared, causal;
+};
+Choice choice_of(PyObject* const* a)     // block, count, sink, window, shared, causal
+{
+    Choice c{as_block(a[0]), as_size(as_long(a[1]), "count"), as_size(as_long(a[2]), "sink"), as_size(as_long(a[3]), "window"), PyObject_IsTrue(a[4]) == 1,
+             PyObject_IsTrue(a[5]) == 1};
+    if (c.count == 0) {
+        refuse(PyExc_ValueError, "count must be positive");
+    }
+    return c;
+}
+
+std::pair<Tensor, Tensor> select_of(const Tensor& qm, const Tensor& km, const Choice& c, int64_t queries, int64_t keys, const int* k_lens, const int* q_start, int dev)
+{
+    const int64_t batch = qm.size(0), heads = qm.size(1), dim = qm.size(3), k_heads = km.size(1), q_blocks = blocks_of(queries, kQueryBlock);
+    if (k_heads == 0 || heads % k_heads != 0) {
+        refuse(PyExc_ValueError, "the query heads must be a multiple of the key heads");
+    }
+    const int64_t lists  = c.shared ? k_heads : heads;
+    const Tensor  index  = empty_like_cuda({batch, lists, q_blocks, c.count}, at::kInt, dev);
+    const Tensor  counts = empty_like_cuda({batch, lists, q_blocks}, at::kInt, dev);
+    const size_t  need   = g_select_ws((size_t)batch, (int)lists, (size_t)queries, (size_t)keys, c.block);
+    const Tensor  ws     = empty_like_cuda({(int64_t)need}, at::kByte, dev);
+    lyraq_select_blocks_t s{};
+    s.q_means  = (const float*)at_contiguous(&qm, "q_means");
+    s.k_means  = (const float*)at_contiguous(&km, "k_means");
+    s.index    = (int*)index.data_ptr();
+    s.counts   = (int*)counts.data_ptr();
+    s.k_lens   = k_lens;
+    s.q_start  = q_start;
+    s.batch    = (size_t)batch;
+    s.queries  = (size_t)queries;
+    s.keys     = (size_t)keys;
+    s.q_heads  = as_size(heads, "the number of heads");
+    s.k_heads  = as_size(k_heads, "the number of heads");
+    s.lists    = (int)lists;
+    s.head_dim = as_size(dim, "head_dim");
+    s.block    = c.block;
+    s.count    = c.count;
+    s.sink     = c.sink;
+    s.window   = c.window;
+    s.causal   = c.causal;
+    check_status(run(g_select, &s, ws.data_ptr(), need, current_stream()), "lyraq_select_blocks");
+    return {index, counts};
+}
+
+// (q_means, k_means, block, count, sink, window, shared, causal, queries, keys, k_lens, q_start) -> (index, counts)
+PyObject* select_blocks(PyObject* const* a)
+{
+    const int     dev = c10::cuda::current_device();
+    const Tensor& qm  = needed(a[0], "q_means", dev);
+    const Tensor& km  = needed(a[1], "k_means", dev);
+    const Choice  c   = choice_of(a + 2);
+    const int64_t queries = as_size(as_long(a[8]), "queries"), keys = as_size(as_long(a[9]), "keys");
+    if (qm.dim() != 4 || km.dim() != 4 || qm.scalar_type() != at::kFloat || km.scalar_type() != at::kFloat || qm.size(2) != blocks_of(queries, kQueryBlock) ||
+        km.size(2) != blocks_of(keys, c.block) || km.size(0) != qm.size(0) || km.size(3) != qm.size(3)) {
+        refuse(PyExc_ValueError, "expected q_means fp32 [batch, heads, %lld, head_dim] and k_means [batch, key heads, %lld, head_dim]",
+               (long long)blocks_of(queries, kQueryBlock), (long long)blocks_of(keys, c.block));
+    }
+    const auto s = select_of(qm, km, c, queries, keys, per_sequence(a[10], "k_lens", qm.size(0), dev), per_sequence(a[11], "q_start", qm.size(0), dev), dev);
+    return Py_BuildValue("(NN)", THPVariable_Wrap(s.first), THPVariable_Wrap(s.second));
+}
+
+void check_qkv(const Tensor& q, const Tensor& k, const Tensor& v)
+{
+    if (k.sizes() != v.sizes() || k.size(0) != q.size(0) || k.size(3) != q.size(3) || k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type()) {
+        refuse(PyExc_ValueError, "k and v must be [%lld, keys, heads, %lld] of q's dtype", (long long)q.size(0), (long long)q.size(3));
+    }
+    if (k.size(2) == 0 || q.size(2) % k.size(2) != 0) {
+        refuse(PyExc_ValueError, "the query heads must be a multiple of the key heads");
+    }
+}
+
+Tensor attend(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& index, const Tensor& counts, int block, const int* k_lens, const int* q_start, bool causal,
+              float scale, const Tensor* out, int dev)
+{
+    const int64_t batch = q.size(0), queries = q.size(1), heads = q.size(2), dim = q.size(3), k_heads = k.size(2), q_blocks = blocks_of(queries, kQueryBlock);
+    if (index.scalar_type() != at::kInt || index.dim() != 4 || index.size(0) != batch || (index.size(1) != heads && index.size(1) != k_heads) ||
+        index.size(2) != q_blocks) {
+        refuse(PyExc_ValueError, "index must be int32 [%lld, %lld or %lld, %lld, count]", (long long)batch, (long long)heads, (long long)k_heads, (long long)q_blocks);
+    }
+    if (counts.scalar_type() != at::kInt || counts.sizes() != index.sizes().slice(0, 3)) {
+        refuse(PyExc_ValueError, "counts must be int32 of index's first three dimensions");
+    }
+    Tensor made;
+    if (out == nullptr) {
+        made = empty_like_cuda(q.sizes(), q.scalar_type(), dev);
+    } else {
+        if (tokens_of(*out, "out").sizes() != q.sizes() || out->scalar_type() != q.scalar_type()) {
+            refuse(PyExc_ValueError, "out must have q's shape and dtype");
+        }
+        if (!out->is_contiguous() && overlaps(*out)) {
+            refuse(PyExc_ValueError, "out has overlapping elements");
+        }
+        made = *out;
+    }
+    lyraq_sparse_attention_t s{};
+    s.q = q.data_ptr(); s.k = k.data_ptr(); s.v = v.data_ptr(); s.out = made.data_ptr();
+    s.q_batch = step_of(q, 0); s.q_token = step_of(q, 1); s.q_head = step_of(q, 2);
+    s.k_batch = step_of(k, 0); s.k_token = step_of(k, 1); s.k_head = step_of(k, 2);
+    s.v_batch = step_of(v, 0); s.v_token = step_of(v, 1); s.v_head = step_of(v, 2);
+    s.o_batch = step_of(made, 0); s.o_token = step_of(made, 1); s.o_head = step_of(made, 2);
+    s.index    = (const int*)at_contiguous(&index, "index");
+    s.counts   = (const int*)at_contiguous(&counts, "counts");
+    s.k_lens   = k_lens;
+    s.q_start  = q_start;
+    s.batch    = (size_t)batch;
+    s.queries  = (size_t)queries;
+    s.keys     = (size_t)k.size(1);
+    s.q_heads  = as_size(heads, "the number of heads");
+    s.k_heads  = as_size(k_heads, "the number of heads");
+    s.lists    = as_size(index.size(1), "the number of lists");
+    s.head_dim = as_size(dim, "head_dim");
+    s.block    = block;
+    s.count    = as_size(index.size(3), "count");
+    s.causal   = causal;
+    s.softmax_scale = scale;
+    s.dtype    = dtype_code(q, "q");
+    check_status(run(g_sparse, &s, current_stream()), "lyraq_sparse_attention");
+    return made;
+}
+
+// (q, k, v, index, counts, block, k_lens, q_start, causal, softmax scale, out) -> out
+PyObject* sparse_attention(PyObject* const* a)
+{
+    const int     dev = c10::cuda::current_device();
+    const Tensor& q = tokens_of(needed(a[0], "q", dev), "q");
+    const Tensor& k = tokens_of(needed(a[1], "k", dev), "k");
+    const Tensor& v = tokens_of(needed(a[2], "v", dev), "v");
+    check_qkv(q, k, v);
+    const Tensor out = attend(q, k, v, needed(a[3], "index", dev), needed(a[4], "counts", dev), as_block(a[5]), per_sequence(a[6], "k_lens", q.size(0), dev),
+                              per_sequence(a[7], "q_start", q.size(0), dev), PyObject_IsTrue(a[8]) == 1, as_float(a[9]), tensor(a[10], "out", dev), dev);
+    return result(a[10], out);
+}
+
+// (q, k, v, block, count, sink, window, shared, causal, softmax scale, k_lens, q_start, k_means, out) -> (out, index, counts): means, selection and attention
+PyObject* select_and_attend(PyObject* const* a)
+{
+    const int     dev = c10::cuda::current_device();
+    const Tensor& q = tokens_of(needed(a[0], "q", dev), "q");
+    const Tensor& k = tokens_of(needed(a[1], "k", dev), "k");
+    const Tensor& v = tokens_of(needed(a[2], "v", dev), "v");
+    check_qkv(q, k, v);
+    const Choice  c       = choice_of(a + 3);
+    const int*    k_lens  = per_sequence(a[10], "k_lens", q.size(0), dev);
+    const int*    q_start = per_sequence(a[11], "q_start", q.size(0), dev);
+    const Tensor* given   = tensor(a[12], "k_means", dev);
+    if (given != nullptr && (given->scalar_type() != at::kFloat || given->sizes() != at::IntArrayRef({k.size(0), k.size(2), blocks_of(k.size(1), c.block), k.size(3)}))) {
+        refuse(PyExc_ValueError, "k_means must be fp32 [batch, key heads, %lld, head_dim]", (long long)blocks_of(k.size(1), c.block));
+    }
+    const Tensor qm = means_of(q, kQueryBlock, nullptr, nullptr, 0, dev);
+    const Tensor km = given != nullptr ? *given : means_of(k, c.block, k_lens, nullptr, 0, dev);
+    const auto   s  = select_of(qm, km, c, q.size(1), k.size(1), k_lens, q_start, dev);
+    const Tensor out = attend(q, k, v, s.first, s.second, c.block, k_lens, q_start, c.causal, as_float(a[9]), tensor(a[13], "out", dev), dev);
+    return Py_BuildValue("(NNN)", result(a[13], out), THPVariable_Wrap(s.first), THPVariable_Wrap(s.second));
+}
+
 template<PyObject* (*F)(PyObject* const*), Py_ssize_t COUNT> PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n)
 {
     HANDLE_TH_ERRORS
@@ -669,7 +908,8 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n)
     if (!take("lyraq_gated_residual_norm", g_norm) || !take("lyraq_rope_axes", g_rope) || !take("lyraq_linear_fp4_forward", g_linear_fp4) ||
         !take("lyraq_gemm_fp4", g_gemm_fp4) || !take("lyraq_quant_fp4", g_quant_fp4) || !take("lyraq_workspace_bytes", g_workspace) ||
         !take("lyraq_linear_fp8_block_forward", g_linear_fp8_block) || !take("lyraq_gemm_fp8_block", g_gemm_fp8_block) ||
-        !take("lyraq_quant_fp8_block", g_quant_fp8_block) || !take("lyraq_fp4_scale_bytes", g_scale_bytes)) {
+        !take("lyraq_quant_fp8_block", g_quant_fp8_block) || !take("lyraq_block_means", g_block_means) || !take("lyraq_select_blocks", g_select) ||
+        !take("lyraq_select_blocks_workspace", g_select_ws) || !take("lyraq_sparse_attention", g_sparse) || !take("lyraq_fp4_scale_bytes", g_scale_bytes)) {
         return nullptr;
     }
     Py_XSETREF(g_error, Py_NewRef(args[1]));
@@ -685,6 +925,10 @@ PyMethodDef g_methods[] = {
     {"linear_fp8_block", (PyCFunction)(void (*)())call<linear_fp8_block, 10>, METH_FASTCALL, nullptr},
     {"gemm_fp8_block", (PyCFunction)(void (*)())call<gemm_fp8_block, 9>, METH_FASTCALL, nullptr},
     {"quant_fp8_block", (PyCFunction)(void (*)())call<quant_fp8_block, 3>, METH_FASTCALL, nullptr},
+    {"block_means", (PyCFunction)(void (*)())call<block_means, 5>, METH_FASTCALL, nullptr},
+    {"select_blocks", (PyCFunction)(void (*)())call<select_blocks, 12>, METH_FASTCALL, nullptr},
+    {"sparse_attention", (PyCFunction)(void (*)())call<sparse_attention, 11>, METH_FASTCALL, nullptr},
+    {"select_and_attend", (PyCFunction)(void (*)())call<select_and_attend, 14>, METH_FASTCALL, nullptr},
     {"fp4_empty", (PyCFunction)(void (*)())call<fp4_empty, 4>, METH_FASTCALL, nullptr},
     {"quant_fp4", (PyCFunction)(void (*)())call<quant_fp4, 5>, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},

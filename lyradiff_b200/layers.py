@@ -125,6 +125,25 @@ class Fp8BlockLinear:
         return _lib.host().linear_fp8_block(x, self.codes, self.scales, self.n, self.k, self.bias, residual, beta, self.epilogue, out)
 
 
+class SparseAttention:
+    """Attention in which every 128 queries go to `count` blocks of `block` keys (64 or 128), chosen by the products of the blocks' means
+    (ops.select_blocks; sink, window, shared and causal as there): for long sequences, where ops.flash_attention would read all keys.  Lists and means live
+    in memory taken from torch's allocator per call.  The reference's attention is dense."""
+
+    def __init__(self, block, count, sink=0, window=0, shared=False, causal=False, softmax_scale=None):
+        if block not in (64, 128) or count < 1 or sink < 0 or window < 0:
+            raise ValueError("expected blocks of 64 or 128 keys, count of 1 or more, sink and window of 0 or more")
+        self.block, self.count, self.sink, self.window, self.shared, self.causal, self.softmax_scale = block, count, sink, window, shared, causal, softmax_scale
+
+    def forward(self, q, k, v, k_lens=None, q_start=None, k_means=None, out=None, with_selection=False):
+        """q [batch, queries, heads, head_dim], k and v [batch, keys, key heads, head_dim], f16 or bf16, any steps with contiguous heads -> like q.
+        k_means: ops.block_means(k, block, lens=k_lens), where a cache keeps them up to date.  with_selection: (out, index, counts)."""
+        scale = self.softmax_scale if self.softmax_scale is not None else float(q.shape[-1]) ** -0.5
+        got = _lib.host().select_and_attend(q, k, v, self.block, self.count, self.sink, self.window, self.shared, self.causal, scale, k_lens, q_start, k_means,
+                                            out)
+        return got if with_selection else got[0]
+
+
 class SmoothQuantLinear:
     """INT8 SmoothQuant W8A8 linear of the SDXL INT8 block: int8 weight + per-channel scale + smoothing vector
     (.weight_int8 / .weight_quant_scale / .pre_quant_scale / .input_quant_scale,
