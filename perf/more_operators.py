@@ -198,6 +198,8 @@ def prepare(case, seed):
     s = _inputs(case, seed)
     if own:
         from lyradiff_b200.layers import Fp8BlockLinear, SparseAttention
+        if "k_means" in s:
+            s["k_means"] = s["k_means"].contiguous()   # as ops.block_means returns them
         if case["kind"] == "linear":
             s["layer"] = Fp8BlockLinear.from_float(s["w"], s["bias"], gelu=case["gelu"])
         elif case["kind"] == "sparse":
