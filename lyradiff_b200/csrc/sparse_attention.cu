@@ -1,17 +1,25 @@
 // Block-sparse attention forward: out[b, i, h, :] = softmax over the keys of the blocks listed for query block i / 128 of (q k^T scale) v.
 //
-// The kernel of attention.cu with lists: a CTA runs two query tiles of 128 rows, which share the tensor pipe and the exponent unit but nothing else,
-// since each has its own list.  So each has its own producer, issuer and part of shared memory, and takes its own query blocks in turn:
-//   warps 8, 10  TMA producers of tile 0, 1: per query block Q, then K and V of each step of 128 keys (two listed blocks of 64, or one of 128), as
-//                boxes of 64 keys x 64 columns.  One buffer for K (free as soon as the scores are there, needed when P V of the step is under way) and
-//                a ring of half steps for V.
-//   warps 9, 11  MMA issuers: S = Q K^T (M 128, N 128), O += P V, P read from tensor memory, in two halves of 64 keys
+// The kernel of attention.cu with lists: a CTA runs two query tiles of 128 rows, which share the tensor pipe and the exponent unit but no operand,
+// since each has its own list.  So each has its own producer and part of shared memory, and takes its own query blocks ("items") in turn:
+//   warps 8, 10  TMA producers of tile 0, 1.  They find each item's list and length and tell the other roles through a ring of two; then Q, and K and V
+//                of each step of 128 keys (two listed blocks of 64, or one of 128), as boxes of 64 keys x 64 columns.  One buffer for K (free as soon as
+//                the scores are there, needed when P V of the step is under way) and a ring of half steps for V.
+//   warp 9       MMA issuer of both tiles, a step of each in turn: O += P V (P from tensor memory, in two halves of 64 keys), then the next step's
+//                S = Q K^T over it
 //   warps 0-3    softmax and epilogue of tile 0, warps 4-7 of tile 1: a thread owns one query row.  Keys of a half step that a row does not see are a
 //                tail of it (beyond the keys, or behind the row's place), so a mask is one number.
-// K V of a step are 64 KB for one tile where the dense kernel reads them once for two: 43 bytes a clock and SM out of L2 at its pace.
 // V rows beyond a sequence's keys may hold anything: the softmax warps clear them in shared memory, since 0 * NaN is NaN.
 // Every wait is bounded; on a timeout the role records it in the status word, raises the block's abort flag and all roles leave; tensor
 // memory is freed at the common exit.
+//
+// What bounds it (32760 tokens, 12 heads of 128, 64 of 512 blocks: 98304 steps of one tile, 824 GFLOP): the chain of a tile's softmax and MMAs, as in
+// the dense kernel; a step of both tiles is 2048 clocks of tensor pipe, 1792 of the exponent unit, 3500 measured for long lists, 2.1 us (the dense
+// kernel, which reads K and V once for two tiles: 1.8), and an item costs 3 us beside its steps.  K and V of a step are 64 KB for one tile; without the loads it takes the same time.
+// Measured, the clip: 908 us with an issuer for each tile (their instructions mix on the pipe and both products end late) -> 759 with one -> 745 with
+// items handed over and keys looked up only where a mask may be (a look at each step's keys by the softmax warps: 6 to 12 %).
+// Not kept: an epilogue in warps of its own, which wait for either tile (their polling and the registers they take from the softmax: 848 to 1030 us); items found by a
+// warp of their own (the same time); a quarter of the exponentials on the FMA pipe (2 % slower than an eighth).
 #include "sparse_attention.cuh"
 #include "sm100_ptx.cuh"
 
@@ -35,10 +43,11 @@ constexpr int kTile    = 128;                       // rows of a query tile, key
 constexpr int kHalf    = 64;
 constexpr int kTiles   = 2;
 constexpr int kThreads = 384;
-constexpr int kRole0   = 8;                         // warps 8 .. 11
+constexpr int kRole0   = 8;                         // warps 8 and 10 producers, 9 issuer
 // registers: 384 threads x 168 at launch = 64512 = 256 x 216 + 128 x 72
 constexpr int kSoftmaxRegs = 216;
 constexpr int kOtherRegs   = 72;
+constexpr int kInfos       = 2;                     // items a producer may be ahead with
 constexpr float kRescaleThreshold = 8.0f;           // in log2 units
 constexpr int kPolyPairs = 2;                       // of 16 pairs of scores, how many take their exponentials from the FMA pipe
 
@@ -54,8 +63,12 @@ template<int D> struct Smem {
     static constexpr int kKOffset = kQBytes;
     static constexpr int kVOffset = kKOffset + kKSlots * kKBytes;
     static constexpr int kPerTile = kVOffset + kVSlots * kVBytes;
-    static constexpr int kBars    = 2 + 2 * kKSlots + 2 * kVSlots + 4;   // of a tile
-    static constexpr int kBarOffset = kTiles * kPerTile;
+    // barriers of a tile, by number
+    static constexpr int kQFull = 0, kQEmpty = 1, kSFull = 2, kPHalf = 3, kOFull = 5, kInfoFull = 6,
+                         kInfoEmpty = kInfoFull + kInfos, kKFull = kInfoEmpty + kInfos, kKEmpty = kKFull + kKSlots, kVFull = kKEmpty + kKSlots,
+                         kVEmpty = kVFull + kVSlots, kBars = kVEmpty + kVSlots;
+    static constexpr int kInfoOffset = kTiles * kPerTile;
+    static constexpr int kBarOffset  = kInfoOffset + kTiles * kInfos * 48;
     static constexpr int kUsed    = kBarOffset + 8 * kBars * kTiles + 16;
     static constexpr int kTotal   = kUsed + 1024;                 // + alignment slack
     static_assert(kTotal <= 232448 && kPerTile % 1024 == 0, "");
@@ -69,12 +82,15 @@ __device__ __forceinline__ void tma_load_4d(uint32_t smem_dst, const CUtensorMap
         : "memory");
 }
 
-// The work of one tile: query block `qb` of head `h` of sequence `b`, and its list.
-struct Item {
-    int        qb, h, b;
-    const int* list;
-    int        entries;
+// What a producer tells the other roles of an item: query block `qb` of head `h` of sequence `b`, its steps (-1: no item any more), the row of its list, how
+// much of the list counts, the keys that exist, the last key its row 0 sees, the first step in which a row may miss a key, the first keys of the
+// halves of its first step.
+struct alignas(16) Info {
+    int qb, h, b, steps;
+    int list, entries, len, place;
+    int masked, key[2], spare;
 };
+static_assert(sizeof(Info) == 48, "");
 
 template<typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -85,17 +101,8 @@ sparse_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t*       gen_base  = smem_raw + (smem_base - smem_u32(smem_raw));
-    auto bar       = [&](int t, int i) { return smem_base + S::kBarOffset + 8u * (uint32_t)(t * S::kBars + i); };
-    auto q_full    = [&](int t) { return bar(t, 0); };
-    auto q_empty   = [&](int t) { return bar(t, 1); };
-    auto s_full    = [&](int t) { return bar(t, 2); };    // scores of a step
-    auto p_first   = [&](int t) { return bar(t, 3); };    // P of the step's keys 0 .. 63 is in tensor memory
-    auto p_second  = [&](int t) { return bar(t, 4); };    // ... and of keys 64 .. 127
-    auto o_full    = [&](int t) { return bar(t, 5); };    // accumulator of a query block is final
-    auto k_full    = [&](int t, int s) { return bar(t, 6 + s); };
-    auto k_empty   = [&](int t, int s) { return bar(t, 6 + S::kKSlots + s); };
-    auto v_full    = [&](int t, int s) { return bar(t, 6 + 2 * S::kKSlots + s); };
-    auto v_empty   = [&](int t, int s) { return bar(t, 6 + 2 * S::kKSlots + S::kVSlots + s); };
+    auto bars_of = [&](int t) { return smem_base + S::kBarOffset + 8u * (uint32_t)(t * S::kBars); };
+    auto info_of = [&](int t, int slot) { return reinterpret_cast<Info*>(gen_base + S::kInfoOffset) + t * kInfos + slot; };
     uint32_t*     tmem_slot  = reinterpret_cast<uint32_t*>(gen_base + S::kBarOffset + 8 * S::kBars * kTiles);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -106,7 +113,9 @@ sparse_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     if (threadIdx.x == 0) {
         for (int t = 0; t < kTiles; ++t) {
             for (int i = 0; i < S::kBars; ++i) {
-                mbar_init(bar(t, i), i == 3 || i == 4 ? 4u : 1u);   // P comes from four warps
+                // P comes from four warps, "item taken" from these and the issuer
+                const bool four = i == S::kPHalf || i == S::kPHalf + 1, five = i >= S::kInfoEmpty && i < S::kInfoEmpty + kInfos;
+                mbar_init(bars_of(t) + 8u * (uint32_t)i, four ? 4u : five ? 5u : 1u);
             }
         }
         *abort_flag = 0;
@@ -129,80 +138,112 @@ sparse_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         report_timeout(p.status, code);
         *abort_flag = 1;
     };
-    // tile 0 of every CTA first: few items spread over all SMs
-    auto item_of = [&](int i) {
-        Item it;
-        it.qb      = i % p.q_blocks;
-        it.h       = i / p.q_blocks % p.q_heads;
-        it.b       = i / (p.q_blocks * p.q_heads);
-        const size_t row = ((size_t)it.b * (size_t)p.lists + (size_t)(it.h / (p.q_heads / p.lists))) * (size_t)p.q_blocks + (size_t)it.qb;
-        it.list    = p.index + row * (size_t)p.count;
-        it.entries = min(max(load_int(p.counts + row), 0), p.count);
-        return it;
+    auto wait = [&](uint32_t b, uint32_t parity, unsigned code) {
+        const bool ok = mbar_wait_warp(b, parity, abort_flag, p.wait_limit_ns);
+        if (!ok) {
+            give_up(code);
+        }
+        return ok;
     };
-    auto steps_of = [&](const Item& it) { return p.block == kTile ? it.entries : (it.entries + 1) / 2; };
-    // first key of half s of step i, or `keys` where there is none: a box there is filled with zeros and its keys are masked
-    auto key_of = [&](const Item& it, int i, int s) {
+    // first key of half s of step i of a list, or `keys` where there is none: a box there is filled with zeros and its keys are masked
+    auto key_of = [&](int list, int entries, int i, int s) {
         const int e = p.block == kTile ? i : 2 * i + s;
-        if (e >= it.entries) {
+        if (e >= entries) {
             return p.keys;
         }
-        const int j = load_int(it.list + e);
+        const int j = load_int(p.index + (size_t)list * (size_t)p.count + (size_t)e);
         return j >= 0 && j <= (p.keys - 1) / p.block ? min(j * p.block + (p.block == kTile ? s * kHalf : 0), p.keys) : p.keys;
     };
-    const int t     = warp < kRole0 ? warp >> 2 : (warp - kRole0) >> 1;
-    const int first = (int)blockIdx.x + t * (int)gridDim.x, stride = kTiles * (int)gridDim.x;
-    const uint32_t tile_smem = smem_base + (uint32_t)(t * S::kPerTile);
 
     if (warp >= kRole0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-        if (((warp - kRole0) & 1) == 0) {
+        if ((warp & 1) == 0) {
             // -------------------------------------------------------------- TMA producer
-            int      k_slot = 0, v_slot = 0, k_issued = 0, v_issued = 0, q_issued = 0;
+            const int      t    = (warp - kRole0) >> 1;
+            const uint32_t bars = bars_of(t), smem = smem_base + (uint32_t)(t * S::kPerTile);
+            int      k_slot = 0, v_slot = 0, k_issued = 0, v_issued = 0, q_issued = 0, infos = 0;
             uint32_t k_phase = 0, v_phase = 0;
-            bool     ok = true;
-            auto wait_for = [&](uint32_t b, uint32_t parity, unsigned code) {
-                if (!mbar_wait_warp(b, parity, abort_flag, p.wait_limit_ns)) {
-                    give_up(code);
-                    ok = false;
+            bool     ok = p.skip_loads == 0;
+            // tile 0 of every CTA first: few items spread over all SMs
+            auto look = [&](int i) {
+                Info it{0, 0, 0, -1, 0, 0, 0, 0, 0, {p.keys, p.keys}, 0};
+                if (i < p.items) {
+                    it.qb      = i % p.q_blocks;
+                    it.h       = i / p.q_blocks % p.q_heads;
+                    it.b       = i / (p.q_blocks * p.q_heads);
+                    it.list    = (it.b * p.lists + it.h / (p.q_heads / p.lists)) * p.q_blocks + it.qb;
+                    it.entries = min(max(load_int(p.counts + it.list), 0), p.count);
+                    it.steps   = p.block == kTile ? it.entries : (it.entries + 1) / 2;
+                    it.len     = key_count(p, it.b);
+                    it.place   = p.causal ? (int)min((long long)first_place(p, it.b) + it.qb * kTile, (long long)kMaxKeys) : p.keys;
+                    // The lists as select_blocks leaves them ascend, so blocks that end behind the keys or a row's place are at their end; the softmax warps
+                    // look at no list before the first of them (a look at each step's keys there took 6 to 12 % of the time).
+                    const int least = min(it.len, p.causal ? it.place + 1 : it.len);     // keys that row 0 sees
+                    int       first = it.entries;
+                    for (int e = lane; e < it.entries; e += 32) {
+                        const int j = load_int(p.index + (size_t)it.list * (size_t)p.count + (size_t)e);
+                        if (j < 0 || j >= least / p.block) {
+                            first = min(first, e);
+                        }
+                    }
+                    first     = __reduce_min_sync(0xffffffffu, first);
+                    it.masked = p.block == kTile ? first : first / 2;
+                    it.key[0] = key_of(it.list, it.entries, 0, 0);
+                    it.key[1] = key_of(it.list, it.entries, 0, 1);
                 }
-                return ok;
+                return it;
             };
-            for (int i = first; ok && i < p.items && p.skip_loads == 0; i += stride) {
-                const Item it    = item_of(i);
-                const int  steps = steps_of(it), kh = it.h / (p.q_heads / p.k_heads);
-                if (steps == 0) {
-                    continue;
-                }
-                if (!wait_for(q_empty(t), (uint32_t)(q_issued & 1) ^ 1u, 0x8110u)) {
+            const int stride = kTiles * (int)gridDim.x;
+            int       i      = (int)blockIdx.x + t * (int)gridDim.x;
+            Info      it     = look(i);
+            while (ok) {
+                const int slot = infos % kInfos;
+                if (!(ok = wait(bars + 8u * (S::kInfoEmpty + slot), (uint32_t)(infos / kInfos & 1) ^ 1u, 0x8130u))) {
                     break;
                 }
+                if (lane == 0) {
+                    *info_of(t, slot) = it;
+                    mbar_arrive(bars + 8u * (S::kInfoFull + slot));
+                }
+                ++infos;
+                if (it.steps < 0) {
+                    break;
+                }
+                i += stride;
+                if (it.steps == 0) {
+                    it = look(i);
+                    continue;
+                }
+                if (!(ok = wait(bars + 8u * S::kQEmpty, (uint32_t)(q_issued & 1) ^ 1u, 0x8110u))) {
+                    break;
+                }
+                const int kh = it.h / (p.q_heads / p.k_heads);
                 if (elect_one()) {
-                    mbar_arrive_expect_tx(q_full(t), (uint32_t)S::kQBytes);
+                    mbar_arrive_expect_tx(bars + 8u * S::kQFull, (uint32_t)S::kQBytes);
 #pragma unroll
                     for (int c = 0; c < S::kPanels; ++c) {
-                        tma_load_4d(tile_smem + c * S::kPanelQ, &tmap_q, q_full(t), c * 64, it.qb * kTile, it.h, (p.fixed & 1) != 0 ? 0 : it.b);
+                        tma_load_4d(smem + c * S::kPanelQ, &tmap_q, bars + 8u * S::kQFull, c * 64, it.qb * kTile, it.h, (p.fixed & 1) != 0 ? 0 : it.b);
                     }
                 }
                 ++q_issued;
-                int key[2] = {key_of(it, 0, 0), key_of(it, 0, 1)};
-                for (int s = 0; ok && s < steps; ++s) {
-                    int next[2] = {p.keys, p.keys};
-                    if (s + 1 < steps) {      // on their way while the buffers are waited for
-                        next[0] = key_of(it, s + 1, 0);
-                        next[1] = key_of(it, s + 1, 1);
+                int key[2] = {it.key[0], it.key[1]};
+                for (int s = 0; ok && s < it.steps; ++s) {
+                    int ahead[2] = {p.keys, p.keys};
+                    if (s + 1 < it.steps) {      // on their way while the buffers are waited for
+                        ahead[0] = key_of(it.list, it.entries, s + 1, 0);
+                        ahead[1] = key_of(it.list, it.entries, s + 1, 1);
                     }
-                    if (!wait_for(k_empty(t, k_slot), k_phase ^ 1u, 0x8100u)) {
+                    if (!(ok = wait(bars + 8u * (S::kKEmpty + k_slot), k_phase ^ 1u, 0x8100u))) {
                         break;
                     }
                     if (elect_one()) {
-                        const uint32_t dst = tile_smem + S::kKOffset + k_slot * S::kKBytes;
-                        mbar_arrive_expect_tx(k_full(t, k_slot), (uint32_t)S::kKBytes);
+                        const uint32_t dst = smem + S::kKOffset + k_slot * S::kKBytes, full = bars + 8u * (S::kKFull + k_slot);
+                        mbar_arrive_expect_tx(full, (uint32_t)S::kKBytes);
 #pragma unroll
                         for (int c = 0; c < S::kPanels; ++c) {
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
-                                tma_load_4d(dst + c * S::kPanelQ + h * S::kPanelV, &tmap_k, k_full(t, k_slot), c * 64, key[h], kh, (p.fixed & 2) != 0 ? 0 : it.b);
+                                tma_load_4d(dst + c * S::kPanelQ + h * S::kPanelV, &tmap_k, full, c * 64, key[h], kh, (p.fixed & 2) != 0 ? 0 : it.b);
                             }
                         }
                     }
@@ -213,15 +254,15 @@ sparse_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                     }
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        if (!ok || !wait_for(v_empty(t, v_slot), v_phase ^ 1u, 0x8120u)) {
+                        if (!ok || !(ok = wait(bars + 8u * (S::kVEmpty + v_slot), v_phase ^ 1u, 0x8120u))) {
                             break;
                         }
                         if (elect_one()) {
-                            const uint32_t dst = tile_smem + S::kVOffset + v_slot * S::kVBytes;
-                            mbar_arrive_expect_tx(v_full(t, v_slot), (uint32_t)S::kVBytes);
+                            const uint32_t dst = smem + S::kVOffset + v_slot * S::kVBytes, full = bars + 8u * (S::kVFull + v_slot);
+                            mbar_arrive_expect_tx(full, (uint32_t)S::kVBytes);
 #pragma unroll
                             for (int c = 0; c < S::kPanels; ++c) {
-                                tma_load_4d(dst + c * S::kPanelV, &tmap_v, v_full(t, v_slot), c * 64, key[h], kh, (p.fixed & 4) != 0 ? 0 : it.b);
+                                tma_load_4d(dst + c * S::kPanelV, &tmap_v, full, c * 64, key[h], kh, (p.fixed & 4) != 0 ? 0 : it.b);
                             }
                         }
                         ++v_issued;
@@ -230,9 +271,10 @@ sparse_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                             v_phase ^= 1u;
                         }
                     }
-                    key[0] = next[0];
-                    key[1] = next[1];
+                    key[0] = ahead[0];
+                    key[1] = ahead[1];
                 }
+                it = look(i);
             }
             // no copy may be in flight when the block leaves: wait (bounded) for the buffers filled last
             auto settle = [&](uint32_t b, uint32_t parity, unsigned code) {
@@ -244,148 +286,224 @@ sparse_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                     }
                 }
             };
-            for (int i = 0; i < S::kKSlots && i < k_issued; ++i) {
+            for (int n = 0; n < S::kKSlots && n < k_issued; ++n) {
                 if (k_slot == 0) {
                     k_slot = S::kKSlots;
                     k_phase ^= 1u;
                 }
                 --k_slot;
-                settle(k_full(t, k_slot), k_phase, 0x8400u);
+                settle(bars + 8u * (S::kKFull + k_slot), k_phase, 0x8400u);
             }
-            for (int i = 0; i < S::kVSlots && i < v_issued; ++i) {
+            for (int n = 0; n < S::kVSlots && n < v_issued; ++n) {
                 if (v_slot == 0) {
                     v_slot = S::kVSlots;
                     v_phase ^= 1u;
                 }
                 --v_slot;
-                settle(v_full(t, v_slot), v_phase, 0x8420u);
+                settle(bars + 8u * (S::kVFull + v_slot), v_phase, 0x8420u);
             }
             if (q_issued > 0) {
-                settle(q_full(t), (uint32_t)((q_issued - 1) & 1), 0x8410u);
+                settle(bars + 8u * S::kQFull, (uint32_t)((q_issued - 1) & 1), 0x8410u);
             }
-        } else {
-            // -------------------------------------------------------------- MMA issuer
+        } else if (warp == kRole0 + 1) {
+            // -------------------------------------------------------------- MMA issuer of both tiles
             constexpr uint32_t kAb = TypeTag<T>::value == LYRAQ_BF16 ? 1u : 0u;
             constexpr uint32_t idesc_qk = umma_idesc(1u, kAb, 128, kTile);
             constexpr uint32_t idesc_pv = umma_idesc(1u, kAb, 128, D) | kIdescBMajorMN;
-            const uint32_t s_acc = tmem_base + (uint32_t)(t * 128), o_acc = tmem_base + (uint32_t)(256 + t * 128);
-            int      k_slot = 0, v_slot = 0;
-            uint32_t k_phase = 0, v_phase = 0, step = 0, taken = 0;
-            bool     ok = true;
+            // One copy of the code serves both tiles in turn, and a wait that runs out is reported behind the loop: what the issuer runs between two
+            // MMAs is fetched anew every time, as the other warps run theirs in between.
+            struct Tile {
+                int      t, steps, step;         // steps of the item under way (0: none yet, -1: no item any more)
+                int      infos, v_slot, k_slot;
+                uint32_t v_phase, k_phase, parity, item_parity;   // parity: of the steps of all items; item_parity: of the items with steps
+            };
+            Tile     c{0, 0, 0, 0, 0, 0, 0u, 0u, 0u, 0u}, other{1, 0, 0, 0, 0, 0, 0u, 0u, 0u, 0u};
+            unsigned bad = 0;
             auto wait_for = [&](uint32_t b, uint32_t parity, unsigned code) {
                 if (!mbar_wait_warp(b, parity, abort_flag, p.wait_limit_ns)) {
-                    give_up(code);
-                    ok = false;
+                    bad = code;
+                    return false;
                 }
-                return ok;
+                return true;
             };
-            // S = Q K^T with the k tile in k_slot
-            auto scores = [&](bool last) {
-                if (!wait_for(k_full(t, k_slot), k_phase, 0x8210u)) {
-                    return;
-                }
-                tc_fence_after_sync();
-                if (elect_one()) {
-                    const uint64_t qdesc = umma_desc_k_sw128(tile_smem);
-                    const uint64_t kdesc = umma_desc_k_sw128(tile_smem + S::kKOffset + k_slot * S::kKBytes);
-#pragma unroll
-                    for (int ks = 0; ks < D / 16; ++ks) {
-                        const uint64_t off = (uint64_t)(((ks >> 2) * S::kPanelQ + (ks & 3) * 32) >> 4);
-                        mma_f16(s_acc, qdesc + off, kdesc + off, idesc_qk, ks > 0 ? 1u : 0u);
-                    }
-                    tc_commit(s_full(t));
-                    tc_commit(k_empty(t, k_slot));
-                    if (last) {
-                        tc_commit(q_empty(t));
-                    }
-                }
-                if (++k_slot == S::kKSlots) {
-                    k_slot = 0;
-                    k_phase ^= 1u;
-                }
-            };
-            for (int i = first; ok && i < p.items; i += stride) {
-                const int steps = steps_of(item_of(i));
-                if (steps == 0) {
-                    continue;
-                }
-                if (!wait_for(q_full(t), taken & 1u, 0x8200u)) {
-                    break;
-                }
-                ++taken;
-                scores(steps == 1);
+            while (bad == 0 && (c.steps >= 0 || other.steps >= 0)) {
+                if (c.steps >= 0) {
+                    const uint32_t smem = smem_base + (uint32_t)(c.t * S::kPerTile), bars = bars_of(c.t);
+                    const uint32_t s_acc = tmem_base + (uint32_t)(c.t * 128), o_acc = tmem_base + (uint32_t)(256 + c.t * 128);
+                    bool           ok = true;
+                    if (c.steps > 0) {
+                        // O += P V of the step
+                        const bool last = c.step + 1 == c.steps;
 #pragma unroll 1
-                for (int s = 0; ok && s < steps; ++s, ++step) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (!ok || !wait_for(v_full(t, v_slot), v_phase, 0x8230u) || !wait_for(h == 0 ? p_first(t) : p_second(t), step & 1u, 0x8240u)) {
-                            break;
-                        }
-                        tc_fence_after_sync();
-                        if (elect_one()) {
-                            const uint64_t vdesc = umma_desc_mn_sw128(tile_smem + S::kVOffset + v_slot * S::kVBytes, (uint32_t)S::kPanelV);
-#pragma unroll
-                            for (int k4 = 0; k4 < 4; ++k4) {   // 16 keys each: 8 columns of P, 2048 bytes of v
-                                mma_f16_ts(o_acc, s_acc + (uint32_t)((4 * h + k4) * 8), vdesc + (uint64_t)(k4 * 128), idesc_pv, s > 0 || h > 0 || k4 > 0 ? 1u : 0u);
+                        for (int h = 0; h < 2 && ok; ++h) {
+                            ok = wait_for(bars + 8u * (uint32_t)(S::kVFull + c.v_slot), c.v_phase, 0x8230u) &&
+                                 wait_for(bars + 8u * (uint32_t)(S::kPHalf + h), c.parity, 0x8240u);
+                            if (!ok) {
+                                break;
                             }
-                            tc_commit(v_empty(t, v_slot));
-                            if (h == 1 && s + 1 == steps) {
-                                tc_commit(o_full(t));
+                            tc_fence_after_sync();
+                            if (elect_one()) {
+                                const uint64_t vdesc = umma_desc_mn_sw128(smem + S::kVOffset + c.v_slot * S::kVBytes, (uint32_t)S::kPanelV);
+                                const uint32_t acc = c.step > 0 || h > 0 ? 1u : 0u, p_in = s_acc + (uint32_t)(h * 32);
+#pragma unroll
+                                for (int k4 = 0; k4 < 4; ++k4) {   // 16 keys each: 8 columns of P, 2048 bytes of v
+                                    mma_f16_ts(o_acc, p_in + (uint32_t)(k4 * 8), vdesc + (uint64_t)(k4 * 128), idesc_pv, k4 > 0 ? 1u : acc);
+                                }
+                                tc_commit(bars + 8u * (uint32_t)(S::kVEmpty + c.v_slot));
+                                if (h == 1 && last) {
+                                    tc_commit(bars + 8u * S::kOFull);
+                                }
+                            }
+                            if (++c.v_slot == S::kVSlots) {
+                                c.v_slot = 0;
+                                c.v_phase ^= 1u;
                             }
                         }
-                        if (++v_slot == S::kVSlots) {
-                            v_slot = 0;
-                            v_phase ^= 1u;
+                        c.parity ^= 1u;
+                        ++c.step;
+                        if (last) {
+                            c.step = c.steps = 0;
+                            c.item_parity ^= 1u;
                         }
                     }
-                    if (ok && s + 1 < steps) {
-                        scores(s + 2 == steps);   // over P, which the MMAs before read, in order
+                    // the next item that has steps
+                    while (ok && c.steps == 0) {
+                        const int slot = c.infos % kInfos;
+                        ok = wait_for(bars + 8u * (uint32_t)(S::kInfoFull + slot), (uint32_t)(c.infos / kInfos & 1), 0x8250u);
+                        if (ok) {
+                            c.steps = info_of(c.t, slot)->steps;
+                            __syncwarp();
+                            if (lane == 0) {
+                                mbar_arrive(bars + 8u * (uint32_t)(S::kInfoEmpty + slot));
+                            }
+                            ++c.infos;
+                        }
+                    }
+                    // S = Q K^T of its next step, over P, which the MMAs before read, in order
+                    if (ok && c.steps > 0) {
+                        ok = (c.step > 0 || wait_for(bars + 8u * S::kQFull, c.item_parity, 0x8200u)) &&
+                             wait_for(bars + 8u * (uint32_t)(S::kKFull + c.k_slot), c.k_phase, 0x8210u);
+                        if (ok) {
+                            tc_fence_after_sync();
+                            if (elect_one()) {
+                                const uint64_t qdesc = umma_desc_k_sw128(smem);
+                                const uint64_t kdesc = umma_desc_k_sw128(smem + S::kKOffset + c.k_slot * S::kKBytes);
+#pragma unroll
+                                for (int ks = 0; ks < D / 16; ++ks) {
+                                    const uint64_t off = (uint64_t)(((ks >> 2) * S::kPanelQ + (ks & 3) * 32) >> 4);
+                                    mma_f16(s_acc, qdesc + off, kdesc + off, idesc_qk, ks > 0 ? 1u : 0u);
+                                }
+                                tc_commit(bars + 8u * S::kSFull);
+                                tc_commit(bars + 8u * (uint32_t)(S::kKEmpty + c.k_slot));
+                                if (c.step + 1 == c.steps) {
+                                    tc_commit(bars + 8u * S::kQEmpty);
+                                }
+                            }
+                            if (++c.k_slot == S::kKSlots) {
+                                c.k_slot = 0;
+                                c.k_phase ^= 1u;
+                            }
+                        }
                     }
                 }
+                const Tile was = c;
+                c     = other;
+                other = was;
+            }
+            if (bad != 0) {
+                give_up(bad);
             }
         }
     } else {
-        // ------------------------------------------------------------------ softmax and epilogue, one thread per query row
+        // ------------------------------------------------------------------ softmax, one thread per query row
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        const int      t        = warp >> 2;
         const int      quadrant = warp & 3;                                    // tensor-memory lane quadrant of this warp
         const int      r        = quadrant * 32 + lane;                        // row of the tile
+        const uint32_t bars     = bars_of(t);
         const uint32_t lanes    = tmem_base + ((uint32_t)(quadrant * 32) << 16);
         const uint32_t s_addr   = lanes + (uint32_t)(t * 128);
         const uint32_t o_addr   = lanes + (uint32_t)(256 + t * 128);
         const float    c        = p.scale_log2;
+        const bool     wide     = (reinterpret_cast<uintptr_t>(p.out) & 31u) == 0 && ((p.os.batch | p.os.token | p.os.head) & 15) == 0;   // rows on 32 bytes
         bool           ok       = true;
-        uint32_t       g        = 0, done = 0;                                 // steps and query blocks of this tile
-        for (int i = first; ok && i < p.items; i += stride) {
-            const Item it    = item_of(i);
-            const int  steps = steps_of(it);
-            const int  row   = it.qb * kTile + r;
-            const int  len   = key_count(p, it.b);
-            // the last key this row sees
-            const int  place = p.causal ? (int)min((long long)first_place(p, it.b) + row, (long long)p.keys) : p.keys;
+        uint32_t       g        = 0;                                           // steps of all items
+        int            infos = 0, done = 0;
+        while (ok) {
+            const int slot = infos % kInfos;
+            if (!(ok = wait(bars + 8u * (S::kInfoFull + slot), (uint32_t)(infos / kInfos & 1), 0x8340u))) {
+                break;
+            }
+            const Info it = *info_of(t, slot);
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(bars + 8u * (uint32_t)(S::kInfoEmpty + slot));
+            }
+            ++infos;
+            const int steps = it.steps, row = it.qb * kTile + r;
+            if (steps < 0) {
+                break;
+            }
+            // O / l, rounded to T
+            uint32_t w[D / 2];
+            auto store = [&]() {
+                if (row < p.queries) {
+                    T* dst = reinterpret_cast<T*>(p.out) + (long long)it.b * p.os.batch + (long long)row * p.os.token + (long long)it.h * p.os.head;
+                    if (wide) {
+#pragma unroll
+                        for (int k = 0; k < D / 16; ++k) {
+                            const Vec16 x = {w[8 * k], w[8 * k + 1], w[8 * k + 2], w[8 * k + 3]}, y = {w[8 * k + 4], w[8 * k + 5], w[8 * k + 6], w[8 * k + 7]};
+                            st_32(dst + 16 * k, x, y);
+                        }
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < D / 8; ++k) {
+                            reinterpret_cast<uint4*>(dst)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+                        }
+                    }
+                }
+            };
+            if (steps == 0) {
+#pragma unroll
+                for (int k = 0; k < D / 2; ++k) {
+                    w[k] = 0u;
+                }
+                store();
+                continue;
+            }
             float m = -INFINITY;                                               // reference maximum of this row's raw scores; -inf: no key seen
             float l = 0.0f;                                                    // sum of exp2((s - m) c)
-            int   key[2] = {p.keys, p.keys};
-            if (steps > 0) {
-                key[0] = key_of(it, 0, 0);
-                key[1] = key_of(it, 0, 1);
-            }
 #pragma unroll 1
             for (int s_i = 0; s_i < steps; ++s_i, ++g) {
-                // keys [0, see[h]) of a half are this row's, of which [0, full[h]) exist
-                int see[2], exist[2];
+                // Keys [0, see[h]) of a half are this row's.  V rows that do not exist but lie in the tensor are cleared before the issuer hears of P.
+                int see[2] = {kHalf, kHalf};
+                if (s_i >= it.masked) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    exist[h] = min(max(len - key[h], 0), kHalf);
-                    see[h]   = min(max(place - key[h] + 1, 0), exist[h]);
+                    for (int h = 0; h < 2; ++h) {
+                        const int key = key_of(it.list, it.entries, s_i, h), exist = min(max(it.len - key, 0), kHalf);
+                        see[h]        = p.causal ? min(max(it.place + r - key + 1, 0), exist) : exist;
+                        if (exist < kHalf && key + exist < p.keys) {
+                            const uint32_t n = 2u * g + (uint32_t)h, slot_v = n % (uint32_t)S::kVSlots;
+                            ok = ok && wait(bars + 8u * (S::kVFull + slot_v), n / (uint32_t)S::kVSlots & 1u, 0x8310u | (unsigned)t);
+                            // two threads a row, which is 128 bytes in every panel
+                            if (ok && (r >> 1) >= exist) {
+                                uint8_t* at = gen_base + t * S::kPerTile + S::kVOffset + (int)slot_v * S::kVBytes + (r >> 1) * 128 + (r & 1) * 64;
+#pragma unroll
+                                for (int cc = 0; cc < S::kPanels; ++cc) {
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) {
+                                        *reinterpret_cast<uint4*>(at + cc * S::kPanelV + e * 16) = make_uint4(0u, 0u, 0u, 0u);
+                                    }
+                                }
+                            }
+                            fence_proxy_async_smem();
+                        }
+                    }
                 }
-                const bool clear[2] = {exist[0] < kHalf && key[0] + exist[0] < p.keys, exist[1] < kHalf && key[1] + exist[1] < p.keys};
-                if (s_i + 1 < steps) {
-                    key[0] = key_of(it, s_i + 1, 0);
-                    key[1] = key_of(it, s_i + 1, 1);
+                if (!ok) {
+                    break;
                 }
-                if (!mbar_wait_warp(s_full(t), g & 1u, abort_flag, p.wait_limit_ns)) {
-                    give_up(0x8300u | (unsigned)t);
-                    ok = false;
+                if (!(ok = wait(bars + 8u * S::kSFull, g & 1u, 0x8300u | (unsigned)t))) {
                     break;
                 }
                 tc_fence_after_sync();
@@ -395,7 +513,7 @@ sparse_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                     tmem_ld_32x32(s_addr + cc * 32, s + cc * 32);
                 }
                 tmem_ld_wait();
-                if (__any_sync(0xffffffffu, see[0] < kHalf || see[1] < kHalf)) {
+                if (s_i >= it.masked) {
 #pragma unroll
                     for (int k = 0; k < 128; ++k) {
                         if ((k & 63) >= see[k >> 6]) {
@@ -444,35 +562,6 @@ sparse_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                         tmem_st_wait();
                     }
                 }
-                // V rows beyond the sequence's keys: cleared before the issuer hears of P
-                if (clear[0] || clear[1]) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (clear[h]) {
-                            const uint32_t n = 2u * g + (uint32_t)h, slot = n % (uint32_t)S::kVSlots;
-                            if (ok && !mbar_wait_warp(v_full(t, (int)slot), n / (uint32_t)S::kVSlots & 1u, abort_flag, p.wait_limit_ns)) {
-                                give_up(0x8310u | (unsigned)t);
-                                ok = false;
-                            }
-                            // two threads a row, which is 128 bytes in every panel
-                            const int key_row = r >> 1;
-                            if (ok && key_row >= exist[h]) {
-                                uint8_t* at = gen_base + t * S::kPerTile + S::kVOffset + (int)slot * S::kVBytes + key_row * 128 + (r & 1) * 64;
-#pragma unroll
-                                for (int cc = 0; cc < S::kPanels; ++cc) {
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e) {
-                                        *reinterpret_cast<uint4*>(at + cc * S::kPanelV + e * 16) = make_uint4(0u, 0u, 0u, 0u);
-                                    }
-                                }
-                            }
-                        }
-                    }
-                    if (!ok) {
-                        break;
-                    }
-                    fence_proxy_async_smem();
-                }
                 const float2 c2   = make_float2(c, c);
                 const float  nmc  = m == -INFINITY ? 0.0f : -m * c;            // no key seen: every weight is exp2(-inf)
                 const float2 nmc2 = make_float2(nmc, nmc);
@@ -499,7 +588,7 @@ sparse_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                         tc_fence_before_sync();
                         __syncwarp();
                         if (lane == 0) {
-                            mbar_arrive(cc == 1 ? p_first(t) : p_second(t));
+                            mbar_arrive(bars + 8u * (uint32_t)(S::kPHalf + (cc >> 1)));
                         }
                     }
                 }
@@ -509,42 +598,26 @@ sparse_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
             if (!ok) {
                 break;
             }
-            // O / l, rounded to T; a row that saw no key: zeros
-            const bool none  = m == -INFINITY;
+            if (!(ok = wait(bars + 8u * S::kOFull, (uint32_t)(done & 1), 0x8320u))) {
+                break;
+            }
+            ++done;
+            tc_fence_after_sync();
+            const bool  none  = m == -INFINITY;                                // a row that saw no key: zeros
             const float inv_l = 1.0f / l;
-            uint32_t w[D / 2];
 #pragma unroll
-            for (int k = 0; k < D / 2; ++k) {
-                w[k] = 0u;
-            }
-            if (steps > 0) {
-                if (!mbar_wait_warp(o_full(t), done & 1u, abort_flag, p.wait_limit_ns)) {
-                    give_up(0x8320u | (unsigned)t);
-                    ok = false;
-                    break;
-                }
-                ++done;
-                tc_fence_after_sync();
+            for (int cc = 0; cc < D / 32; ++cc) {
+                uint32_t o[32];
+                tmem_ld_32x32(o_addr + cc * 32, o);
+                tmem_ld_wait();
 #pragma unroll
-                for (int cc = 0; cc < D / 32; ++cc) {
-                    uint32_t o[32];
-                    tmem_ld_32x32(o_addr + cc * 32, o);
-                    tmem_ld_wait();
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        const float2 x = mul_f32x2(make_float2(__uint_as_float(o[2 * k]), __uint_as_float(o[2 * k + 1])), make_float2(inv_l, inv_l));
-                        w[cc * 16 + k] = none ? 0u : Pair<T>::from_f32(x.x, x.y);
-                    }
-                }
-                tc_fence_before_sync();
-            }
-            if (row < p.queries) {
-                T* dst = reinterpret_cast<T*>(p.out) + (long long)it.b * p.os.batch + (long long)row * p.os.token + (long long)it.h * p.os.head;
-#pragma unroll
-                for (int k = 0; k < D / 8; ++k) {
-                    reinterpret_cast<uint4*>(dst)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+                for (int k = 0; k < 16; ++k) {
+                    const float2 x = mul_f32x2(make_float2(__uint_as_float(o[2 * k]), __uint_as_float(o[2 * k + 1])), make_float2(inv_l, inv_l));
+                    w[cc * 16 + k] = none ? 0u : Pair<T>::from_f32(x.x, x.y);
                 }
             }
+            tc_fence_before_sync();   // the next item's P lets the issuer overwrite it
+            store();
         }
     }
 
