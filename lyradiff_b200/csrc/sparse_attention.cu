@@ -630,7 +630,7 @@ sparse_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
 }
 
 // [batch, heads, tokens, D] with any steps, boxes of `rows` tokens x 64 columns.  A dimension that does not move is one of size one.
-static int make_map(CUtensorMap* map, const void* base, const Steps& s, int batch, int heads, int tokens, int dim, int rows)
+int make_map(CUtensorMap* map, const void* base, const Steps& s, int batch, int heads, int tokens, int dim, int rows)
 {
     static EncodeTiledFnSparse encode = nullptr;
     if (encode == nullptr) {
@@ -780,6 +780,9 @@ int lyraq_sparse_attention(const lyraq_sparse_attention_t* a, void* stream)
         return LYRAQ_ERR_CUDA;
     }
     cudaStream_t s = (cudaStream_t)stream;
+    if (sattn::few_rows(p)) {
+        return sattn::launch_rows(p, a->dtype, a->head_dim, s);
+    }
     if (a->dtype == LYRAQ_BF16) {
         return dim == 128 ? sattn::launch<__nv_bfloat16, 128>(p, sms, s) : sattn::launch<__nv_bfloat16, 64>(p, sms, s);
     }

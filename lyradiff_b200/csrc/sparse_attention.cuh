@@ -49,6 +49,7 @@ __device__ __forceinline__ int first_place(const Params& p, int b)
     return p.q_start == nullptr ? p.keys - p.queries : min(max(load_int(p.q_start + b), -kMaxKeys), kMaxKeys);
 }
 
+bool few_rows(const Params& p);   // whether the few-row kernel takes the call
 int launch_rows(const Params& p, int dtype, int head_dim, cudaStream_t stream);   // sparse_attention_rows.cu
 
 }  // namespace sattn

@@ -390,18 +390,20 @@ def test_refusals(ops):
     check_status()
 
 
-def test_a_wait_that_runs_out_is_reported(ops):
+@pytest.mark.parametrize("nq,kernel", [(300, 8), (1, 9)])
+def test_a_wait_that_runs_out_is_reported(ops, nq, kernel):
     from lyradiff_b200 import _lib
-    q = torch.randn(1, 300, 2, 128, device="cuda").bfloat16()
-    index, counts = torch.zeros(1, 2, 3, 1, dtype=torch.int32, device="cuda"), torch.ones(1, 2, 3, dtype=torch.int32, device="cuda")
-    want = ops.sparse_attention(q, q, q, index, counts, 64)
+    q, k = torch.randn(1, nq, 2, 128, device="cuda").bfloat16(), torch.randn(1, 600, 2, 128, device="cuda").bfloat16()
+    qb = sparse.blocks(nq, 128)
+    index, counts = torch.arange(5, dtype=torch.int32, device="cuda").expand(1, 2, qb, 5).contiguous(), torch.full((1, 2, qb), 5, dtype=torch.int32, device="cuda")
+    want = ops.sparse_attention(q, k, k, index, counts, 64)
     check_status()
     _lib.check(_lib.lib().lyraq_debug_sparse_attention_wait_test(1, 200), "hook")
     try:
-        ops.sparse_attention(q, q, q, index, counts, 64)
+        ops.sparse_attention(q, k, k, index, counts, 64)
         status, detail = ops.last_status()
-        assert status == 4 and detail >> 12 == 8
+        assert status == 4 and detail >> 12 == kernel
     finally:
         _lib.lib().lyraq_debug_sparse_attention_wait_test(0, 0)
-    assert torch.equal(ops.sparse_attention(q, q, q, index, counts, 64), want)     # tensor memory was given back
+    assert torch.equal(ops.sparse_attention(q, k, k, index, counts, 64), want)     # tensor memory was given back
     check_status()
