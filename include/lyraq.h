@@ -118,6 +118,9 @@ LYRAQ_API int lyraq_debug_force_fp4_tile(int code);
 /* lyraq_debug_attention_wait_test for lyraq_sparse_attention.  It has no counterpart in the reference. */
 LYRAQ_API int lyraq_debug_sparse_attention_wait_test(int skip_loads, unsigned int wait_limit_ms);
 
+/* lyraq_debug_skinny_wait_test for the few-row kernel of lyraq_gemm_fp8_block.  It has no counterpart in the reference. */
+LYRAQ_API int lyraq_debug_fp8_block_rows_wait_test(int stalled_rank, unsigned int wait_limit_ms);
+
 /* Test / sweep hook: the kernel of lyraq_gemm_fp8_block.  0 = automatic (default); 2562 = CTA pair, 256 x 256 tile; 1281 = one CTA, 128 x 128; 16 = the few-row kernel wherever it can, the automatic choice elsewhere.  Process-wide, not thread-safe.  It has no counterpart in the reference. */
 LYRAQ_API int lyraq_debug_force_fp8_block_tile(int code);
 

@@ -18,7 +18,7 @@ CLASSES_SRC = os.path.join(CSRC, "torch_classes.cpp")
 HOST_LIB = os.path.join(HERE, "_host" + sysconfig.get_config_var("EXT_SUFFIX"))
 HOST_SRC = os.path.join(CSRC, "host_calls.cpp")
 
-SOURCES = ["api.cu", "quant_kernels.cu", "gemm_dense.cu", "gemm_skinny.cu", "gemm_w4a4.cu", "gemm_w4a4_wide.cu", "fp4_quant.cu", "gemm_fp4.cu", "gemm_fp4_skinny.cu", "fp8_block_quant.cu", "gemm_fp8_block.cu", "norm_residual.cu", "rope_axes.cu", "lora_down.cu", "block_kernels.cu", "attention.cu", "block_select.cu", "sparse_attention.cu", "sparse_attention_rows.cu", "linear_layers.cu", "noalloc.cu"]
+SOURCES = ["api.cu", "quant_kernels.cu", "gemm_dense.cu", "gemm_skinny.cu", "gemm_w4a4.cu", "gemm_w4a4_wide.cu", "fp4_quant.cu", "gemm_fp4.cu", "gemm_fp4_skinny.cu", "fp8_block_quant.cu", "gemm_fp8_block.cu", "gemm_fp8_block_rows.cu", "norm_residual.cu", "rope_axes.cu", "lora_down.cu", "block_kernels.cu", "attention.cu", "block_select.cu", "sparse_attention.cu", "sparse_attention_rows.cu", "linear_layers.cu", "noalloc.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

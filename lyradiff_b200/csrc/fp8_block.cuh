@@ -129,9 +129,11 @@ template<typename T> __device__ __forceinline__ Vec16 encode16(const Vec16* v, c
 }
 
 int check_quant(const void* q, const void* scale, const void* x, int dtype, size_t ldx, size_t rows, size_t k);   // fp8_block_quant.cu
-// gemm_fp8_block_rows.cu: whether the few-row kernel can take the call, and whether it pays; and its launch
-bool few_rows(int m, int n, int k);
-int  launch_rows(const Input& X, const uint8_t* W, const GemmParams& p, cudaStream_t stream);
+bool few_rows(int m, int n, int k);              // whether a product takes the few-row kernel (gemm_fp8_block.cu),
+bool few_rows_quantize(int m, int n, int k);     // and whether a linear leaves the quantize to it
+bool rows_fit(int n, int k, int sms);            // gemm_fp8_block_rows.cu: whether a CTA's shared memory holds its part of the rows
+bool rows_quantize_pays(int m, int n, int k, int sms);
+int  launch_rows(const Input& X, const uint8_t* W, const GemmParams& p, int sms, cudaStream_t stream);
 // lyraq_gemm_fp8_block behind its checks (gemm_fp8_block.cu); rows that are not FP8 yet only where few_rows
 int  product(const Input& X, const uint8_t* W, const float* ws, void* Y, int c_dtype, const void* bias, const void* residual, float beta, int epilogue, int m,
              int n, int k, cudaStream_t stream);

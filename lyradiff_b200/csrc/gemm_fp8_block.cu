@@ -515,11 +515,25 @@ template<int BLOCK_N, int CTAS, bool RES> static int launch(const uint8_t* X, co
                        "cudaLaunchKernelEx(gemm_fp8_block_kernel)");
 }
 
-// forced kernel for tests and sweeps: 0 = automatic, 2562 = CTA pair with 256 x 256, 1281 = one CTA with 128 x 128
+// forced kernel for tests and sweeps: 0 = automatic, 16 = the few-row kernel (up to 16 rows), 2562 = CTA pair with 256 x 256, 1281 = one CTA with 128 x 128
 static int g_forced_tile = 0;
+
+bool few_rows(int m, int n, int k)
+{
+    // The few-row kernel's time grows with the rows (their partial sums cross shared memory and leave row by row), the other's does not; what it gains
+    // grows with K.  Dense against few-row, a linear, us: 6 rows of [256, 256] 4.7 / 4.6, of [1280, 768] 5.9 / 5.8, 8 rows of it 5.9 / 6.2, 16 rows of [1280, 1024] 6.5 /
+    // 6.5, of [1280, 5120] 16.2 / 7.4, of [13824, 5120] 25 / 20; one row of [5120, 5120] 16.9 / 9.5.
+    const bool pays = m <= 6 || k > 7 * kBlock;
+    return m <= kFewRows && (g_forced_tile == 16 || (g_forced_tile == 0 && pays)) && rows_fit(n, k, device_sm_count());
+}
+
+bool few_rows_quantize(int m, int n, int k) { return few_rows(m, n, k) && (g_forced_tile == 16 || rows_quantize_pays(m, n, k, device_sm_count())); }
 
 static int run(const Input& X, const uint8_t* W, const GemmParams& p, int sms, cudaStream_t stream)
 {
+    if (few_rows(p.M, p.N, p.K)) {
+        return launch_rows(X, W, p, sms, stream);
+    }
     const long m128 = ((long)p.M + 127) / 128, n128 = ((long)p.N + 127) / 128, m256 = ((long)p.M + 255) / 256, n256 = ((long)p.N + 255) / 256;
     const long pairs = sms / 2;
     const int  num_kb = (p.K + kBlock - 1) / kBlock;

@@ -170,6 +170,10 @@ int lyraq_linear_fp8_block_forward(void* Y, const void* x, int dtype, size_t ldx
         result_clashes(work, nullptr, {w, ws, b, view_of(residual, rows * cols * bytes), view_of(x, bytes, rows, ldx, 1, 0, 1, 0, depth)})) {
         return LYRAQ_ERR_INVALID_ARG;
     }
+    // One launch, which quantizes the rows on their way.  Every thread block reads all rows, so a result in their place needs them quantized before.
+    if (fp8b::few_rows_quantize(m, n, k) && !views_meet(y, view_of(x, bytes, rows, ldx, 1, 0, 1, 0, depth))) {
+        return fp8b::product({nullptr, {nullptr, 0, 0}, x, dtype, ldx}, W, w_scale, Y, dtype, bias, residual, beta, epilogue, m, n, k, (cudaStream_t)stream);
+    }
     const size_t pitch = fp8b::scale_pitch(rows);
     st = lyraq_quant_fp8_block(qx, sx, 1, pitch, x, dtype, ldx, rows, depth, stream);
     if (st != LYRAQ_OK) {

@@ -299,3 +299,58 @@ def test_encode_matches_torch(ops):
     codes, s = ops.quant_fp8_block(cu(x))
     assert bool((s == 1).all())
     assert torch.equal(codes.cpu(), x.to(torch.float8_e4m3fn).view(torch.uint8))
+
+
+@pytest.mark.parametrize("m", [1, 3, 8, 16])
+@pytest.mark.parametrize("n,k", [(264, 4096), (4224, 2560), (9088, 1024), (9216, 2048), (18944, 512), (19072, 1152), (130, 16), (33000, 400), (200, 33008)])
+def test_few_rows_with_every_split_of_k(ops, tile, m, n, k):
+    """One, two, four and eight CTAs along K, both sides of the tile counts at which fewer are taken, more K blocks than tensor memory has buffers: integers, exact."""
+    tile(16)
+    g = torch.Generator(device="cuda").manual_seed(n + m)
+    table = torch.tensor([0, 0x38, 0xB8, 0x40], dtype=torch.uint8, device="cuda")
+    value = torch.tensor([0.0, 1.0, -1.0, 2.0], dtype=torch.float64, device="cuda")
+    i, j = (torch.randint(0, 4, (rows, k), generator=g, device="cuda") for rows in (m, n))
+    xs, ws = torch.ones(m, (k + 127) // 128, device="cuda"), torch.ones((n + 127) // 128, (k + 127) // 128, device="cuda")
+    y = torch.full((m, n), float("nan"), dtype=torch.float32, device="cuda")
+    ops.gemm_fp8_block(table[j], ws, table[i], xs, y)
+    check_status()
+    assert torch.equal(y.double(), value[i] @ value[j].t())
+
+
+@pytest.mark.parametrize("m", [1, 2, 7, 16])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_quantized_in_the_product_are_the_same(ops, tile, m, dtype):
+    """The few-row kernel's own quantize against the quantizer and the product on its codes: the same bits."""
+    from lyradiff_b200.layers import Fp8BlockLinear
+    g = torch.Generator().manual_seed(m)
+    for n, k in ((200, 1040), (1300, 336), (264, 6416)):
+        x = values(m, k, dtype, m + k).clamp(-1e4, 1e4)
+        layer = Fp8BlockLinear.from_float(cu((torch.randn(n, k, generator=g) * 0.02).to(dtype)))
+        tile(16)
+        y = layer.forward(cu(x))
+        codes, s = ops.quant_fp8_block(cu(x))
+        assert torch.equal(ops.gemm_fp8_block(layer.codes, layer.scales, codes, s, dtype), y)
+        tile(0)
+        assert torch.equal(layer.forward(cu(x)), y) or m > 6 and k <= 7 * 128
+        check_status()
+
+
+def test_a_wait_that_runs_out_is_reported(ops):
+    from lyradiff_b200 import _lib
+    from lyradiff_b200.layers import Fp8BlockLinear
+    layer = Fp8BlockLinear.from_float(torch.randn(640, 4096, device="cuda").bfloat16())
+    x = torch.randn(3, 4096, device="cuda").bfloat16()
+    want = layer.forward(x)
+    check_status()
+    _lib.check(_lib.lib().lyraq_debug_fp8_block_rows_wait_test(1, 200), "hook")
+    try:
+        y = torch.zeros(3, 640, dtype=torch.bfloat16, device="cuda")
+        layer.forward(x, out=y)
+        from lyradiff_b200 import ops as _ops
+        status, detail = _ops.last_status()
+        assert status == 4 and detail >> 12 == 10
+        assert not bool(y.any())                                 # none of a cluster stores anything
+    finally:
+        _lib.lib().lyraq_debug_fp8_block_rows_wait_test(-1, 0)
+    assert torch.equal(layer.forward(x), want)                   # tensor memory was given back
+    check_status()
