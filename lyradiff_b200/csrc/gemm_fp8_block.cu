@@ -33,22 +33,21 @@ namespace fp8b {
 using namespace tiles;
 
 constexpr int kBlockM    = 128;
-constexpr int kThreads   = 384;
+constexpr int kThreads   = 640;
 constexpr int kEpiWarp0  = 4;
-constexpr int kEpiWarps  = 8;
+constexpr int kEpiWarps  = 16;
 constexpr int kBox       = 32 * 64;      // one warp's staging box: 32 rows x 32 columns of a 16-bit type
-constexpr int kBoxes     = 2;            // the store of one chunk drains its box while the next chunk is computed and fills the other
-constexpr int kBiasBytes = 128 * 2;      // one warp's bias: up to 128 columns of a 16-bit type (fp32, which uses no boxes, keeps its there)
+constexpr int kBiasBytes = 64 * 2;       // one warp's bias: up to 64 columns of a 16-bit type (fp32, which uses no boxes, keeps its there)
 constexpr int kBarBytes  = 256;
-constexpr int kOtherRegs = 72;
-constexpr int kEpiRegs   = 216;
-static_assert(128 * kOtherRegs + 256 * kEpiRegs <= kThreads * 168, "the split draws on what the block was launched with");
+constexpr int kOtherRegs = 32;
+constexpr int kEpiRegs   = 112;
+static_assert(128 * kOtherRegs + 512 * kEpiRegs <= kThreads * 96, "the split draws on what the block was launched with");
 
 template<int BLOCK_N, int CTAS> struct Smem {
     static constexpr int kABytes     = kBlockM * kBlock;
     static constexpr int kBBytes     = BLOCK_N / CTAS * kBlock;
     static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kEpiBytes   = kEpiWarps * (kBoxes * kBox + kBiasBytes);
+    static constexpr int kEpiBytes   = kEpiWarps * (kBox + kBiasBytes);
     static constexpr int kStages     = (227 * 1024 - 1024 - kBarBytes - kEpiBytes) / kStageBytes;
     static constexpr int kEpiOffset  = kStages * kStageBytes;
     static constexpr int kBarOffset  = kEpiOffset + kEpiBytes;
@@ -67,9 +66,9 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
     constexpr int kStages = S::kStages;
     constexpr int kBufs   = S::kBufs;
     constexpr int kTileM  = kBlockM * CTAS;
-    constexpr int kHalfN  = BLOCK_N / 2;      // columns per epilogue warp: 128 or 64, all of one block of W
-    constexpr int kChunks = kHalfN / 32;
-    constexpr int kAhead  = 4;                // K blocks whose scales are fetched together
+    constexpr int kCols   = BLOCK_N / 4;      // columns per epilogue warp: 64 or 32, all of one block of W
+    constexpr int kChunks = kCols / 32;
+    constexpr int kAhead  = 2;                // K blocks whose scales are fetched together
 
     extern __shared__ uint8_t smem_raw[];
     // the dynamic shared window starts at the same offset in every CTA of the kernel, so both CTAs of a pair get the same layout
@@ -248,11 +247,11 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
         // ------------------------------------------------------------------ epilogue (warps 4..11)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
         const int      quad      = warp & 3;                 // the TMEM lane quadrant this warp may read
-        const int      half      = (warp - kEpiWarp0) >> 2;  // which half of the tile's columns
+        const int      quarter   = (warp - kEpiWarp0) >> 2;  // which quarter of the tile's columns
         const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
-        uint8_t*       boxes     = gen_base + S::kEpiOffset + (warp - kEpiWarp0) * kBoxes * kBox;
-        const uint32_t boxes_at  = smem_base + S::kEpiOffset + (warp - kEpiWarp0) * kBoxes * kBox;
-        uint8_t*       bias      = p.c_dtype == LYRAQ_F32 ? boxes : gen_base + S::kEpiOffset + kEpiWarps * kBoxes * kBox + (warp - kEpiWarp0) * kBiasBytes;
+        uint8_t*       boxes     = gen_base + S::kEpiOffset + (warp - kEpiWarp0) * kBox;
+        const uint32_t boxes_at  = smem_base + S::kEpiOffset + (warp - kEpiWarp0) * kBox;
+        uint8_t*       bias      = p.c_dtype == LYRAQ_F32 ? boxes : gen_base + S::kEpiOffset + kEpiWarps * kBox + (warp - kEpiWarp0) * kBiasBytes;
         const bool     vec_ok    = p.c_dtype == LYRAQ_F32 ? (p.N & 3) == 0 : (p.N & 7) == 0;
         int            buf       = 0;
         uint32_t       buf_phase = 0;
@@ -262,7 +261,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
             tile_coords(tile, p.m_tiles, p.n_tiles, m_blk, n_blk);
             const int row0  = m_blk * kTileM + (int)rank * kBlockM + quad * 32;  // first row of this warp
             const int row   = row0 + lane;
-            const int ncol0 = n_blk * BLOCK_N + half * kHalfN;
+            const int ncol0 = n_blk * BLOCK_N + quarter * kCols;
             // factors: a row or columns beyond the matrix take part with 0
             const bool   there = row < p.M && ncol0 < p.N;
             const float* xs    = p.xs.p + (there ? (size_t)row * p.xs.row_step : 0);
@@ -315,16 +314,14 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                             ok = false;
                         } else {
                             tc_fence_after_sync();
-                            const uint32_t t_addr = tmem_base + lane_addr + (uint32_t)(buf * BLOCK_N + half * kHalfN);
+                            const uint32_t t_addr = tmem_base + lane_addr + (uint32_t)(buf * BLOCK_N + quarter * kCols);
                             const float2   f2     = make_float2(f[i], f[i]);
-                            uint32_t       part[2][32];
-                            tmem_ld_32x32(t_addr, part[0]);
 #pragma unroll
                             for (int c = 0; c < kChunks; ++c) {
+                                uint32_t part[32];
+                                tmem_ld_32x32(t_addr + (uint32_t)(c * 32), part);
                                 tmem_ld_wait();
-                                if (c + 1 < kChunks) {
-                                    tmem_ld_32x32(t_addr + (uint32_t)((c + 1) * 32), part[(c + 1) & 1]);
-                                } else {
+                                if (c + 1 == kChunks) {
                                     // this warp's share of the product is in registers: its buffer may be overwritten
                                     tc_fence_before_sync();
                                     __syncwarp();
@@ -338,7 +335,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                                 }
 #pragma unroll
                                 for (int e = 0; e < 16; ++e) {
-                                    const float2 a = fma_f32x2(f2, make_float2(__uint_as_float(part[c & 1][2 * e]), __uint_as_float(part[c & 1][2 * e + 1])),
+                                    const float2 a = fma_f32x2(f2, make_float2(__uint_as_float(part[2 * e]), __uint_as_float(part[2 * e + 1])),
                                                                make_float2(__uint_as_float(acc[c][2 * e]), __uint_as_float(acc[c][2 * e + 1])));
                                     acc[c][2 * e]     = __float_as_uint(a.x);
                                     acc[c][2 * e + 1] = __float_as_uint(a.y);
@@ -369,10 +366,9 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                 __syncwarp();
             }
             // Residual of a 16-bit output: a lane that fetched its own row would touch 32 lines an instruction and use half a sector of each.
-            // Instead four lanes fetch the 64 bytes of a row, eight rows an instruction, two chunks ahead, and hand them over through the box
-            // that the result leaves by.
+            // Instead four lanes fetch the 64 bytes of a row, eight rows an instruction, and hand them over through the box that the result leaves by.
             const bool staged = RES && p.residual != nullptr && p.tma_store;
-            Vec16      rr[2][RES ? 4 : 1];
+            Vec16      rr[RES ? 4 : 1];
             auto fetch_residual = [&](int c, Vec16* dst) {
                 const int col = ncol0 + c * 32 + (lane & 3) * 8;
 #pragma unroll
@@ -385,8 +381,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                 }
             };
             if (staged) {
-                fetch_residual(0, rr[0]);
-                fetch_residual(1, rr[1]);
+                fetch_residual(0, rr);
             }
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
@@ -396,17 +391,12 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                     continue;
                 }
                 float     v[32];
-                uint8_t*  box  = boxes + (c % kBoxes) * kBox;
+                uint8_t*  box  = boxes;
                 uint8_t*  brow = box + lane * 64;
                 const int sw_  = (lane >> 1) & 3;
                 if (p.tma_store) {
                     if (lane == 0) {
-                        // the store before the last has drained this box; the tile before may have ended with either box
-                        if (c == 0) {
-                            tma_store_wait_read();
-                        } else {
-                            tma_store_wait_read_but_one();
-                        }
+                        tma_store_wait_read();   // the last store has drained the box
                     }
                     __syncwarp();
                 }
@@ -414,11 +404,11 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
 #pragma unroll
                     for (int i = 0; i < (RES ? 4 : 1); ++i) {
                         const int r = i * 8 + (lane >> 2);
-                        *reinterpret_cast<Vec16*>(box + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4)) = rr[c & 1][i];
+                        *reinterpret_cast<Vec16*>(box + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4)) = rr[i];
                     }
                     __syncwarp();
-                    if (c + 2 < kChunks) {
-                        fetch_residual(c + 2, rr[c & 1]);
+                    if (c + 1 < kChunks) {
+                        fetch_residual(c + 1, rr);
                     }
                 }
                 if (p.c_dtype == LYRAQ_F32) {
@@ -453,7 +443,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0 && row0 < p.M) {
-                    tma_store_2d(&tmap_c, boxes_at + (uint32_t)((c % kBoxes) * kBox), col0, row0);
+                    tma_store_2d(&tmap_c, boxes_at, col0, row0);
                     tma_store_commit();
                 }
             }
