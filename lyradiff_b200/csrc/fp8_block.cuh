@@ -78,20 +78,29 @@ __device__ __forceinline__ Divisor divisor_of(uint32_t amax_bits)
 }
 
 // Codes of eight values.  The quotient is rounded to fp32 as a division rounds it, so that a quotient on a tie of e4m3 comes out as that tie; it
-// is found without one, by two corrections with the remainder, the second of which rounds correctly (P. Markstein, "Computation of elementary
-// functions on the IBM RISC System/6000 processor", 1990: r within half an ulp of 1 / t and a quotient within an ulp).
-__device__ __forceinline__ uint2 encode8(const float* x, const Divisor& d)
+// is found without one, by corrections with the remainder (P. Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor",
+// 1990: r within half an ulp of 1 / t).  Two corrections round any quotient correctly.
+// One is enough for 16-bit values (SHORT).  Behind it the quotient is off by 2^-45 before it is rounded, which could only matter if x lay within 2^-45 of t (q + ulp / 2) for
+// a tie q of e4m3.  In units of the last places, with q = a 2^19 (a of five bits) and T the 24 bits of t, that is T (a 2^20 + 1) within 16 of a number of 11
+// bits times 2^36, so T within 16 of a multiple of 2^20.  T is the quotient of an 11-bit number by 7, shifted: either its bits repeat every three places, and 15 equal
+// ones never follow one another, or it has nine bits, and is a multiple of 2^15 (too far from one of 2^20) or b 2^20, and T (a 2^20 + 1) is b 2^20 off.
+template<bool SHORT> __device__ __forceinline__ uint2 encode8(const float* x, const Divisor& d)
 {
     const float2 r2 = make_float2(d.r, d.r), m2 = make_float2(-d.t, -d.t), c2 = make_float2(d.c, d.c);
     uint32_t     h[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        // a block that is not finite: its values are replaced, not multiplied, so that no NaN reaches a code
-        const float2 v = d.r == 0.0f ? make_float2(0.0f, 0.0f) : mul_f32x2(make_float2(x[2 * j], x[2 * j + 1]), c2);
-        float2       q = mul_f32x2(v, r2);
-        q              = fma_f32x2(fma_f32x2(q, m2, v), r2, q);
-        q              = fma_f32x2(fma_f32x2(q, m2, v), r2, q);
-        h[j]           = f32x2_to_e4m3x2(q.x, q.y);
+        float2 v = make_float2(x[2 * j], x[2 * j + 1]);
+        if (__builtin_expect(d.c != 1.0f, 0)) {
+            // a block that is not finite: its values are replaced, not multiplied, so that no NaN reaches a code
+            v = d.r == 0.0f ? make_float2(0.0f, 0.0f) : mul_f32x2(v, c2);
+        }
+        float2 q = mul_f32x2(v, r2);
+        q        = fma_f32x2(fma_f32x2(q, m2, v), r2, q);
+        if (!SHORT) {
+            q = fma_f32x2(fma_f32x2(q, m2, v), r2, q);
+        }
+        h[j] = f32x2_to_e4m3x2(q.x, q.y);
     }
     return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
 }
@@ -121,7 +130,7 @@ template<typename T> __device__ __forceinline__ Vec16 encode16(const Vec16* v, c
         } else {
             unpack8<T>(v[a], f);
         }
-        const uint2 w  = encode8(f, d);
+        const uint2 w  = encode8<sizeof(T) == 2>(f, d);
         o.w[2 * a]     = w.x;
         o.w[2 * a + 1] = w.y;
     }

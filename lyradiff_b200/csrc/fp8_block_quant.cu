@@ -4,12 +4,12 @@
 namespace lyraq {
 namespace fp8b {
 
-// Activations, blocks of 1 x 128.  A pass over memory: 2 bytes a value are read, one and a 32nd are written.  A lane owns 16 values, eight lanes a block, a
-// warp the same 128 columns of four rows (whole lines of each; their scales are 16 bytes where scales of a block lie together), the warps of a
+// Activations, blocks of 1 x 128.  A pass over memory: 2 bytes a value are read, one and a 32nd are written.  A lane owns 16 values of each of two blocks, eight
+// lanes a block, a warp 256 columns of four rows (whole lines of each; their scales are 16 bytes where scales of a block lie together), the warps of a
 // thread block neighbouring columns.
 template<typename T>
 __global__ void __launch_bounds__(256)
-fp8_block_quant_kernel(uint8_t* q, float* scale, size_t scale_row, size_t scale_block, const T* x, size_t ldx, size_t rows, size_t k, unsigned blocks_k,
+fp8_block_quant_kernel(uint8_t* q, float* scale, size_t scale_row, size_t scale_block, const T* x, size_t ldx, size_t rows, size_t k, unsigned pairs_k,
                        size_t pieces, int wide)
 {
     constexpr int kPer  = 16 / (int)sizeof(T);
@@ -17,36 +17,42 @@ fp8_block_quant_kernel(uint8_t* q, float* scale, size_t scale_row, size_t scale_
     grid_launch_dependents();
     const size_t   piece = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     const unsigned lane  = threadIdx.x & 31;
-    const size_t   quad  = piece / blocks_k, kb = piece - quad * blocks_k;
+    const size_t   quad  = piece / pairs_k, kb = (piece - quad * pairs_k) * 2;
     const size_t   row   = quad * 4 + (lane >> 3), col = kb * kBlock + (lane & 7) * 16;
-    const bool     in    = piece < pieces && row < rows && col < k;   // k is a multiple of 16: a lane's values are there or not
+    const bool     there = piece < pieces && row < rows;
     grid_dependency_wait();
 
-    Vec16 v[kVecs] = {};
-    if (in) {
-        const T* src = x + row * ldx + col;
-        if (wide) {
+    Vec16 v[2][kVecs] = {};
 #pragma unroll
-            for (int a = 0; a < kVecs; a += 2) {
-                ld_nc_32(src + a * kPer, v[a], v[a + 1]);
-            }
-        } else {
+    for (int u = 0; u < 2; ++u) {
+        if (there && col + u * kBlock < k) {   // k is a multiple of 16: a lane's values are there or not
+            const T* src = x + row * ldx + col + u * kBlock;
+            if (wide) {
 #pragma unroll
-            for (int a = 0; a < kVecs; ++a) {
-                v[a] = ld_nc_16(src + a * kPer);
+                for (int a = 0; a < kVecs; a += 2) {
+                    ld_nc_32(src + a * kPer, v[u][a], v[u][a + 1]);
+                }
+            } else {
+#pragma unroll
+                for (int a = 0; a < kVecs; ++a) {
+                    v[u][a] = ld_nc_16(src + a * kPer);
+                }
             }
         }
     }
-    uint32_t amax = amax16_values<T>(v);
 #pragma unroll
-    for (int d = 1; d < 8; d *= 2) {
-        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, d));
-    }
-    const Divisor d = divisor_of(amax);
-    if (in) {
-        st_16(q + row * k + col, encode16<T>(v, d));
-        if ((lane & 7) == 0) {
-            scale[row * scale_row + kb * scale_block] = d.s;
+    for (int u = 0; u < 2; ++u) {
+        uint32_t amax = amax16_values<T>(v[u]);
+#pragma unroll
+        for (int d = 1; d < 8; d *= 2) {
+            amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+        }
+        const Divisor d = divisor_of(amax);
+        if (there && col + u * kBlock < k) {
+            st_16(q + row * k + col + u * kBlock, encode16<T>(v[u], d));
+            if ((lane & 7) == 0) {
+                scale[row * scale_row + (kb + u) * scale_block] = d.s;
+            }
         }
     }
 }
@@ -143,7 +149,7 @@ int lyraq_quant_fp8_block(uint8_t* q, float* scale, size_t scale_row, size_t sca
     if (!nested || views_meet(vs, vq) || views_meet(vx, vq) || views_meet(vx, vs)) {
         return LYRAQ_ERR_INVALID_ARG;
     }
-    const size_t pieces = (rows + 3) / 4 * blocks_k, blocks = (pieces + 7) / 8;
+    const size_t pairs_k = (blocks_k + 1) / 2, pieces = (rows + 3) / 4 * pairs_k, blocks = (pieces + 7) / 8;
     if (blocks > 0x7fffffffu) {
         return LYRAQ_ERR_UNSUPPORTED;
     }
@@ -151,7 +157,7 @@ int lyraq_quant_fp8_block(uint8_t* q, float* scale, size_t scale_row, size_t sca
     auto      launch = [&](auto type) {
         using T = decltype(type);
         return launch_kernel(fp8b::fp8_block_quant_kernel<T>, (unsigned)blocks, 256u, (size_t)0, (cudaStream_t)stream, 1u, q, scale, scale_row, scale_block,
-                             (const T*)x, ldx, rows, k, (unsigned)blocks_k, pieces, wide);
+                             (const T*)x, ldx, rows, k, (unsigned)pairs_k, pieces, wide);
     };
     const cudaError_t e = x_dtype == LYRAQ_BF16 ? launch(__nv_bfloat16{}) : x_dtype == LYRAQ_F16 ? launch(__half{}) : launch(float{});
     return cuda_status(e, "cudaLaunchKernelEx(fp8_block_quant_kernel)");

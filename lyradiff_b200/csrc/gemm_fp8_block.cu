@@ -190,57 +190,65 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
         } else if (warp == 1 && leader) {
             // -------------------------------------------------------------- MMA issuer (the leader CTA only)
             constexpr uint32_t kIdesc = umma_idesc(1u, 0u, kTileM, BLOCK_N);
-            int      stage = 0, buf = 0;
-            uint32_t phase = 0, buf_phase = 0;
-            bool     ok = true;
-            for (int tile = unit; ok && tile < num_tiles; tile += n_units) {
-                for (int kb = 0; kb < num_kb; ++kb) {
-                    if (!mbar_wait_warp(full_bar(stage), phase, abort_flag)) {
-                        report_timeout(p.status, 0x7300u | (unsigned)stage);
-                        *abort_flag = 1;
-                        ok = false;
-                        break;
-                    }
-                    if (!mbar_wait_warp(tmem_empty_bar(buf), buf_phase ^ 1u, abort_flag)) {
-                        report_timeout(p.status, 0x7200u | (unsigned)buf);
-                        *abort_flag = 1;
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after_sync();
-                    if (elect_one()) {
-                        const uint32_t sa     = smem_base + stage * S::kStageBytes;
-                        const uint64_t adesc  = umma_desc_k_sw128(sa);
-                        const uint64_t bdesc  = umma_desc_k_sw128(sa + S::kABytes);
-                        const uint32_t d_tmem = tmem_base + (uint32_t)(buf * BLOCK_N);
-                        const int      steps  = min(kBlock, p.K - kb * kBlock + 31) / 32;   // MMAs of this K block; TMA fills its end with zeros
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            if (k < steps) {
-                                if (CTAS == 2) {
-                                    mma_f8f6f4_pair(d_tmem, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), kIdesc, k > 0 ? 1u : 0u);
-                                } else {
-                                    mma_f8f6f4(d_tmem, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), kIdesc, k > 0 ? 1u : 0u);
-                                }
-                            }
-                        }
+            int       stage = 0, buf = 0, kb = 0;
+            uint32_t  phase = 0, buf_phase = 0;
+            long long left  = (long long)((num_tiles - unit + n_units - 1) / n_units) * num_kb;   // K blocks of all its tiles
+            // The waits for the next K block stand between the MMAs of this one: the pipe has work while they pass (a passed wait costs about 100 clocks,
+            // as much as two MMAs; [1317, 1280, 5120] 18.1 -> 16.2 us).  With two products in tensor memory the one before is still being taken then, and
+            // they stand in front of them (388 us against 315 for [4680, 13824, 5120]).
+            constexpr bool kEarly = kBufs > 2;
+            bool           ok     = !kEarly || mbar_wait_warp2(full_bar(0), 0u, tmem_empty_bar(0), 1u, abort_flag);
+            for (; ok && left > 0; --left) {
+                if (!kEarly && !(ok = mbar_wait_warp2(full_bar(stage), phase, tmem_empty_bar(buf), buf_phase ^ 1u, abort_flag))) {
+                    break;
+                }
+                const uint32_t sa     = smem_base + stage * S::kStageBytes;
+                const uint64_t adesc  = umma_desc_k_sw128(sa);
+                const uint64_t bdesc  = umma_desc_k_sw128(sa + S::kABytes);
+                const uint32_t d_tmem = tmem_base + (uint32_t)(buf * BLOCK_N);
+                const int      steps  = min(kBlock, p.K - kb * kBlock + 31) / 32;   // MMAs of this K block; TMA fills its end with zeros
+                const int      was_stage = stage, was_buf = buf;
+                auto mma = [&](int k) {
+                    if (k < steps) {
                         if (CTAS == 2) {
-                            tc_commit_both(empty_bar(stage));
-                            tc_commit_both(tmem_full_bar(buf));
+                            mma_f8f6f4_pair(d_tmem, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), kIdesc, k > 0 ? 1u : 0u);
                         } else {
-                            tc_commit(empty_bar(stage));
-                            tc_commit(tmem_full_bar(buf));
+                            mma_f8f6f4(d_tmem, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), kIdesc, k > 0 ? 1u : 0u);
                         }
                     }
-                    if (++stage == kStages) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
-                    if (++buf == kBufs) {
-                        buf = 0;
-                        buf_phase ^= 1u;
+                };
+                tc_fence_after_sync();
+                if (elect_one()) {
+                    mma(0);
+                    mma(1);
+                }
+                kb = kb + 1 == num_kb ? 0 : kb + 1;
+                if (++stage == kStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+                if (++buf == kBufs) {
+                    buf = 0;
+                    buf_phase ^= 1u;
+                }
+                if (kEarly && left > 1) {
+                    ok = mbar_wait_warp2(full_bar(stage), phase, tmem_empty_bar(buf), buf_phase ^ 1u, abort_flag);
+                }
+                if (elect_one()) {
+                    mma(2);
+                    mma(3);
+                    if (CTAS == 2) {
+                        tc_commit_both(empty_bar(was_stage));
+                        tc_commit_both(tmem_full_bar(was_buf));
+                    } else {
+                        tc_commit(empty_bar(was_stage));
+                        tc_commit(tmem_full_bar(was_buf));
                     }
                 }
+            }
+            if (!ok) {
+                report_timeout(p.status, 0x7200u | (unsigned)(stage << 4) | (unsigned)buf);
+                *abort_flag = 1;
             }
         }
     } else {
@@ -527,8 +535,10 @@ static int run(const Input& X, const uint8_t* W, const GemmParams& p, int sms, c
     const long m128 = ((long)p.M + 127) / 128, n128 = ((long)p.N + 127) / 128, m256 = ((long)p.M + 255) / 256, n256 = ((long)p.N + 255) / 256;
     const long pairs = sms / 2;
     const int  num_kb = (p.K + kBlock - 1) / kBlock;
-    const double c1   = (double)((m128 * n128 + sms - 1) / sms) * (1.0 + 0.2 * num_kb);
-    const double c2   = pairs > 0 ? (double)((m256 * n256 + pairs - 1) / pairs) * (2.0 + 0.35 * num_kb) : 1e30;
+    // Rounds of each tile times what one takes, us: 0.6 + 0.33 a K block for 128 x 128, 1.0 + 0.53 for a pair's 256 x 256, from [4608, 3072, 12288] (194 / 157),
+    // [4608, 3072, 3072] (53 / 42), [512, 5120, 5120] (30 / 23), [1317, 5120, 1280] (15.0 / 16.6), [2309, 4808, 1136] (26.6 / 24.3).
+    const double c1   = (double)((m128 * n128 + sms - 1) / sms) * (0.6 + 0.33 * num_kb);
+    const double c2   = pairs > 0 ? (double)((m256 * n256 + pairs - 1) / pairs) * (1.0 + 0.53 * num_kb) : 1e30;
     const int    tile = g_forced_tile > 16 ? g_forced_tile : c2 <= c1 ? 2562 : 1281;
     auto pick = [&](auto res) {
         constexpr bool kRes = decltype(res)::value;

@@ -157,6 +157,30 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
     }
 }
 
+// The same for two barriers at once: one loop and one verdict.
+__device__ __forceinline__ bool mbar_wait_warp2(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1, volatile int* abort_flag,
+                                                uint64_t limit_ns = kWaitLimitNs)
+{
+    uint64_t t0 = 0;
+#pragma unroll 1
+    for (uint32_t i = 0;; ++i) {
+        const bool first = mbar_try_wait(bar0, parity0), second = mbar_try_wait(bar1, parity1);
+        if (__all_sync(0xffffffffu, first && second)) {
+            return true;
+        }
+        if (i >= 64u) {
+            __nanosleep(kPollSleepNs);
+            if ((i & 255u) == 255u) {
+                const uint64_t now = global_timer_ns();
+                t0 = t0 == 0 ? now : t0;
+                if (__any_sync(0xffffffffu, *abort_flag != 0 || now - t0 > limit_ns)) {
+                    return false;
+                }
+            }
+        }
+    }
+}
+
 // A whole-warp wait that is expected to be long: it looks rarely, and so costs the working warps nothing.
 __device__ __forceinline__ bool mbar_wait_lazy(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t limit_ns = kWaitLimitNs)
 {
