@@ -8,6 +8,8 @@
 #include "common.cuh"
 #include "views.h"
 
+#include <type_traits>
+
 namespace lyraq {
 
 int device_sm_count();  // gemm_dense.cu
@@ -16,13 +18,25 @@ namespace bsel {
 
 constexpr int kQueryBlock  = 128;     // queries that share a list
 constexpr int kMeanThreads = 128;
+constexpr int kAtOnce      = 16;      // tokens of a thread on their way together
 constexpr int kMaxHeadDim  = 256;
 constexpr int kMaxKeys     = 1 << 30;
 constexpr int kMaxBlocks   = 32768;   // key blocks: the keys of a row are held in the registers of one thread block
 
+// A fp32 number in 64 bits by shifts: its bits, the exponent under a double's, read as the value times 2^-896, subnormals and zeros included (infinities and
+// NaN do not: their users look for them).
+__device__ __forceinline__ double widen_f32(uint32_t u) { return __hiloint2double(((int)u >> 3) & (int)0x8fffffffu, (int)(u << 29)); }
+
 // ------------------------------------------------------------------------------- means
-// A pass over memory.  A thread block takes one block of tokens of one head: D / 8 lanes a token, 16 bytes each, as many tokens at a time as the
-// threads allow; their sums meet in shared memory.  Where only the newest tokens changed, only the blocks that hold them are taken.
+// A pass over memory: 100 MB, 15 us, for q of 32760 tokens in 12 heads of 128 (measured: 28, the additions).  WARPS warps take one block of tokens of one head: D / 8 lanes a token, 16 bytes
+// each, as many tokens at a time as there are lanes for; their sums meet in shared memory.  One warp a block where there are many, which spares
+// instructions (the sums' way through shared memory, a division a channel), four where few have to be quick.
+// An addition in 64 bits for every value took 35 us: B200 does six of them a clock and SM.  So 16 tokens at a time are added in fp32 with their
+// rounding errors beside them (D. Knuth's two-sum), and the sum and the sum of errors then go to 64 bits.  Both are exact as long as
+// the exponents of the values lie close enough: with the largest E (below 2^(E + 1)) a sum of 16 is below 2^(E + 5), an error at most 2^(E - 19) and 16 of them
+// 2^(E - 15); with the smallest e all are multiples of 2^(e - M), M bits behind the point, so 24 bits hold them if E - e <= 39 - M.  Blocks whose values lie further
+// apart, or that hold infinities or NaN, are added again in 64 bits.
+// Where only the newest tokens changed, only the blocks that hold them are taken.
 struct MeansParams {
     float*      means;          // [batch][heads][blocks][head_dim]
     const void* x;
@@ -30,62 +44,148 @@ struct MeansParams {
     const int*  lens;           // tokens of each sequence, or null
     int         tokens, heads, head_dim, block, blocks;
     int         newest;         // 0: all blocks
-    int         per_head;       // thread blocks of one head
+    int         per_head;       // blocks of one head that are taken
+    int         heads_first;    // neighbouring blocks: those of the same tokens in all heads (which lie side by side), or of the same head
+    int         units;
 };
 
-template<typename T> __global__ void __launch_bounds__(kMeanThreads) block_means_kernel(const MeansParams p)
+// LANES: D / 8 where it is 8 or 16, else 0 (any)
+template<typename T, int WARPS, int LANES> __global__ void __launch_bounds__(kMeanThreads) block_means_kernel(const MeansParams p)
 {
-    __shared__ double part[kMeanThreads * 8];
+    constexpr int kUnits = kMeanThreads / (WARPS * 32), kLanes = WARPS * 32;
+    __shared__ double part_all[kUnits][kLanes * 8];
     grid_launch_dependents();
     grid_dependency_wait();
-    const int unit = (int)blockIdx.x / p.per_head, h = unit % p.heads, b = unit / p.heads;
-    int       j    = (int)blockIdx.x % p.per_head;
-    const int len  = p.lens == nullptr ? p.tokens : min(max(__ldg(p.lens + b), 0), p.tokens);
+    double* const   part = part_all[kUnits == 1 ? 0 : (int)threadIdx.x / kLanes];
+    const int       me   = (int)threadIdx.x % kLanes;
+    const int       unit = (int)blockIdx.x * kUnits + (int)threadIdx.x / kLanes;
+    if (unit >= p.units) {
+        return;    // whole warps, and with one unit a thread block never
+    }
+    auto meet = [] {
+        if (kUnits == 1) {
+            __syncthreads();
+        } else {
+            __syncwarp();
+        }
+    };
+    const int inner = p.heads_first ? p.heads : p.per_head, outer = p.heads_first ? p.per_head : p.heads;
+    const int whole = unit / inner, in = unit - whole * inner, b = whole / outer, out_of = whole - b * outer;
+    const int h  = p.heads_first ? in : out_of;
+    int       j  = p.heads_first ? out_of : in;
+    const int len = p.lens == nullptr ? p.tokens : min(max(__ldg(p.lens + b), 0), p.tokens);
     if (p.newest > 0) {
         j += max(len - p.newest, 0) / p.block;
         if (len == 0 || j > (len - 1) / p.block) {
             return;
         }
     }
-    const int lanes = p.head_dim / 8, slots = kMeanThreads / lanes;
-    const int slot = (int)threadIdx.x / lanes, c = (int)threadIdx.x % lanes * 8;
-    const int first = j * p.block, end = min(first + p.block, len);
-    double    sum[8] = {};
-    if (slot < slots) {
-        const T* src = reinterpret_cast<const T*>(p.x) + (size_t)b * p.batch_step + (size_t)h * p.head_step + (size_t)c;
-        for (int t0 = first + slot; t0 < end; t0 += 8 * slots) {
-            Vec16 v[8];
+    const int  lanes = LANES > 0 ? LANES : p.head_dim / 8, slots = kLanes / lanes;
+    const int  slot = me / lanes, c = me % lanes * 8;
+    const int  first = j * p.block, count = max(min(p.block, len - first), 0);
+    const T*   src  = reinterpret_cast<const T*>(p.x) + (size_t)b * p.batch_step + (size_t)h * p.head_step + (size_t)(first + slot) * p.token_step + (size_t)c;
+    const size_t step = (size_t)slots * p.token_step;
+    double     sum[8] = {};
+    // this thread's tokens, 16 at a time, as words of two channels each; those that do not exist are zeros
+    auto each = [&](auto take) {
+        if (slot < slots) {
+            const T* at = src;
+            for (int t = slot; t < count; t += kAtOnce * slots) {
+                Vec16 v[kAtOnce];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int t = t0 + i * slots;
-                v[i]        = Vec16{};
-                if (t < end) {
-                    v[i] = ld_nc_16(src + (size_t)t * p.token_step);
+                for (int i = 0; i < kAtOnce; ++i) {
+                    v[i] = Vec16{};
+                    if (t + i * slots < count) {
+                        v[i] = ld_nc_16(at);
+                    }
+                    at += step;
                 }
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float f[8];
-                unpack8<T>(v[i], f);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    sum[e] += (double)f[e];
-                }
+                take(v);
             }
         }
+    };
+    uint32_t most = 0, least = 0xffffffffu;      // of both channels of a word: the largest magnitude, and the smallest that is not 0, less 1
+    each([&](const Vec16* v) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float2 s = make_float2(0.0f, 0.0f), lost = s;
+            auto minus = [](float2 x, float2 y) { return fma_f32x2(y, make_float2(-1.0f, -1.0f), x); };
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) {
+                const uint32_t w = v[i].w[e], m = w & 0x7fff7fffu;
+                most  = __vmaxu2(most, m);
+                least = __viaddmin_u16x2(m, 0xffffffffu, least);
+                const float2 x = Pair<T>::to_f32(w);
+                const float2 t = add_f32x2(s, x), y = minus(t, s);
+                lost = add_f32x2(lost, add_f32x2(minus(s, minus(t, y)), minus(x, y)));
+                s    = t;
+            }
+            sum[2 * e] += (double)s.x;
+            sum[2 * e + 1] += (double)s.y;
+            sum[2 * e] += (double)lost.x;
+            sum[2 * e + 1] += (double)lost.y;
+        }
+    });
+    // exponents as the type holds them (of a subnormal: the least normal number's); bf16 sums stay below fp32's largest
+    constexpr bool kBf16 = TypeTag<T>::value == LYRAQ_BF16;
+    constexpr int  kMantissa = kBf16 ? 7 : 10, kTop = kBf16 ? 0xff - 5 : 0x1f;
+    const int  top   = (int)(max(most & 0xffffu, most >> 16) >> kMantissa), low = max((int)((min(least & 0xffffu, least >> 16) + 1u) >> kMantissa), 1);
+    const bool exact = top < kTop && top - low <= 39 - kMantissa;
+    if (kUnits == 1 ? __syncthreads_or(exact ? 0 : 1) != 0 : !__all_sync(0xffffffffu, exact)) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            part[slot * p.head_dim + c + e] = sum[e];
+            sum[e] = 0.0;
         }
+        each([&](const Vec16* v) {
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 f = Pair<T>::to_f32(v[i].w[e]);
+                    sum[2 * e] += (double)f.x;
+                    sum[2 * e + 1] += (double)f.y;
+                }
+            }
+        });
     }
-    __syncthreads();
-    float* out = p.means + (((size_t)b * (size_t)p.heads + (size_t)h) * (size_t)p.blocks + (size_t)j) * (size_t)p.head_dim;
-    for (int d = (int)threadIdx.x; d < p.head_dim; d += kMeanThreads) {
-        double s = 0.0;
-        for (int i = 0; i < slots; ++i) {
-            s += part[i * p.head_dim + d];
+    float*       out  = p.means + (((size_t)b * (size_t)p.heads + (size_t)h) * (size_t)p.blocks + (size_t)j) * (size_t)p.head_dim;
+    const bool   even = (count & (count - 1)) == 0;                   // a power of two: the product with its reciprocal is the quotient
+    const double n    = (double)max(count, 1);
+    const double inv  = __hiloint2double((1023 - (31 - __clz(max(count, 1)))) << 20, 0);   // 1 / n of a power of two, by its exponent
+    auto mean = [&](double s) {
+        return (float)(even ? s * inv : s / n);
+    };
+    if constexpr (LANES > 0 && kUnits > 1) {
+#pragma unroll
+        for (int d = LANES; d < 32; d *= 2) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], d);
+            }
         }
-        out[d] = end > first ? (float)(s / (double)(end - first)) : 0.0f;
+        if (slot < 2) {      // half of the lane's channels each
+            float4 v;
+            v.x = mean(slot == 0 ? sum[0] : sum[4]);
+            v.y = mean(slot == 0 ? sum[1] : sum[5]);
+            v.z = mean(slot == 0 ? sum[2] : sum[6]);
+            v.w = mean(slot == 0 ? sum[3] : sum[7]);
+            *reinterpret_cast<float4*>(out + c + slot * 4) = v;
+        }
+    } else {
+        if (slot < slots) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                part[slot * p.head_dim + e * lanes + c / 8] = sum[e];      // neighbouring threads beside each other
+            }
+        }
+        meet();
+        for (int d = me; d < p.head_dim; d += kLanes) {
+            double s = 0.0;
+            for (int i = 0; i < slots; ++i) {
+                s += part[i * p.head_dim + d];
+            }
+            out[d % lanes * 8 + d / lanes] = mean(s);
+        }
     }
 }
 
@@ -103,19 +203,22 @@ struct SelectParams {
     int          q_tiles, k_tiles;
 };
 
-// Products on the 64-bit tensor path (mma m8n8k4): QR x KT scores a thread block, a warp (QR / 2 or QR) x 16, K chunk by chunk through shared memory,
-// queries already in 64 bits (they may be sums over heads), keys in 32.  201 million products of [256 x 512] blocks in 12 heads of 128 are 11.5 us at
-// 64 a clock and SM.
-constexpr int kScoreThreads = 256;
-constexpr int kChunk        = 64;
+// Products on the 64-bit tensor path (mma m8n8k4): QR x KT scores a thread block, a warp (QR / 2 or QR) x 16, chunk by chunk through shared memory, already in
+// 64 bits (the queries may be sums over heads), the next chunk on its way.  201 million products of [256 x 512] blocks in 12 heads of 128 take 26 us, 30 a clock
+// and SM; the vector pipe does six.
+constexpr int    kScoreThreads = 256;
+constexpr int    kChunk        = 32;
+constexpr double kDown         = 1.8928834978668395e-270;     // 2^-896
+constexpr double kUp           = 5.282945311356653e269;       // 2^896
 
-template<int QR> __global__ void __launch_bounds__(kScoreThreads) block_scores_kernel(const SelectParams p)
+template<int QR> __global__ void __launch_bounds__(kScoreThreads, 4) block_scores_kernel(const SelectParams p)
 {
     constexpr int kWarpsQ = QR == 32 ? 2 : 1, kWarpsK = 8 / kWarpsQ;
     constexpr int kMt = QR / kWarpsQ / 8;     // fragments of 8 queries a warp
     constexpr int KT  = kWarpsK * 16;
+    constexpr int kQ  = QR * kChunk / kScoreThreads, kK = KT * kChunk / 4 / kScoreThreads;   // queries' values and keys' vectors of a thread
     __shared__ double qs[QR][kChunk + 4];     // pitches that spread a fragment's 8 x 4 values over all banks
-    __shared__ float  ks[KT][kChunk + 4];
+    __shared__ double ks[KT][kChunk + 4];
     grid_launch_dependents();
     grid_dependency_wait();
     const int kt = (int)blockIdx.x % p.k_tiles, qt = (int)blockIdx.x / p.k_tiles % p.q_tiles, unit = (int)blockIdx.x / (p.k_tiles * p.q_tiles);
@@ -127,28 +230,53 @@ template<int QR> __global__ void __launch_bounds__(kScoreThreads) block_scores_k
     const int warp = (int)threadIdx.x >> 5, lane = (int)threadIdx.x & 31;
     const int wq = warp % kWarpsQ * (QR / kWarpsQ), wk = warp / kWarpsQ * 16;
     double    acc[kMt][2][2] = {};
+    float     qv[kQ];
+    float4    kv[kK];
+    auto load = [&](int d0) {
+#pragma unroll
+        for (int u = 0; u < kQ; ++u) {
+            const int i = u * kScoreThreads + (int)threadIdx.x, r = i / kChunk, d = d0 + i % kChunk, row = qt * QR + r;
+            qv[u] = row < p.q_blocks && d < p.head_dim && heads == 1 ? ld_f32(q + (size_t)row * (size_t)p.head_dim + (size_t)d) : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < kK; ++u) {
+            const int i = u * kScoreThreads + (int)threadIdx.x, r = i / (kChunk / 4), d = d0 + i % (kChunk / 4) * 4, row = kt * KT + r;
+            kv[u] = row < p.k_blocks && d < p.head_dim ? ld_f32x4(reinterpret_cast<const float4*>(k + (size_t)row * (size_t)p.head_dim + (size_t)d))
+                                                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+    };
+    load(0);
     for (int d0 = 0; d0 < p.head_dim; d0 += kChunk) {
         const int width = min(kChunk, p.head_dim - d0);                  // a multiple of 8
         __syncthreads();
-        for (int i = (int)threadIdx.x; i < QR * kChunk; i += kScoreThreads) {
-            const int r = i / kChunk, d = i % kChunk, row = qt * QR + r;
-            double    v = 0.0;
-            if (row < p.q_blocks && d < width) {
+#pragma unroll
+        for (int u = 0; u < kQ; ++u) {
+            const int i = u * kScoreThreads + (int)threadIdx.x, r = i / kChunk, d = i % kChunk, row = qt * QR + r;
+            double    v = (double)qv[u];
+            if (heads > 1 && row < p.q_blocks && d < width) {
+                v = 0.0;
                 for (int h = 0; h < heads; ++h) {
                     v += (double)ld_f32(q + ((size_t)h * (size_t)p.q_blocks + (size_t)row) * (size_t)p.head_dim + (size_t)(d0 + d));
                 }
             }
             qs[r][d] = v;
         }
-        for (int i = (int)threadIdx.x; i < KT * (kChunk / 4); i += kScoreThreads) {
-            const int r = i / (kChunk / 4), d = i % (kChunk / 4) * 4, row = kt * KT + r;
-            float4    v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (row < p.k_blocks && d < width) {
-                v = ld_f32x4(reinterpret_cast<const float4*>(k + (size_t)row * (size_t)p.head_dim + (size_t)(d0 + d)));
+        // keys times 2^-896, and the scores times 2^896: exact but for what is far below the least fp32 number
+#pragma unroll
+        for (int u = 0; u < kK; ++u) {
+            const int    i = u * kScoreThreads + (int)threadIdx.x, r = i / (kChunk / 4), d = i % (kChunk / 4) * 4;
+            const float4 v = kv[u];
+            const float  f[4] = {v.x, v.y, v.z, v.w};
+            const bool   finite = fabsf(v.x) < INFINITY && fabsf(v.y) < INFINITY && fabsf(v.z) < INFINITY && fabsf(v.w) < INFINITY;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                ks[r][d + e] = finite ? widen_f32(__float_as_uint(f[e])) : (double)f[e] * kDown;
             }
-            *reinterpret_cast<float4*>(&ks[r][d]) = v;
         }
         __syncthreads();
+        if (d0 + kChunk < p.head_dim) {
+            load(d0 + kChunk);
+        }
 #pragma unroll 4
         for (int d = 0; d < width; d += 4) {
             double a[kMt], c[2];
@@ -158,7 +286,7 @@ template<int QR> __global__ void __launch_bounds__(kScoreThreads) block_scores_k
             }
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-                c[n] = (double)ks[wk + n * 8 + (lane >> 2)][d + (lane & 3)];
+                c[n] = ks[wk + n * 8 + (lane >> 2)][d + (lane & 3)];
             }
 #pragma unroll
             for (int m = 0; m < kMt; ++m) {
@@ -180,7 +308,7 @@ template<int QR> __global__ void __launch_bounds__(kScoreThreads) block_scores_k
             for (int e = 0; e < 2; ++e) {
                 const int row = qt * QR + wq + m * 8 + (lane >> 2), col = kt * KT + wk + n * 8 + (lane & 3) * 2 + e;
                 if (row < p.q_blocks && col < p.k_blocks) {
-                    out[(size_t)row * (size_t)p.k_blocks + (size_t)col] = (float)acc[m][n][e];
+                    out[(size_t)row * (size_t)p.k_blocks + (size_t)col] = (float)(acc[m][n][e] * kUp);
                 }
             }
         }
@@ -204,14 +332,17 @@ struct Range {
         const int  len   = p.k_lens == nullptr ? p.keys : min(max(__ldg(p.k_lens + b), 0), p.keys);
         // places beyond the keys, on either side, are all alike
         const int  start = p.q_start == nullptr ? p.keys - p.queries : min(max(__ldg(p.q_start + b), -kMaxKeys), kMaxKeys);
-        const long long first = (long long)start + (long long)i * kQueryBlock;
-        const long long last  = first + min(kQueryBlock, p.queries - i * kQueryBlock) - 1;
-        auto block_of = [&](long long t) { return (t >= 0 ? t : t - (p.block - 1)) / p.block; };   // downwards
-        const long long e = (len + (long long)p.block - 1) / p.block;
-        end  = (int)(p.causal ? min(e, max(block_of(last) + 1, 0ll)) : e);
+        // in 32 bits: a place beyond the keys by 2^30 and more is as good as one there
+        const int first = (int)min((long long)start + (long long)i * kQueryBlock, (long long)kMaxKeys);
+        const int last  = min(first + min(kQueryBlock, p.queries - i * kQueryBlock) - 1, kMaxKeys);
+        auto block_of = [&](int t) { return t >= 0 ? t / p.block : -((p.block - 1 - t) / p.block); };   // downwards
+        const int e = (int)(((unsigned)len + (unsigned)p.block - 1u) / (unsigned)p.block);
+        end  = p.causal ? min(e, max(block_of(last) + 1, 0)) : e;
         sink = p.sink;
-        low  = p.window > 0 ? (int)max(block_of(first) - (p.window - 1), -1ll) : 0;
-        high = p.window > 0 ? (int)max(min(block_of(last) + (p.window - 1), (long long)kMaxKeys), -1ll) : -1;
+        // windows wider than the keys are as good as all of them
+        const int w = min(p.window - 1, kMaxKeys / 2);
+        low  = p.window > 0 ? max(block_of(first) - w, -1) : 0;
+        high = p.window > 0 ? max(min(block_of(last) + w, kMaxKeys), -1) : -1;
     }
     __device__ __forceinline__ uint32_t key(int j, float s) const { return j >= end ? 0u : j < sink || (j >= low && j <= high) ? 0xffffffffu : score_key(s); }
 };
@@ -372,15 +503,28 @@ int lyraq_block_means(float* means, const void* x, int dtype, size_t batch_step,
     }
     // `newest` tokens touch one block more than they fill, at most
     const size_t touched  = newest == 0 ? blocks : ((size_t)newest + (size_t)block - 2) / (size_t)block + 1;
-    const size_t per_head = touched < blocks ? touched : blocks, grid = per_head * batch * (size_t)heads;
-    if (grid > 0x7fffffffu) {
+    const size_t per_head = touched < blocks ? touched : blocks, units = per_head * batch * (size_t)heads;
+    const bool   few      = units <= 592;      // a warp for each would leave schedulers without one
+    const size_t grid     = few ? units : (units + 3) / 4;
+    if (units > 0x7ffffff0u) {
         return LYRAQ_ERR_UNSUPPORTED;
     }
     const bsel::MeansParams p{means,       x,     batch_step, token_step, head_step, lens, (int)tokens, heads, head_dim, block, (int)blocks,
-                              newest < bsel::kMaxKeys ? newest : bsel::kMaxKeys, (int)per_head};
-    const cudaError_t e = dtype == LYRAQ_BF16
-                              ? launch_kernel(bsel::block_means_kernel<__nv_bfloat16>, (unsigned)grid, (unsigned)bsel::kMeanThreads, (size_t)0, (cudaStream_t)stream, 1u, p)
-                              : launch_kernel(bsel::block_means_kernel<__half>, (unsigned)grid, (unsigned)bsel::kMeanThreads, (size_t)0, (cudaStream_t)stream, 1u, p);
+                              newest < bsel::kMaxKeys ? newest : bsel::kMaxKeys, (int)per_head, head_step < token_step ? 1 : 0, (int)units};
+    auto launch = [&](auto* kernel) {
+        return launch_kernel(kernel, (unsigned)grid, (unsigned)bsel::kMeanThreads, (size_t)0, (cudaStream_t)stream, 1u, p);
+    };
+    auto pick = [&](auto type, auto lanes) {
+        using T = decltype(type);
+        constexpr int kLanes = decltype(lanes)::value;
+        return few ? launch(bsel::block_means_kernel<T, 4, kLanes>) : launch(bsel::block_means_kernel<T, 1, kLanes>);
+    };
+    auto pick_lanes = [&](auto type) {
+        return head_dim == 128 ? pick(type, std::integral_constant<int, 16>{})
+               : head_dim == 64 ? pick(type, std::integral_constant<int, 8>{})
+                                : pick(type, std::integral_constant<int, 0>{});
+    };
+    const cudaError_t e = dtype == LYRAQ_BF16 ? pick_lanes(__nv_bfloat16{}) : pick_lanes(__half{});
     return cuda_status(e, "cudaLaunchKernelEx(block_means_kernel)");
 }
 
@@ -476,7 +620,9 @@ int lyraq_select_blocks(const lyraq_select_blocks_t* s, void* workspace, size_t 
     auto top = [&](auto* kernel, int warps) {
         return launch_kernel(kernel, (unsigned)(warps == 1 ? (rows + 3) / 4 : rows), warps == 1 ? 128u : (unsigned)(warps * 32), (size_t)0, st, 1u, p);
     };
-    const cudaError_t e = k_blocks <= 128 ? top(bsel::block_top_kernel<1, 4>, 1)
+    // few rows are spread over more warps each: 32 rows of 512 7.4 us instead of 13; 864 rows of 72 5.6 us with one warp each, 13.9 with eight
+    const cudaError_t e = rows <= 148 && k_blocks <= 1024 ? top(bsel::block_top_kernel<8, 4>, 8)
+                          : k_blocks <= 128 ? top(bsel::block_top_kernel<1, 4>, 1)
                           : k_blocks <= 512 ? top(bsel::block_top_kernel<1, 16>, 1)
                           : k_blocks <= 2048 ? top(bsel::block_top_kernel<4, 16>, 4)
                           : k_blocks <= 8192 ? top(bsel::block_top_kernel<16, 16>, 16)

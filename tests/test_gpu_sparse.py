@@ -1,5 +1,7 @@
 """GPU tests of attention over selected key blocks against the 64-bit restatement in oracle/sparse.py."""
 
+import math
+
 import pytest
 import torch
 
@@ -81,6 +83,41 @@ def test_means_of_numbers_at_the_ends_of_the_type(ops):
         got = ops.block_means(x.cuda(), 64).cpu()
         want = sparse.means(x, 64)
         assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(7.0), want.nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("n,block", [(128, 128), (640, 64), (50000, 64)])
+def test_means_of_values_far_apart(ops, dtype, n, block):
+    """Exponents on both sides of what sums in fp32 with their errors hold exactly, cancellation, and blocks that need 64 bits beside others: the means are
+    those of exact sums."""
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(1, n, 2, 128, generator=g)
+    low, high = (-126, 126) if dtype == BF16 else (-14, 15)
+    for i, spread in enumerate((0, 10, 28, 29, 30, 31, 32, 33, 34, 40, 100, 250)):
+        c = slice(i * 8, i * 8 + 8)
+        at = torch.randint(0, spread + 1, (n, 2, 8), generator=g) + low
+        x[0, :, :, c] = torch.ldexp(1 + torch.rand(n, 2, 8, generator=g), at.clamp(low, high - 1)) * (1 - 2 * torch.randint(0, 2, (n, 2, 8), generator=g))
+    x[0, 1::2, :, 100:104] = -x[0, ::2, :, 100:104]                    # sums of 0
+    x[0, ::3, :, 104] = 2.0 ** high * 1.5                             # sums beyond fp32's largest on the way, for bf16
+    x[0, 1::3, :, 104] = -2.0 ** high * 1.5
+    x = x.to(dtype)
+    got = ops.block_means(x.cuda(), block).cpu()
+    check_status()
+    m = torch.zeros(1, 2, sparse.blocks(n, block), 128, dtype=torch.float64)
+    for j in range(m.shape[2] if n < 10000 else 3):
+        part = x[0, j * block:(j + 1) * block].double()
+        for h in range(2):
+            for c in range(128):
+                m[0, h, j, c] = math.fsum(part[:, h, c].tolist()) / part.shape[0]
+        want = m[0, :, j]
+        # an exact sum, against one in 64 bits: 2^-50 of the magnitudes before it is rounded
+        slack = part.abs().sum(0) / part.shape[0] * 2.0 ** -50
+        half = torch.maximum(want.abs() * 2.0 ** -24, torch.tensor(2.0 ** -150, dtype=torch.float64))
+        assert bool(((got[0, :, j].double() - want).abs() <= half + slack).all())
+    # every block against the restatement: either side is half a step of fp32 and 2^-50 of the magnitudes from the exact mean
+    size = sparse.means(x.double().abs(), block).double()
+    want = sparse.means(x, block).double()
+    assert bool(((got.double() - want).abs() <= want.abs() * 2.0 ** -23 + size * 2.0 ** -48 + 2.0 ** -149).all())
 
 
 # ----------------------------------------------------------------------------- selection
