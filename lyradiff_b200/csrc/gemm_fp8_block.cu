@@ -3,17 +3,23 @@
 //   Y[M,N] = T( epi( sum_kb s_x[m,kb] s_w[n/128,kb] sum_{k in kb} X[m,k] W[n,k]  + beta R + bias ) )
 //
 // The scales are any fp32 numbers, so the tensor cores cannot apply them: a K block of 128 is one product of its own in tensor memory, and the
-// epilogue warps add it, times its factor, to fp32 sums that they hold in registers for the whole tile (128 a thread).  Tensor memory holds two
-// products, so that the next is formed while one is taken; a pair's 256 x 256 product is 512 clocks of tensor pipe, and taking it is 256 clocks of
-// tensor-memory loads and as many of packed multiply-adds, shared by two warps per scheduler.
+// epilogue warps add it, times its factor, to fp32 sums that they hold in registers for the whole tile (64 a thread).  Tensor memory holds two products of a
+// pair's tile (four of a lone CTA's), so that the next is formed while one is taken.
 //
-// Persistent, 384 threads, warp-specialised, as a CTA pair (256 x 256 tile, cta_group::2) or one CTA (128 x 128):
+// Persistent, 640 threads, warp-specialised, as a CTA pair (256 x 256 tile, cta_group::2) or one CTA (128 x 128):
 //   warp 0    : TMA producer   - operand tiles (128-byte swizzle) into a ring of stages, one K block each; each CTA of a pair loads its own A rows
 //                                and its half of the B rows.
 //   warp 1    : MMA issuer     - four MMAs a K block into the product buffer that is free; commits the stage and the product.
 //   warp 2    : allocates / frees tensor memory.
-//   warps 4-11: epilogue       - per K block: products -> sums; at the end of a tile residual, bias, GELU, store.  A lane owns a row, so its factor is
+//   warps 4-19: epilogue       - per K block: products -> sums; at the end of a tile residual, bias, GELU, store.  A lane owns a row, so its factor is
 //                                one number per K block: its row's scale times the scale of the warp's columns, which lie in one block of W.
+//
+// What bounds it: the way of a product from its last MMA to the next one in its place (completion, loads out of tensor memory, the word back to the issuer, about
+// 1400 clocks with two in flight), against 512 of MMAs for a pair's K block, which take about 600 beside the loads into shared memory; 1000 measured.
+// [4680, 13824, 5120]: 311 us in a burst (2.1 PFLOP/s), [4608, 3072, 12288] 155; the framework's FP8 product with one scale takes 117 for the latter.
+// Measured on the way: eight epilogue warps with 128 sums a thread 360 and 180 (two a scheduler do not hide the loads' latency).  Not kept: products in pieces
+// of 128 columns (an A tile read twice bounds the MMAs: 180), a pair's tile of 256 x 128 (198), the next product's loads ahead of the additions (229), two or
+// four CTAs of a cluster along K where tiles are few (the cluster's launch takes the 5 us that it saves).
 // Every mbarrier wait is bounded; on a timeout the role records it in the status word, raises the block's abort flag and all roles fall
 // through to the common exit, where tensor memory is freed.
 #include "fp8_block.cuh"
