@@ -701,7 +701,7 @@ int lyraq_debug_sparse_attention_wait_test(int skip_loads, unsigned int wait_lim
 int lyraq_sparse_attention(const lyraq_sparse_attention_t* a, void* stream)
 {
     if (a == nullptr || a->q_heads < 0 || a->k_heads < 0 || a->lists < 0 || a->head_dim < 0 || a->count < 0 || !(a->softmax_scale > 0.0f) ||
-        !(a->softmax_scale < INFINITY)) {
+        !(a->softmax_scale * 1.4426950408889634f < INFINITY)) {
         return LYRAQ_ERR_INVALID_ARG;
     }
     if ((a->dtype != LYRAQ_F16 && a->dtype != LYRAQ_BF16) || (a->head_dim != 64 && a->head_dim != 128) || (a->block != 64 && a->block != 128)) {
@@ -735,6 +735,9 @@ int lyraq_sparse_attention(const lyraq_sparse_attention_t* a, void* stream)
     if ((a->queries > 1 && a->q_token == 0) || (a->q_heads > 1 && a->q_head == 0) || (a->keys > 1 && (a->k_token == 0 || a->v_token == 0)) ||
         (a->k_heads > 1 && (a->k_head == 0 || a->v_head == 0))) {
         return LYRAQ_ERR_UNSUPPORTED;
+    }
+    if ((a->batch > 1 && a->o_batch == 0) || (a->queries > 1 && a->o_token == 0) || (a->q_heads > 1 && a->o_head == 0)) {
+        return LYRAQ_ERR_INVALID_ARG;      // results in one place
     }
     const size_t dim = (size_t)a->head_dim;
     auto view = [&](const void* p, size_t sb, size_t n, size_t st, int heads, size_t sh) { return view_of(p, 2, a->batch, sb, n, st, (size_t)heads, sh, dim); };

@@ -80,7 +80,8 @@ def test_attention_refusals(lib):
         return lib.lyraq_sparse_attention(ctypes.byref(_lib.SparseAttentionArgs(**f)), None)
     assert lib.lyraq_sparse_attention(None, None) == INVALID
     assert attend(batch=0) == attend(queries=0) == attend(q_heads=0) == 0
-    for scale in (0.0, -1.0, float("inf"), float("nan")):
+    assert attend(o_batch=0) == attend(o_token=0) == attend(o_head=0) == INVALID
+    for scale in (0.0, -1.0, float("inf"), float("nan"), 3e38):
         assert attend(softmax_scale=scale) == INVALID
     assert attend(k_heads=3) == attend(lists=1) == attend(count=-1) == attend(q=None) == attend(k=None) == attend(index=None) == attend(counts=None) == INVALID
     assert attend(q=P[0] + 2) == attend(out=P[3] + 8) == attend(k_token=130) == attend(v_head=1 << 40) == attend(counts=P[5] + 1) == INVALID
