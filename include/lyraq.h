@@ -121,7 +121,7 @@ LYRAQ_API int lyraq_debug_sparse_attention_wait_test(int skip_loads, unsigned in
 /* lyraq_debug_skinny_wait_test for the few-row kernel of lyraq_gemm_fp8_block.  It has no counterpart in the reference. */
 LYRAQ_API int lyraq_debug_fp8_block_rows_wait_test(int stalled_rank, unsigned int wait_limit_ms);
 
-/* Test / sweep hook: the kernel of lyraq_gemm_fp8_block.  0 = automatic (default); 2562 = CTA pair, 256 x 256 tile; 1281 = one CTA, 128 x 128; 16 = the few-row kernel wherever it can, the automatic choice elsewhere.  Process-wide, not thread-safe.  It has no counterpart in the reference. */
+/* Test / sweep hook: the kernel of lyraq_gemm_fp8_block.  0 = automatic (default); 2562 = CTA pair, 256 x 256 tile; 1281 = one CTA, 128 x 128; 1282, 1284, 1288 = that with 2, 4 or 8 CTAs along K; 16 = the few-row kernel wherever it can, the automatic choice elsewhere.  Process-wide, not thread-safe.  It has no counterpart in the reference. */
 LYRAQ_API int lyraq_debug_force_fp8_block_tile(int code);
 
 /* lyraq_debug_skinny_wait_test for the few-row FP4 kernel.  It has no counterpart in the reference. */

@@ -40,6 +40,7 @@ struct Input {
 struct GemmParams {
     int           M, N, K;
     int           m_tiles, n_tiles;
+    int           splits;     // CTAs along K
     unsigned int* status;
     void*         C;          // [M, N] of c_dtype: F16, BF16 or F32
     int           c_dtype;

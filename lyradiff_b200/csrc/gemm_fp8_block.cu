@@ -18,8 +18,8 @@
 // 1400 clocks with two in flight), against 512 of MMAs for a pair's K block, which take about 600 beside the loads into shared memory; 1000 measured.
 // [4680, 13824, 5120]: 311 us in a burst (2.1 PFLOP/s), [4608, 3072, 12288] 155; the framework's FP8 product with one scale takes 117 for the latter.
 // Measured on the way: eight epilogue warps with 128 sums a thread 360 and 180 (two a scheduler do not hide the loads' latency).  Not kept: products in pieces
-// of 128 columns (an A tile read twice bounds the MMAs: 180), a pair's tile of 256 x 128 (198), the next product's loads ahead of the additions (229), two or
-// four CTAs of a cluster along K where tiles are few (the cluster's launch takes the 5 us that it saves).
+// of 128 columns (an A tile read twice bounds the MMAs: 180), a pair's tile of 256 x 128 (198), the next product's loads ahead of the additions (229).
+// Where few tiles have many K blocks, a cluster of 2, 4 or 8 CTAs shares out the K blocks of a tile.
 // Every mbarrier wait is bounded; on a timeout the role records it in the status word, raises the block's abort flag and all roles fall
 // through to the common exit, where tensor memory is freed.
 #include "fp8_block.cuh"
@@ -45,6 +45,7 @@ constexpr int kEpiWarps  = 16;
 constexpr int kBox       = 32 * 64;      // one warp's staging box: 32 rows x 32 columns of a 16-bit type
 constexpr int kBiasBytes = 64 * 2;       // one warp's bias: up to 64 columns of a 16-bit type (fp32, which uses no boxes, keeps its there)
 constexpr int kBarBytes  = 256;
+constexpr int kPartBytes = 32 * 32 * 4;  // one warp's sums of one CTA along K, [column][row]
 constexpr int kOtherRegs = 32;
 constexpr int kEpiRegs   = 112;
 static_assert(128 * kOtherRegs + 512 * kEpiRegs <= kThreads * 96, "the split draws on what the block was launched with");
@@ -107,9 +108,16 @@ template<bool IN> __device__ __forceinline__ void move_box(uint8_t* box, uint16_
     }
 }
 
+__device__ __forceinline__ void st_cluster_u32(uint32_t cluster_addr, uint32_t v)
+{
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+}
+
 // NARROW: 16-bit rows that start on less than 16 bytes, which no TMA store takes.  A kernel of its own: its stores beside the others cost 340 us for 318 with
 // [4680, 13824, 5120].
-template<int BLOCK_N, int CTAS, bool RES, bool NARROW>
+// SPLIT: a tile is a cluster's, its K blocks shared out among the CTAs.  Each warp sends its sums to the CTA that owns its part of the tile, which adds them in
+// rank order and finishes that part.
+template<int BLOCK_N, int CTAS, bool RES, bool NARROW, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_c,
                       const GemmParams p)
@@ -121,6 +129,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
     constexpr int kCols   = BLOCK_N / 4;      // columns per epilogue warp: 64 or 32, all of one block of W
     constexpr int kChunks = kCols / 32;
     constexpr int kAhead  = 2;                // K blocks whose scales are fetched together
+    static_assert(!SPLIT || (CTAS == 1 && kChunks == 1 && S::kEpiOffset >= kEpiWarps * kPartBytes), "the partial sums take the operands' place");
 
     extern __shared__ uint8_t smem_raw[];
     // the dynamic shared window starts at the same offset in every CTA of the kernel, so both CTAs of a pair get the same layout
@@ -138,8 +147,10 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
     const int      lane    = threadIdx.x & 31;
     const uint32_t rank    = (CTAS == 2) ? cluster_ctarank() : 0u;  // position in the pair; 0 = leader
     const bool     leader  = (rank == 0);
-    const int      unit    = (CTAS == 2) ? (int)(blockIdx.x >> 1) : (int)blockIdx.x;
-    const int      n_units = (CTAS == 2) ? (int)(gridDim.x >> 1) : (int)gridDim.x;
+    const int      splits  = SPLIT ? p.splits : 1;                  // CTAs along K
+    const int      unit    = SPLIT ? (int)blockIdx.x / splits : (CTAS == 2) ? (int)(blockIdx.x >> 1) : (int)blockIdx.x;
+    const int      n_units = SPLIT ? (int)gridDim.x / splits : (CTAS == 2) ? (int)(gridDim.x >> 1) : (int)gridDim.x;   // SPLIT: one for each tile
+    const int      part    = SPLIT ? (int)cluster_ctarank() : 0;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -177,6 +188,8 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
 
     const int num_tiles = p.m_tiles * p.n_tiles;
     const int num_kb    = (p.K + kBlock - 1) / kBlock;
+    const int kb_first  = SPLIT ? num_kb * part / splits : 0;        // this CTA's K blocks
+    const int kb_end    = SPLIT ? num_kb * (part + 1) / splits : num_kb;
 
     if (warp < kEpiWarp0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
@@ -190,7 +203,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                 tile_coords(tile, p.m_tiles, p.n_tiles, m_blk, n_blk);
                 const int a_row = m_blk * kTileM + (int)rank * kBlockM;
                 const int b_row = n_blk * BLOCK_N + (int)rank * (BLOCK_N / CTAS);
-                for (int kb = 0; kb < num_kb; ++kb) {
+                for (int kb = kb_first; kb < kb_end; ++kb) {
                     if (!mbar_wait_warp(empty_bar(stage), phase ^ 1u, abort_flag)) {
                         report_timeout(p.status, 0x7100u | (unsigned)stage);
                         *abort_flag = 1;
@@ -242,9 +255,9 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
         } else if (warp == 1 && leader) {
             // -------------------------------------------------------------- MMA issuer (the leader CTA only)
             constexpr uint32_t kIdesc = umma_idesc(1u, 0u, kTileM, BLOCK_N);
-            int       stage = 0, buf = 0, kb = 0;
+            int       stage = 0, buf = 0, kb = kb_first;
             uint32_t  phase = 0, buf_phase = 0;
-            long long left  = (long long)((num_tiles - unit + n_units - 1) / n_units) * num_kb;   // K blocks of all its tiles
+            long long left  = (long long)((num_tiles - unit + n_units - 1) / n_units) * (kb_end - kb_first);   // K blocks of all its tiles
             // The waits for the next K block stand between the MMAs of this one: the pipe has work while they pass (a passed wait costs about 100 clocks,
             // as much as two MMAs; [1317, 1280, 5120] 18.1 -> 16.2 us).  With two products in tensor memory the one before is still being taken then, and
             // they stand in front of them (388 us against 315 for [4680, 13824, 5120]).
@@ -274,7 +287,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                     mma(0);
                     mma(1);
                 }
-                kb = kb + 1 == num_kb ? 0 : kb + 1;
+                kb = kb + 1 == kb_end ? kb_first : kb + 1;
                 if (++stage == kStages) {
                     stage = 0;
                     phase ^= 1u;
@@ -303,6 +316,10 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                 *abort_flag = 1;
             }
         }
+        if constexpr (SPLIT) {
+            cluster_sync_all();   // the two around the partial sums
+            cluster_sync_all();
+        }
     } else {
         // ------------------------------------------------------------------ epilogue (warps 4..19)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
@@ -329,13 +346,13 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
             auto fetch = [&](int kb, float* sx, float* sw) {
 #pragma unroll
                 for (int i = 0; i < kAhead; ++i) {
-                    const bool in = there && kb + i < num_kb;
+                    const bool in = there && kb + i < kb_end;
                     sx[i] = in ? ld_f32(xs + (size_t)(kb + i) * p.xs.block_step) : 0.0f;
                     sw[i] = in ? ld_f32(ws + kb + i) : 0.0f;
                 }
             };
             float sx[kAhead], sw[kAhead];
-            fetch(0, sx, sw);
+            fetch(kb_first, sx, sw);
             uint32_t bias_here[kChunks];
 #pragma unroll
             for (int i = 0; i < kChunks; ++i) {
@@ -354,18 +371,18 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                     acc[c][i] = 0u;
                 }
             }
-            for (int kb0 = 0; ok && kb0 < num_kb; kb0 += kAhead) {
+            for (int kb0 = kb_first; ok && kb0 < kb_end; kb0 += kAhead) {
                 float f[kAhead];
 #pragma unroll
                 for (int i = 0; i < kAhead; ++i) {
                     f[i] = sx[i] * sw[i];
                 }
-                if (kb0 + kAhead < num_kb) {
+                if (kb0 + kAhead < kb_end) {
                     fetch(kb0 + kAhead, sx, sw);
                 }
 #pragma unroll
                 for (int i = 0; i < kAhead; ++i) {
-                    if (kb0 + i < num_kb && ok) {
+                    if (kb0 + i < kb_end && ok) {
                         if (!mbar_wait_warp(tmem_full_bar(buf), buf_phase, abort_flag)) {
                             if (lane == 0) {
                                 report_timeout(p.status, 0x7400u | (unsigned)buf);
@@ -409,7 +426,38 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                     }
                 }
             }
-            if (!ok) {
+            if constexpr (SPLIT) {
+                cluster_sync_all();   // every CTA has taken its last product: the operands' stages are free
+                const int w = warp - kEpiWarp0, own = kEpiWarps / splits, owner = w / own;
+                const uint32_t to = smem_base + (uint32_t)((w % own * splits + part) * kPartBytes + lane * 4);
+                if (ok) {
+                    const uint32_t there_at = map_to_cta(to, (uint32_t)owner);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        st_cluster_u32(there_at + (uint32_t)i * 128u, acc[0][i]);
+                    }
+                } else if (lane == 0) {
+                    // one CTA that gave up leaves every part of the tile without its sums, so none of the cluster stores anything
+                    for (int r = 0; r < splits; ++r) {
+                        st_cluster_u32(map_to_cta(smem_u32(const_cast<int*>(abort_flag)), (uint32_t)r), 1u);
+                    }
+                }
+                cluster_sync_all();
+                if (owner != part || *abort_flag != 0) {
+                    break;
+                }
+                const float* from = reinterpret_cast<const float*>(gen_base + (w % own * splits) * kPartBytes) + lane;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    acc[0][i] = __float_as_uint(from[i * 32]);
+                }
+                for (int r = 1; r < splits; ++r) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        acc[0][i] = __float_as_uint(__uint_as_float(acc[0][i]) + from[r * (kPartBytes / 4) + i * 32]);
+                    }
+                }
+            } else if (!ok) {
                 break;
             }
             if (p.bias != nullptr) {
@@ -534,7 +582,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
     }
 }
 
-template<int BLOCK_N, int CTAS, bool RES, bool NARROW> static int launch(const uint8_t* X, const uint8_t* W, GemmParams p, int sms, cudaStream_t stream)
+template<int BLOCK_N, int CTAS, bool RES, bool NARROW, bool SPLIT> static int launch(const uint8_t* X, const uint8_t* W, GemmParams p, int sms, cudaStream_t stream)
 {
     using S = Smem<BLOCK_N, CTAS>;
     CUtensorMap ta, tb;
@@ -553,22 +601,23 @@ template<int BLOCK_N, int CTAS, bool RES, bool NARROW> static int launch(const u
     p.m_tiles = (int)(((long)p.M + kBlockM * CTAS - 1) / (kBlockM * CTAS));
     p.n_tiles = (int)(((long)p.N + BLOCK_N - 1) / BLOCK_N);
     const long long tiles = (long long)p.m_tiles * p.n_tiles;
-    if (tiles > 0x40000000ll) {
+    if (tiles > (SPLIT ? 0x1000000ll : 0x40000000ll)) {
         return LYRAQ_ERR_UNSUPPORTED;
     }
     const long long units = sms / CTAS;
-    const int       grid  = (int)(tiles < units ? tiles : units) * CTAS;
-    auto            kern  = gemm_fp8_block_kernel<BLOCK_N, CTAS, RES, NARROW>;
+    const int       grid  = SPLIT ? (int)tiles * p.splits : (int)(tiles < units ? tiles : units) * CTAS;
+    auto            kern  = gemm_fp8_block_kernel<BLOCK_N, CTAS, RES, NARROW, SPLIT>;
     static bool     smem_raised[64] = {};
     st = raise_dynamic_smem_once(kern, (int)S::kTotal, smem_raised, "cudaFuncSetAttribute(gemm_fp8_block_kernel, dynamic shared memory)");
     if (st != LYRAQ_OK) {
         return st;
     }
-    return cuda_status(launch_kernel(kern, (unsigned)grid, (unsigned)kThreads, (size_t)S::kTotal, stream, (unsigned)CTAS, ta, tb, tc, p),
+    return cuda_status(launch_kernel(kern, (unsigned)grid, (unsigned)kThreads, (size_t)S::kTotal, stream, (unsigned)(SPLIT ? p.splits : CTAS), ta, tb, tc, p),
                        "cudaLaunchKernelEx(gemm_fp8_block_kernel)");
 }
 
-// forced kernel for tests and sweeps: 0 = automatic, 16 = the few-row kernel (up to 16 rows), 2562 = CTA pair with 256 x 256, 1281 = one CTA with 128 x 128
+// forced kernel for tests and sweeps: 0 = automatic, 16 = the few-row kernel (up to 16 rows), 2562 = CTA pair with 256 x 256, 1281 = one CTA with 128 x 128,
+// 1282, 1284, 1288 = that with 2, 4 or 8 CTAs along K
 static int g_forced_tile = 0;
 
 bool few_rows(int m, int n, int k)
@@ -582,7 +631,11 @@ bool few_rows(int m, int n, int k)
 
 bool few_rows_quantize(int m, int n, int k) { return few_rows(m, n, k) && (g_forced_tile == 16 || rows_quantize_pays(m, n, k, device_sm_count())); }
 
-static int run(const Input& X, const uint8_t* W, const GemmParams& p, int sms, cudaStream_t stream)
+// What a split costs, us: the cluster's launch and the partial sums' way (2.5 with 2 CTAs, 3.2 with 4, 3.6 with 8).  One CTA / the split it picks, us:
+// [64, 5120, 13824] 35.9 / 25.0, [300, 1280, 5120] 15.3 / 10.1, [28, 1290, 12480] 33.7 / 11.7, [154, 1280, 2048] 8.1 / 7.3; [17, 1280, 1280] 5.7 against 6.9 stays whole.
+constexpr double kSplitCost = 3.2;
+
+static int run(const Input& X, const uint8_t* W, GemmParams p, int sms, cudaStream_t stream)
 {
     if (few_rows(p.M, p.N, p.K)) {
         return launch_rows(X, W, p, sms, stream);
@@ -594,11 +647,34 @@ static int run(const Input& X, const uint8_t* W, const GemmParams& p, int sms, c
     // [4608, 3072, 3072] (53 / 42), [512, 5120, 5120] (30 / 23), [1317, 5120, 1280] (15.0 / 16.6), [2309, 4808, 1136] (26.6 / 24.3).
     const double c1   = (double)((m128 * n128 + sms - 1) / sms) * (0.6 + 0.33 * num_kb);
     const double c2   = pairs > 0 ? (double)((m256 * n256 + pairs - 1) / pairs) * (1.0 + 0.53 * num_kb) : 1e30;
-    const int    tile = g_forced_tile > 16 ? g_forced_tile : c2 <= c1 ? 2562 : 1281;
+    int          tile = g_forced_tile > 16 ? g_forced_tile : c2 <= c1 ? 2562 : 1281;
+    p.splits = 1;
+    if (g_forced_tile > 1281 && g_forced_tile < 1289) {
+        p.splits = g_forced_tile - 1280;
+        while (p.splits > num_kb) {
+            p.splits /= 2;
+        }
+    } else if (g_forced_tile == 0) {
+        // CTAs along K where few tiles have many K blocks, in one wave of clusters (of 4 and 8 some SMs of a GPC are left over): kSplitCost more a call
+        double best = c1 < c2 ? c1 : c2;
+        for (int s = 2; s <= 8 && s <= num_kb; s *= 2) {
+            const long   room = s == 2 ? sms / 2 : s == 4 ? sms * 35l / 148 : sms * 16l / 148;
+            const double cost = kSplitCost + 0.6 + 0.33 * ((num_kb + s - 1) / s);
+            if (m128 * n128 <= room && cost < best) {
+                best     = cost;
+                p.splits = s;
+            }
+        }
+    }
+    if (p.splits > 1) {
+        tile = 1282;
+    }
     const bool narrow = p.c_dtype != LYRAQ_F32 && (p.N & 7) != 0;
     auto pick = [&](auto res, auto nar) {
         constexpr bool kRes = decltype(res)::value, kNarrow = decltype(nar)::value;
-        return tile == 2562 ? launch<256, 2, kRes, kNarrow>(X.codes, W, p, sms, stream) : launch<128, 1, kRes, kNarrow>(X.codes, W, p, sms, stream);
+        return tile == 2562   ? launch<256, 2, kRes, kNarrow, false>(X.codes, W, p, sms, stream)
+               : tile == 1282 ? launch<128, 1, kRes, kNarrow, true>(X.codes, W, p, sms, stream)
+                              : launch<128, 1, kRes, kNarrow, false>(X.codes, W, p, sms, stream);
     };
     using Yes = std::true_type;
     using No  = std::false_type;
@@ -637,7 +713,7 @@ extern "C" {
 
 int lyraq_debug_force_fp8_block_tile(int code)
 {
-    if (code != 0 && code != 16 && code != 1281 && code != 2562) {
+    if (code != 0 && code != 16 && code != 1281 && code != 1282 && code != 1284 && code != 1288 && code != 2562) {
         return LYRAQ_ERR_INVALID_ARG;
     }
     fp8b::g_forced_tile = code;

@@ -200,6 +200,50 @@ def test_large_products_are_exact(ops, tile, code, m, n, k):
         assert torch.equal(y, want.to(dtype))
 
 
+SPLIT = [1282, 1284, 1288]      # CTAs along K
+
+
+@pytest.mark.parametrize("code", SPLIT)
+@pytest.mark.parametrize("m,n,k", SHAPES + [(20, 136, 144), (77, 1300, 5136)])
+def test_product_with_k_over_a_cluster(ops, tile, code, m, n, k):
+    test_product_of_every_kernel(ops, tile, code, m, n, k)
+
+
+@pytest.mark.parametrize("code", SPLIT)
+@pytest.mark.parametrize("dtype", TYPES + [torch.float32])
+@pytest.mark.parametrize("gelu,bias,residual", [(True, True, False), (True, True, True)])
+@pytest.mark.parametrize("m,n", [(33, 72), (140, 300), (260, 131)])
+def test_epilogues_with_k_over_a_cluster(ops, tile, code, dtype, gelu, bias, residual, m, n):
+    test_epilogues_and_types(ops, tile, code, dtype, gelu, bias, residual, m, n)
+
+
+@pytest.mark.parametrize("code,m", [(code, m) for code in SPLIT for m in (17, 300)])
+def test_scales_with_k_over_a_cluster(ops, tile, code, m):
+    test_scales_of_every_row_and_block_reach_their_values(ops, tile, code, m)
+
+
+@pytest.mark.parametrize("code,m,n,k", [(0, 64, 5120, 13824), (0, 17, 33, 40000), (1282, 700, 3000, 1136), (1284, 300, 2100, 9232), (1288, 129, 1111, 13824)])
+def test_large_products_with_k_over_a_cluster_are_exact(ops, tile, code, m, n, k):
+    """More clusters than run at once, and the automatic choice."""
+    test_large_products_are_exact(ops, tile, code, m, n, k)
+
+
+def test_k_over_a_cluster_gives_the_same_bits_again_and_captured(ops, tile):
+    x, w, b, r = (cu(t) if torch.is_tensor(t) else tuple(cu(u) for u in t) for t in problem(40, 300, 9232, torch.bfloat16, 11, True, True))
+    first = torch.empty(40, 300, dtype=torch.bfloat16, device="cuda")
+    ops.gemm_fp8_block(*w, *x, first, b, r)
+    check_status()
+    again = torch.empty_like(first)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.gemm_fp8_block(*w, *x, again, b, r)
+    for _ in range(3):
+        again.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(again, first)
+
+
 def test_a_scale_that_is_no_number_spoils_its_rows_and_no_others(ops, tile):
     for code, m in ((0, 3), (1281, 200), (2562, 300)):
         tile(code)
