@@ -157,7 +157,7 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
     }
 }
 
-// The same for two barriers at once: one loop and one verdict.
+// The same for two barriers at once: one loop, one answer.
 __device__ __forceinline__ bool mbar_wait_warp2(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1, volatile int* abort_flag,
                                                 uint64_t limit_ns = kWaitLimitNs)
 {
