@@ -513,8 +513,10 @@ LYRAQ_API int lyraq_load_lora(void* weight, const void* lora, int dtype, float a
 /* ------------------------------------------------------------------ attention over selected key blocks
  * Queries in blocks of 128, keys in blocks of `block` tokens.  Every 128 queries of a head share a list of key blocks, chosen by the products of the
  * blocks' means; lists belong to query heads, or one to all query heads of a key head ("lists" = q_heads or k_heads).  k_lens (int32 [batch], NULL: all)
- * says how many keys of a sequence exist, values beyond 0 .. keys are taken as these; q_start (int32 [batch], NULL: keys - queries) at which key the
- * first query stands, which causal order and the window go by. */
+ * says how many keys of a sequence exist, values beyond 0 .. keys are taken as these; q_lens (int32 [batch], NULL: all) the same of its queries, whose
+ * means are lyraq_block_means with these lengths; q_start (int32 [batch], NULL: keys - queries) at which key the first query stands, which causal order
+ * and the window go by.  In a padded batch q_lens and k_lens are both given: without q_lens the rows behind a sequence are queries like the others, and
+ * choose with those of their block. */
 
 /* Means of blocks of tokens: means fp32 [batch, heads, ceil(tokens / block), head_dim] of x (f16 or bf16, element (b, t, h, c) at b * batch_step + t *
  * token_step + h * head_step + c, steps multiples of 8); sums in 64 bits, over the tokens below lens[b]; 0 for a block without any.  newest = n > 0
@@ -529,6 +531,7 @@ typedef struct {
     int*         index;        /* [batch, lists, ceil(queries / 128), count]: the blocks taken in ascending order, then -1 */
     int*         counts;       /* [batch, lists, ceil(queries / 128)]: how many */
     const int*   k_lens;
+    const int*   q_lens;
     const int*   q_start;
     size_t       batch, queries, keys;
     int          q_heads, k_heads, lists, head_dim;
@@ -541,7 +544,7 @@ typedef struct {
 
 /* The count key blocks with the largest fl(q_mean . k_mean) (sum in 64 bits; q_mean the sum over the list's query heads) among those that hold a key a query of
  * the block may see, ties to the lowest index; blocks taken in any case come first, the lowest of them where they are more than count.  A score that
- * is no number comes last.  Up to 32768 key blocks.  workspace: lyraq_select_blocks_workspace bytes, 16-byte aligned.  Outputs and workspace share no memory with anything
+ * is no number comes last.  A query block without an existing query takes none.  Up to 32768 key blocks.  workspace: lyraq_select_blocks_workspace bytes, 16-byte aligned.  Outputs and workspace share no memory with anything
  * else.  It has no counterpart in the reference. */
 LYRAQ_API int lyraq_select_blocks(const lyraq_select_blocks_t* args, void* workspace, size_t workspace_bytes, void* stream);
 
@@ -555,6 +558,7 @@ typedef struct {
     const int*  index;                                /* as lyraq_select_blocks leaves them */
     const int*  counts;
     const int*  k_lens;
+    const int*  q_lens;
     const int*  q_start;
     size_t      batch, queries, keys;
     int         q_heads, k_heads, lists, head_dim;    /* head_dim 64 or 128 */
@@ -565,7 +569,7 @@ typedef struct {
 } lyraq_sparse_attention_t;
 
 /* out = softmax(q k^T * softmax_scale) v over the keys of the first counts[...] listed blocks that are below k_lens[b] and, if causal, not behind the
- * query's place; a query without any gets zeros.  An index outside the keys adds nothing, a block listed twice counts twice.  Keys and values
+ * query's place; a query without any, or beyond q_lens, gets zeros.  An index outside the keys adds nothing, a block listed twice counts twice.  Keys and values
  * beyond k_lens may hold anything; in causal order the values within a listed block are finite.  All pointers of tensors 16-byte aligned, steps
  * multiples of 8; out shares no memory with what is read.  lyraq_attention over a part of the keys; no counterpart in the reference. */
 LYRAQ_API int lyraq_sparse_attention(const lyraq_sparse_attention_t* args, void* stream);

@@ -28,7 +28,7 @@ class GatedNormArgs(ctypes.Structure):
 
 class SelectBlocksArgs(ctypes.Structure):
     """lyraq_select_blocks_t."""
-    _fields_ = ([(n, c_void_p) for n in ("q_means", "k_means", "index", "counts", "k_lens", "q_start")]
+    _fields_ = ([(n, c_void_p) for n in ("q_means", "k_means", "index", "counts", "k_lens", "q_lens", "q_start")]
                 + [(n, c_size_t) for n in ("batch", "queries", "keys")]
                 + [(n, c_int) for n in ("q_heads", "k_heads", "lists", "head_dim", "block", "count", "sink", "window", "causal")])
 
@@ -36,7 +36,7 @@ class SelectBlocksArgs(ctypes.Structure):
 class SparseAttentionArgs(ctypes.Structure):
     """lyraq_sparse_attention_t."""
     _fields_ = ([(n, c_void_p) for n in ("q", "k", "v", "out")] + [(a + n, c_size_t) for a in ("q_", "k_", "v_", "o_") for n in ("batch", "token", "head")]
-                + [(n, c_void_p) for n in ("index", "counts", "k_lens", "q_start")] + [(n, c_size_t) for n in ("batch", "queries", "keys")]
+                + [(n, c_void_p) for n in ("index", "counts", "k_lens", "q_lens", "q_start")] + [(n, c_size_t) for n in ("batch", "queries", "keys")]
                 + [(n, c_int) for n in ("q_heads", "k_heads", "lists", "head_dim", "block", "count", "causal")] + [("softmax_scale", c_float), ("dtype", c_int)])
 
 

@@ -197,6 +197,7 @@ struct SelectParams {
     int*         index;        // [batch][lists][q_blocks][count]
     int*         counts;       // [batch][lists][q_blocks]
     const int*   k_lens;       // keys of each sequence, or null
+    const int*   q_lens;       // queries of each sequence, or null
     const int*   q_start;      // place of each sequence's first query among the keys, or null
     int          batch, q_heads, k_heads, lists, head_dim, queries, keys, block, q_blocks, k_blocks;
     int          count, sink, window, causal;
@@ -334,10 +335,11 @@ struct Range {
         const int  start = p.q_start == nullptr ? p.keys - p.queries : min(max(__ldg(p.q_start + b), -kMaxKeys), kMaxKeys);
         // in 32 bits: a place beyond the keys by 2^30 and more is as good as one there
         const int first = (int)min((long long)start + (long long)i * kQueryBlock, (long long)kMaxKeys);
-        const int last  = min(first + min(kQueryBlock, p.queries - i * kQueryBlock) - 1, kMaxKeys);
+        const int rows  = min(kQueryBlock, (p.q_lens == nullptr ? p.queries : min(max(__ldg(p.q_lens + b), 0), p.queries)) - i * kQueryBlock);
+        const int last  = min(first + max(rows, 1) - 1, kMaxKeys);
         auto block_of = [&](int t) { return t >= 0 ? t / p.block : -((p.block - 1 - t) / p.block); };   // downwards
         const int e = (int)(((unsigned)len + (unsigned)p.block - 1u) / (unsigned)p.block);
-        end  = p.causal ? min(e, max(block_of(last) + 1, 0)) : e;
+        end  = rows <= 0 ? 0 : p.causal ? min(e, max(block_of(last) + 1, 0)) : e;      // no query: nothing
         sink = p.sink;
         // windows wider than the keys are as good as all of them
         const int w = min(p.window - 1, kMaxKeys / 2);
@@ -564,7 +566,7 @@ int lyraq_select_blocks(const lyraq_select_blocks_t* s, void* workspace, size_t 
     if (s->q_means == nullptr || s->index == nullptr || s->counts == nullptr || !aligned16(s->q_means) || (k_blocks > 0 && s->k_means == nullptr) ||
         !aligned16(s->k_means) ||
         ((reinterpret_cast<uintptr_t>(s->index) | reinterpret_cast<uintptr_t>(s->counts) | reinterpret_cast<uintptr_t>(s->k_lens) |
-          reinterpret_cast<uintptr_t>(s->q_start)) & 3u) != 0) {
+          reinterpret_cast<uintptr_t>(s->q_lens) | reinterpret_cast<uintptr_t>(s->q_start)) & 3u) != 0) {
         return LYRAQ_ERR_INVALID_ARG;
     }
     if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace))) {
@@ -572,8 +574,8 @@ int lyraq_select_blocks(const lyraq_select_blocks_t* s, void* workspace, size_t 
     }
     const size_t dim = (size_t)s->head_dim;
     const View   out[3] = {view_of(s->index, rows * (size_t)s->count * 4), view_of(s->counts, rows * 4), view_of(workspace, need)};
-    const View   in[4]  = {view_of(s->q_means, s->batch * (size_t)s->q_heads * q_blocks * dim * 4), view_of(s->k_means, s->batch * (size_t)s->k_heads * k_blocks * dim * 4),
-                           view_of(s->k_lens, s->batch * 4), view_of(s->q_start, s->batch * 4)};
+    const View   in[5]  = {view_of(s->q_means, s->batch * (size_t)s->q_heads * q_blocks * dim * 4), view_of(s->k_means, s->batch * (size_t)s->k_heads * k_blocks * dim * 4),
+                           view_of(s->k_lens, s->batch * 4), view_of(s->q_lens, s->batch * 4), view_of(s->q_start, s->batch * 4)};
     for (int i = 0; i < 3; ++i) {
         for (const View& v : in) {
             if (views_meet(out[i], v)) {
@@ -591,6 +593,7 @@ int lyraq_select_blocks(const lyraq_select_blocks_t* s, void* workspace, size_t 
     p.index    = s->index;
     p.counts   = s->counts;
     p.k_lens   = s->k_lens;
+    p.q_lens   = s->q_lens;
     p.q_start  = s->q_start;
     p.batch    = (int)s->batch;
     p.q_heads  = s->q_heads;

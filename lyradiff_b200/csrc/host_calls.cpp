@@ -725,7 +725,16 @@ Choice choice_of(PyObject* const* a)     // block, count, sink, window, shared, 
     return c;
 }
 
-std::pair<Tensor, Tensor> select_of(const Tensor& qm, const Tensor& km, const Choice& c, int64_t queries, int64_t keys, const int* k_lens, const int* q_start, int dev)
+// Of each sequence, int32 [batch] or null.
+struct Lengths {
+    const int *k_lens, *q_lens, *q_start;
+};
+Lengths lengths_of(PyObject* k_lens, PyObject* q_lens, PyObject* q_start, int64_t batch, int dev)
+{
+    return {per_sequence(k_lens, "k_lens", batch, dev), per_sequence(q_lens, "q_lens", batch, dev), per_sequence(q_start, "q_start", batch, dev)};
+}
+
+std::pair<Tensor, Tensor> select_of(const Tensor& qm, const Tensor& km, const Choice& c, int64_t queries, int64_t keys, const Lengths& n, int dev)
 {
     const int64_t batch = qm.size(0), heads = qm.size(1), dim = qm.size(3), k_heads = km.size(1), q_blocks = blocks_of(queries, kQueryBlock);
     if (k_heads == 0 || heads % k_heads != 0) {
@@ -741,8 +750,9 @@ std::pair<Tensor, Tensor> select_of(const Tensor& qm, const Tensor& km, const Ch
     s.k_means  = (const float*)at_contiguous(&km, "k_means");
     s.index    = (int*)index.data_ptr();
     s.counts   = (int*)counts.data_ptr();
-    s.k_lens   = k_lens;
-    s.q_start  = q_start;
+    s.k_lens   = n.k_lens;
+    s.q_lens   = n.q_lens;
+    s.q_start  = n.q_start;
     s.batch    = (size_t)batch;
     s.queries  = (size_t)queries;
     s.keys     = (size_t)keys;
@@ -759,7 +769,7 @@ std::pair<Tensor, Tensor> select_of(const Tensor& qm, const Tensor& km, const Ch
     return {index, counts};
 }
 
-// (q_means, k_means, block, count, sink, window, shared, causal, queries, keys, k_lens, q_start) -> (index, counts)
+// (q_means, k_means, block, count, sink, window, shared, causal, queries, keys, k_lens, q_start, q_lens) -> (index, counts)
 PyObject* select_blocks(PyObject* const* a)
 {
     const int     dev = c10::cuda::current_device();
@@ -772,7 +782,7 @@ PyObject* select_blocks(PyObject* const* a)
         refuse(PyExc_ValueError, "expected q_means fp32 [batch, heads, %lld, head_dim] and k_means [batch, key heads, %lld, head_dim]",
                (long long)blocks_of(queries, kQueryBlock), (long long)blocks_of(keys, c.block));
     }
-    const auto s = select_of(qm, km, c, queries, keys, per_sequence(a[10], "k_lens", qm.size(0), dev), per_sequence(a[11], "q_start", qm.size(0), dev), dev);
+    const auto s = select_of(qm, km, c, queries, keys, lengths_of(a[10], a[12], a[11], qm.size(0), dev), dev);
     return Py_BuildValue("(NN)", THPVariable_Wrap(s.first), THPVariable_Wrap(s.second));
 }
 
@@ -786,8 +796,8 @@ void check_qkv(const Tensor& q, const Tensor& k, const Tensor& v)
     }
 }
 
-Tensor attend(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& index, const Tensor& counts, int block, const int* k_lens, const int* q_start, bool causal,
-              float scale, const Tensor* out, int dev)
+Tensor attend(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& index, const Tensor& counts, int block, const Lengths& n, bool causal, float scale,
+              const Tensor* out, int dev)
 {
     const int64_t batch = q.size(0), queries = q.size(1), heads = q.size(2), dim = q.size(3), k_heads = k.size(2), q_blocks = blocks_of(queries, kQueryBlock);
     if (index.scalar_type() != at::kInt || index.dim() != 4 || index.size(0) != batch || (index.size(1) != heads && index.size(1) != k_heads) ||
@@ -817,8 +827,9 @@ Tensor attend(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& i
     s.o_batch = step_of(made, 0); s.o_token = step_of(made, 1); s.o_head = step_of(made, 2);
     s.index    = (const int*)at_contiguous(&index, "index");
     s.counts   = (const int*)at_contiguous(&counts, "counts");
-    s.k_lens   = k_lens;
-    s.q_start  = q_start;
+    s.k_lens   = n.k_lens;
+    s.q_lens   = n.q_lens;
+    s.q_start  = n.q_start;
     s.batch    = (size_t)batch;
     s.queries  = (size_t)queries;
     s.keys     = (size_t)k.size(1);
@@ -835,7 +846,7 @@ Tensor attend(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& i
     return made;
 }
 
-// (q, k, v, index, counts, block, k_lens, q_start, causal, softmax scale, out) -> out
+// (q, k, v, index, counts, block, k_lens, q_start, causal, softmax scale, out, q_lens) -> out
 PyObject* sparse_attention(PyObject* const* a)
 {
     const int     dev = c10::cuda::current_device();
@@ -843,12 +854,12 @@ PyObject* sparse_attention(PyObject* const* a)
     const Tensor& k = tokens_of(needed(a[1], "k", dev), "k");
     const Tensor& v = tokens_of(needed(a[2], "v", dev), "v");
     check_qkv(q, k, v);
-    const Tensor out = attend(q, k, v, needed(a[3], "index", dev), needed(a[4], "counts", dev), as_block(a[5]), per_sequence(a[6], "k_lens", q.size(0), dev),
-                              per_sequence(a[7], "q_start", q.size(0), dev), PyObject_IsTrue(a[8]) == 1, as_float(a[9]), tensor(a[10], "out", dev), dev);
+    const Tensor out = attend(q, k, v, needed(a[3], "index", dev), needed(a[4], "counts", dev), as_block(a[5]), lengths_of(a[6], a[11], a[7], q.size(0), dev),
+                              PyObject_IsTrue(a[8]) == 1, as_float(a[9]), tensor(a[10], "out", dev), dev);
     return result(a[10], out);
 }
 
-// (q, k, v, block, count, sink, window, shared, causal, softmax scale, k_lens, q_start, k_means, out) -> (out, index, counts): means, selection and attention
+// (q, k, v, block, count, sink, window, shared, causal, softmax scale, k_lens, q_start, k_means, out, q_lens) -> (out, index, counts): means, selection and attention
 PyObject* select_and_attend(PyObject* const* a)
 {
     const int     dev = c10::cuda::current_device();
@@ -856,17 +867,16 @@ PyObject* select_and_attend(PyObject* const* a)
     const Tensor& k = tokens_of(needed(a[1], "k", dev), "k");
     const Tensor& v = tokens_of(needed(a[2], "v", dev), "v");
     check_qkv(q, k, v);
-    const Choice  c       = choice_of(a + 3);
-    const int*    k_lens  = per_sequence(a[10], "k_lens", q.size(0), dev);
-    const int*    q_start = per_sequence(a[11], "q_start", q.size(0), dev);
-    const Tensor* given   = tensor(a[12], "k_means", dev);
+    const Choice  c     = choice_of(a + 3);
+    const Lengths n     = lengths_of(a[10], a[14], a[11], q.size(0), dev);
+    const Tensor* given = tensor(a[12], "k_means", dev);
     if (given != nullptr && (given->scalar_type() != at::kFloat || given->sizes() != at::IntArrayRef({k.size(0), k.size(2), blocks_of(k.size(1), c.block), k.size(3)}))) {
         refuse(PyExc_ValueError, "k_means must be fp32 [batch, key heads, %lld, head_dim]", (long long)blocks_of(k.size(1), c.block));
     }
-    const Tensor qm = means_of(q, kQueryBlock, nullptr, nullptr, 0, dev);
-    const Tensor km = given != nullptr ? *given : means_of(k, c.block, k_lens, nullptr, 0, dev);
-    const auto   s  = select_of(qm, km, c, q.size(1), k.size(1), k_lens, q_start, dev);
-    const Tensor out = attend(q, k, v, s.first, s.second, c.block, k_lens, q_start, c.causal, as_float(a[9]), tensor(a[13], "out", dev), dev);
+    const Tensor qm = means_of(q, kQueryBlock, n.q_lens, nullptr, 0, dev);
+    const Tensor km = given != nullptr ? *given : means_of(k, c.block, n.k_lens, nullptr, 0, dev);
+    const auto   s  = select_of(qm, km, c, q.size(1), k.size(1), n, dev);
+    const Tensor out = attend(q, k, v, s.first, s.second, c.block, n, c.causal, as_float(a[9]), tensor(a[13], "out", dev), dev);
     return Py_BuildValue("(NNN)", result(a[13], out), THPVariable_Wrap(s.first), THPVariable_Wrap(s.second));
 }
 
@@ -926,9 +936,9 @@ PyMethodDef g_methods[] = {
     {"gemm_fp8_block", (PyCFunction)(void (*)())call<gemm_fp8_block, 9>, METH_FASTCALL, nullptr},
     {"quant_fp8_block", (PyCFunction)(void (*)())call<quant_fp8_block, 3>, METH_FASTCALL, nullptr},
     {"block_means", (PyCFunction)(void (*)())call<block_means, 5>, METH_FASTCALL, nullptr},
-    {"select_blocks", (PyCFunction)(void (*)())call<select_blocks, 12>, METH_FASTCALL, nullptr},
-    {"sparse_attention", (PyCFunction)(void (*)())call<sparse_attention, 11>, METH_FASTCALL, nullptr},
-    {"select_and_attend", (PyCFunction)(void (*)())call<select_and_attend, 14>, METH_FASTCALL, nullptr},
+    {"select_blocks", (PyCFunction)(void (*)())call<select_blocks, 13>, METH_FASTCALL, nullptr},
+    {"sparse_attention", (PyCFunction)(void (*)())call<sparse_attention, 12>, METH_FASTCALL, nullptr},
+    {"select_and_attend", (PyCFunction)(void (*)())call<select_and_attend, 15>, METH_FASTCALL, nullptr},
     {"fp4_empty", (PyCFunction)(void (*)())call<fp4_empty, 4>, METH_FASTCALL, nullptr},
     {"quant_fp4", (PyCFunction)(void (*)())call<quant_fp4, 5>, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},

@@ -84,11 +84,11 @@ __device__ __forceinline__ void tma_load_4d(uint32_t smem_dst, const CUtensorMap
 
 // What a producer tells the other roles of an item: query block `qb` of head `h` of sequence `b`, its steps (-1: no item any more), the row of its list, how
 // much of the list counts, the keys that exist, the last key its row 0 sees, the first step in which a row may miss a key, the first keys of the
-// halves of its first step.
+// halves of its first step, its rows that exist (the others get zeros).
 struct alignas(16) Info {
     int qb, h, b, steps;
     int list, entries, len, place;
-    int masked, key[2], spare;
+    int masked, key[2], rows;
 };
 static_assert(sizeof(Info) == 48, "");
 
@@ -172,7 +172,8 @@ sparse_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                     it.h       = i / p.q_blocks % p.q_heads;
                     it.b       = i / (p.q_blocks * p.q_heads);
                     it.list    = (it.b * p.lists + it.h / (p.q_heads / p.lists)) * p.q_blocks + it.qb;
-                    it.entries = min(max(load_int(p.counts + it.list), 0), p.count);
+                    it.rows    = query_count(p, it.b) - it.qb * kTile;
+                    it.entries = it.rows > 0 ? min(max(load_int(p.counts + it.list), 0), p.count) : 0;
                     it.steps   = p.block == kTile ? it.entries : (it.entries + 1) / 2;
                     it.len     = key_count(p, it.b);
                     it.place   = p.causal ? (int)min((long long)first_place(p, it.b) + it.qb * kTile, (long long)kMaxKeys) : p.keys;
@@ -603,7 +604,7 @@ sparse_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
             }
             ++done;
             tc_fence_after_sync();
-            const bool  none  = m == -INFINITY;                                // a row that saw no key: zeros
+            const bool  none  = m == -INFINITY || r >= it.rows;                // a row that saw no key, or does not exist: zeros
             const float inv_l = 1.0f / l;
 #pragma unroll
             for (int cc = 0; cc < D / 32; ++cc) {
@@ -728,7 +729,7 @@ int lyraq_sparse_attention(const lyraq_sparse_attention_t* a, void* stream)
     if (a->q == nullptr || a->out == nullptr || !aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out) ||
         (!none && (a->k == nullptr || a->v == nullptr || a->index == nullptr)) || a->counts == nullptr ||
         ((reinterpret_cast<uintptr_t>(a->index) | reinterpret_cast<uintptr_t>(a->counts) | reinterpret_cast<uintptr_t>(a->k_lens) |
-          reinterpret_cast<uintptr_t>(a->q_start)) & 3u) != 0) {
+          reinterpret_cast<uintptr_t>(a->q_lens) | reinterpret_cast<uintptr_t>(a->q_start)) & 3u) != 0) {
         return LYRAQ_ERR_INVALID_ARG;
     }
     // a step of 0 repeats a sequence; tokens and heads have places of their own
@@ -745,7 +746,7 @@ int lyraq_sparse_attention(const lyraq_sparse_attention_t* a, void* stream)
     if (result_clashes(out, nullptr,
                        {view(a->q, a->q_batch, a->queries, a->q_token, a->q_heads, a->q_head), view(a->k, a->k_batch, a->keys, a->k_token, a->k_heads, a->k_head),
                         view(a->v, a->v_batch, a->keys, a->v_token, a->k_heads, a->v_head), view_of(a->index, rows * (size_t)a->count * 4),
-                        view_of(a->counts, rows * 4), view_of(a->k_lens, a->batch * 4), view_of(a->q_start, a->batch * 4)})) {
+                        view_of(a->counts, rows * 4), view_of(a->k_lens, a->batch * 4), view_of(a->q_lens, a->batch * 4), view_of(a->q_start, a->batch * 4)})) {
         return LYRAQ_ERR_INVALID_ARG;
     }
     sattn::Params p{};
@@ -761,6 +762,7 @@ int lyraq_sparse_attention(const lyraq_sparse_attention_t* a, void* stream)
     p.index      = a->index;
     p.counts     = a->counts;
     p.k_lens     = a->k_lens;
+    p.q_lens     = a->q_lens;
     p.q_start    = a->q_start;
     p.batch      = (int)a->batch;
     p.queries    = (int)a->queries;

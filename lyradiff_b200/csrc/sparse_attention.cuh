@@ -24,6 +24,7 @@ struct Params {
     const int*    index;
     const int*    counts;
     const int*    k_lens;
+    const int*    q_lens;
     const int*    q_start;
     int           batch, queries, keys;
     int           q_heads, k_heads, lists;
@@ -44,6 +45,8 @@ __device__ __forceinline__ int load_int(const int* p)
 }
 // keys of a sequence, and the place of its first query
 __device__ __forceinline__ int key_count(const Params& p, int b) { return p.k_lens == nullptr ? p.keys : min(max(load_int(p.k_lens + b), 0), p.keys); }
+// its queries
+__device__ __forceinline__ int query_count(const Params& p, int b) { return p.q_lens == nullptr ? p.queries : min(max(load_int(p.q_lens + b), 0), p.queries); }
 __device__ __forceinline__ int first_place(const Params& p, int b)
 {
     return p.q_start == nullptr ? p.keys - p.queries : min(max(load_int(p.q_start + b), -kMaxKeys), kMaxKeys);

@@ -135,7 +135,8 @@ sparse_attention_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const _
     }
     grid_dependency_wait();
     const int halves_per = p.block / kKeys;
-    const int entries    = min(max(load_int(p.counts + unit), 0), p.count);
+    const int q_count    = query_count(p, b);
+    const int entries    = q_count > 0 ? min(max(load_int(p.counts + unit), 0), p.count) : 0;
     const int halves     = entries * halves_per;
     const int len        = key_count(p, b);
     if (warp < kWarps) {
@@ -381,12 +382,12 @@ sparse_attention_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const _
                 a[6] += f * y.z;
                 a[7] += f * y.w;
             }
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;      // no key seen: zeros
+            const int   head = list * heads + r / p.queries, qi = r % p.queries;
+            const float inv  = sum == 0.0f ? 0.0f : 1.0f / sum;      // no key seen: zeros
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                a[e] *= inv;
+                a[e] = qi < q_count ? a[e] * inv : 0.0f;             // nor does a row behind the sequence's queries have a result
             }
-            const int head = list * heads + r / p.queries, qi = r % p.queries;
             st_16(reinterpret_cast<T*>(p.out) + (long long)b * p.os.batch + (long long)qi * p.os.token + (long long)head * p.os.head + d, pack8<T>(a));
         }
     }

@@ -135,12 +135,14 @@ class SparseAttention:
             raise ValueError("expected blocks of 64 or 128 keys, count of 1 or more, sink and window of 0 or more")
         self.block, self.count, self.sink, self.window, self.shared, self.causal, self.softmax_scale = block, count, sink, window, shared, causal, softmax_scale
 
-    def forward(self, q, k, v, k_lens=None, q_start=None, k_means=None, out=None, with_selection=False):
+    def forward(self, q, k, v, k_lens=None, q_start=None, k_means=None, out=None, with_selection=False, q_lens=None):
         """q [batch, queries, heads, head_dim], k and v [batch, keys, key heads, head_dim], f16 or bf16, any steps with contiguous heads -> like q.
-        k_means: ops.block_means(k, block, lens=k_lens), where a cache keeps them up to date.  with_selection: (out, index, counts)."""
+        k_lens, q_lens: int32 [batch], the keys and the queries of each sequence; a padded batch gives its lengths as both, and then neither a list nor a
+        result depends on what lies behind a sequence (without q_lens its rows choose like queries).  k_means: ops.block_means(k, block, lens=k_lens),
+        where a cache keeps them up to date.  with_selection: (out, index, counts)."""
         scale = self.softmax_scale if self.softmax_scale is not None else float(q.shape[-1]) ** -0.5
         got = _lib.host().select_and_attend(q, k, v, self.block, self.count, self.sink, self.window, self.shared, self.causal, scale, k_lens, q_start, k_means,
-                                            out)
+                                            out, q_lens)
         return got if with_selection else got[0]
 
 

@@ -362,25 +362,26 @@ def block_means(x, block, lens=None, out=None, newest=0):
     return _lib.host().block_means(x, block, lens, out, newest)
 
 
-def select_blocks(q_means, k_means, count, queries, keys, block, k_lens=None, q_start=None, causal=False, sink=0, window=0, shared=False):
+def select_blocks(q_means, k_means, count, queries, keys, block, k_lens=None, q_start=None, causal=False, sink=0, window=0, shared=False, q_lens=None):
     """Key blocks that attention goes to (lyraq_select_blocks): for each QUERY_BLOCK queries of a head the `count` blocks of `block` keys with the largest
     product of means, ties to the lowest; the first `sink` blocks in any case, and with window = n > 0 those that hold the queries' own places and n - 1
     on either side.  q_means, k_means: block_means of q (with QUERY_BLOCK) and of k; queries, keys: tokens of both; k_lens int32 [batch]: keys of each
     sequence (default: all); q_start int32 [batch]: the key at which the first query stands (default: keys - queries); causal: only blocks with a key
-    at or before the last query's; shared: one list for the query heads of a key head.  Returns (index int32 [batch, heads or key heads,
+    at or before the last query's; shared: one list for the query heads of a key head.  q_lens int32 [batch]: queries of each sequence (default: all), with
+    q_means = block_means(q, QUERY_BLOCK, q_lens); blocks of queries that do not exist take nothing.  Returns (index int32 [batch, heads or key heads,
     ceil(queries / 128), count] in ascending order with -1 behind, counts int32)."""
-    return _lib.host().select_blocks(q_means, k_means, block, count, sink, window, shared, causal, queries, keys, k_lens, q_start)
+    return _lib.host().select_blocks(q_means, k_means, block, count, sink, window, shared, causal, queries, keys, k_lens, q_start, q_lens)
 
 
-def sparse_attention(q, k, v, index, counts, block, k_lens=None, q_start=None, causal=False, softmax_scale=None, out=None):
+def sparse_attention(q, k, v, index, counts, block, k_lens=None, q_start=None, causal=False, softmax_scale=None, out=None, q_lens=None):
     """Attention over the listed key blocks (lyraq_sparse_attention): q [batch, queries, heads, head_dim], k and v [batch, keys, key heads, head_dim], f16 or
     bf16, any steps with contiguous heads (views of a packed projection, a cache with heads before tokens by transpose), head_dim 64 or 128, block 64 or
     128.  index, counts: as select_blocks returns them, or any lists of that form.  Keys beyond k_lens, or behind a query's place in causal order, take no
-    part; a query that sees no key gets zeros.  In causal order the values within a listed block have to be finite.  softmax_scale: head_dim ** -0.5
+    part; a query that sees no key, or is beyond q_lens, gets zeros.  In causal order the values within a listed block have to be finite.  softmax_scale: head_dim ** -0.5
     when omitted.  out is created when omitted and shares no memory with the inputs."""
     if softmax_scale is None:
         softmax_scale = float(q.shape[-1]) ** -0.5
-    return _lib.host().sparse_attention(q, k, v, index, counts, block, k_lens, q_start, causal, softmax_scale, out)
+    return _lib.host().sparse_attention(q, k, v, index, counts, block, k_lens, q_start, causal, softmax_scale, out, q_lens)
 
 
 def quant_fp8_into_columns(dst, col0, src, scale):

@@ -26,7 +26,7 @@ def means(x, block, lens=None):
     return out
 
 
-def select(q_means, k_means, count, queries, keys, block, k_lens=None, q_start=None, causal=False, sink=0, window=0, shared=False):
+def select(q_means, k_means, count, queries, keys, block, k_lens=None, q_start=None, causal=False, sink=0, window=0, shared=False, q_lens=None):
     """One query block after the other, by sorting (score, -index)."""
     batch, heads, qb, _ = q_means.shape
     k_heads, kb = k_means.shape[1:3]
@@ -36,15 +36,16 @@ def select(q_means, k_means, count, queries, keys, block, k_lens=None, q_start=N
     for b in range(batch):
         n = keys if k_lens is None else min(max(int(k_lens[b]), 0), keys)
         start = keys - queries if q_start is None else int(q_start[b])
+        nq = queries if q_lens is None else min(max(int(q_lens[b]), 0), queries)
         for h in range(lists):
             if shared:
                 q, k = q_means[b, h * group:(h + 1) * group].double().sum(0), k_means[b, h].double()
             else:
                 q, k = q_means[b, h].double(), k_means[b, h // group].double()
             scores = (q @ k.t()).float()
-            for i in range(qb):
+            for i in range(blocks(nq, QUERY_BLOCK)):
                 first = start + i * QUERY_BLOCK
-                last = first + min(QUERY_BLOCK, queries - i * QUERY_BLOCK) - 1
+                last = first + min(QUERY_BLOCK, nq - i * QUERY_BLOCK) - 1
                 rank = []
                 for j in range(kb):
                     if j * block >= n or (causal and j * block > last):
@@ -58,7 +59,7 @@ def select(q_means, k_means, count, queries, keys, block, k_lens=None, q_start=N
     return index, counts
 
 
-def attend(q, k, v, index, counts, block, k_lens=None, q_start=None, causal=False, scale=None):
+def attend(q, k, v, index, counts, block, k_lens=None, q_start=None, causal=False, scale=None, q_lens=None):
     """Key by key as the lists name them (a block listed twice counts twice); also returns what bounds the rounding of the weights: the sum of |weight * value|."""
     batch, nq, heads, dim = q.shape
     nk, k_heads = k.shape[1:3]
@@ -69,12 +70,13 @@ def attend(q, k, v, index, counts, block, k_lens=None, q_start=None, causal=Fals
     for b in range(batch):
         n = nk if k_lens is None else min(max(int(k_lens[b]), 0), nk)
         start = nk - nq if q_start is None else int(q_start[b])
+        end = nq if q_lens is None else min(max(int(q_lens[b]), 0), nq)
         for h in range(heads):
             for i in range(index.shape[2]):
                 lists = index[b, h // per, i, :max(0, min(int(counts[b, h // per, i]), index.shape[3]))].tolist()
                 pos = [p for j in lists if 0 <= j < blocks(nk, block) for p in range(j * block, min((j + 1) * block, n))]
-                rows = torch.arange(i * QUERY_BLOCK, min(nq, (i + 1) * QUERY_BLOCK))
-                if not pos:
+                rows = torch.arange(min(end, i * QUERY_BLOCK), min(end, (i + 1) * QUERY_BLOCK))
+                if not pos or not len(rows):
                     continue
                 at = torch.tensor(pos)
                 s = q[b, rows, h].double() @ k[b, at, h // group].double().t() * scale
