@@ -555,7 +555,8 @@ int lyraq_select_blocks(const lyraq_select_blocks_t* s, void* workspace, size_t 
         return LYRAQ_ERR_INVALID_ARG;
     }
     const size_t k_blocks = (s->keys + (size_t)s->block - 1) / (size_t)s->block, q_blocks = (s->queries + bsel::kQueryBlock - 1) / bsel::kQueryBlock;
-    if (s->keys > (size_t)bsel::kMaxKeys || s->queries > (size_t)bsel::kMaxKeys || k_blocks > (size_t)bsel::kMaxBlocks || s->batch > 0xffffu ||
+    // a longer block than 2^30: its end less a place in front of the keys (Range) would leave 32 bits
+    if (s->block > bsel::kMaxKeys || s->keys > (size_t)bsel::kMaxKeys || s->queries > (size_t)bsel::kMaxKeys || k_blocks > (size_t)bsel::kMaxBlocks || s->batch > 0xffffu ||
         s->q_heads > 0xffff || s->head_dim == 0 || (s->head_dim & 7) != 0 || s->head_dim > bsel::kMaxHeadDim || s->count > bsel::kMaxBlocks) {
         return LYRAQ_ERR_UNSUPPORTED;
     }

@@ -8,7 +8,7 @@ import torch
 from lyradiff_b200 import _lib, build
 from oracle import sparse
 
-INVALID = 1
+INVALID, UNSUPPORTED = 1, 2
 P = [0x100000 + (i << 34) for i in range(10)]
 
 
@@ -35,6 +35,14 @@ def test_query_lengths(lib):
         return lib.lyraq_sparse_attention(ctypes.byref(_lib.SparseAttentionArgs(**{**f, **k})), None)
     assert select(q_lens=P[5] + 2) == select(counts=P[5]) == select(q_lens=P[7] + 64) == select(q_lens=P[2] + 4) == INVALID
     assert attend(q_lens=P[7] + 1) == attend(out=P[7]) == INVALID
+
+
+def test_blocks_beyond_30_bits(lib):
+    """As the means: the distance of a place 2^30 in front of the keys to the end of a longer block does not fit 32 bits."""
+    def select(**k):
+        return lib.lyraq_select_blocks(ctypes.byref(_lib.SelectBlocksArgs(**select_args(**k))), P[7], 1 << 20, None)
+    assert select(block=2 ** 31 - 1, causal=1) == select(block=2 ** 30 + 1) == UNSUPPORTED
+    assert lib.lyraq_block_means(P[0], P[1], 1, 4096, 64, 32, None, 2 ** 30 + 1, 0, 2, 60, 2, 32, None) == UNSUPPORTED
 
 
 def test_rows_behind_a_sequence_choose_nothing_and_for_no_one():
