@@ -101,17 +101,20 @@ class Fp4Linear:
 
 
 class Fp8BlockLinear:
-    """Linear in FP8 with a scale for each block of 128: weight codes uint8 [n, k] with scales fp32 [ceil(n / 128), ceil(k / 128)], as block-scaled
-    checkpoints hold them (k a multiple of 16); activations are quantized by the forward with a scale for each 128 values of a row, so nothing is
-    calibrated; bias / GELU-tanh / residual fused into the GEMM epilogue.  The quantized activation lives in memory taken from torch's allocator
-    per call, so calls on several streams and captured graphs do not share it.  The reference has no such linear; this is Fp8Linear's counterpart."""
+    """Linear in FP8 with a scale for each block of 128: weight codes [n, k] (torch.float8_e4m3fn, or their bytes in uint8) with scales fp32 [ceil(n / 128),
+    ceil(k / 128)], as block-scaled checkpoints hold them (k a multiple of 16); activations are quantized by the forward with a scale for each 128 values of
+    a row, so nothing is calibrated; bias / GELU-tanh / residual fused into the GEMM epilogue.  The quantized activation lives in memory taken from torch's
+    allocator per call, so calls on several streams and captured graphs do not share it.  The reference has no such linear; this is Fp8Linear's
+    counterpart."""
 
     def __init__(self, codes, scales, bias=None, gelu=False):
         self.n, self.k = codes.shape
         if self.k % 16:
             raise ValueError("k must be a multiple of 16")
+        if codes.dtype == torch.float8_e4m3fn:
+            codes = codes.view(torch.uint8)
         if codes.dtype != torch.uint8 or scales.dtype != torch.float32 or tuple(scales.shape) != ((self.n + 127) // 128, (self.k + 127) // 128):
-            raise ValueError("expected uint8 codes [n, k] and fp32 scales, one for each 128 x 128")
+            raise ValueError("expected codes [n, k] in float8_e4m3fn or uint8 and fp32 scales, one for each 128 x 128")
         self.codes, self.scales, self.gelu = codes.contiguous(), scales.contiguous(), gelu
         self.bias = None if bias is None else bias.contiguous()
         self.epilogue = ops.EPI_GELU_TANH if gelu else ops.EPI_NONE
