@@ -118,6 +118,10 @@ LYRAQ_API int lyraq_debug_force_fp4_tile(int code);
 /* lyraq_debug_attention_wait_test for lyraq_sparse_attention.  It has no counterpart in the reference. */
 LYRAQ_API int lyraq_debug_sparse_attention_wait_test(int skip_loads, unsigned int wait_limit_ms);
 
+/* lyraq_debug_skinny_wait_test for the tiled kernel of lyraq_gemm_fp8_block, by the rank in a CTA pair or of the CTAs along K (one CTA alone: 0).
+ * It has no counterpart in the reference. */
+LYRAQ_API int lyraq_debug_fp8_block_wait_test(int stalled_rank, unsigned int wait_limit_ms);
+
 /* lyraq_debug_skinny_wait_test for the few-row kernel of lyraq_gemm_fp8_block.  It has no counterpart in the reference. */
 LYRAQ_API int lyraq_debug_fp8_block_rows_wait_test(int stalled_rank, unsigned int wait_limit_ms);
 

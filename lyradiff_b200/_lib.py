@@ -62,6 +62,7 @@ SIGNATURES = {
     "lyraq_debug_force_w4a4_wide": (c_int, [c_int]),
     "lyraq_debug_force_fp4_tile": (c_int, [c_int]),
     "lyraq_debug_sparse_attention_wait_test": (c_int, [c_int, ctypes.c_uint]),
+    "lyraq_debug_fp8_block_wait_test": (c_int, [c_int, ctypes.c_uint]),
     "lyraq_debug_fp8_block_rows_wait_test": (c_int, [c_int, ctypes.c_uint]),
     "lyraq_debug_force_fp8_block_tile": (c_int, [c_int]),
     "lyraq_debug_fp4_skinny_wait_test": (c_int, [c_int, ctypes.c_uint]),

@@ -51,6 +51,8 @@ struct GemmParams {
     const void*   residual;   // [M, N] of c_dtype or null
     float         beta;
     int           gelu;
+    unsigned long long wait_limit_ns;   // of the tiled kernel's waits
+    int           stalled_rank;         // test hook: this CTA of a cluster issues no loads there (-1: none)
 };
 
 // What a block's values are divided by, and how.

@@ -197,14 +197,14 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
             // -------------------------------------------------------------- TMA producer
             int      stage = 0, issued = 0;
             uint32_t phase = 0;
-            bool     ok = true;
+            bool     ok = (SPLIT ? part : (int)rank) != p.stalled_rank;
             for (int tile = unit; ok && tile < num_tiles; tile += n_units) {
                 int m_blk, n_blk;
                 tile_coords(tile, p.m_tiles, p.n_tiles, m_blk, n_blk);
                 const int a_row = m_blk * kTileM + (int)rank * kBlockM;
                 const int b_row = n_blk * BLOCK_N + (int)rank * (BLOCK_N / CTAS);
                 for (int kb = kb_first; kb < kb_end; ++kb) {
-                    if (!mbar_wait_warp(empty_bar(stage), phase ^ 1u, abort_flag)) {
+                    if (!mbar_wait_warp(empty_bar(stage), phase ^ 1u, abort_flag, p.wait_limit_ns)) {
                         report_timeout(p.status, 0x7100u | (unsigned)stage);
                         *abort_flag = 1;
                         ok = false;
@@ -245,7 +245,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                     --s;
                     const uint64_t t0 = global_timer_ns();
                     while (!mbar_try_wait(full_bar(s), ph)) {
-                        if (global_timer_ns() - t0 > kWaitLimitNs) {
+                        if (global_timer_ns() - t0 > p.wait_limit_ns) {
                             report_timeout(p.status, 0x7500u | (unsigned)s);
                             break;
                         }
@@ -262,9 +262,9 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
             // as much as two MMAs; [1317, 1280, 5120] 18.1 -> 16.2 us).  With two products in tensor memory the one before is still being taken then, and
             // they stand in front of them (388 us against 315 for [4680, 13824, 5120]).
             constexpr bool kEarly = kBufs > 2;
-            bool           ok     = !kEarly || mbar_wait_warp2(full_bar(0), 0u, tmem_empty_bar(0), 1u, abort_flag);
+            bool           ok     = !kEarly || mbar_wait_warp2(full_bar(0), 0u, tmem_empty_bar(0), 1u, abort_flag, p.wait_limit_ns);
             for (; ok && left > 0; --left) {
-                if (!kEarly && !(ok = mbar_wait_warp2(full_bar(stage), phase, tmem_empty_bar(buf), buf_phase ^ 1u, abort_flag))) {
+                if (!kEarly && !(ok = mbar_wait_warp2(full_bar(stage), phase, tmem_empty_bar(buf), buf_phase ^ 1u, abort_flag, p.wait_limit_ns))) {
                     break;
                 }
                 const uint32_t sa     = smem_base + stage * S::kStageBytes;
@@ -297,7 +297,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                     buf_phase ^= 1u;
                 }
                 if (kEarly && left > 1) {
-                    ok = mbar_wait_warp2(full_bar(stage), phase, tmem_empty_bar(buf), buf_phase ^ 1u, abort_flag);
+                    ok = mbar_wait_warp2(full_bar(stage), phase, tmem_empty_bar(buf), buf_phase ^ 1u, abort_flag, p.wait_limit_ns);
                 }
                 if (elect_one()) {
                     mma(2);
@@ -383,7 +383,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
 #pragma unroll
                 for (int i = 0; i < kAhead; ++i) {
                     if (kb0 + i < kb_end && ok) {
-                        if (!mbar_wait_warp(tmem_full_bar(buf), buf_phase, abort_flag)) {
+                        if (!mbar_wait_warp(tmem_full_bar(buf), buf_phase, abort_flag, p.wait_limit_ns)) {
                             if (lane == 0) {
                                 report_timeout(p.status, 0x7400u | (unsigned)buf);
                             }
@@ -619,6 +619,9 @@ template<int BLOCK_N, int CTAS, bool RES, bool NARROW, bool SPLIT> static int la
 // forced kernel for tests and sweeps: 0 = automatic, 16 = the few-row kernel (up to 16 rows), 2562 = CTA pair with 256 x 256, 1281 = one CTA with 128 x 128,
 // 1282, 1284, 1288 = that with 2, 4 or 8 CTAs along K
 static int g_forced_tile = 0;
+// Test hook (lyraq_debug_fp8_block_wait_test)
+static int                g_stalled_rank  = -1;
+static unsigned long long g_wait_limit_ns = kWaitLimitNs;
 
 bool few_rows(int m, int n, int k)
 {
@@ -697,6 +700,8 @@ int product(const Input& X, const uint8_t* W, const float* ws, void* Y, int c_dt
     p.beta     = beta;
     p.gelu     = epilogue == LYRAQ_EPI_GELU_TANH;
     p.status   = status_word_ptr();
+    p.wait_limit_ns = g_wait_limit_ns;
+    p.stalled_rank  = g_stalled_rank;
     const int sms = device_sm_count();
     if (p.status == nullptr || sms <= 0) {
         return LYRAQ_ERR_CUDA;
@@ -717,6 +722,13 @@ int lyraq_debug_force_fp8_block_tile(int code)
         return LYRAQ_ERR_INVALID_ARG;
     }
     fp8b::g_forced_tile = code;
+    return LYRAQ_OK;
+}
+
+int lyraq_debug_fp8_block_wait_test(int stalled_rank, unsigned int wait_limit_ms)
+{
+    fp8b::g_stalled_rank  = stalled_rank;
+    fp8b::g_wait_limit_ns = wait_limit_ms == 0 ? kWaitLimitNs : (unsigned long long)wait_limit_ms * 1000000ull;
     return LYRAQ_OK;
 }
 
