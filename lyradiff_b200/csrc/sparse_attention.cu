@@ -84,11 +84,11 @@ __device__ __forceinline__ void tma_load_4d(uint32_t smem_dst, const CUtensorMap
 
 // What a producer tells the other roles of an item: query block `qb` of head `h` of sequence `b`, its steps (-1: no item any more), the row of its list, how
 // much of the list counts, the keys that exist, the last key its row 0 sees, the first step in which a row may miss a key, the first keys of the
-// halves of its first step, its rows that exist (the others get zeros).
+// halves of its first step.
 struct alignas(16) Info {
     int qb, h, b, steps;
     int list, entries, len, place;
-    int masked, key[2], rows;
+    int masked, key[2], spare;
 };
 static_assert(sizeof(Info) == 48, "");
 
@@ -172,8 +172,7 @@ sparse_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                     it.h       = i / p.q_blocks % p.q_heads;
                     it.b       = i / (p.q_blocks * p.q_heads);
                     it.list    = (it.b * p.lists + it.h / (p.q_heads / p.lists)) * p.q_blocks + it.qb;
-                    it.rows    = query_count(p, it.b) - it.qb * kTile;
-                    it.entries = it.rows > 0 ? min(max(load_int(p.counts + it.list), 0), p.count) : 0;
+                    it.entries = min(max(load_int(p.counts + it.list), 0), p.count);
                     it.steps   = p.block == kTile ? it.entries : (it.entries + 1) / 2;
                     it.len     = key_count(p, it.b);
                     it.place   = p.causal ? (int)min((long long)first_place(p, it.b) + it.qb * kTile, (long long)kMaxKeys) : p.keys;
@@ -604,7 +603,8 @@ sparse_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
             }
             ++done;
             tc_fence_after_sync();
-            const bool  none  = m == -INFINITY || r >= it.rows;                // a row that saw no key, or does not exist: zeros
+            // a row that saw no key, or does not exist: zeros (its length is read here, as one more number kept through the steps cost up to 0.4 us a call)
+            const bool  none  = m == -INFINITY || (p.q_lens != nullptr && row >= query_count(p, it.b));
             const float inv_l = 1.0f / l;
 #pragma unroll
             for (int cc = 0; cc < D / 32; ++cc) {

@@ -135,8 +135,7 @@ sparse_attention_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const _
     }
     grid_dependency_wait();
     const int halves_per = p.block / kKeys;
-    const int q_count    = query_count(p, b);
-    const int entries    = q_count > 0 ? min(max(load_int(p.counts + unit), 0), p.count) : 0;
+    const int entries    = min(max(load_int(p.counts + unit), 0), p.count);
     const int halves     = entries * halves_per;
     const int len        = key_count(p, b);
     if (warp < kWarps) {
@@ -386,9 +385,10 @@ sparse_attention_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const _
             const float inv  = sum == 0.0f ? 0.0f : 1.0f / sum;      // no key seen: zeros
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                a[e] = qi < q_count ? a[e] * inv : 0.0f;             // nor does a row behind the sequence's queries have a result
+                a[e] *= inv;
             }
-            st_16(reinterpret_cast<T*>(p.out) + (long long)b * p.os.batch + (long long)qi * p.os.token + (long long)head * p.os.head + d, pack8<T>(a));
+            const Vec16 y = p.q_lens == nullptr || qi < query_count(p, b) ? pack8<T>(a) : Vec16{};    // a row behind the sequence's queries: zeros too
+            st_16(reinterpret_cast<T*>(p.out) + (long long)b * p.os.batch + (long long)qi * p.os.token + (long long)head * p.os.head + d, y);
         }
     }
     cluster_sync_all();   // no CTA leaves while a peer reads its shared memory
