@@ -30,7 +30,7 @@ __device__ __forceinline__ double widen_f32(uint32_t u) { return __hiloint2doubl
 // ------------------------------------------------------------------------------- means
 // A pass over memory: 100 MB, 15 us, for q of 32760 tokens in 12 heads of 128 (measured: 28, the additions).  WARPS warps take one block of tokens of one head: D / 8 lanes a token, 16 bytes
 // each, as many tokens at a time as there are lanes for; their sums meet in shared memory.  One warp a block where there are many, which spares
-// instructions (the sums' way through shared memory, a division a channel), four where few have to be quick.
+// instructions (the sums' way through shared memory, a division a channel), four where there are few.
 // An addition in 64 bits for every value took 35 us: B200 does six of them a clock and SM.  So 16 tokens at a time are added in fp32 with their
 // rounding errors beside them (D. Knuth's two-sum), and the sum and the sum of errors then go to 64 bits.  Both are exact as long as
 // the exponents of the values lie close enough: with the largest E (below 2^(E + 1)) a sum of 16 is below 2^(E + 5), an error at most 2^(E - 19) and 16 of them
@@ -511,11 +511,17 @@ int lyraq_block_means(float* means, const void* x, int dtype, size_t batch_step,
     // `newest` tokens touch one block more than they fill, at most
     const size_t touched  = newest == 0 ? blocks : ((size_t)newest + (size_t)block - 2) / (size_t)block + 1;
     const size_t per_head = touched < blocks ? touched : blocks, units = per_head * batch * (size_t)heads;
-    const bool   few      = units <= 592;      // a warp for each would leave schedulers without one
-    const size_t grid     = few ? units : (units + 3) / 4;
     if (units > 0x7ffffff0u) {
         return LYRAQ_ERR_UNSUPPORTED;
     }
+    const int sms = device_sm_count();
+    if (sms <= 0) {
+        return LYRAQ_ERR_CUDA;
+    }
+    // Four warps a block of tokens where one each would leave schedulers of an SM without one.  Four / one, us, changing buffers: 144 blocks of 128 x 128 6.6 / 10.4,
+    // 432 8.1 / 11.9, 580 13.4 / 12.0 (fp16: 13.1 / 14.7), 888 14.7 / 12.9; 144 of 64 x 128 4.4 / 6.3, 432 5.3 / 7.4, 588 7.6 / 7.2, 888 9.1 / 7.5.
+    const bool   few  = units <= 4 * (size_t)sms;
+    const size_t grid = few ? units : (units + 3) / 4;
     const bsel::MeansParams p{means,       x,     batch_step, token_step, head_step, lens, (int)tokens, heads, head_dim, block, (int)blocks,
                               newest < bsel::kMaxKeys ? newest : bsel::kMaxKeys, (int)per_head, head_step < token_step ? 1 : 0, (int)units};
     auto launch = [&](auto* kernel) {
@@ -611,6 +617,10 @@ int lyraq_select_blocks(const lyraq_select_blocks_t* s, void* workspace, size_t 
     p.window   = s->window;
     p.causal   = s->causal;
     cudaStream_t st = (cudaStream_t)stream;
+    const int    sms = device_sm_count();
+    if (sms <= 0) {
+        return LYRAQ_ERR_CUDA;
+    }
     if (k_blocks > 0) {
         const bool   few = q_blocks <= 8;
         const size_t qr = few ? 8 : 32, kt = few ? 128 : 64;
@@ -629,10 +639,10 @@ int lyraq_select_blocks(const lyraq_select_blocks_t* s, void* workspace, size_t 
     auto top = [&](auto* kernel, int warps) {
         return launch_kernel(kernel, (unsigned)(warps == 1 ? (rows + 3) / 4 : rows), warps == 1 ? 128u : (unsigned)(warps * 32), (size_t)0, st, 1u, p);
     };
-    // few rows are spread over more warps each: 32 rows of 512 7.4 us instead of 13; 864 rows of 72 5.6 us with one warp each, 13.9 with eight (all 32 halvings;
-    // 6.0 and 4.8 since they end as soon as the count is met, 3072 rows of 512 13.6 for 17.5)
-    const cudaError_t e = rows <= 148 && k_blocks <= 1024 ? top(bsel::block_top_kernel<8, 4>, 8)
-                          : k_blocks <= 128 ? top(bsel::block_top_kernel<1, 4>, 1)
+    // Few rows of many blocks are spread over eight warps each.  Eight warps / one, us, with the scores: 1 row of 128 7.8 / 6.6, of 129 6.7 / 8.5, of 512 7.5 / 11.9; 148 rows of
+    // 128 9.6 / 8.6, of 129 11.1 / 12.9, of 512 14.9 / 15.2; 600 rows of 129 15.4 / 11.7, 3000 of 512 42 / 29.
+    const cudaError_t e = k_blocks <= 128 ? top(bsel::block_top_kernel<1, 4>, 1)
+                          : rows <= (size_t)sms && k_blocks <= 1024 ? top(bsel::block_top_kernel<8, 4>, 8)
                           : k_blocks <= 512 ? top(bsel::block_top_kernel<1, 16>, 1)
                           : k_blocks <= 2048 ? top(bsel::block_top_kernel<4, 16>, 4)
                           : k_blocks <= 8192 ? top(bsel::block_top_kernel<16, 16>, 16)
