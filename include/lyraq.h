@@ -380,7 +380,8 @@ LYRAQ_API int lyraq_gemm_w4a4(const uint8_t* A, const uint8_t* B, const float* s
 
 /* FP8 with a scale for each block of 128: Y[m,n] = T( epi( sum_b s_x[m,b] s_w[n/128,b] * sum_{k in block b} X[m,k] W[n,k] + beta * R[m,n] + bias[n] ) ),
  * e4m3 codes X [m, k] and W [n, k], scales as lyraq_quant_fp8_block (element (row, block) of X's at row * x_scale_row + block * x_scale_block) and
- * lyraq_weight_quant_fp8_block leave them, fp32 accumulation, epi = identity or GELU-tanh.  Y, R and bias have element type c_dtype (f16, bf16, f32).
+ * lyraq_weight_quant_fp8_block leave them, fp32 accumulation (the factor s_x s_w is formed first, in fp32: below 2^-126 it loses digits,
+ * beyond the largest number it is infinite), epi = identity or GELU-tanh.  Y, R and bias have element type c_dtype (f16, bf16, f32).
  * k a multiple of 16; code, result, bias and residual pointers 16-byte aligned.  Y may be R; otherwise it shares no memory with the operands, or the call
  * is refused (LYRAQ_ERR_INVALID_ARG).  lyraq_gemm_fp8 for checkpoints with block scales; no counterpart in the reference. */
 LYRAQ_API int lyraq_gemm_fp8_block(const uint8_t* X, const float* x_scale, size_t x_scale_row, size_t x_scale_block, const uint8_t* W,
@@ -548,8 +549,10 @@ typedef struct {
 
 /* The count key blocks with the largest fl(q_mean . k_mean) (sum in 64 bits; q_mean the sum over the list's query heads) among those that hold a key a query of
  * the block may see, ties to the lowest index; blocks taken in any case come first, the lowest of them where they are more than count.  A score that
- * is no number comes last.  A query block without an existing query takes none.  Up to 32768 key blocks.  workspace: lyraq_select_blocks_workspace bytes, 16-byte aligned.  Outputs and workspace share no memory with anything
- * else.  It has no counterpart in the reference. */
+ * is no number comes last.  A query block without an existing query takes none.  causal says which blocks may be taken, not what a choice depends on: the means are
+ * over all 128 queries and over whole key blocks, so a list (and with it the result of each of its queries) also depends on tokens behind a query's place, and a
+ * sequence given at once and the same one token by token choose differently.  block up to 2^30, up to 32768 key blocks.  workspace: lyraq_select_blocks_workspace
+ * bytes, 16-byte aligned.  Outputs and workspace share no memory with anything else.  It has no counterpart in the reference. */
 LYRAQ_API int lyraq_select_blocks(const lyraq_select_blocks_t* args, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Workspace of lyraq_select_blocks (no counterpart in the reference). */
@@ -573,9 +576,10 @@ typedef struct {
 } lyraq_sparse_attention_t;
 
 /* out = softmax(q k^T * softmax_scale) v over the keys of the first counts[...] listed blocks that are below k_lens[b] and, if causal, not behind the
- * query's place; a query without any, or beyond q_lens, gets zeros.  An index outside the keys adds nothing, a block listed twice counts twice.  Keys and values
- * beyond k_lens may hold anything; in causal order the values within a listed block are finite.  All pointers of tensors 16-byte aligned, steps
- * multiples of 8; out shares no memory with what is read.  lyraq_attention over a part of the keys; no counterpart in the reference. */
+ * query's place; a query without any, or beyond q_lens, gets zeros, and so does one whose every score is -infinity.  An index outside the keys adds nothing, a
+ * block listed twice counts twice.  Keys and values beyond k_lens may hold anything; in causal order the values within a listed block are finite.  Scores and
+ * sums are held in 32 bits; the softmax's weights are rounded to the tensors' type for the product with v (half a step: 2^-8 of a weight in bf16, 2^-11 in f16),
+ * their sum is not.  All pointers of tensors 16-byte aligned, steps multiples of 8; out shares no memory with what is read.  lyraq_attention over a part of the keys; no counterpart in the reference. */
 LYRAQ_API int lyraq_sparse_attention(const lyraq_sparse_attention_t* args, void* stream);
 
 /* ------------------------------------------------------------------ quantized-Linear layer forwards

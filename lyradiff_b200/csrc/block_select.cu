@@ -3,8 +3,9 @@
 //   mean(block) = fl( sum of its existing tokens, in 64 bits, / their number )                     fl: rounding to fp32
 //   score(i, j) = fl( sum over the head's channels of q_mean(i) k_mean(j), in 64 bits )            for a shared list q_mean is the sum over its heads
 //
-// What is selected jumps where two scores change places, so the scores must not depend on the order of a sum: in 64 bits two orders differ by 2^-50
-// of a score, and both round to the same fp32 number but once in 2^26.  The means are held in 32 bits, which is part of the definition.
+// What is selected jumps where two scores change places, so the scores should not depend on the order of a sum.  In 64 bits two orders differ by some 2^-50 of
+// the sum of |q_mean k_mean|, and round to the same fp32 score unless it lies that close to the border of two: once in 2^26 where its terms hardly cancel, more
+// often the more they do.  The means are held in 32 bits, which is part of the definition.
 #include "common.cuh"
 #include "views.h"
 

@@ -2,7 +2,9 @@
 //
 // A row of k values is stored as k bytes of e4m3 codes (k a multiple of 16) and one fp32 scale for each 128 of them, the last block of a row
 // being shorter where k is no multiple of 128; a weight has one scale for each 128 rows x 128 columns.  value = code * s.
-//   s = fl(max|x| / 448), at least 2^-100 (below it every product with another operand's block is lost anyway); code = e4m3(fl(x / s))
+//   s = fl(max|x| / 448), at least 2^-100; code = e4m3(fl(x / s))
+// The least scale keeps a block of zeros from a division by 0, and the arithmetic of the quotients among normal numbers; blocks below 448 * 2^-100 = 3.5e-28 are
+// held in steps of 2^-109.
 // with fl rounding to fp32.  A block that holds an infinity or a NaN gets the scale NaN and zero codes: all of it reads back as NaN.
 #pragma once
 

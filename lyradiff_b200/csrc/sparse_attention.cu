@@ -10,6 +10,7 @@
 //   warps 0-3    softmax and epilogue of tile 0, warps 4-7 of tile 1: a thread owns one query row.  Keys of a half step that a row does not see are a
 //                tail of it (beyond the keys, or behind the row's place), so a mask is one number.
 // V rows beyond a sequence's keys may hold anything: the softmax warps clear them in shared memory, since 0 * NaN is NaN.
+// P is rounded to the tensors' type, which the MMAs ask for (both operands of one type); its sum l is of the numbers before.
 // Every wait is bounded; on a timeout the role records it in the status word, raises the block's abort flag and all roles leave; tensor
 // memory is freed at the common exit.
 //

@@ -8,6 +8,7 @@
 //   warp 4     TMA producer: K and V of a half block (64 keys x 64 columns a box) into a ring of stages
 //   warps 0-3  16 keys of each stage: S = Q K^T, running maximum and sum, O += P V; keys and values as they lie in shared memory by ldmatrix
 // V rows beyond a sequence's keys may hold anything: their registers are cleared, since 0 * NaN is NaN.
+// Weights are rounded to the tensors' type, as mma.sync asks for and as the kernel of many queries does; their sum is of the numbers before.
 // All waits are bounded.  A timeout sets the status word and the abort flag of every CTA of the cluster, and none of them stores anything.
 #include "sparse_attention.cuh"
 #include "sm100_ptx.cuh"

@@ -131,7 +131,8 @@ class Fp8BlockLinear:
 class SparseAttention:
     """Attention in which every 128 queries go to `count` blocks of `block` keys (64 or 128), chosen by the products of the blocks' means
     (ops.select_blocks; sink, window, shared and causal as there): for long sequences, where ops.flash_attention would read all keys.  Lists and means live
-    in memory taken from torch's allocator per call.  The reference's attention is dense."""
+    in memory taken from torch's allocator per call.  causal masks keys; a list is chosen by means over its 128 queries and over whole key blocks, so a token's
+    result also depends on later tokens of its block, and differs from the one it gets token by token.  The reference's attention is dense."""
 
     def __init__(self, block, count, sink=0, window=0, shared=False, causal=False, softmax_scale=None):
         if block not in (64, 128) or count < 1 or sink < 0 or window < 0:

@@ -367,7 +367,8 @@ def select_blocks(q_means, k_means, count, queries, keys, block, k_lens=None, q_
     product of means, ties to the lowest; the first `sink` blocks in any case, and with window = n > 0 those that hold the queries' own places and n - 1
     on either side.  q_means, k_means: block_means of q (with QUERY_BLOCK) and of k; queries, keys: tokens of both; k_lens int32 [batch]: keys of each
     sequence (default: all); q_start int32 [batch]: the key at which the first query stands (default: keys - queries); causal: only blocks with a key
-    at or before the last query's; shared: one list for the query heads of a key head.  q_lens int32 [batch]: queries of each sequence (default: all), with
+    at or before the last query's (which are chosen from depends on all queries of the block and on whole key blocks, also behind a query's place); shared:
+    one list for the query heads of a key head.  q_lens int32 [batch]: queries of each sequence (default: all), with
     q_means = block_means(q, QUERY_BLOCK, q_lens); blocks of queries that do not exist take nothing.  Returns (index int32 [batch, heads or key heads,
     ceil(queries / 128), count] in ascending order with -1 behind, counts int32)."""
     return _lib.host().select_blocks(q_means, k_means, block, count, sink, window, shared, causal, queries, keys, k_lens, q_start, q_lens)
@@ -377,8 +378,9 @@ def sparse_attention(q, k, v, index, counts, block, k_lens=None, q_start=None, c
     """Attention over the listed key blocks (lyraq_sparse_attention): q [batch, queries, heads, head_dim], k and v [batch, keys, key heads, head_dim], f16 or
     bf16, any steps with contiguous heads (views of a packed projection, a cache with heads before tokens by transpose), head_dim 64 or 128, block 64 or
     128.  index, counts: as select_blocks returns them, or any lists of that form.  Keys beyond k_lens, or behind a query's place in causal order, take no
-    part; a query that sees no key, or is beyond q_lens, gets zeros.  In causal order the values within a listed block have to be finite.  softmax_scale: head_dim ** -0.5
-    when omitted.  out is created when omitted and shares no memory with the inputs."""
+    part; a query that sees no key, or is beyond q_lens, gets zeros.  In causal order the values within a listed block have to be finite.  The weights
+    are rounded to the tensors' type before the product with v.  softmax_scale: head_dim ** -0.5 when omitted.  out is created when omitted and shares no
+    memory with the inputs."""
     if softmax_scale is None:
         softmax_scale = float(q.shape[-1]) ** -0.5
     return _lib.host().sparse_attention(q, k, v, index, counts, block, k_lens, q_start, causal, softmax_scale, out, q_lens)
